@@ -1,7 +1,7 @@
 """Build recipe for the in-tree HIP library ``slideformer_amd/lib/libslideformer_amd.so``.
 
 Usage: ``python -m slideformer_amd.build`` (also called by ``__graft_entry__.build()``);
-it also writes the small-grid test build ``lib/libslideformer_amd_smallgrid.so``, the
+it also writes the model operators' library ``lib/libslideformer_amd_ops.so``, the small-grid test build ``lib/libslideformer_amd_smallgrid.so``, the
 stream-probe library ``lib/libslideformer_amd_probe.so`` (bench only) and the C test
 driver ``tests/native/_build/device_from_c``.
 
@@ -79,6 +79,13 @@ SMALL_GRID_LIB = os.path.join(LIB_DIR, "libslideformer_amd_smallgrid.so")
 SMALL_GRID_DEFINES = {"LA_MAX_GRID": 64, "LA_NORM_MAX_GRID": 2, "LA_NORM_ONE": 16384, "LA_NORM_RUNS": 4096}
 
 
+# The operators at a model's two ends (include/model_ops.h), a library of their own:
+# a process that only steps an optimizer does not load them.
+OPS_LIB = os.path.join(LIB_DIR, "libslideformer_amd_ops.so")
+OPS_SOURCES = [os.path.join(CSRC, "embedding.hip"), os.path.join(CSRC, "rms_norm.hip"),
+               os.path.join(CSRC, "linear_loss.hip")]
+
+
 # The update kernel's memory-ceiling probes (csrc/stream_probe.hip: its exact
 # memory side with the arithmetic removed), loaded only by
 # `bench.py --update-ceiling`; a library of their own, so that the product
@@ -150,9 +157,10 @@ def build_host_calls(verbose: bool = False) -> str:
 
 
 def build_all(verbose: bool = False) -> list:
-    """The product library, the native host module, the small-grid test build, the stream probes and the C test
+    """The product libraries, the native host module, the small-grid test build, the stream probes and the C test
     driver."""
     return [build_library(verbose=verbose),
+            build_library(out=OPS_LIB, sources=OPS_SOURCES, verbose=verbose),
             build_host_calls(verbose=verbose),
             build_library(out=SMALL_GRID_LIB, defines=SMALL_GRID_DEFINES, verbose=verbose),
             build_library(out=PROBE_LIB, sources=PROBE_SOURCES, verbose=verbose),
