@@ -91,17 +91,23 @@ template <bool BY_ROWS> struct Operand {
         stage = wave * 1024;
     }
 
-    // Loads the next stage into `lds`; returns at once.
+    // Loads the next stage into `lds`; returns at once.  Written in assembly,
+    // which takes no result in a register: the compiler would wait for every such
+    // load before the next read of LDS, the one stage in flight included.  The
+    // loop waits itself, once a stage.
     __device__ void load(lds_char* lds)
     {
         const int64_t left = end - at;
         const uint32_t range = left <= 0 ? 0 : left > 0x7ffffff0 ? 0x7ffffff0 : static_cast<uint32_t>(left);
-        const __amdgpu_buffer_rsrc_t rsrc =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, static_cast<int>(range), 0x00020000);
+        const uint64_t address = reinterpret_cast<uint64_t>(at);
+        const u32x4_t rsrc{static_cast<uint32_t>(address), static_cast<uint32_t>(address >> 32), range, 0x00020000u};
+        const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + stage;
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, lds + n * 8192 + stage, 16, static_cast<int>(offset[n]), 0,
-                                                     0, 0);
+        for (uint32_t n = 0; n < 4; ++n)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :
+                         : "s"(to + n * 8192), "v"(offset[n]), "s"(rsrc)
+                         : "m0");
         at += step;
     }
 };
@@ -166,6 +172,7 @@ __device__ void product(const Matrix& inner, uint64_t inner_at, const Matrix& ou
     for (uint32_t stage = 0; stage < stages; ++stage) {
         lds_char* now = lds + (stage & 1) * (2 * kStageBytes);
         // this stage has arrived, and every wave has done with the other half
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (stage + 1 < stages) {
             lds_char* next = lds + (~stage & 1) * (2 * kStageBytes);
