@@ -155,81 +155,91 @@ struct ScoreArgs {
     Part* parts;                    // [rows of the piece][tiles of the vocabulary]
     float* target_scores;           // [rows of the piece]
     void* held;                     // [rows of the piece][tiles * 256], or null
-    uint32_t first, most, vocab, tiles, stages;
+    uint32_t first, most, vocab, tiles, steps;
 };
 
-template <typename T> __global__ __launch_bounds__(tile::kThreads, 2) void scores_kernel(ScoreArgs a)
+template <typename T> __global__ __launch_bounds__(tile::kThreads, 1) void scores_kernel(ScoreArgs a)
 {
-    __shared__ __attribute__((aligned(1024))) char lds[4 * tile::kStageBytes];
+    __shared__ __attribute__((aligned(1024))) char lds[tile::kLdsBytes];
     const uint32_t rows = piece_rows(a.plan, a.first, a.most);
     const tile::Place at = tile::place(blockIdx.x, ceil_div(rows, kTile), a.tiles);
     if (!at.valid) return;
     tile::Sums sums;
-    tile::product<T, true, true>(a.weight, at.inner * kTile, a.x, a.first + at.outer * kTile, 0, a.stages,
-                                 (tile::lds_char*)lds, sums);
+    tile::product<T, true, true>(a.weight, at.inner * kTile, a.x, a.first + at.outer * kTile, 0, a.steps,
+                                 lds, sums);
 
+    // [largest, sum][inner half][row of the tile], after what the tile is handed out through
+    float(*exchange)[2][kTile] = reinterpret_cast<float(*)[2][kTile]>(lds + tile::kHandOutBytes);
     const uint32_t lane = threadIdx.x % kWave, half = threadIdx.x / kWave % 2;
     const uint32_t column = at.inner * kTile + tile::wave_inner() + lane / 16 * 4;
-    float(*exchange)[2][kTile] = reinterpret_cast<float(*)[2][kTile]>(lds);   // [largest, sum][half][row of the tile]
-    __syncthreads();
-    float top[4];
+    if (at.inner * kTile + kTile > a.vocab)                      // columns past the vocabulary take no part
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (column + s * 16 + r >= a.vocab)
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) sums[s][t][r] = -INFINITY;
+    float top[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
         const uint32_t row = tile::wave_outer() + t * 16 + lane % 16;
+        const uint32_t in_piece = at.outer * kTile + row;
+        // the target's score, in the one lane that holds it
+        const uint32_t target = (in_piece < rows ? a.row_targets[a.first + in_piece] : -1) - column;
+        if (target < 128 && target % 16 < 4)
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (target == s * 16u + r) a.target_scores[in_piece] = sums[s][t][r];
         top[t] = -INFINITY;
 #pragma unroll
         for (int s = 0; s < 8; ++s)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if (column + s * 16 + r >= a.vocab) sums[s][t][r] = -INFINITY;
-                top[t] = fmaxf(top[t], sums[s][t][r]);
-            }
+            for (int r = 0; r < 4; ++r) top[t] = fmaxf(top[t], sums[s][t][r]);
         top[t] = fmaxf(top[t], __shfl_xor(top[t], 16));
         top[t] = fmaxf(top[t], __shfl_xor(top[t], 32));
         if (lane < 16) exchange[0][half][row] = top[t];
     }
     __syncthreads();
-    float sum[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 8; ++t) {
         const uint32_t row = tile::wave_outer() + t * 16 + lane % 16;
-        const uint32_t in_piece = at.outer * kTile + row;
-        const int32_t target = in_piece < rows ? a.row_targets[a.first + in_piece] : -1;
         top[t] = fmaxf(exchange[0][0][row], exchange[0][1][row]);
-        const float base = top[t] == -INFINITY ? 0.0f : top[t];   // a row of -inf: exp gives zeros
-        sum[t] = 0.0f;
+        // exp(s - m) as a power of 2, one multiply-add before it; a row of -inf gives zeros
+        constexpr float kLog2e = 1.44269504088896340736f;
+        const float base = top[t] == -INFINITY ? 0.0f : top[t] * -kLog2e;
+        float sum = 0.0f;
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            float e[4];
+        for (int s = 0; s < 8; ++s)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float score = sums[s][t][r];
-                if (static_cast<int32_t>(column + s * 16 + r) == target) a.target_scores[in_piece] = score;
-                e[r] = __expf(score - base);
-                sum[t] += e[r];
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sums[s][t][r], kLog2e, base));
+                sum += e;
+                sums[s][t][r] = e;
             }
-            if (a.held) {
-                typedef T v4 __attribute__((ext_vector_type(4)));
-                v4 v;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = static_cast<T>(e[r] * kHeld<T>);
-                *reinterpret_cast<v4*>(static_cast<T*>(a.held) +
-                                       static_cast<uint64_t>(in_piece) * a.tiles * kTile + column + s * 16) = v;
-            }
-        }
-        sum[t] += __shfl_xor(sum[t], 16);
-        sum[t] += __shfl_xor(sum[t], 32);
-        if (lane < 16) exchange[1][half][row] = sum[t];
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (lane < 16) exchange[1][half][row] = sum;
     }
     __syncthreads();
     if (half == 0 && lane < 16)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < 8; ++t) {
             const uint32_t row = tile::wave_outer() + t * 16 + lane;
-            const uint32_t in_piece = at.outer * kTile + row;
-            a.parts[static_cast<uint64_t>(in_piece) * a.tiles + at.inner] =
+            a.parts[static_cast<uint64_t>(at.outer * kTile + row) * a.tiles + at.inner] =
                 Part{top[t], exchange[1][0][row] + exchange[1][1][row]};
         }
+    if (!a.held) return;
+    T* held = static_cast<T*>(a.held) + static_cast<uint64_t>(at.outer) * kTile * a.tiles * kTile + at.inner * kTile;
+    tile::by_rows(sums, lds, [&](uint32_t outer, uint32_t inner, const float(&v)[8]) {
+        float e[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = v[k] * kHeld<T>;
+        *reinterpret_cast<u32x4_t*>(held + static_cast<uint64_t>(outer) * a.tiles * kTile + inner) =
+            Elem<T>::pack(e);
+    });
 }
 
 // ---------------------------------------------------------------------------
@@ -313,7 +323,7 @@ struct GradXArgs {
     const Plan* plan;
     const uint32_t* rows;
     float* partial;                 // [splits][rows of the piece][hidden]
-    uint32_t first, most, hidden, inners, stages, max_splits;
+    uint32_t first, most, hidden, inners, pairs, max_splits;   // pairs of steps
 };
 
 // Into how many runs of k a product of `tiles` tiles is split.  A compute unit
@@ -335,9 +345,9 @@ __device__ __forceinline__ uint32_t splits_of(uint32_t tiles, uint32_t max_split
     return best;
 }
 
-template <typename T> __global__ __launch_bounds__(tile::kThreads, 2) void grad_x_kernel(GradXArgs a)
+template <typename T> __global__ __launch_bounds__(tile::kThreads, 1) void grad_x_kernel(GradXArgs a)
 {
-    __shared__ __attribute__((aligned(1024))) char lds[4 * tile::kStageBytes];
+    __shared__ __attribute__((aligned(1024))) char lds[tile::kLdsBytes];
     const uint32_t rows = piece_rows(a.plan, a.first, a.most);
     const uint32_t outers = ceil_div(rows, kTile);
     if (outers == 0) return;
@@ -345,25 +355,17 @@ template <typename T> __global__ __launch_bounds__(tile::kThreads, 2) void grad_
     const tile::Place at = tile::place(blockIdx.x, outers * splits, a.inners);
     if (!at.valid) return;
     const uint32_t split = at.outer / outers, outer = at.outer % outers;
-    const uint32_t from = static_cast<uint64_t>(a.stages) * split / splits;
-    const uint32_t to = static_cast<uint64_t>(a.stages) * (split + 1) / splits;
+    const uint32_t from = static_cast<uint64_t>(a.pairs) * split / splits * 2;
+    const uint32_t to = static_cast<uint64_t>(a.pairs) * (split + 1) / splits * 2;
     tile::Sums sums;
     tile::product<T, false, true>(a.weight, at.inner * kTile, a.held, outer * kTile,
-                                  static_cast<uint64_t>(from) * tile::kDepth, to - from, (tile::lds_char*)lds, sums);
-    const uint32_t lane = threadIdx.x % kWave;
-    const uint32_t column = at.inner * kTile + tile::wave_inner() + lane / 16 * 4;
-    float* partial = a.partial + static_cast<uint64_t>(split) * a.most * a.hidden;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const uint32_t row = outer * kTile + tile::wave_outer() + t * 16 + lane % 16;
-        if (row >= rows) continue;
-        float* out = partial + static_cast<uint64_t>(row) * a.hidden;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            const float v[4] = {sums[s][t][0], sums[s][t][1], sums[s][t][2], sums[s][t][3]};
-            store_vec<float, 4>(out, (column + s * 16) / 4, a.hidden, v);
-        }
-    }
+                                  static_cast<uint64_t>(from) * tile::kDepth, to - from, lds, sums);
+    float* partial = a.partial + (static_cast<uint64_t>(split) * a.most + outer * kTile) * a.hidden;
+    tile::by_rows(sums, lds, [&](uint32_t row, uint32_t inner, const float(&v)[8]) {
+        if (outer * kTile + row < rows)
+            store_vec<float, 8>(partial + static_cast<uint64_t>(row) * a.hidden, (at.inner * kTile + inner) / 8,
+                                a.hidden, v);
+    });
 }
 
 template <typename T>
@@ -399,58 +401,42 @@ struct GradWeightArgs {
 };
 
 template <typename T, typename W>
-__global__ __launch_bounds__(tile::kThreads, 2) void grad_weight_kernel(GradWeightArgs a)
+__global__ __launch_bounds__(tile::kThreads, 1) void grad_weight_kernel(GradWeightArgs a)
 {
-    __shared__ __attribute__((aligned(1024))) char lds[4 * tile::kStageBytes];
+    __shared__ __attribute__((aligned(1024))) char lds[tile::kLdsBytes];
     const uint32_t rows = piece_rows(a.plan, a.first, a.most);
     if (rows == 0 && a.first > 0) return;
     const tile::Place at = tile::place(blockIdx.x, a.outers, a.inners);
     if (!at.valid) return;
     tile::Sums sums;
-    tile::product<T, false, false>(a.x, at.inner * kTile, a.held, at.outer * kTile, 0, ceil_div(rows, tile::kDepth),
-                                   (tile::lds_char*)lds, sums);
+    tile::product<T, false, false>(a.x, at.inner * kTile, a.held, at.outer * kTile, 0, ceil_div(rows, 2 * tile::kDepth) * 2,
+                                   lds, sums);
     const bool last = a.first + rows >= a.plan->rows;
     const float factor = a.plan->factor;
-    const uint32_t lane = threadIdx.x % kWave;
-    const uint32_t column = at.inner * kTile + tile::wave_inner() + lane / 16 * 4;
+    tile::by_rows(sums, lds, [&](uint32_t outer, uint32_t inner, const float(&sum)[8]) {
+        const uint32_t row = at.outer * kTile + outer, vec = (at.inner * kTile + inner) / 8;
+        if (row >= a.vocab) return;
+        float v[8];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const uint32_t row = at.outer * kTile + tile::wave_outer() + t * 16 + lane % 16;
-        if (row >= a.vocab) continue;
-        W* out = static_cast<W*>(a.grad_weight) + row * a.stride;
+        for (int k = 0; k < 8; ++k) v[k] = sum[k];
         float* total = a.total + static_cast<uint64_t>(row) * a.hidden;
+        if (a.first > 0)
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            const uint32_t vec = (column + s * 16) / 4;
-            float v[4] = {sums[s][t][0], sums[s][t][1], sums[s][t][2], sums[s][t][3]};
-            if (a.first > 0) {
-                float before[4];
-                load_vec<float>(total, vec, a.hidden, before);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] += before[r];
-            }
-            if (!last) {
-                store_vec<float, 4>(total, vec, a.hidden, v);
-                continue;
-            }
-            if (vec * 4 + 4 <= a.hidden) {
-                typedef W v4 __attribute__((ext_vector_type(4), aligned(sizeof(W))));
-                v4* to = reinterpret_cast<v4*>(out + vec * 4);
-                v4 w;
-                if (a.accumulate) w = *to;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    w[r] = Elem<W>::from_f32(v[r] * factor + (a.accumulate ? Elem<W>::to_f32(w[r]) : 0.0f));
-                *to = w;
-            } else {
-#pragma unroll
-                for (uint32_t r = 0; r < 4; ++r)
-                    if (vec * 4 + r < a.hidden)
-                        out[vec * 4 + r] = Elem<W>::from_f32(
-                            v[r] * factor + (a.accumulate ? Elem<W>::to_f32(out[vec * 4 + r]) : 0.0f));
-            }
+            for (uint32_t k = 0; k < 8; ++k)
+                if (vec * 8 + k < a.hidden) v[k] += total[vec * 8 + k];
+        if (!last) {
+            store_vec<float, 8>(total, vec, a.hidden, v);
+            return;
         }
-    }
+        W* out = static_cast<W*>(a.grad_weight) + row * a.stride;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= factor;
+        if (a.accumulate)
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k)
+                if (vec * 8 + k < a.hidden) v[k] += Elem<W>::to_f32(out[vec * 8 + k]);
+        store_vec<W, 8>(out, vec, a.hidden, v);
+    });
 }
 
 // ---------------------------------------------------------------------------
@@ -462,6 +448,8 @@ constexpr uint64_t kMaxVocab = 1ull << 21;          // a tile's rows stay within
 constexpr uint64_t kForwardRows = 16384;            // rows of a piece without gradients: only `parts` grows with it
 constexpr uint64_t kMostRows = 32768;               // and of any piece: a launch's second dimension has 16 bits
 
+constexpr uint64_t kPair = 2 * tile::kDepth;        // k is padded to: a product takes an even number of steps
+
 bool sizes_ok(const la_linear_loss_t& c)
 {
     return c.n <= kMaxRows && c.hidden > 0 && c.hidden <= kMaxHidden && c.vocab > 0 && c.vocab <= kMaxVocab &&
@@ -471,7 +459,7 @@ bool sizes_ok(const la_linear_loss_t& c)
 // Whether the products can read the matrix where it lies.
 bool reads_in_place(const la_linear_loss_t& c)
 {
-    return c.hidden % tile::kDepth == 0 && c.weight_stride % 8 == 0 && reinterpret_cast<uintptr_t>(c.weight) % 16 == 0;
+    return c.hidden % kPair == 0 && c.weight_stride % 8 == 0 && reinterpret_cast<uintptr_t>(c.weight) % 16 == 0;
 }
 
 // Sizes and the workspace's parts (offsets in bytes).
@@ -481,7 +469,7 @@ struct Layout {
 
     explicit Layout(const la_linear_loss_t& c)
     {
-        padded = ceil_div(c.hidden, tile::kDepth) * tile::kDepth;
+        padded = ceil_div(c.hidden, kPair) * kPair;
         tiles = ceil_div(c.vocab, kTile);
         inners = ceil_div(c.hidden, kTile);
         all = c.n > 0 ? ceil_div(c.n, kTile) * kTile : kTile;     // no rows: one empty piece, which clears grad_weight
@@ -565,7 +553,7 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
         if (rc != LA_OK) return rc;
         const GradXArgs gx{weight, d, plan, rows, reinterpret_cast<float*>(ws + l.partial), first, most,
                            static_cast<uint32_t>(c.hidden), static_cast<uint32_t>(l.inners),
-                           static_cast<uint32_t>(l.tiles * (kTile / tile::kDepth)),
+                           static_cast<uint32_t>(l.tiles * (kTile / kPair)),
                            static_cast<uint32_t>(l.max_splits)};
         rc = launch(grad_x_kernel<T>, dim3(tile::places(most / kTile * l.max_splits, l.inners)), dim3(tile::kThreads),
                     st, gx);

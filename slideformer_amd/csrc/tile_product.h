@@ -9,14 +9,22 @@
 // so no operand is transposed in memory for any of the three products of a linear
 // layer with a loss.
 //
-// A workgroup of 8 waves computes one tile.  Both operands go from memory into
-// LDS 64 k at a time without passing registers, two stages in turn.  The LDS
-// image is permuted so that no read has bank conflicts; since the loads write
-// LDS linearly, the permutation is applied to the addresses that they read:
-//   by rows      [256][64]: 16-byte chunk c of row r is at chunk c ^ (r & 7), so 8
-//                lanes that read one chunk column of 8 rows hit 8 chunks;
-//   by columns   [64][256]: 32-byte segment s of row k is at s ^ (k & 15), so the
-//                four rows that a transposing read takes at one s differ in banks.
+// A workgroup of 4 waves, one on each SIMD, computes one tile, a quarter of it per
+// wave: 128 x 128 sums in 256 registers.  At that size a step of 32 k takes a wave 64
+// matrix instructions (1024 cycles) and the workgroup 64 KB of LDS reads and 32 KB of
+// writes (768 cycles at 128 bytes each), so LDS stays behind the matrix cores; with
+// eight waves of 128 x 64 the reads alone take as long as the products.  What a wave
+// multiplies in one step it reads from LDS during the step before, instruction by
+// instruction between the products, so that neither waits for the other.
+//
+// Operands go from memory into LDS without passing registers, four steps ahead.
+// The LDS image is permuted so that no read has bank conflicts; since the loads
+// write LDS linearly, the permutation is applied to the addresses that they read:
+//   by rows      [256][32]: 16-byte chunk c of row r is at chunk c ^ (r / 2 % 4), so 8
+//                lanes that read one chunk column of 8 rows hit all 128 bytes of banks;
+//   by columns   [32][256]: 32-byte segment s of row k is at s ^ f(k), f taking bits 0, 1, 3
+//                and 2 of k in this order, so the eight rows that two groups of lanes
+//                read at one s by a transposing read differ in banks.
 // Rows and columns beyond a matrix's memory read as zeros through the buffer
 // descriptor's range.
 #ifndef SLIDEFORMER_AMD_TILE_PRODUCT_H
@@ -27,9 +35,12 @@
 namespace tile {
 
 constexpr int kTile = 256;          // both sides of a tile
-constexpr int kDepth = 64;          // k per stage
-constexpr int kThreads = 512;
-constexpr int kStageBytes = kTile * kDepth * 2;
+constexpr int kDepth = 32;          // k per step
+constexpr int kAhead = 4;           // steps in LDS
+constexpr int kThreads = 256;
+constexpr int kPanelBytes = kTile * kDepth * 2;             // one operand's share of a step
+constexpr int kStepBytes = 2 * kPanelBytes;
+constexpr int kLdsBytes = kAhead * kStepBytes;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -38,21 +49,19 @@ typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) s16x8 lds_s16x8;
 
-template <typename T> struct Mfma;
-template <> struct Mfma<__bf16> {
-    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
-    __device__ static f32x4 run(s16x8 a, s16x8 b, f32x4 c)
-    {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
-    }
-};
-template <> struct Mfma<_Float16> {
-    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
-    __device__ static f32x4 run(s16x8 a, s16x8 b, f32x4 c)
-    {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
-    }
-};
+// c += a b^T.  Written in assembly to keep a sum in its registers: left to itself
+// the compiler gives each product a destination of its own, and with all
+// accumulation registers in use it then moves sums about, more often than it
+// multiplies.  It cannot see that the results of these take a while; settle() waits.
+template <typename T> __device__ __forceinline__ void multiply(const s16x8& a, const s16x8& b, f32x4& c);
+template <> __device__ __forceinline__ void multiply<__bf16>(const s16x8& a, const s16x8& b, f32x4& c)
+{
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+template <> __device__ __forceinline__ void multiply<_Float16>(const s16x8& a, const s16x8& b, f32x4& c)
+{
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
 
 // An operand in memory: `count` rows of `width` 16-bit elements, `stride` bytes apart.
 struct Matrix {
@@ -62,58 +71,63 @@ struct Matrix {
 
 // One operand's share of a workgroup's work.  BY_ROWS: see above.
 template <bool BY_ROWS> struct Operand {
-    const char* at;                 // this stage's corner in memory
-    const char* end;                // one past the matrix's last byte
-    uint64_t step;                  // bytes from stage to stage
+    uint64_t at;                    // the next step's corner in memory
+    uint64_t left;                  // bytes from there to the matrix's end
+    uint64_t stride;                // bytes from step to step
+    uint32_t steps;                 // with data to read
     uint32_t offset[4];             // of this lane's four loads
-    uint32_t stage;                 // this wave's place in a stage
+    u32x4_t rsrc;
 
-    __device__ void init(const Matrix& m, uint64_t tile_at, uint64_t k_at)
+    __device__ void init(const Matrix& m, uint64_t tile_at, uint64_t k_at, uint32_t wanted)
     {
-        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-        const char* data = static_cast<const char*>(m.data);
-        end = data + (m.count - 1) * m.stride + m.width * 2;
+        const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+        const uint64_t from = BY_ROWS ? tile_at * m.stride + k_at * 2 : k_at * m.stride + tile_at * 2;
+        at = reinterpret_cast<uint64_t>(m.data) + from;
+        left = (m.count - 1) * m.stride + m.width * 2 - from;
         if constexpr (BY_ROWS) {
-            at = data + tile_at * m.stride + k_at * 2;
-            step = kDepth * 2;
+            stride = kDepth * 2;
+            steps = wanted;
 #pragma unroll
             for (uint32_t n = 0; n < 4; ++n)
-                offset[n] = (n * 64 + wave * 8 + lane / 8) * static_cast<uint32_t>(m.stride) +
-                            ((lane % 8) ^ (lane / 8)) * 16;
+                offset[n] = (n * 64 + wave * 16 + lane / 4) * static_cast<uint32_t>(m.stride) +
+                            ((lane % 4) ^ (lane / 8 % 4)) * 16;
         } else {
-            at = data + k_at * m.stride + tile_at * 2;
-            step = kDepth * m.stride;
-            const uint32_t k = wave * 2 + lane / 32;        // & 15: the rows of one lane's loads are 16 apart
-            const uint32_t chunk = (((lane % 32 / 2) ^ k) * 2 + lane % 2) * 16;
+            stride = kDepth * m.stride;
+            const uint64_t there = m.count > k_at ? (m.count - k_at + kDepth - 1) / kDepth : 0;
+            steps = there < wanted ? static_cast<uint32_t>(there) : wanted;
 #pragma unroll
-            for (uint32_t n = 0; n < 4; ++n) offset[n] = (n * 16 + k) * static_cast<uint32_t>(m.stride) + chunk;
+            for (uint32_t n = 0; n < 4; ++n) {
+                const uint32_t k = n * 8 + wave * 2 + lane / 32;
+                const uint32_t f = (k & 3) | (k >> 3 & 1) << 2 | (k >> 2 & 1) << 3;
+                offset[n] = k * static_cast<uint32_t>(m.stride) + (((lane % 32 / 2) ^ f) * 2 + lane % 2) * 16;
+            }
         }
-        stage = wave * 1024;
     }
 
-    // Loads the next stage into `lds`; returns at once.  Written in assembly,
-    // which takes no result in a register: the compiler would wait for every such
-    // load before the next read of LDS, the one stage in flight included.  The
-    // loop waits itself, once a stage.
-    __device__ void load(lds_char* lds)
+    // Turns to step `step`, the one after the last; one without data reads zeros.
+    __device__ __forceinline__ void turn(uint32_t step)
     {
-        const int64_t left = end - at;
-        const uint32_t range = left <= 0 ? 0 : left > 0x7ffffff0 ? 0x7ffffff0 : static_cast<uint32_t>(left);
-        const uint64_t address = reinterpret_cast<uint64_t>(at);
-        const u32x4_t rsrc{static_cast<uint32_t>(address), static_cast<uint32_t>(address >> 32), range, 0x00020000u};
-        const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + stage;
-#pragma unroll
-        for (uint32_t n = 0; n < 4; ++n)
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                         :
-                         : "s"(to + n * 8192), "v"(offset[n]), "s"(rsrc)
-                         : "m0");
-        at += step;
+        const uint32_t low = static_cast<uint32_t>(left), high = static_cast<uint32_t>(left >> 32);
+        rsrc = u32x4_t{static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32),
+                       step < steps ? (high ? 0xffffffffu : low) : 0u, 0x00020000u};
+        at += stride;
+        left -= stride;
+    }
+
+    // Load `n` of the step, to this wave's place `lds`; returns at once.  Written in
+    // assembly, which takes no result in a register: the compiler would wait for
+    // every load in flight before any read of LDS.  The loop waits itself.
+    __device__ void load(uint32_t lds, int n) const
+    {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                     :
+                     : "s"(lds + n * 4096), "v"(offset[n]), "s"(rsrc)
+                     : "m0");
     }
 };
 
-// The 16 x 32 fragment of tile rows `at`.. and k `half` * 32.., as the matrix
-// instructions take it: lane l holds row l % 16, k (l / 16) * 8 .. + 7.
+// The 16 x 32 fragment of tile rows `tile_at` + 16 n .., as the matrix instructions
+// take it: lane l holds row l % 16, k (l / 16) * 8 .. + 7.
 template <bool BY_ROWS> struct Fragments {
     uint32_t base;
 
@@ -121,76 +135,176 @@ template <bool BY_ROWS> struct Fragments {
     {
         const uint32_t lane = threadIdx.x % 64, row = lane % 16, group = lane / 16;
         if constexpr (BY_ROWS) {
-            base = (tile_at + row) * 128 + ((group ^ (row & 7)) * 16);
+            base = (tile_at + row) * 64 + (group ^ (row / 2 % 4)) * 16;
         } else {
-            const uint32_t k = group * 8 + row / 4;
-            base = k * 512 + (((tile_at / 16) ^ (k & 15)) * 32) + (row % 4) * 8;
+            const uint32_t k = group * 8 + row / 4;         // bit 2 is clear, and set in the second read
+            const uint32_t f = (k & 3) | (k >> 3 & 1) << 2;
+            base = k * 512 + ((tile_at / 16) ^ f) * 32 + (row % 4) * 8;
         }
     }
 
-    __device__ s16x8 read(const lds_char* lds, int n, int half) const
+    __device__ s16x8 read(const lds_char* lds, int n) const
     {
         if constexpr (BY_ROWS) {
-            return *reinterpret_cast<const lds_s16x8*>(lds + (base ^ (half * 64)) + n * 2048);
+            return *reinterpret_cast<const lds_s16x8*>(lds + base + n * 1024);
         } else {
             // lanes 4j .. 4j+3 of a group of 16 read 16 elements of row j; lane l gets column l of the four rows
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_s16x4*)(lds + (base ^ (n * 32)) + half * 16384));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_s16x4*)(lds + (base ^ ((n ^ 4) * 32)) + half * 16384 + 2048));
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + (base ^ (n * 32))));
+            const s16x4 hi =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + (base ^ (n * 32) ^ 256) + 2048));
             return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
 };
 
-// A wave's part of the tile: 128 inner x 64 outer.  Element [s][t][r] of a lane
-// is inner 16 s + (lane / 16) * 4 + r, outer 16 t + lane % 16 of that part.
-typedef f32x4 Sums[8][4];
+// A wave's quarter of the tile.  Element [s][t][r] of a lane is inner
+// 16 s + (lane / 16) * 4 + r, outer 16 t + lane % 16 of that quarter.
+typedef f32x4 Sums[8][8];
+typedef s16x8 Step[2][8];           // a wave's fragments of one step: inner, outer
 
 __device__ __forceinline__ uint32_t wave_inner() { return threadIdx.x / 64 % 2 * 128; }
-__device__ __forceinline__ uint32_t wave_outer() { return threadIdx.x / 128 * 64; }
+__device__ __forceinline__ uint32_t wave_outer() { return threadIdx.x / 128 * 128; }
 
-template <typename T, bool INNER_ROWS, bool OUTER_ROWS>
-__device__ void product(const Matrix& inner, uint64_t inner_at, const Matrix& outer, uint64_t outer_at, uint64_t k_at,
-                        uint32_t stages, lds_char* lds, Sums& sums)
+// Waits until at most `left` loads of this wave are in flight and its reads of
+// LDS are done, then for the other waves to come this far.
+template <int LEFT> __device__ __forceinline__ void arrive()
 {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(LEFT) : "memory");
+}
+
+// Places all sums in accumulation registers, and waits until what wrote them has
+// and what reads them may: longer than any matrix instruction or move needs.
+__device__ __forceinline__ void settle(Sums& sums)
+{
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) asm volatile("" : "+a"(sums[s][t]));
+    asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15");
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) asm volatile("" : "+a"(sums[s][t]));
+}
+
+template <typename T, bool INNER_ROWS, bool OUTER_ROWS> struct Product {
     Operand<INNER_ROWS> load_inner;
     Operand<OUTER_ROWS> load_outer;
     Fragments<INNER_ROWS> read_inner;
     Fragments<OUTER_ROWS> read_outer;
-    load_inner.init(inner, inner_at, k_at);
-    load_outer.init(outer, outer_at, k_at);
-    read_inner.init(wave_inner());
-    read_outer.init(wave_outer());
+    lds_char* lds;
+    uint32_t place;                 // of this wave's loads in a panel
+
+    // One step: multiplies `now`, reads the fragments of the next step into `then`,
+    // and loads the step kAhead from here over this one, whose reads are over.
+    __device__ __forceinline__ void step(uint32_t at, const Step& now, Step& then, Sums& sums)
+    {
+        // the next step's loads have arrived: only those of two steps more are in flight
+        arrive<(kAhead - 2) * 8>();
+        const lds_char* from = lds + (at + 1) % kAhead * kStepBytes;
+        const uint32_t to =
+            __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) +
+                                           at % kAhead * kStepBytes + place);
 #pragma unroll
-    for (int s = 0; s < 8; ++s)
+        for (int g = 0; g < 16; ++g) {
+            if (g < 8) {
+                then[0][g] = read_inner.read(from, g);
+                then[1][g] = read_outer.read(from + kPanelBytes, g);
+            }
+            if (g == 6) load_inner.turn(at + kAhead);
+            if (g == 9) load_outer.turn(at + kAhead);
+            if (g >= 8 && g < 12) load_inner.load(to, g - 8);
+            if (g >= 12) load_outer.load(to + kPanelBytes, g - 12);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) sums[s][t] = f32x4{0, 0, 0, 0};
-    if (stages == 0) return;
-    load_inner.load(lds);
-    load_outer.load(lds + kStageBytes);
-    for (uint32_t stage = 0; stage < stages; ++stage) {
-        lds_char* now = lds + (stage & 1) * (2 * kStageBytes);
-        // this stage has arrived, and every wave has done with the other half
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (stage + 1 < stages) {
-            lds_char* next = lds + (~stage & 1) * (2 * kStageBytes);
-            load_inner.load(next);
-            load_outer.load(next + kStageBytes);
+            for (int k = 0; k < 4; ++k) {
+                const int s = g / 2, t = g % 2 * 4 + k;
+                multiply<T>(now[0][s], now[1][t], sums[s][t]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
+    }
+
+    __device__ __forceinline__ void run(const Matrix& inner, uint64_t inner_at, const Matrix& outer, uint64_t outer_at,
+                                        uint64_t k_at, uint32_t steps, char* shared, Sums& sums)
+    {
+        lds = (lds_char*)shared;
+        place = threadIdx.x / 64 * 1024;
+        load_inner.init(inner, inner_at, k_at, steps);
+        load_outer.init(outer, outer_at, k_at, steps);
+        read_inner.init(wave_inner());
+        read_outer.init(wave_outer());
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            s16x8 a[8], b[4];
+        for (int s = 0; s < 8; ++s)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) b[t] = read_outer.read(now + kStageBytes, t, half);
+            for (int t = 0; t < 8; ++t) sums[s][t] = f32x4{0, 0, 0, 0};
+        if (steps == 0) return;
 #pragma unroll
-            for (int s = 0; s < 8; ++s) a[s] = read_inner.read(now, s, half);
+        for (int ahead = 0; ahead < kAhead; ++ahead) {
+            const uint32_t to = __builtin_amdgcn_readfirstlane(
+                static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + ahead * kStepBytes + place);
+            load_inner.turn(ahead);
+            load_outer.turn(ahead);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) load_inner.load(to, n);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) load_outer.load(to + kPanelBytes, n);
+        }
+        arrive<(kAhead - 1) * 8>();
+        Step even, odd;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            even[0][n] = read_inner.read(lds, n);
+            even[1][n] = read_outer.read(lds + kPanelBytes, n);
+        }
+        settle(sums);
+        for (uint32_t at = 0; at < steps; at += 2) {
+            step(at, even, odd, sums);
+            step(at + 1, odd, even, sums);
+        }
+        settle(sums);
+        // the loads that read zeros are over, and every wave has done with LDS
+        arrive<0>();
+    }
+};
+
+// sums = the tile at (inner_at, outer_at) over `steps` steps from k_at, an even number.
+template <typename T, bool INNER_ROWS, bool OUTER_ROWS>
+__device__ __forceinline__ void product(const Matrix& inner, uint64_t inner_at, const Matrix& outer, uint64_t outer_at,
+                                        uint64_t k_at, uint32_t steps, char* shared, Sums& sums)
+{
+    Product<T, INNER_ROWS, OUTER_ROWS> p;
+    p.run(inner, inner_at, outer, outer_at, k_at, steps, shared, sums);
+}
+
+// Hands a wave's quarter of the tile out by rows: emit(outer, inner, v) with eight
+// consecutive inner elements, 16 lanes to a row, so that what is stored from them
+// fills whole lines.  Goes through this wave's part of LDS, a quarter of the rows at
+// a time; the row distance of 132 keeps its accesses free of bank conflicts.
+constexpr int kHandOutBytes = 4 * 32 * 132 * 4;
+
+template <typename Emit> __device__ __forceinline__ void by_rows(const Sums& sums, char* shared, const Emit& emit)
+{
+    constexpr uint32_t kRow = 132;
+    const uint32_t lane = threadIdx.x % 64;
+    float* mine = reinterpret_cast<float*>(shared) + threadIdx.x / 64 * (32 * kRow);
+#pragma unroll
+    for (int part = 0; part < 4; ++part) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int s = 0; s < 8; ++s)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) sums[s][t] = Mfma<T>::run(a[s], b[t], sums[s][t]);
+                *reinterpret_cast<f32x4*>(mine + (t * 16 + lane % 16) * kRow + s * 16 + lane / 16 * 4) =
+                    sums[s][part * 2 + t];
+        // the wave's own stores, seen by its own loads: the hardware keeps them in order
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+        for (uint32_t row = lane / 16; row < 32; row += 4) {
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(mine + row * kRow + lane % 16 * 8);
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(mine + row * kRow + lane % 16 * 8 + 4);
+            const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            emit(wave_outer() + part * 32 + row, wave_inner() + lane % 16 * 8, v);
         }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
