@@ -49,9 +49,9 @@ int la_embedding(int token_dtype, const void* tokens, uint64_t n, int dtype, con
  * held in fp32 in the order of i, in groups whose bounds depend on the tokens
  * alone: equal calls give equal bits.  Tokens outside [0, vocab) and those equal
  * to padding_idx (negative: none) contribute nothing.
- * workspace: la_embedding_grad_workspace(n, hidden) bytes, 16-byte aligned.
+ * workspace: la_embedding_grad_workspace(n, vocab, hidden) bytes, 16-byte aligned.
  */
-uint64_t la_embedding_grad_workspace(uint64_t n, uint64_t hidden);
+uint64_t la_embedding_grad_workspace(uint64_t n, uint64_t vocab, uint64_t hidden);
 int la_embedding_grad(int token_dtype, const void* tokens, uint64_t n, int g_dtype, const void* grad_out,
                       uint64_t grad_stride, int out_dtype, void* grad_weight, uint64_t vocab, uint64_t hidden,
                       uint64_t weight_stride, float scale, int64_t padding_idx, int accumulate, void* workspace,

@@ -63,51 +63,64 @@ __global__ __launch_bounds__(256) void embedding_kernel(const I* tokens, uint64_
 // sorting the tokens
 // ---------------------------------------------------------------------------
 // A chunk of kChunk tokens is sorted by counting, for each, the tokens of the
-// chunk that come before it: kChunk compares a token, spread over the whole GPU
+// chunk that come before it: kChunk compares a token, spread over many workgroups
 // with no data exchanged.  Chunks are then merged by binary search: a token's
 // place is its place in its own chunk plus, for each other chunk, the number of
-// tokens before it there (equal ones count in earlier chunks only).
-constexpr int kChunk = 4096;
-constexpr int kRankTokens = 64;           // tokens ranked by one workgroup, four lanes each
-constexpr int32_t kNone = INT32_MAX;      // sorts after every token
+// tokens before it there (equal ones count in earlier chunks only).  Two launches
+// whatever the vocabulary; with chunks of 1024 they take 8192 tokens 5.6 + 5.0 us, with
+// chunks of 4096 the counting alone took 54.
+constexpr int kChunk = 1024;
+constexpr int kRankLanes = 16;            // that share one token's compares
+constexpr int kRankTokens = 256 / kRankLanes;   // ranked by one workgroup
+constexpr int kRankGroups = kChunk / kRankTokens;
+constexpr uint32_t kNone = 0x7fffffffu;   // sorts after every token
 
-__device__ __forceinline__ int32_t sort_key(uint64_t t, uint64_t vocab, int64_t padding)
+__device__ __forceinline__ uint32_t sort_key(uint64_t t, uint64_t vocab, int64_t padding)
 {
-    return t < vocab && t != static_cast<uint64_t>(padding) ? static_cast<int32_t>(t) : kNone;
+    return t < vocab && t != static_cast<uint64_t>(padding) ? static_cast<uint32_t>(t) : kNone;
 }
 
+// The workgroups after the first `groups` clear the marks of the tokens that occur.
 template <typename I>
 __global__ __launch_bounds__(256) void rank_kernel(const I* tokens, uint32_t n, uint64_t vocab, int64_t padding,
-                                                   int32_t* keys, uint32_t* places)
+                                                   uint32_t* keys, uint32_t* places, uint32_t groups, uint4* marks)
 {
-    __shared__ __attribute__((aligned(16))) int32_t chunk[kChunk];
-    const uint32_t base = blockIdx.x / (kChunk / kRankTokens) * kChunk;
-    const uint32_t mine = blockIdx.x % (kChunk / kRankTokens) * kRankTokens + threadIdx.x / 4;
+    const uint32_t group = blockIdx.x;
+    if (group >= groups) {
+        const uint64_t at = static_cast<uint64_t>(group - groups) * 256 + threadIdx.x;
+        if (at * 16 < vocab) marks[at] = uint4{0, 0, 0, 0};
+        return;
+    }
+    __shared__ __attribute__((aligned(16))) uint32_t chunk[kChunk];
+    const uint32_t base = group / kRankGroups * kChunk;
+    const uint32_t mine = group % kRankGroups * kRankTokens + threadIdx.x / kRankLanes;
     const uint32_t size = n - base < kChunk ? n - base : kChunk;
-    if (mine - threadIdx.x / 4 >= size) return;                    // the whole workgroup
+    if (group % kRankGroups * kRankTokens >= size) return;          // the whole workgroup
+#pragma unroll
     for (uint32_t k = threadIdx.x; k < kChunk; k += 256)
         chunk[k] = k < size ? sort_key(token_at(tokens, base + k), vocab, padding) : kNone;
     __syncthreads();
-    const int32_t key = chunk[mine];
-    const uint32_t lane = threadIdx.x % 4;
+    const uint32_t key = chunk[mine];
+    const uint32_t lane = threadIdx.x % kRankLanes;
     uint32_t before = 0;
-    for (uint32_t quad = lane; quad * 4 < size; quad += 4) {
-        const int4 k = *reinterpret_cast<const int4*>(chunk + quad * 4);
-        const int32_t other[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll 4
+    for (uint32_t quad = lane; quad < kChunk / 4; quad += kRankLanes) {
+        const uint4 k = *reinterpret_cast<const uint4*>(chunk + quad * 4);
+        const uint32_t other[4] = {k.x, k.y, k.z, k.w};
+        // an equal key counts where it stands before
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e)
-            before += other[e] < key || (other[e] == key && quad * 4 + e < mine);
+        for (uint32_t e = 0; e < 4; ++e) before += other[e] < key + (quad * 4 + e < mine);
     }
-    before += __shfl_xor(before, 1);
-    before += __shfl_xor(before, 2);
+#pragma unroll
+    for (int d = kRankLanes / 2; d > 0; d >>= 1) before += __shfl_xor(before, d);
     if (lane == 0 && mine < size) {
         keys[base + before] = key;
         places[base + before] = base + mine;
     }
 }
 
-__global__ __launch_bounds__(256) void merge_kernel(const int32_t* keys, const uint32_t* places, uint32_t n,
-                                                    int32_t* sorted, uint32_t* sorted_places)
+__global__ __launch_bounds__(256) void merge_kernel(const uint32_t* keys, const uint32_t* places, uint32_t n,
+                                                    uint32_t* sorted, uint32_t* sorted_places, uint8_t* marks)
 {
     // 16 lanes a token, each searching every 16th chunk
     const uint32_t at = blockIdx.x * 16 + threadIdx.x / 16;
@@ -115,14 +128,14 @@ __global__ __launch_bounds__(256) void merge_kernel(const int32_t* keys, const u
     const uint32_t own = at / kChunk;
     uint32_t before = 0;
     if (at < n) {
-        const int32_t key = keys[at];
+        const uint32_t key = keys[at];
         for (uint32_t c = lane; c * kChunk < n; c += 16) {
             if (c == own) continue;
             uint32_t lo = c * kChunk, hi = n - lo < kChunk ? n : lo + kChunk;
             const uint32_t start = lo;
             while (lo < hi) {
                 const uint32_t mid = (lo + hi) / 2;
-                const int32_t k = keys[mid];
+                const uint32_t k = keys[mid];
                 if (k < key || (k == key && c < own)) lo = mid + 1;
                 else hi = mid;
             }
@@ -133,33 +146,25 @@ __global__ __launch_bounds__(256) void merge_kernel(const int32_t* keys, const u
     for (int d = 8; d > 0; d >>= 1) before += __shfl_xor(before, d);
     if (at < n && lane == 0) {
         const uint32_t to = at % kChunk + before;
-        sorted[to] = keys[at];
+        const uint32_t key = keys[at];
+        sorted[to] = key;
         sorted_places[to] = places[at];
+        if (marks && key != kNone) marks[key] = 1;
     }
 }
 
 // ---------------------------------------------------------------------------
 // sums over runs of equal tokens
 // ---------------------------------------------------------------------------
-constexpr int kBlock = 16;                // sorted positions walked by one wave
-
-template <typename T>
-__global__ __launch_bounds__(256) void clear_kernel(T* weight, uint64_t rows, uint32_t hidden, uint64_t stride,
-                                                    uint32_t units)
-{
-    constexpr int E = Elem<T>::kCount;
-    const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
-    const uint64_t row = unit / units;
-    if (row >= rows) return;
-    const uint32_t first = static_cast<uint32_t>(unit % units) * (kLookup * kWave) + threadIdx.x % kWave;
-    const float zero[E] = {};
-#pragma unroll
-    for (int k = 0; k < kLookup; ++k)
-        if ((first + k * kWave) * E < hidden) store_vec<T, E>(weight + row * stride, first + k * kWave, hidden, zero);
-}
+// A wave sums kBlock positions, all of whose rows it loads before it stores the
+// first sum: a later load would wait for the stores before it too.  Alone, 8192
+// tokens 4096 wide take 39 us in blocks of 8, 59 us in blocks of 32 by four trips.
+constexpr int kBlock = 8;
+constexpr int kJoinWaves = 4;             // that share the blocks of a long run
+constexpr int kFlight = 4;                // partials in flight in each
 
 template <typename O, int E>
-__device__ __forceinline__ void write_row(O* weight, int32_t key, uint64_t stride, uint32_t vec, uint32_t hidden,
+__device__ __forceinline__ void write_row(O* weight, uint32_t key, uint64_t stride, uint32_t vec, uint32_t hidden,
                                           float scale, bool accumulate, const float (&sum)[E])
 {
     O* row = weight + static_cast<uint64_t>(key) * stride;
@@ -172,74 +177,145 @@ __device__ __forceinline__ void write_row(O* weight, int32_t key, uint64_t strid
     store_vec<O, E>(row, vec, hidden, x);
 }
 
+struct SumArgs {
+    const uint32_t* keys;
+    const uint32_t* places;
+    const void* grad;
+    void* weight;
+    float* partial;
+    const uint8_t* marks;           // of the tokens that occur
+    uint64_t grad_stride, weight_stride, vocab;
+    uint32_t n, hidden, slices, groups;
+    float scale;
+    int accumulate;
+};
+
+// Zeros in a row whose token does not occur, a wave each.  They are not read here
+// again, and nontemporal stores leave the caches to the sums: 241 -> 235 us for
+// 8192 tokens of 128256 x 4096, 47 -> 41 us for 4095 of 50257 x 768 in fp32.
+template <typename O> __device__ void clear_row(const SumArgs& a, uint64_t row)
+{
+    constexpr uint32_t E = Elem<O>::kCount;
+    if (row >= a.vocab || a.marks[row]) return;
+    O* to = static_cast<O*>(a.weight) + row * a.weight_stride;
+    for (uint32_t vec = threadIdx.x % kWave; vec * E < a.hidden; vec += kWave) {
+        if (vec * E + E <= a.hidden) {
+            __builtin_nontemporal_store(u32x4_t{0, 0, 0, 0}, reinterpret_cast<u32x4_any*>(to + vec * E));
+        } else {
+            const float zero[E] = {};
+            store_vec<O, E>(to, vec, a.hidden, zero);
+        }
+    }
+}
+
 // partial[2 * block]: the sum of the run that came in from the block before;
 // partial[2 * block + 1]: that of the run that starts here and goes on.
-template <typename T, typename O>
-__global__ __launch_bounds__(256) void run_sums_kernel(const int32_t* keys, const uint32_t* places, uint32_t n,
-                                                       const T* grad, uint64_t grad_stride, uint32_t hidden,
-                                                       O* weight, uint64_t weight_stride, float scale, int accumulate,
-                                                       float* partial, uint32_t slices)
+// The workgroups after the first `groups` clear the rows of tokens that do not occur:
+// the sums wait for scattered rows, and the zeros keep memory busy meanwhile.
+template <typename T, typename O> __global__ __launch_bounds__(256, 8) void run_sums_kernel(SumArgs a)
 {
+    if (blockIdx.x >= a.groups) {
+        clear_row<O>(a, __builtin_amdgcn_readfirstlane((blockIdx.x - a.groups) * 4 + threadIdx.x / kWave));
+        return;
+    }
+    const uint32_t* keys = a.keys;
+    const uint32_t* places = a.places;
+    const T* grad = static_cast<const T*>(a.grad);
+    O* weight = static_cast<O*>(a.weight);
+    float* partial = a.partial;
+    const uint32_t n = a.n, hidden = a.hidden, slices = a.slices;
     constexpr int E = Elem<T>::kCount;
-    const uint32_t unit = blockIdx.x * 4 + threadIdx.x / kWave;
+    const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / kWave);
     const uint32_t block = unit / slices;
     const uint32_t vec = unit % slices * kWave + threadIdx.x % kWave;
     const uint32_t first = block * kBlock;
     if (first >= n || vec * E >= hidden) return;
-    const uint32_t last = n - first < kBlock ? n : first + kBlock;
-    int32_t key = keys[first];
+    uint32_t key = keys[first];
+    if (key == kNone) return;                                       // nothing but tokens that are left out
     bool came_in = first > 0 && keys[first - 1] == key;
+    uint32_t next[kBlock];
+    u32x4_t x[kBlock];                                              // as loaded: half the registers
     float sum[E] = {};
-    for (uint32_t at = first; at < last && key != kNone; ++at) {
-        float x[E];
-        load_vec<T>(grad + static_cast<uint64_t>(places[at]) * grad_stride, vec, hidden, x);
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] += x[e];
-        const int32_t next = at + 1 < n ? keys[at + 1] : kNone;
-        if (next == key && at + 1 < last) continue;
-        if (next == key || came_in)
+    for (uint32_t k = 0; k < kBlock; ++k) {
+        const uint32_t at = first + k;
+        next[k] = at + 1 < n ? keys[at + 1] : kNone;
+        const uint64_t place = at < n ? places[at] : places[first];  // beyond the end: any row, not added
+        x[k] = load_raw<T>(grad + place * a.grad_stride, vec, hidden);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kBlock; ++k) {
+        if (key == kNone) break;
+        float row[E];
+        Elem<T>::unpack(x[k], row);
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e] += row[e];
+        if (next[k] == key && k + 1 < kBlock) continue;
+        if (next[k] == key || came_in)
             store_vec<float, E>(partial + (2ull * block + (came_in ? 0 : 1)) * hidden, vec, hidden, sum);
         else
-            write_row<O, E>(weight, key, weight_stride, vec, hidden, scale, accumulate, sum);
-        key = next;
+            write_row<O, E>(weight, key, a.weight_stride, vec, hidden, a.scale, a.accumulate, sum);
+        key = next[k];
         came_in = false;
 #pragma unroll
         for (int e = 0; e < E; ++e) sum[e] = 0.0f;
     }
 }
 
-template <typename T, typename O>
-__global__ __launch_bounds__(256) void join_runs_kernel(const int32_t* keys, uint32_t n, uint32_t hidden, O* weight,
-                                                        uint64_t weight_stride, float scale, int accumulate,
-                                                        const float* partial, uint32_t slices)
+// A workgroup joins the run that starts in block `unit / slices` and goes on.  Its
+// waves take turns of kFlight partials and their sums are added in order.
+template <typename T, typename O> __global__ __launch_bounds__(256) void join_runs_kernel(SumArgs a)
 {
     constexpr int E = Elem<T>::kCount;
-    const uint32_t unit = blockIdx.x * 4 + threadIdx.x / kWave;
-    uint32_t block = unit / slices;
-    const uint32_t vec = unit % slices * kWave + threadIdx.x % kWave;
-    uint32_t end = (block + 1) * kBlock;                            // the position after this block
-    if (end >= n || vec * E >= hidden) return;
-    const int32_t key = keys[end - 1];
+    __shared__ float lds[kJoinWaves - 1][E][kWave];
+    const uint32_t* keys = a.keys;
+    const uint32_t n = a.n, hidden = a.hidden;
+    const uint32_t block = blockIdx.x / a.slices, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const uint32_t vec = blockIdx.x % a.slices * kWave + lane;
+    const uint32_t end = (block + 1) * kBlock;                      // the position after this block
+    if (end >= n) return;
+    const uint32_t key = keys[end - 1];
     if (key == kNone || keys[end] != key) return;                   // nothing goes on
-    if (block > 0 && keys[block * kBlock] == key && keys[block * kBlock - 1] == key) return;   // it started earlier
-    float sum[E], x[E];
+    if (block > 0 && keys[end - kBlock] == key && keys[end - kBlock - 1] == key) return;   // it started earlier
+    const auto load = [&](uint64_t which, float(&x)[E]) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const uint32_t at = vec * E + e;
-        sum[e] = at < hidden ? partial[(2ull * block + 1) * hidden + at] : 0.0f;
-    }
-    do {
-        ++block;
+        for (int e = 0; e < E; e += 4) {
+            float part[4];
+            load_vec<float>(a.partial + which * hidden, (vec * E + e) / 4, hidden, part);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint32_t at = vec * E + e;
-            x[e] = at < hidden ? partial[2ull * block * hidden + at] : 0.0f;
+            for (int k = 0; k < 4; ++k) x[e + k] = part[k];
         }
+    };
+    float sum[E] = {};
+    if (wave == 0) load(2ull * block + 1, sum);
+    // the blocks that begin with the same token, found 64 at a time
+    for (uint32_t from = block + 1;; from += kWave) {
+        const uint64_t start = static_cast<uint64_t>(from + lane) * kBlock;
+        const uint64_t same = __ballot(start < n && keys[start < n ? start : 0] == key);
+        const uint32_t count = same == ~0ull ? kWave : __builtin_ctzll(~same);
+        for (uint32_t k = wave * kFlight; k < count; k += kJoinWaves * kFlight) {
+            float x[kFlight][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] += x[e];
-        end += kBlock;
-    } while (end < n && keys[end - 1] == key && keys[end] == key);
-    write_row<O, E>(weight, key, weight_stride, vec, hidden, scale, accumulate, sum);
+            for (uint32_t f = 0; f < kFlight; ++f)
+                if (k + f < count) load(2ull * (from + k + f), x[f]);
+#pragma unroll
+            for (uint32_t f = 0; f < kFlight; ++f)
+                if (k + f < count)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) sum[e] += x[f][e];
+        }
+        if (count < kWave) break;
+    }
+    if (wave > 0)
+#pragma unroll
+        for (int e = 0; e < E; ++e) lds[wave - 1][e][lane] = sum[e];
+    __syncthreads();
+    if (wave > 0 || vec * E >= hidden) return;
+#pragma unroll
+    for (int w = 0; w < kJoinWaves - 1; ++w)
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e] += lds[w][e][lane];
+    write_row<O, E>(static_cast<O*>(a.weight), key, a.weight_stride, vec, hidden, a.scale, a.accumulate, sum);
 }
 
 // ---------------------------------------------------------------------------
@@ -251,11 +327,21 @@ constexpr uint64_t kMaxGrid = (1ull << 24) - 1;   // a launch has under 2^32 thr
 
 uint64_t pad(uint64_t bytes) { return ceil_div(bytes, 256) * 256; }
 
-// keys and places of the sorted chunks, of the sorted whole, then the partials
-uint64_t grad_workspace(uint64_t n, uint64_t hidden)
-{
-    return 4 * pad(4 * n) + pad(ceil_div(n, kBlock) * 2 * hidden * 4);
-}
+// Keys and places of the sorted chunks, of the sorted whole, the marks, then the partials.
+struct Workspace {
+    uint64_t keys, places, sorted, sorted_places, marks, partial, size;
+
+    Workspace(uint64_t n, uint64_t vocab, uint64_t hidden)
+    {
+        keys = 0;
+        places = keys + pad(4 * n);
+        sorted = places + pad(4 * n);
+        sorted_places = sorted + pad(4 * n);
+        marks = sorted_places + pad(4 * n);
+        partial = marks + pad(vocab);
+        size = partial + pad(ceil_div(n, kBlock) * 2 * hidden * 4);
+    }
+};
 
 template <typename T>
 int lookup(int token_dtype, const void* tokens, uint64_t n, const void* weight, uint64_t vocab, uint64_t hidden,
@@ -290,51 +376,51 @@ struct GradCall {
     hipStream_t st;
 };
 
-template <typename T, typename O> int sum_runs(const GradCall& c, const int32_t* keys, const uint32_t* places)
+template <typename I> int sort(const GradCall& c, const Workspace& w)
 {
-    float* partial = reinterpret_cast<float*>(c.workspace + 4 * pad(4ull * c.n));
-    const uint32_t slices = ceil_div(c.hidden, kWave * Elem<T>::kCount);
-    const uint64_t blocks = ceil_div(c.n, kBlock);
-    const uint64_t grid = ceil_div(blocks * slices, 4);
-    if (grid > kMaxGrid) return LA_EINVAL;
-    int rc = launch(run_sums_kernel<T, O>, dim3(grid), dim3(256), c.st, keys, places, c.n,
-                    static_cast<const T*>(c.grad), c.grad_stride, c.hidden, static_cast<O*>(c.weight), c.weight_stride,
-                    c.scale, c.accumulate, partial, slices);
-    if (rc != LA_OK || blocks == 1) return rc;
-    return launch(join_runs_kernel<T, O>, dim3(grid), dim3(256), c.st, keys, c.n, c.hidden, static_cast<O*>(c.weight),
-                  c.weight_stride, c.scale, c.accumulate, partial, slices);
+    uint32_t* keys = reinterpret_cast<uint32_t*>(c.workspace + w.keys);
+    uint32_t* places = reinterpret_cast<uint32_t*>(c.workspace + w.places);
+    uint8_t* marks = c.accumulate ? nullptr : reinterpret_cast<uint8_t*>(c.workspace + w.marks);
+    const uint64_t groups = ceil_div(c.n, kChunk) * kRankGroups;
+    const uint64_t clear = marks ? ceil_div(c.vocab, 256 * 16) : 0;
+    if (groups + clear == 0) return LA_OK;
+    int rc = launch(rank_kernel<I>, dim3(groups + clear), dim3(256), c.st, static_cast<const I*>(c.tokens), c.n,
+                    c.vocab, c.padding, keys, places, groups, reinterpret_cast<uint4*>(marks));
+    if (rc != LA_OK || c.n == 0) return rc;
+    return launch(merge_kernel, dim3(ceil_div(c.n, 16)), dim3(256), c.st, keys, places, c.n,
+                  reinterpret_cast<uint32_t*>(c.workspace + w.sorted),
+                  reinterpret_cast<uint32_t*>(c.workspace + w.sorted_places), marks);
 }
 
 template <typename T, typename O> int grad(const GradCall& c)
 {
-    if (!c.accumulate) {
-        const uint64_t units = ceil_div(c.hidden, kLookup * kWave * Elem<O>::kCount);
-        const uint64_t grid = ceil_div(c.vocab * units, 4);
-        if (grid > kMaxGrid) return LA_EINVAL;
-        const int rc = launch(clear_kernel<O>, dim3(grid), dim3(256), c.st, static_cast<O*>(c.weight), c.vocab,
-                              c.hidden, c.weight_stride, units);
-        if (rc != LA_OK) return rc;
-    }
-    if (c.n == 0) return LA_OK;
-    int32_t* keys = reinterpret_cast<int32_t*>(c.workspace);
-    uint32_t* places = reinterpret_cast<uint32_t*>(c.workspace + pad(4ull * c.n));
-    const uint32_t chunks = ceil_div(c.n, kChunk);
-    const dim3 rank_grid(chunks * (kChunk / kRankTokens));
-    int rc = c.token_dtype == LA_I32
-                 ? launch(rank_kernel<int32_t>, rank_grid, dim3(256), c.st, static_cast<const int32_t*>(c.tokens), c.n,
-                          c.vocab, c.padding, keys, places)
-                 : launch(rank_kernel<int64_t>, rank_grid, dim3(256), c.st, static_cast<const int64_t*>(c.tokens), c.n,
-                          c.vocab, c.padding, keys, places);
+    const Workspace w(c.n, c.vocab, c.hidden);
+    SumArgs a{};
+    a.keys = reinterpret_cast<const uint32_t*>(c.workspace + w.sorted);
+    a.places = reinterpret_cast<const uint32_t*>(c.workspace + w.sorted_places);
+    a.grad = c.grad;
+    a.weight = c.weight;
+    a.partial = reinterpret_cast<float*>(c.workspace + w.partial);
+    a.marks = reinterpret_cast<const uint8_t*>(c.workspace + w.marks);
+    a.grad_stride = c.grad_stride;
+    a.weight_stride = c.weight_stride;
+    a.vocab = c.vocab;
+    a.n = c.n;
+    a.hidden = c.hidden;
+    a.slices = ceil_div(c.hidden, kWave * Elem<T>::kCount);
+    a.scale = c.scale;
+    a.accumulate = c.accumulate;
+    const uint64_t blocks = ceil_div(c.n, kBlock);
+    const uint64_t groups = ceil_div(blocks * a.slices, 4);
+    const uint64_t clear = c.accumulate ? 0 : ceil_div(c.vocab, 4);
+    a.groups = groups;
+    if (blocks * a.slices > kMaxGrid || groups + clear > kMaxGrid) return LA_EINVAL;
+    if (groups + clear == 0) return LA_OK;
+    int rc = c.token_dtype == LA_I32 ? sort<int32_t>(c, w) : sort<int64_t>(c, w);
     if (rc != LA_OK) return rc;
-    if (chunks > 1) {
-        int32_t* sorted = reinterpret_cast<int32_t*>(c.workspace + 2 * pad(4ull * c.n));
-        uint32_t* sorted_places = reinterpret_cast<uint32_t*>(c.workspace + 3 * pad(4ull * c.n));
-        rc = launch(merge_kernel, dim3(ceil_div(c.n, 16)), dim3(256), c.st, keys, places, c.n, sorted, sorted_places);
-        if (rc != LA_OK) return rc;
-        keys = sorted;
-        places = sorted_places;
-    }
-    return sum_runs<T, O>(c, keys, places);
+    rc = launch(run_sums_kernel<T, O>, dim3(groups + clear), dim3(256), c.st, a);
+    if (rc != LA_OK || blocks <= 1) return rc;
+    return launch(join_runs_kernel<T, O>, dim3(blocks * a.slices), dim3(256), c.st, a);
 }
 
 bool token_types(int dtype) { return dtype == LA_I32 || dtype == LA_I64; }
@@ -367,9 +453,10 @@ int la_embedding(int token_dtype, const void* tokens, uint64_t n, int dtype, con
     return lookup<_Float16>(token_dtype, tokens, n, weight, vocab, hidden, weight_stride, scale, out, out_stride, st);
 }
 
-uint64_t la_embedding_grad_workspace(uint64_t n, uint64_t hidden)
+uint64_t la_embedding_grad_workspace(uint64_t n, uint64_t vocab, uint64_t hidden)
 {
-    return n > kMaxTokens || hidden > kMaxHidden ? 0 : grad_workspace(n, hidden);
+    const bool fits = n <= kMaxTokens && hidden <= kMaxHidden && vocab <= static_cast<uint64_t>(INT32_MAX);
+    return fits ? Workspace(n, vocab, hidden).size : 0;
 }
 
 int la_embedding_grad(int token_dtype, const void* tokens, uint64_t n, int g_dtype, const void* grad_out,
@@ -384,11 +471,11 @@ int la_embedding_grad(int token_dtype, const void* tokens, uint64_t n, int g_dty
     int rc = check_matrix(grad_weight, out_dtype, hidden, weight_stride);
     if (rc == LA_OK && n > 0) rc = check_matrix(tokens, token_dtype, 1, 1);
     if (rc == LA_OK && n > 0) rc = check_matrix(grad_out, g_dtype, hidden, grad_stride);
-    if (rc == LA_OK && n > 0) rc = check_workspace(workspace, workspace_bytes, grad_workspace(n, hidden), 16);
+    if (rc == LA_OK) rc = check_workspace(workspace, workspace_bytes, Workspace(n, vocab, hidden).size, 16);
     if (rc != LA_OK) return rc;
     if (!la_ptr::device_accessible(grad_weight) ||
-        (n > 0 && (!la_ptr::device_accessible(tokens) || !la_ptr::device_accessible(grad_out) ||
-                   !la_ptr::device_accessible(workspace))))
+        !la_ptr::device_accessible(workspace) ||
+        (n > 0 && (!la_ptr::device_accessible(tokens) || !la_ptr::device_accessible(grad_out))))
         return LA_EFAULT;
     const GradCall c{token_dtype, tokens, static_cast<uint32_t>(n), grad_out, grad_stride, grad_weight, vocab,
                      static_cast<uint32_t>(hidden), weight_stride, scale, padding_idx, accumulate != 0,

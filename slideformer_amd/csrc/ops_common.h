@@ -100,6 +100,18 @@ __device__ __forceinline__ void load_vec(const T* row, uint32_t vec, uint32_t hi
     }
 }
 
+// The same as it lies in memory.
+template <typename T> __device__ __forceinline__ u32x4_t load_raw(const T* row, uint32_t vec, uint32_t hidden)
+{
+    constexpr uint32_t E = Elem<T>::kCount;
+    const uint32_t at = vec * E;
+    if (at + E <= hidden) return *reinterpret_cast<const u32x4_any*>(row + at);
+    T x[E];
+#pragma unroll
+    for (uint32_t i = 0; i < E; ++i) x[i] = at + i < hidden ? row[at + i] : Elem<T>::from_f32(0.0f);
+    return __builtin_bit_cast(u32x4_t, x);
+}
+
 template <typename T, int E>
 __device__ __forceinline__ void store_vec(T* row, uint32_t vec, uint32_t hidden, const float (&x)[E])
 {

@@ -69,7 +69,7 @@ def test_embedding_refusals():
     assert f(I64, HP, 4, F32, HP, 4, 8, 8, 1.0, HP, 8, None) == _lib.LA_EFAULT          # host memory
     assert f(I64, None, 0, F32, None, 4, 8, 8, 1.0, None, 8, None) == _lib.LA_OK        # nothing to do
     g = L.la_embedding_grad
-    need = L.la_embedding_grad_workspace(4, 8)
+    need = L.la_embedding_grad_workspace(4, 4, 8)
     assert need > 0
     assert g(I64, HP, 4, F32, HP, 8, BF16, HP, 4, 8, 8, 1.0, -1, 0, HP, need, None) == _lib.LA_EDTYPE
     assert g(I64, HP, 4, F32, HP, 8, F32, HP, 4, 8, 8, 1.0, -1, 0, HP, need - 1, None) == _lib.LA_EINVAL
