@@ -6,6 +6,7 @@ if it is missing, ``load()`` raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
@@ -15,6 +16,9 @@ from . import _lib
 
 # where slideformer_amd/build.py writes the library
 LIB_PATH = os.path.join(os.path.dirname(_lib.LIB_PATH), "libslideformer_amd_ops.so")
+
+# where it writes the native host module
+CALLS_PATH = os.path.join(os.path.dirname(LIB_PATH), "_ops_calls.so")
 
 # LA_OPS_ABI_VERSION of include/model_ops.h that these bindings declare
 ABI_VERSION = 1
@@ -76,7 +80,7 @@ def _declare(L):
     L.la_ops_abi_version.restype = i
     L.la_embedding.argtypes = [i, P, u64, i, P, u64, u64, u64, f, P, u64, P]
     L.la_embedding.restype = i
-    L.la_embedding_grad_workspace.argtypes = [u64, u64]
+    L.la_embedding_grad_workspace.argtypes = [u64, u64, u64]
     L.la_embedding_grad_workspace.restype = u64
     L.la_embedding_grad.argtypes = [i, P, u64, i, P, u64, i, P, u64, u64, u64, f, i64, i, P, u64, P]
     L.la_embedding_grad.restype = i
@@ -111,3 +115,26 @@ def load():
                                   f"{ABI_VERSION}; rebuild it with `python -m slideformer_amd.build`")
             _loaded = _declare(raw)
         return _loaded
+
+
+_calls = None
+
+
+def calls():
+    """The native host module (csrc/ops_calls.cpp), bound once to the loaded
+    library.  Raises ImportError if it has not been built."""
+    global _calls
+    if _calls is None:
+        L = load()
+        with _lock:
+            if _calls is None:
+                if not os.path.exists(CALLS_PATH):
+                    raise ImportError(f"{CALLS_PATH} not found; build it with `python -m slideformer_amd.build`")
+                spec = importlib.util.spec_from_file_location("_ops_calls", CALLS_PATH)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                module.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+                    L.la_embedding, L.la_embedding_grad_workspace, L.la_embedding_grad, L.la_rms_norm,
+                    L.la_rms_norm_grad_workspace, L.la_rms_norm_grad)))
+                _calls = module
+    return _calls

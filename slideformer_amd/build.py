@@ -128,8 +128,13 @@ HOST_CALLS_SRC = os.path.join(CSRC, "host_calls.cpp")
 HOST_CALLS = os.path.join(LIB_DIR, "_host_calls.so")
 
 
-def build_host_calls(verbose: bool = False) -> str:
-    """Compile csrc/host_calls.cpp with g++ against torch's and Python's headers."""
+# The same for the smallest calls of the model operators.
+OPS_CALLS_SRC = os.path.join(CSRC, "ops_calls.cpp")
+OPS_CALLS = os.path.join(LIB_DIR, "_ops_calls.so")
+
+
+def build_host_calls(verbose: bool = False, source: str = HOST_CALLS_SRC, out: str = HOST_CALLS) -> str:
+    """Compile one of these modules with g++ against torch's and Python's headers."""
     import sysconfig
 
     import torch
@@ -143,25 +148,26 @@ def build_host_calls(verbose: bool = False) -> str:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-isystem", os.path.join(root, "include"),
            "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
-           "-isystem", sysconfig.get_paths()["include"], HOST_CALLS_SRC,
+           "-isystem", sysconfig.get_paths()["include"], source,
            "-L", os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
-           f"-Wl,-rpath,{os.path.join(root, 'lib')}", "-o", HOST_CALLS + ".tmp"]
+           f"-Wl,-rpath,{os.path.join(root, 'lib')}", "-o", out + ".tmp"]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError(f"g++ failed with code {res.returncode}")
-    os.replace(HOST_CALLS + ".tmp", HOST_CALLS)
-    return HOST_CALLS
+    os.replace(out + ".tmp", out)
+    return out
 
 
 def build_all(verbose: bool = False) -> list:
-    """The product libraries, the native host module, the small-grid test build, the stream probes and the C test
+    """The product libraries, the native host modules, the small-grid test build, the stream probes and the C test
     driver."""
     return [build_library(verbose=verbose),
             build_library(out=OPS_LIB, sources=OPS_SOURCES, verbose=verbose),
             build_host_calls(verbose=verbose),
+            build_host_calls(verbose=verbose, source=OPS_CALLS_SRC, out=OPS_CALLS),
             build_library(out=SMALL_GRID_LIB, defines=SMALL_GRID_DEFINES, verbose=verbose),
             build_library(out=PROBE_LIB, sources=PROBE_SOURCES, verbose=verbose),
             build_c_driver(verbose=verbose)]

@@ -28,7 +28,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib, _ops_lib
-from .layer_adam import _on_device, _stream_handle, _torch_stream
+from .layer_adam import _on_device, _raw_current_stream, _stream_handle, _torch_stream
 
 __all__ = ["embedding", "embedding_grad", "rms_norm", "rms_norm_8bit", "rms_norm_grad", "linear_cross_entropy",
            "linear_cross_entropy_grad", "PIECE_BYTES"]
@@ -80,6 +80,20 @@ def _vector(t: torch.Tensor, name: str, device, size: int, dtypes) -> None:
         raise RuntimeError(f"unsupported dtype of {name}: {t.dtype}")
 
 
+def _here():
+    """(current device, its current stream's handle), what the native host module takes."""
+    device = torch.cuda.current_device()
+    return device, _stream_handle(None, torch.device("cuda", device)) if _raw_current_stream is None \
+        else _raw_current_stream(device)
+
+
+def _got(result, what: str):
+    """What the native host module returned: outputs, or a code of the library's."""
+    if type(result) is int:
+        _check(result, what)
+    return result
+
+
 class _Scratch:
     """Allocations of one call, made on its stream so that the caching allocator
     orders their reuse after it."""
@@ -117,6 +131,10 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
 
     tokens: int32 or int64; one outside [0, vocab) gives a row of NaN.  ``out``: a
     matrix [tokens.numel(), hidden] to write instead of a new tensor."""
+    if out is None and stream is None and tokens.is_cuda:
+        done = _ops_lib.calls().embedding(tokens, weight, scale, *_here())
+        if done is not None:
+            return _got(done, "la_embedding")
     stride = _matrix(weight, "weight", weight.device)
     vocab, hidden = weight.shape
     _vector(tokens, "tokens", weight.device, tokens.numel(), _TOKEN)
@@ -143,6 +161,11 @@ def embedding_grad(tokens: torch.Tensor, grad_out: torch.Tensor, grad_weight: to
     are added to what is there and other rows stay untouched.  ``padding_idx`` and
     out-of-range tokens contribute nothing.  Sums are fp32 in a fixed order: equal
     calls give equal bits."""
+    if stream is None and tokens.is_cuda:
+        done = _ops_lib.calls().embedding_grad(tokens, grad_out, grad_weight, scale,
+                                               -1 if padding_idx is None else padding_idx, accumulate, *_here())
+        if done is not None:
+            return _got(done, "la_embedding_grad")
     device = grad_weight.device
     stride = _matrix(grad_weight, "grad_weight", device)
     vocab, hidden = grad_weight.shape
@@ -158,7 +181,7 @@ def embedding_grad(tokens: torch.Tensor, grad_out: torch.Tensor, grad_weight: to
         raise RuntimeError(f"grad_weight is {grad_weight.dtype}, expected {grad_out.dtype} or torch.float32")
     lib = _ops_lib.load()
     with _on_device(device), _Scratch(device, stream) as s:
-        size = lib.la_embedding_grad_workspace(n, hidden)
+        size = lib.la_embedding_grad_workspace(n, vocab, hidden)
         work = s.workspace(size)
         _check(lib.la_embedding_grad(_TOKEN[tokens.dtype], tokens.data_ptr(), n, _FLOAT[grad_out.dtype],
                                      grad_out.data_ptr(), grad_stride, _FLOAT[grad_weight.dtype],
@@ -188,6 +211,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
     ``(out, z, rstd)``: z (x itself without a residual) is what the next residual
     takes, and it and the fp32 ``rstd`` [n] are what ``rms_norm_grad`` takes.  The norm
     is that of the unrounded sum."""
+    if stream is None and x.is_cuda:
+        done = _ops_lib.calls().rms_norm(x, weight, eps, residual, *_here())
+        if done is not None:
+            return _got(done, "la_rms_norm")
     device, n, hidden, x_stride, r_stride = _norm_inputs(x, weight, residual)
     with _on_device(device), _Scratch(device, stream) as s:
         out = s.empty((n, hidden), x.dtype)
@@ -211,6 +238,10 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6,
     of zeros has scale 0; one that holds an infinity or NaN has scale NaN."""
     if dtype not in _EIGHT:
         raise RuntimeError(f"unsupported 8-bit dtype: {dtype}")
+    if stream is None and x.is_cuda:
+        done = _ops_lib.calls().rms_norm_8bit(x, weight, eps, residual, dtype is not torch.int8, *_here())
+        if done is not None:
+            return _got(done, "la_rms_norm")
     device, n, hidden, x_stride, r_stride = _norm_inputs(x, weight, residual)
     with _on_device(device), _Scratch(device, stream) as s:
         out = s.empty((n, hidden), dtype)
@@ -232,6 +263,11 @@ def rms_norm_grad(grad_out: torch.Tensor, summed: torch.Tensor, rstd: torch.Tens
     residual; it is added.  ``grad_weight``: the tensor [hidden] to write (weight's type
     or float32; new by default), added to with ``accumulate``.  Returns
     ``(grad_x, grad_weight)``.  Sums are fp32 in a fixed order."""
+    if stream is None and grad_out.is_cuda:
+        done = _ops_lib.calls().rms_norm_grad(grad_out, summed, rstd, weight, grad_summed, grad_weight, accumulate,
+                                              *_here())
+        if done is not None:
+            return _got(done, "la_rms_norm_grad")
     device = grad_out.device
     go_stride = _matrix(grad_out, "grad_out", device)
     n, hidden = grad_out.shape
