@@ -29,9 +29,9 @@
 namespace {
 
 using tile::f32x4;
-using tile::kTile;
 
 constexpr int kWave = 64;
+constexpr int kTile = 256;          // rows and columns are padded to: whole tiles of either side
 
 // What the device finds out: trained rows, and the factor of every gradient.
 struct Plan {
@@ -56,14 +56,44 @@ __device__ __forceinline__ uint32_t piece_rows(const Plan* plan, uint32_t first,
 __device__ __forceinline__ uint32_t round_up(uint32_t x, uint32_t to) { return (x + to - 1) / to * to; }
 
 // ---------------------------------------------------------------------------
+// which tiles, how many runs of k
+// ---------------------------------------------------------------------------
+// About how long a product of `tiles` tiles over `steps` steps of k takes in `splits`
+// runs of k, in us.  The chip holds 256 tiles of 256 x 256 at a time, or 512 of
+// 128 x 128, so they run in rounds; those of the larger ones end together.  A round
+// costs its steps and a start and an end; the partial sums of a split product are
+// written and read once more.  The constants are from products of 1000 to 3072
+// rows, 20000 to 128256 columns and 768 to 4096 k: of 256, 0.86 us a step and 12 us
+// a round; of 128, 0.53 to 0.78 us (two on a compute unit) and 5.5 us.
+__host__ __device__ __forceinline__ float product_us(int side, uint32_t tiles, uint32_t steps, uint32_t splits,
+                                                     float partial_bytes)
+{
+    const float k = static_cast<float>(steps) / static_cast<float>(splits);
+    const float all = static_cast<float>(tiles) * static_cast<float>(splits);
+    const float join = static_cast<float>(splits) * partial_bytes * (2.0f / 4.0e6f);
+    if (side == 256) return ceilf(all / 256.0f) * (0.86f * k + 12.0f) + join;
+    return fmaxf(1.0f, all / 512.0f) * (0.65f * k + 5.5f) + join;
+}
+
+constexpr uint32_t kMostSplits = 64;
+
+// ---------------------------------------------------------------------------
 // the trained rows
 // ---------------------------------------------------------------------------
+// What the states' gradient needs decided once the rows are known: in how many runs
+// of k each piece is taken.
+struct SplitArgs {
+    uint32_t* splits;               // [pieces], null without gradients
+    uint32_t pieces, most, hidden, steps, side, max_splits;
+};
+
 // One workgroup lists the rows whose target is not `ignore`, in order.
 constexpr uint32_t kListed = 8;                                  // targets per thread and trip
 
 __global__ __launch_bounds__(1024) void list_rows_kernel(const int64_t* targets, uint32_t n, int64_t ignore,
                                                          uint64_t vocab, int mean, const float* grad_scale, float held,
-                                                         uint32_t* rows, int32_t* row_targets, Plan* plan)
+                                                         uint32_t* rows, int32_t* row_targets, Plan* plan,
+                                                         SplitArgs split)
 {
     __shared__ uint32_t counts[16];
     uint32_t done = 0;
@@ -101,6 +131,27 @@ __global__ __launch_bounds__(1024) void list_rows_kernel(const int64_t* targets,
     if (threadIdx.x == 0) {
         plan->rows = done;
         plan->factor = (grad_scale ? *grad_scale : 1.0f) / (mean && done > 0 ? static_cast<float>(done) : 1.0f) / held;
+    }
+    if (!split.splits) return;
+    const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    for (uint32_t p = wave; p < split.pieces; p += 16) {
+        const uint32_t first = p * split.most;
+        const uint32_t piece = done <= first ? 0 : done - first < split.most ? done - first : split.most;
+        const uint32_t tiles = ceil_div(piece, split.side) * ceil_div(split.hidden, split.side);
+        float least = lane < split.max_splits
+                          ? product_us(split.side, tiles, split.steps, lane + 1, 4.0f * piece * split.hidden)
+                          : 3.0e38f;
+        uint32_t best = lane + 1;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            const float other = __shfl_xor(least, d);
+            const uint32_t its = __shfl_xor(best, d);
+            if (other < least || (other == least && its < best)) {
+                least = other;
+                best = its;
+            }
+        }
+        if (lane == 0) split.splits[p] = best;
     }
 }
 
@@ -154,65 +205,67 @@ struct ScoreArgs {
     const int32_t* row_targets;
     Part* parts;                    // [rows of the piece][tiles of the vocabulary]
     float* target_scores;           // [rows of the piece]
-    void* held;                     // [rows of the piece][tiles * 256], or null
-    uint32_t first, most, vocab, tiles, steps;
+    void* held;                     // [rows of the piece][columns], or null
+    uint32_t first, most, vocab, columns, tiles, steps;
 };
 
-template <typename T> __global__ __launch_bounds__(tile::kThreads, 1) void scores_kernel(ScoreArgs a)
-{
-    __shared__ __attribute__((aligned(1024))) char lds[tile::kLdsBytes];
-    const uint32_t rows = piece_rows(a.plan, a.first, a.most);
-    const tile::Place at = tile::place(blockIdx.x, ceil_div(rows, kTile), a.tiles);
-    if (!at.valid) return;
-    tile::Sums sums;
-    tile::product<T, true, true>(a.weight, at.inner * kTile, a.x, a.first + at.outer * kTile, 0, a.steps,
-                                 lds, sums);
+// What the waves that share a tile's rows tell each other: [largest, sum][wave][row of the tile].
+template <int WAVES, int ROWS> struct Exchange {
+    float at[2][WAVES][ROWS];
+};
 
-    // [largest, sum][inner half][row of the tile], after what the tile is handed out through
-    float(*exchange)[2][kTile] = reinterpret_cast<float(*)[2][kTile]>(lds + tile::kHandOutBytes);
-    const uint32_t lane = threadIdx.x % kWave, half = threadIdx.x / kWave % 2;
-    const uint32_t column = at.inner * kTile + tile::wave_inner() + lane / 16 * 4;
-    if (at.inner * kTile + kTile > a.vocab)                      // columns past the vocabulary take no part
+// Reduces a wave's INNER x OUTER fragments of scores (inner the vocabulary, from
+// `inner_at` of vocabulary tile `inner`; outer rows, from `outer_at` of the tile that
+// starts at row `first` of the piece): target scores and the tile's part of each row
+// are written, and the sums become exp(s - m).  `part` of WAVES shares the rows.
+template <int SIDE, int INNER, int OUTER, int WAVES, int ROWS>
+__device__ __forceinline__ void reduce_scores(const ScoreArgs& a, uint32_t inner, uint32_t first, uint32_t rows,
+                                              uint32_t part, uint32_t inner_at, uint32_t outer_at,
+                                              f32x4 (&sums)[INNER][OUTER], Exchange<WAVES, ROWS>& exchange)
+{
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint32_t column = inner * SIDE + inner_at + lane / 16 * 4;
+    if (inner * SIDE + SIDE > a.vocab)                           // columns past the vocabulary take no part
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
+        for (int s = 0; s < INNER; ++s)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 if (column + s * 16 + r >= a.vocab)
 #pragma unroll
-                    for (int t = 0; t < 8; ++t) sums[s][t][r] = -INFINITY;
-    float top[8];
+                    for (int t = 0; t < OUTER; ++t) sums[s][t][r] = -INFINITY;
+    float top[OUTER];
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-        const uint32_t row = tile::wave_outer() + t * 16 + lane % 16;
-        const uint32_t in_piece = at.outer * kTile + row;
+    for (int t = 0; t < OUTER; ++t) {
+        const uint32_t row = outer_at + t * 16 + lane % 16;
         // the target's score, in the one lane that holds it
-        const uint32_t target = (in_piece < rows ? a.row_targets[a.first + in_piece] : -1) - column;
-        if (target < 128 && target % 16 < 4)
+        const uint32_t target = (first + row < rows ? a.row_targets[a.first + first + row] : -1) - column;
+        if (target < INNER * 16 && target % 16 < 4)
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
+            for (int s = 0; s < INNER; ++s)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (target == s * 16u + r) a.target_scores[in_piece] = sums[s][t][r];
+                    if (target == s * 16u + r) a.target_scores[first + row] = sums[s][t][r];
         top[t] = -INFINITY;
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
+        for (int s = 0; s < INNER; ++s)
 #pragma unroll
             for (int r = 0; r < 4; ++r) top[t] = fmaxf(top[t], sums[s][t][r]);
         top[t] = fmaxf(top[t], __shfl_xor(top[t], 16));
         top[t] = fmaxf(top[t], __shfl_xor(top[t], 32));
-        if (lane < 16) exchange[0][half][row] = top[t];
+        if (lane < 16) exchange.at[0][part][row] = top[t];
     }
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-        const uint32_t row = tile::wave_outer() + t * 16 + lane % 16;
-        top[t] = fmaxf(exchange[0][0][row], exchange[0][1][row]);
+    for (int t = 0; t < OUTER; ++t) {
+        const uint32_t row = outer_at + t * 16 + lane % 16;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) top[t] = fmaxf(top[t], exchange.at[0][w][row]);
         // exp(s - m) as a power of 2, one multiply-add before it; a row of -inf gives zeros
         constexpr float kLog2e = 1.44269504088896340736f;
         const float base = top[t] == -INFINITY ? 0.0f : top[t] * -kLog2e;
         float sum = 0.0f;
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
+        for (int s = 0; s < INNER; ++s)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sums[s][t][r], kLog2e, base));
@@ -221,25 +274,112 @@ template <typename T> __global__ __launch_bounds__(tile::kThreads, 1) void score
             }
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
-        if (lane < 16) exchange[1][half][row] = sum;
+        if (lane < 16) exchange.at[1][part][row] = sum;
     }
     __syncthreads();
-    if (half == 0 && lane < 16)
+    if (part == 0 && lane < 16)
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            const uint32_t row = tile::wave_outer() + t * 16 + lane;
-            a.parts[static_cast<uint64_t>(at.outer * kTile + row) * a.tiles + at.inner] =
-                Part{top[t], exchange[1][0][row] + exchange[1][1][row]};
+        for (int t = 0; t < OUTER; ++t) {
+            const uint32_t row = outer_at + t * 16 + lane;
+            float sum = exchange.at[1][0][row];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) sum += exchange.at[1][w][row];
+            a.parts[static_cast<uint64_t>(first + row) * a.tiles + inner] = Part{top[t], sum};
         }
+}
+
+template <typename T, int SIDE>
+__global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void scores_kernel(ScoreArgs a)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[tile::Sizes<SIDE>::kLdsBytes];
+    const uint32_t rows = piece_rows(a.plan, a.first, a.most);
+    const tile::Place at = tile::place(blockIdx.x, ceil_div(rows, SIDE), a.tiles);
+    if (!at.valid) return;
+    tile::Sums<SIDE> sums;
+    tile::product<T, SIDE, true, true>(a.weight, at.inner * SIDE, a.x, a.first + at.outer * SIDE, 0, a.steps, lds, sums);
+
+    // after what the tile is handed out through
+    auto* exchange = reinterpret_cast<Exchange<2, SIDE>*>(lds + tile::Sizes<SIDE>::kHandOutBytes);
+    reduce_scores<SIDE>(a, at.inner, at.outer * SIDE, rows, threadIdx.x / kWave % 2, tile::wave_inner<SIDE>(),
+                        tile::wave_outer<SIDE>(), sums, *exchange);
     if (!a.held) return;
-    T* held = static_cast<T*>(a.held) + static_cast<uint64_t>(at.outer) * kTile * a.tiles * kTile + at.inner * kTile;
-    tile::by_rows(sums, lds, [&](uint32_t outer, uint32_t inner, const float(&v)[8]) {
+    T* held = static_cast<T*>(a.held) + static_cast<uint64_t>(at.outer) * SIDE * a.columns + at.inner * SIDE;
+    tile::by_rows<SIDE>(sums, lds, [&](uint32_t outer, uint32_t inner, const float(&v)[8]) {
         float e[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) e[k] = v[k] * kHeld<T>;
-        *reinterpret_cast<u32x4_t*>(held + static_cast<uint64_t>(outer) * a.tiles * kTile + inner) =
-            Elem<T>::pack(e);
+        *reinterpret_cast<u32x4_t*>(held + static_cast<uint64_t>(outer) * a.columns + inner) = Elem<T>::pack(e);
     });
+}
+
+// The same for at most 16 * OUTER rows: the time is that of reading the vocabulary
+// matrix, which goes from memory to registers in the order that the matrix
+// instructions take it, 64 of its rows a wave; the states come from the caches.
+// Rows of any alignment and width are read where they lie.  13 rows of
+// 128256 x 4096: tiles of 256 rows XX us, this YY us.
+template <typename T, int OUTER> __global__ __launch_bounds__(256) void few_scores_kernel(ScoreArgs a)
+{
+    __shared__ Exchange<4, 16 * OUTER> exchange;
+    const uint32_t rows = piece_rows(a.plan, a.first, a.most);
+    if (rows == 0) return;
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const uint32_t width = a.weight.width, steps = a.steps;
+    const T* weight[4];
+    const T* x[OUTER];
+#pragma unroll
+    for (uint32_t s = 0; s < 4; ++s) {
+        const uint32_t row = blockIdx.x * kTile + wave * 64 + s * 16 + lane % 16;
+        weight[s] = reinterpret_cast<const T*>(static_cast<const char*>(a.weight.data) +
+                                               (row < a.vocab ? row : a.vocab - 1) * a.weight.stride);
+    }
+#pragma unroll
+    for (uint32_t t = 0; t < OUTER; ++t)
+        x[t] = static_cast<const T*>(a.x.data) + (a.first + t * 16 + lane % 16) * (a.x.stride / 2);
+    f32x4 sums[4][OUTER] = {};
+    u32x4_t w[2][2][4], v[2][2][OUTER];                              // [buffer][step of the pair]
+    const auto load = [&](int b, uint32_t step) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t vec = (step + h) * 4 + lane / 16;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) w[b][h][s] = load_raw<T>(weight[s], vec, width);
+#pragma unroll
+            for (int t = 0; t < OUTER; ++t) v[b][h][t] = *reinterpret_cast<const u32x4_t*>(x[t] + vec * 8);
+        }
+    };
+    const auto multiply = [&](int b) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int t = 0; t < OUTER; ++t)
+                    sums[s][t] = tile::product_of<T>(__builtin_bit_cast(tile::s16x8, w[b][h][s]),
+                                                     __builtin_bit_cast(tile::s16x8, v[b][h][t]), sums[s][t]);
+    };
+    load(0, 0);
+    for (uint32_t step = 0; step < steps; step += 4) {              // steps come in pairs
+        if (step + 2 < steps) load(1, step + 2);
+        multiply(0);
+        if (step + 4 < steps) load(0, step + 4);
+        if (step + 2 < steps) multiply(1);
+    }
+    reduce_scores<kTile>(a, blockIdx.x, 0, rows, wave, wave * 64, 0, sums, exchange);
+    if (!a.held) return;
+    // the rows after these, up to a whole tile, are written as zeros with D
+#pragma unroll
+    for (int t = 0; t < OUTER; ++t) {
+        T* held = static_cast<T*>(a.held) + static_cast<uint64_t>(t * 16 + lane % 16) * a.columns +
+                  blockIdx.x * kTile + wave * 64 + lane / 16 * 4;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            typedef T v4 __attribute__((ext_vector_type(4)));
+            v4 e;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) e[r] = static_cast<T>(sums[s][t][r] * kHeld<T>);
+            *reinterpret_cast<v4*>(held + s * 16) = e;
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -290,11 +430,12 @@ constexpr uint32_t kPerGroup = 4;                                // 16-byte vect
 template <typename T>
 __global__ __launch_bounds__(256) void softmax_grad_kernel(T* held, const Part* parts, const float* lse,
                                                            const int32_t* row_targets, const Plan* plan,
-                                                           uint32_t first, uint32_t most, uint32_t tiles)
+                                                           uint32_t first, uint32_t most, uint32_t width,
+                                                           uint32_t tiles)
 {
     const uint32_t row = blockIdx.y, rows = piece_rows(plan, first, most);
     if (row >= round_up(rows, kTile)) return;
-    const uint32_t width = tiles * kTile;
+    const uint32_t side = width / tiles;
     T* mine = held + static_cast<uint64_t>(row) * width;
     const int32_t target = row < rows ? row_targets[first + row] : -1;
     const float total = row < rows ? lse[row] : 0.0f;
@@ -305,7 +446,7 @@ __global__ __launch_bounds__(256) void softmax_grad_kernel(T* held, const Part* 
         float d[8] = {};
         if (row < rows) {
             load_vec<T>(mine, vec, width, d);
-            const float top = parts[static_cast<uint64_t>(row) * tiles + vec / (kTile / 8)].top;
+            const float top = parts[static_cast<uint64_t>(row) * tiles + vec * 8 / side].top;
             const float f = expf(top - total);
 #pragma unroll
             for (uint32_t e = 0; e < 8; ++e)
@@ -323,47 +464,30 @@ struct GradXArgs {
     const Plan* plan;
     const uint32_t* rows;
     float* partial;                 // [splits][rows of the piece][hidden]
-    uint32_t first, most, hidden, inners, pairs, max_splits;   // pairs of steps
+    const uint32_t* splits;         // runs of k of this piece
+    uint32_t first, most, hidden, inners, pairs;               // pairs of steps
 };
 
-// Into how many runs of k a product of `tiles` tiles is split.  A compute unit
-// holds one workgroup, so the tiles run in rounds of 256 and the last round may be
-// nearly empty; with more, shorter runs it is fuller.  Each run costs a pass over
-// its partial sums, counted here as a fiftieth of a round.
-__device__ __forceinline__ uint32_t splits_of(uint32_t tiles, uint32_t max_splits)
+template <typename T, int SIDE>
+__global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void grad_x_kernel(GradXArgs a)
 {
-    uint32_t best = 1;
-    float least = 3.0e38f;
-    for (uint32_t s = 1; s <= max_splits; ++s) {
-        const float cost = static_cast<float>((tiles * s + 255) / 256) / static_cast<float>(s) +
-                           0.02f * static_cast<float>(s);
-        if (cost < least) {
-            least = cost;
-            best = s;
-        }
-    }
-    return best;
-}
-
-template <typename T> __global__ __launch_bounds__(tile::kThreads, 1) void grad_x_kernel(GradXArgs a)
-{
-    __shared__ __attribute__((aligned(1024))) char lds[tile::kLdsBytes];
+    __shared__ __attribute__((aligned(1024))) char lds[tile::Sizes<SIDE>::kLdsBytes];
     const uint32_t rows = piece_rows(a.plan, a.first, a.most);
-    const uint32_t outers = ceil_div(rows, kTile);
+    const uint32_t outers = ceil_div(rows, SIDE);
     if (outers == 0) return;
-    const uint32_t splits = splits_of(outers * a.inners, a.max_splits);
+    const uint32_t splits = *a.splits;
     const tile::Place at = tile::place(blockIdx.x, outers * splits, a.inners);
     if (!at.valid) return;
     const uint32_t split = at.outer / outers, outer = at.outer % outers;
     const uint32_t from = static_cast<uint64_t>(a.pairs) * split / splits * 2;
     const uint32_t to = static_cast<uint64_t>(a.pairs) * (split + 1) / splits * 2;
-    tile::Sums sums;
-    tile::product<T, false, true>(a.weight, at.inner * kTile, a.held, outer * kTile,
-                                  static_cast<uint64_t>(from) * tile::kDepth, to - from, lds, sums);
-    float* partial = a.partial + (static_cast<uint64_t>(split) * a.most + outer * kTile) * a.hidden;
-    tile::by_rows(sums, lds, [&](uint32_t row, uint32_t inner, const float(&v)[8]) {
-        if (outer * kTile + row < rows)
-            store_vec<float, 8>(partial + static_cast<uint64_t>(row) * a.hidden, (at.inner * kTile + inner) / 8,
+    tile::Sums<SIDE> sums;
+    tile::product<T, SIDE, false, true>(a.weight, at.inner * SIDE, a.held, outer * SIDE,
+                                        static_cast<uint64_t>(from) * tile::kDepth, to - from, lds, sums);
+    float* partial = a.partial + (static_cast<uint64_t>(split) * a.most + outer * SIDE) * a.hidden;
+    tile::by_rows<SIDE>(sums, lds, [&](uint32_t row, uint32_t inner, const float(&v)[8]) {
+        if (outer * SIDE + row < rows)
+            store_vec<float, 8>(partial + static_cast<uint64_t>(row) * a.hidden, (at.inner * SIDE + inner) / 8,
                                 a.hidden, v);
     });
 }
@@ -373,7 +497,7 @@ __global__ __launch_bounds__(256) void join_grad_x_kernel(GradXArgs a, T* grad_x
 {
     const uint32_t row = blockIdx.x, rows = piece_rows(a.plan, a.first, a.most);
     if (row >= rows) return;
-    const uint32_t splits = splits_of(ceil_div(rows, kTile) * a.inners, a.max_splits);
+    const uint32_t splits = *a.splits;
     const float factor = a.plan->factor;
     T* out = grad_x + a.rows[a.first + row] * grad_x_stride;
     for (uint32_t vec = threadIdx.x; vec * 4 < a.hidden; vec += 256) {
@@ -400,21 +524,21 @@ struct GradWeightArgs {
     int accumulate;
 };
 
-template <typename T, typename W>
-__global__ __launch_bounds__(tile::kThreads, 1) void grad_weight_kernel(GradWeightArgs a)
+template <typename T, typename W, int SIDE>
+__global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void grad_weight_kernel(GradWeightArgs a)
 {
-    __shared__ __attribute__((aligned(1024))) char lds[tile::kLdsBytes];
+    __shared__ __attribute__((aligned(1024))) char lds[tile::Sizes<SIDE>::kLdsBytes];
     const uint32_t rows = piece_rows(a.plan, a.first, a.most);
     if (rows == 0 && a.first > 0) return;
     const tile::Place at = tile::place(blockIdx.x, a.outers, a.inners);
     if (!at.valid) return;
-    tile::Sums sums;
-    tile::product<T, false, false>(a.x, at.inner * kTile, a.held, at.outer * kTile, 0, ceil_div(rows, 2 * tile::kDepth) * 2,
-                                   lds, sums);
+    tile::Sums<SIDE> sums;
+    tile::product<T, SIDE, false, false>(a.x, at.inner * SIDE, a.held, at.outer * SIDE, 0,
+                                         ceil_div(rows, 2 * tile::kDepth) * 2, lds, sums);
     const bool last = a.first + rows >= a.plan->rows;
     const float factor = a.plan->factor;
-    tile::by_rows(sums, lds, [&](uint32_t outer, uint32_t inner, const float(&sum)[8]) {
-        const uint32_t row = at.outer * kTile + outer, vec = (at.inner * kTile + inner) / 8;
+    tile::by_rows<SIDE>(sums, lds, [&](uint32_t outer, uint32_t inner, const float(&sum)[8]) {
+        const uint32_t row = at.outer * SIDE + outer, vec = (at.inner * SIDE + inner) / 8;
         if (row >= a.vocab) return;
         float v[8];
 #pragma unroll
@@ -462,26 +586,53 @@ bool reads_in_place(const la_linear_loss_t& c)
     return c.hidden % kPair == 0 && c.weight_stride % 8 == 0 && reinterpret_cast<uintptr_t>(c.weight) % 16 == 0;
 }
 
+// Up to so many rows the scores are bound by reading the matrix.
+constexpr uint64_t kFewRows = 64;
+
+bool copies_weight(const la_linear_loss_t& c) { return !reads_in_place(c) && (c.grads || c.n > kFewRows); }
+
+// The least time of a product of rows x columns in tiles of this side, over the ways to split it.
+float least_us(int side, uint64_t rows, uint64_t columns, uint64_t k, uint64_t max_splits)
+{
+    const uint64_t tiles = ceil_div(rows, side) * ceil_div(columns, side), steps = ceil_div(k, kPair) * 2;
+    float least = product_us(side, tiles, steps, 1, max_splits > 1 ? 4.0f * rows * columns : 0.0f);
+    for (uint32_t s = 2; s <= max_splits; ++s) {
+        const float us = product_us(side, tiles, steps, s, 4.0f * rows * columns);
+        if (us < least) least = us;
+    }
+    return least;
+}
+
+int side_of(uint64_t rows, uint64_t columns, uint64_t k, uint64_t max_splits)
+{
+    return least_us(128, rows, columns, k, max_splits) < least_us(256, rows, columns, k, max_splits) ? 128 : 256;
+}
+
 // Sizes and the workspace's parts (offsets in bytes).
 struct Layout {
-    uint64_t padded, tiles, inners, all, piece, pieces, max_splits;
-    uint64_t plan, rows, row_targets, gathered, weight, parts, target_scores, lse, row_loss, held, partial, total, size;
+    int score_side, grad_x_side, grad_w_side;
+    uint64_t padded, columns, all, piece, pieces, max_splits;
+    uint64_t plan, splits, rows, row_targets, gathered, weight, parts, target_scores, lse, row_loss, held, partial, total, size;
 
     explicit Layout(const la_linear_loss_t& c)
     {
         padded = ceil_div(c.hidden, kPair) * kPair;
-        tiles = ceil_div(c.vocab, kTile);
-        inners = ceil_div(c.hidden, kTile);
+        columns = ceil_div(c.vocab, kTile) * kTile;
         all = c.n > 0 ? ceil_div(c.n, kTile) * kTile : kTile;     // no rows: one empty piece, which clears grad_weight
         piece = ceil_div(c.grads ? c.piece_rows : kForwardRows, kTile) * kTile;
         if (piece > kMostRows) piece = kMostRows;
         if (piece == 0 || piece > all) piece = all;
         pieces = ceil_div(all, piece);
-        // enough runs of k for four rounds of workgroups
-        const uint64_t grad_x_tiles = piece / kTile * inners;
-        max_splits = ceil_div(1024, grad_x_tiles);
-        if (max_splits > 64) max_splits = 64;
-        if (max_splits > tiles) max_splits = tiles;
+        // partial sums of the states' gradient take at most the memory of a piece's D, or 64 MiB
+        const uint64_t partials = piece * columns * 2 > (64u << 20) ? piece * columns * 2 : 64u << 20;
+        max_splits = partials / (piece * c.hidden * 4);
+        if (max_splits > columns / kTile) max_splits = columns / kTile;
+        if (max_splits > kMostSplits) max_splits = kMostSplits;
+        if (max_splits == 0) max_splits = 1;
+        const uint64_t rows_of_piece = c.n < piece ? c.n : piece;
+        score_side = c.n <= kFewRows ? kTile : side_of(rows_of_piece, c.vocab, c.hidden, 1);
+        grad_x_side = side_of(rows_of_piece, c.hidden, c.vocab, max_splits);
+        grad_w_side = side_of(c.vocab, c.hidden, rows_of_piece, 1);
         uint64_t at = 0;
         const auto take = [&](uint64_t bytes) {
             const uint64_t here = at;
@@ -489,25 +640,53 @@ struct Layout {
             return here;
         };
         plan = take(sizeof(Plan));
+        splits = take(pieces * 4);
         rows = take(c.n * 4);
         row_targets = take(c.n * 4);
         gathered = take(all * padded * 2);
-        weight = reads_in_place(c) ? 0 : take(c.vocab * padded * 2);
-        parts = take(piece * tiles * sizeof(Part));
+        weight = !copies_weight(c) ? 0 : take(c.vocab * padded * 2);
+        parts = take(piece * (columns / score_side) * sizeof(Part));
         target_scores = take(piece * 4);
         lse = take(piece * 4);
         row_loss = c.row_loss ? 0 : take(c.n * 4);
-        held = c.grads ? take(piece * tiles * kTile * 2) : 0;
+        held = c.grads ? take(piece * columns * 2) : 0;
         partial = c.grads ? take(max_splits * piece * c.hidden * 4) : 0;
         total = c.grads && pieces > 1 ? take(c.vocab * c.hidden * 4) : 0;
         size = at;
     }
 };
 
+template <typename T> int run_scores(const la_linear_loss_t& c, const Layout& l, const ScoreArgs& a, hipStream_t st)
+{
+    if (c.n <= 16) return launch(few_scores_kernel<T, 1>, dim3(a.tiles), dim3(256), st, a);
+    if (c.n <= kFewRows) return launch(few_scores_kernel<T, 4>, dim3(a.tiles), dim3(256), st, a);
+    const dim3 grid(tile::places(l.piece / l.score_side, a.tiles)), block(tile::kThreads);
+    return l.score_side == 128 ? launch(scores_kernel<T, 128>, grid, block, st, a)
+                               : launch(scores_kernel<T, 256>, grid, block, st, a);
+}
+
+template <typename T, int SIDE>
+int run_grad_x(const Layout& l, GradXArgs a, T* grad_x, uint64_t grad_x_stride, hipStream_t st)
+{
+    a.inners = ceil_div(a.hidden, SIDE);
+    const int rc = launch(grad_x_kernel<T, SIDE>, dim3(tile::places(l.piece / SIDE * l.max_splits, a.inners)),
+                          dim3(tile::kThreads), st, a);
+    if (rc != LA_OK) return rc;
+    return launch(join_grad_x_kernel<T>, dim3(l.piece), dim3(256), st, a, grad_x, grad_x_stride);
+}
+
+template <typename T, typename W, int SIDE> int run_grad_weight(GradWeightArgs a, hipStream_t st)
+{
+    a.inners = ceil_div(a.hidden, SIDE);
+    a.outers = ceil_div(a.vocab, SIDE);
+    return launch(grad_weight_kernel<T, W, SIDE>, dim3(tile::places(a.outers, a.inners)), dim3(tile::kThreads), st, a);
+}
+
 template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, hipStream_t st)
 {
     const Layout l(c);
     Plan* plan = reinterpret_cast<Plan*>(ws + l.plan);
+    uint32_t* splits = reinterpret_cast<uint32_t*>(ws + l.splits);
     uint32_t* rows = reinterpret_cast<uint32_t*>(ws + l.rows);
     int32_t* row_targets = reinterpret_cast<int32_t*>(ws + l.row_targets);
     T* gathered = reinterpret_cast<T*>(ws + l.gathered);
@@ -519,13 +698,17 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
     T* grad_x = c.grads ? static_cast<T*>(c.grad_x) : nullptr;
 
     int rc = launch(list_rows_kernel, dim3(1), dim3(1024), st, c.targets, c.n, c.ignore_index, c.vocab, c.mean,
-                    c.grad_scale, kHeld<T>, rows, row_targets, plan);
+                    c.grad_scale, kHeld<T>, rows, row_targets, plan,
+                    SplitArgs{c.grads ? splits : nullptr, static_cast<uint32_t>(l.pieces),
+                              static_cast<uint32_t>(l.piece), static_cast<uint32_t>(c.hidden),
+                              static_cast<uint32_t>(l.columns / tile::kDepth), static_cast<uint32_t>(l.grad_x_side),
+                              static_cast<uint32_t>(l.max_splits)});
     if (rc != LA_OK) return rc;
     rc = launch(gather_kernel<T>, dim3(l.all + c.n), dim3(256), st, static_cast<const T*>(c.x), c.x_stride, c.hidden,
                 l.padded, rows, plan, gathered, l.all, c.targets, c.ignore_index, row_loss, grad_x, c.grad_x_stride);
     if (rc != LA_OK) return rc;
     tile::Matrix weight{c.weight, c.vocab, c.hidden, c.weight_stride * 2};
-    if (!reads_in_place(c)) {
+    if (copies_weight(c)) {
         T* copy = reinterpret_cast<T*>(ws + l.weight);
         rc = launch(pad_kernel<T>, dim3(c.vocab), dim3(256), st, static_cast<const T*>(c.weight), c.weight_stride,
                     c.hidden, l.padded, copy);
@@ -533,40 +716,32 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
         weight = tile::Matrix{copy, c.vocab, l.padded, l.padded * 2};
     }
     const tile::Matrix x{gathered, l.all, l.padded, l.padded * 2};
-    const tile::Matrix d{held, l.piece, l.tiles * kTile, l.tiles * kTile * 2};
+    const tile::Matrix d{held, l.piece, l.columns, l.columns * 2};
+    const uint32_t vocab = c.vocab, hidden = c.hidden, columns = l.columns, tiles = l.columns / l.score_side;
 
     for (uint64_t p = 0; p < l.pieces; ++p) {
         const uint32_t first = p * l.piece, most = l.piece;
-        const ScoreArgs scores{weight, x, plan, row_targets, parts, target_scores, held, first, most,
-                               static_cast<uint32_t>(c.vocab), static_cast<uint32_t>(l.tiles),
-                               static_cast<uint32_t>(l.padded / tile::kDepth)};
-        rc = launch(scores_kernel<T>, dim3(tile::places(most / kTile, l.tiles)), dim3(tile::kThreads), st, scores);
+        rc = run_scores<T>(c, l, ScoreArgs{weight, x, plan, row_targets, parts, target_scores, held, first, most, vocab,
+                                           columns, tiles, static_cast<uint32_t>(l.padded / tile::kDepth)}, st);
         if (rc != LA_OK) return rc;
-        rc = launch(row_loss_kernel, dim3(most / 4), dim3(256), st, parts, l.tiles, plan, first, most, rows,
-                    row_targets, target_scores, lse, row_loss);
-        if (rc != LA_OK || !c.grads) {
-            if (rc != LA_OK) return rc;
-            continue;
-        }
-        rc = launch(softmax_grad_kernel<T>, dim3(ceil_div(l.tiles * kTile, 8 * 256 * kPerGroup), most), dim3(256), st,
-                    held, parts, lse, row_targets, plan, first, most, l.tiles);
+        rc = launch(row_loss_kernel, dim3(most / 4), dim3(256), st, parts, tiles, plan, first, most, rows, row_targets,
+                    target_scores, lse, row_loss);
         if (rc != LA_OK) return rc;
-        const GradXArgs gx{weight, d, plan, rows, reinterpret_cast<float*>(ws + l.partial), first, most,
-                           static_cast<uint32_t>(c.hidden), static_cast<uint32_t>(l.inners),
-                           static_cast<uint32_t>(l.tiles * (kTile / kPair)),
-                           static_cast<uint32_t>(l.max_splits)};
-        rc = launch(grad_x_kernel<T>, dim3(tile::places(most / kTile * l.max_splits, l.inners)), dim3(tile::kThreads),
-                    st, gx);
+        if (!c.grads) continue;
+        rc = launch(softmax_grad_kernel<T>, dim3(ceil_div(columns, 8 * 256 * kPerGroup), most), dim3(256), st, held,
+                    parts, lse, row_targets, plan, first, most, columns, tiles);
         if (rc != LA_OK) return rc;
-        rc = launch(join_grad_x_kernel<T>, dim3(most), dim3(256), st, gx, grad_x, c.grad_x_stride);
+        const GradXArgs gx{weight, d, plan, rows, reinterpret_cast<float*>(ws + l.partial), splits + p, first, most,
+                           hidden, 0, static_cast<uint32_t>(columns / kPair)};
+        rc = l.grad_x_side == 128 ? run_grad_x<T, 128>(l, gx, grad_x, c.grad_x_stride, st)
+                                  : run_grad_x<T, 256>(l, gx, grad_x, c.grad_x_stride, st);
         if (rc != LA_OK) return rc;
         const tile::Matrix piece_x{gathered + first * l.padded, l.piece < l.all - first ? l.piece : l.all - first,
                                    l.padded, l.padded * 2};
         const GradWeightArgs gw{piece_x, d, plan, c.grad_weight,
                                 l.pieces > 1 ? reinterpret_cast<float*>(ws + l.total) : nullptr, c.grad_weight_stride,
-                                first, most, static_cast<uint32_t>(c.vocab), static_cast<uint32_t>(c.hidden),
-                                static_cast<uint32_t>(l.inners), static_cast<uint32_t>(l.tiles), c.accumulate};
-        rc = launch(grad_weight_kernel<T, W>, dim3(tile::places(l.tiles, l.inners)), dim3(tile::kThreads), st, gw);
+                                first, most, vocab, hidden, 0, 0, c.accumulate};
+        rc = l.grad_w_side == 128 ? run_grad_weight<T, W, 128>(gw, st) : run_grad_weight<T, W, 256>(gw, st);
         if (rc != LA_OK) return rc;
     }
     if (!c.loss) return LA_OK;
