@@ -161,6 +161,10 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs a)
     float square = 0.0f;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) load_sum<T>(a, row, k * THREADS + tid, z[k]);
+    u32x4_t weight[VPT];                                    // on its way while the row is summed
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
+        weight[k] = load_raw<T>(static_cast<const T*>(a.weight), k * THREADS + tid, a.hidden);
 #pragma unroll
     for (int k = 0; k < VPT; ++k)
 #pragma unroll
@@ -175,7 +179,7 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs a)
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         float w[E];
-        load_vec<T>(static_cast<const T*>(a.weight), k * THREADS + tid, a.hidden, w);
+        Elem<T>::unpack(weight[k], w);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             z[k][e] = z[k][e] * r * w[e];
@@ -294,42 +298,70 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_grad_kerne
 {
     constexpr int E = Elem<T>::kCount;
     constexpr int WORKERS = THREADS < 256 ? 256 / THREADS : 1;
+    constexpr bool kLean = THREADS == 1024;                 // 128 registers a thread: less is kept and fetched ahead
     __shared__ float lds[THREADS / kWave];
     const uint32_t worker = blockIdx.x * WORKERS + threadIdx.x / THREADS;
     if (worker >= a.workers) return;
     const uint32_t tid = threadIdx.x % THREADS;
-    float w[VPT][E], dw[VPT][E];
+    u32x4_t weight[VPT];                                    // kept as it lies in memory: half the registers
+    float dw[VPT][E];
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-        load_vec<T>(static_cast<const T*>(a.weight), k * THREADS + tid, a.hidden, w[k]);
+        if constexpr (!kLean)
+            weight[k] = load_raw<T>(static_cast<const T*>(a.weight), k * THREADS + tid, a.hidden);
 #pragma unroll
         for (int e = 0; e < E; ++e) dw[k][e] = 0.0f;
     }
+    // a row's three inputs as they lie in memory, loaded while the row before is computed
+    u32x4_t next[3][VPT];
+    const auto fetch = [&](uint64_t row) {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const uint32_t vec = k * THREADS + tid;
+            next[0][k] = load_raw<T>(static_cast<const T*>(a.grad_out) + row * a.grad_out_stride, vec, a.hidden);
+            next[1][k] = load_raw<T>(static_cast<const T*>(a.summed) + row * a.summed_stride, vec, a.hidden);
+            if constexpr (!kLean)
+                next[2][k] = a.grad_summed ? load_raw<T>(static_cast<const T*>(a.grad_summed) +
+                                                         row * a.grad_summed_stride, vec, a.hidden)
+                                       : u32x4_t{0, 0, 0, 0};
+        }
+    };
+    fetch(worker);
     for (uint64_t row = worker; row < a.n; row += a.workers) {
         float u[VPT][E], g[VPT][E];
+        u32x4_t through[VPT];
         const float r = a.rstd[row];
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            Elem<T>::unpack(next[0][k], g[k]);
+            Elem<T>::unpack(next[1][k], u[k]);
+            through[k] = next[2][k];
+            if constexpr (kLean) {
+                through[k] = a.grad_summed ? load_raw<T>(static_cast<const T*>(a.grad_summed) +
+                                                             row * a.grad_summed_stride, k * THREADS + tid, a.hidden)
+                                           : u32x4_t{0, 0, 0, 0};
+                weight[k] = load_raw<T>(static_cast<const T*>(a.weight), k * THREADS + tid, a.hidden);
+            }
+        }
+        if (row + a.workers < a.n) fetch(row + a.workers);
         float inner = 0.0f;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            load_vec<T>(static_cast<const T*>(a.grad_out) + row * a.grad_out_stride, k * THREADS + tid, a.hidden, g[k]);
-            load_vec<T>(static_cast<const T*>(a.summed) + row * a.summed_stride, k * THREADS + tid, a.hidden, u[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < VPT; ++k)
+            float w[E];
+            Elem<T>::unpack(weight[k], w);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 u[k][e] *= r;
                 dw[k][e] = __builtin_fmaf(g[k][e], u[k][e], dw[k][e]);
-                g[k][e] *= w[k][e];
+                g[k][e] *= w[e];
                 inner = __builtin_fmaf(g[k][e], u[k][e], inner);
             }
+        }
         inner = row_sum<THREADS>(inner, lds) / static_cast<float>(a.hidden);
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             float past[E] = {};
-            if (a.grad_summed)
-                load_vec<T>(static_cast<const T*>(a.grad_summed) + row * a.grad_summed_stride, k * THREADS + tid,
-                            a.hidden, past);
+            if (a.grad_summed) Elem<T>::unpack(through[k], past);
 #pragma unroll
             for (int e = 0; e < E; ++e) g[k][e] = __builtin_fmaf(g[k][e] - u[k][e] * inner, r, past[e]);
             store_vec<T, E>(static_cast<T*>(a.grad_x) + row * a.grad_x_stride, k * THREADS + tid, a.hidden, g[k]);
@@ -409,13 +441,21 @@ __global__ __launch_bounds__(1024) void join_weight_grad_kernel(const float* par
 }
 
 // Workers that share the rows out, and the weight gradient's partials.
-constexpr uint64_t kWorkers = 512;
+// A worker prefetches its next row, so few are enough to keep memory busy, and each
+// costs a row of partials.  8192 rows: of 4096 (a workgroup each) 512 workers 53 us,
+// 1024 62 us, without the prefetch 82 us; of 512 (a wave each) 1024 16 us, 512 20 us.
+constexpr uint64_t kWaveWorkers = 1024;
+constexpr uint64_t kGroupWorkers = 512;
 
-uint64_t workers_for(uint64_t n) { return n < kWorkers ? n : kWorkers; }
+uint64_t most_workers(uint64_t n) { return n < kWaveWorkers ? n : kWaveWorkers; }
 
-template <typename T> int norm_grad_rows(const NormGradArgs& a, hipStream_t st)
+template <typename T> int norm_grad_rows(NormGradArgs& a, hipStream_t st)
 {
     const uint32_t vecs = ceil_div(a.hidden, static_cast<uint32_t>(Elem<T>::kCount));
+    const uint64_t most = vecs <= 128 ? kWaveWorkers : kGroupWorkers;
+    a.workers = static_cast<uint32_t>(a.n < most ? a.n : most);
+    if (vecs <= 128 && vecs > 64)
+        return launch(norm_grad_kernel<T, 64, 2>, dim3(ceil_div(a.workers, 4)), dim3(256), st, a);
     if (vecs <= 64) return launch(norm_grad_kernel<T, 64, 1>, dim3(ceil_div(a.workers, 4)), dim3(256), st, a);
     if (vecs <= 256) return launch(norm_grad_kernel<T, 256, 1>, dim3(a.workers), dim3(256), st, a);
     if (vecs <= 512) return launch(norm_grad_kernel<T, 256, 2>, dim3(a.workers), dim3(256), st, a);
@@ -469,7 +509,7 @@ int la_rms_norm(int dtype, const void* x, uint64_t x_stride, const void* residua
 
 uint64_t la_rms_norm_grad_workspace(uint64_t n, uint64_t hidden)
 {
-    return n > kMaxRows || hidden > kMaxHidden ? 0 : workers_for(n) * hidden * sizeof(float);
+    return n > kMaxRows || hidden > kMaxHidden ? 0 : most_workers(n) * hidden * sizeof(float);
 }
 
 int la_rms_norm_grad(int dtype, const void* grad_out, uint64_t grad_out_stride, const void* summed,
@@ -490,7 +530,7 @@ int la_rms_norm_grad(int dtype, const void* grad_out, uint64_t grad_out_stride, 
         if (rc == LA_OK && grad_summed) rc = check_matrix(grad_summed, dtype, hidden, grad_summed_stride);
         if (rc == LA_OK) rc = check_matrix(grad_x, dtype, hidden, grad_x_stride);
         if (rc == LA_OK && grad_weight)
-            rc = check_workspace(workspace, workspace_bytes, workers_for(n) * hidden * sizeof(float), 16);
+            rc = check_workspace(workspace, workspace_bytes, most_workers(n) * hidden * sizeof(float), 16);
     }
     if (rc == LA_OK && grad_weight) rc = check_matrix(grad_weight, w_dtype, hidden, hidden);
     if (rc != LA_OK) return rc;
@@ -498,10 +538,10 @@ int la_rms_norm_grad(int dtype, const void* grad_out, uint64_t grad_out_stride, 
         (n > 0 && (!reachable(grad_out) || !reachable(summed) || !reachable(rstd) || !reachable(weight) ||
                    !reachable(grad_summed) || !reachable(grad_x) || (grad_weight && !reachable(workspace)))))
         return LA_EFAULT;
-    const NormGradArgs a{grad_out, summed, rstd, weight, grad_summed, grad_x,
+    NormGradArgs a{grad_out, summed, rstd, weight, grad_summed, grad_x,
                          grad_weight ? static_cast<float*>(workspace) : nullptr, n, grad_out_stride, summed_stride,
                          grad_summed_stride, grad_x_stride, static_cast<uint32_t>(hidden),
-                         static_cast<uint32_t>(workers_for(n))};
+                         0};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (n > 0) {
         rc = dtype == LA_F32    ? norm_grad_rows<float>(a, st)
