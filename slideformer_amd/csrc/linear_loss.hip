@@ -87,6 +87,8 @@ struct SplitArgs {
     uint32_t pieces, most, hidden, steps, side, max_splits;
 };
 
+constexpr uint32_t kFewRows = 64;                                // up to so many, a call is bound by the vocabulary matrix
+
 // One workgroup lists the rows whose target is not `ignore`, in order.
 constexpr uint32_t kListed = 8;                                  // targets per thread and trip
 
@@ -161,10 +163,16 @@ template <typename T>
 __global__ __launch_bounds__(256) void gather_kernel(const T* x, uint64_t x_stride, uint32_t hidden, uint32_t padded,
                                                      const uint32_t* rows, const Plan* plan, T* gathered,
                                                      uint32_t gathered_rows, const int64_t* targets, int64_t ignore,
-                                                     float* row_loss, T* grad_x, uint64_t grad_x_stride)
+                                                     float* row_loss, T* grad_x, uint64_t grad_x_stride,
+                                                     T* transposed)
 {
     if (blockIdx.x < gathered_rows) {
         const uint32_t row = blockIdx.x, count = plan->rows;
+        // few rows with gradients: X^T too, [padded][kFewRows]
+        if (transposed && row < kFewRows)
+            for (uint32_t h = threadIdx.x; h < padded; h += 256)
+                transposed[static_cast<uint64_t>(h) * kFewRows + row] =
+                    row < count && h < hidden ? x[rows[row] * x_stride + h] : Elem<T>::from_f32(0.0f);
         if (row >= round_up(count, kTile)) return;
         T* to = gathered + static_cast<uint64_t>(row) * padded;
         for (uint32_t vec = threadIdx.x; vec * 8 < padded; vec += 256) {
@@ -316,7 +324,7 @@ __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void 
 // matrix, which goes from memory to registers in the order that the matrix
 // instructions take it, 64 of its rows a wave; the states come from the caches.
 // Rows of any alignment and width are read where they lie.  13 rows of
-// 128256 x 4096: tiles of 256 rows XX us, this YY us.
+// 128256 x 4096: 232 us (4.5 TB/s), with tiles of 256 rows 300 us.
 template <typename T, int OUTER> __global__ __launch_bounds__(256) void few_scores_kernel(ScoreArgs a)
 {
     __shared__ Exchange<4, 16 * OUTER> exchange;
@@ -563,6 +571,84 @@ __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void 
     });
 }
 
+// The same for at most kFewRows rows, all of whose k fits two steps: the time is that
+// of writing the gradient.  A wave holds the D of 64 columns in registers, as the
+// matrix instructions take it, and goes along the hidden dimension with X^T out of
+// the caches.  Row m of a fragment of X^T is hidden element 16 (m / 4) + 4 s + m % 4,
+// s counting four fragments, so that a lane ends up with 16 neighbouring elements
+// of a row.  13 rows of 128256 x 4096: 260 us, with tiles of 128 354 us;
+// without the next chunk's loads before this one's stores 400 us.
+template <typename T, typename W>
+__global__ __launch_bounds__(256) void few_grad_weight_kernel(GradWeightArgs a, const T* transposed, uint32_t runs)
+{
+    using Z = tile::Sizes<kTile>;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * Z::kPanelBytes];
+    const uint32_t columns = blockIdx.x / runs * kTile, run = blockIdx.x % runs;
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const bool some = a.plan->rows > 0;
+    const float factor = a.plan->factor;
+    tile::Operand<kTile, false> load;
+    tile::Fragments<kTile, false> read;
+    load.init(a.held, columns, 0, some ? 2 : 0);
+    read.init(wave * 64);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        load.turn(half);
+        const uint32_t to = __builtin_amdgcn_readfirstlane(
+            static_cast<uint32_t>(reinterpret_cast<uintptr_t>((tile::lds_char*)lds)) + half * Z::kPanelBytes +
+            wave * 1024);
+#pragma unroll
+        for (int n = 0; n < Z::kLoads; ++n) load.load(to, n);
+    }
+    tile::arrive<0>();
+    tile::s16x8 d[2][4];
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) d[half][t] = read.read((tile::lds_char*)lds + half * Z::kPanelBytes, t);
+
+    const uint32_t chunks = ceil_div(a.hidden, 64u);
+    const T* x = transposed + (lane % 16 / 4 * 8 + lane % 4) * kFewRows + lane / 16 * 8;
+    const uint32_t end = chunks * (run + 1) / runs;
+    tile::s16x8 next[2][4];
+    const auto fetch = [&](uint32_t chunk) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                next[half][s] = *reinterpret_cast<const tile::s16x8*>(x + (chunk * 64 + s / 2 * 32 + s % 2 * 4) * kFewRows + half * 32);
+    };
+    fetch(chunks * run / runs);
+    for (uint32_t chunk = chunks * run / runs; chunk < end; ++chunk) {
+        f32x4 sums[4][4] = {};
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) sums[s][t] = tile::product_of<T>(next[half][s], d[half][t], sums[s][t]);
+        // before this chunk's stores: a load after them would wait for them
+        fetch(chunk + 1 < end ? chunk + 1 : chunk);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const uint32_t row = columns + wave * 64 + t * 16 + lane % 16;
+            if (row >= a.vocab) continue;
+            W* out = static_cast<W*>(a.grad_weight) + row * a.stride;
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                const uint32_t vec = chunk * 8 + part * 4 + lane / 16;
+                float v[8];
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) {
+                    v[k] = sums[part * 2 + k / 4][t][k % 4] * factor;
+                    if (a.accumulate && vec * 8 + k < a.hidden) v[k] += Elem<W>::to_f32(out[vec * 8 + k]);
+                }
+                store_vec<W, 8>(out, vec, a.hidden, v);
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -585,9 +671,6 @@ bool reads_in_place(const la_linear_loss_t& c)
 {
     return c.hidden % kPair == 0 && c.weight_stride % 8 == 0 && reinterpret_cast<uintptr_t>(c.weight) % 16 == 0;
 }
-
-// Up to so many rows the scores are bound by reading the matrix.
-constexpr uint64_t kFewRows = 64;
 
 bool copies_weight(const la_linear_loss_t& c) { return !reads_in_place(c) && (c.grads || c.n > kFewRows); }
 
@@ -612,7 +695,7 @@ int side_of(uint64_t rows, uint64_t columns, uint64_t k, uint64_t max_splits)
 struct Layout {
     int score_side, grad_x_side, grad_w_side;
     uint64_t padded, columns, all, piece, pieces, max_splits;
-    uint64_t plan, splits, rows, row_targets, gathered, weight, parts, target_scores, lse, row_loss, held, partial, total, size;
+    uint64_t plan, splits, rows, row_targets, gathered, weight, parts, target_scores, lse, row_loss, held, partial, transposed, total, size;
 
     explicit Layout(const la_linear_loss_t& c)
     {
@@ -651,6 +734,7 @@ struct Layout {
         row_loss = c.row_loss ? 0 : take(c.n * 4);
         held = c.grads ? take(piece * columns * 2) : 0;
         partial = c.grads ? take(max_splits * piece * c.hidden * 4) : 0;
+        transposed = c.grads && c.n <= kFewRows ? take(kFewRows * padded * 2) : 0;
         total = c.grads && pieces > 1 ? take(c.vocab * c.hidden * 4) : 0;
         size = at;
     }
@@ -696,6 +780,7 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
     float* row_loss = c.row_loss ? c.row_loss : reinterpret_cast<float*>(ws + l.row_loss);
     T* held = c.grads ? reinterpret_cast<T*>(ws + l.held) : nullptr;
     T* grad_x = c.grads ? static_cast<T*>(c.grad_x) : nullptr;
+    T* transposed = c.grads && c.n <= kFewRows ? reinterpret_cast<T*>(ws + l.transposed) : nullptr;
 
     int rc = launch(list_rows_kernel, dim3(1), dim3(1024), st, c.targets, c.n, c.ignore_index, c.vocab, c.mean,
                     c.grad_scale, kHeld<T>, rows, row_targets, plan,
@@ -705,7 +790,7 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
                               static_cast<uint32_t>(l.max_splits)});
     if (rc != LA_OK) return rc;
     rc = launch(gather_kernel<T>, dim3(l.all + c.n), dim3(256), st, static_cast<const T*>(c.x), c.x_stride, c.hidden,
-                l.padded, rows, plan, gathered, l.all, c.targets, c.ignore_index, row_loss, grad_x, c.grad_x_stride);
+                l.padded, rows, plan, gathered, l.all, c.targets, c.ignore_index, row_loss, grad_x, c.grad_x_stride, transposed);
     if (rc != LA_OK) return rc;
     tile::Matrix weight{c.weight, c.vocab, c.hidden, c.weight_stride * 2};
     if (copies_weight(c)) {
@@ -741,6 +826,14 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
         const GradWeightArgs gw{piece_x, d, plan, c.grad_weight,
                                 l.pieces > 1 ? reinterpret_cast<float*>(ws + l.total) : nullptr, c.grad_weight_stride,
                                 first, most, vocab, hidden, 0, 0, c.accumulate};
+        if (transposed) {
+            // runs along the hidden dimension: enough workgroups to fill the chip
+            const uint32_t chunks = ceil_div(hidden, 64u), groups = columns / kTile;
+            const uint32_t wanted = ceil_div(2048u, groups), runs = wanted < chunks ? wanted : chunks;
+            rc = launch(few_grad_weight_kernel<T, W>, dim3(groups * runs), dim3(256), st, gw, transposed, runs);
+            if (rc != LA_OK) return rc;
+            continue;
+        }
         rc = l.grad_w_side == 128 ? run_grad_weight<T, W, 128>(gw, st) : run_grad_weight<T, W, 256>(gw, st);
         if (rc != LA_OK) return rc;
     }
