@@ -393,74 +393,108 @@ template <typename T, int OUTER> __global__ __launch_bounds__(256) void few_scor
 // ---------------------------------------------------------------------------
 // the rows' losses
 // ---------------------------------------------------------------------------
+// lse of a row from its parts, by the THREADS threads that call it together.
+template <int THREADS> __device__ __forceinline__ float row_lse(const Part* parts, uint32_t tiles, float* lds)
+{
+    const uint32_t thread = threadIdx.x % THREADS, wave = threadIdx.x / kWave;
+    float top = -INFINITY, sum = 0.0f;
+    for (uint32_t k = thread; k < tiles; k += THREADS) top = fmaxf(top, parts[k].top);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if constexpr (THREADS > kWave) {
+        if (threadIdx.x % kWave == 0) lds[wave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < THREADS / kWave; ++w) top = fmaxf(top, lds[w]);
+    }
+    const float base = top == -INFINITY ? 0.0f : top;
+    for (uint32_t k = thread; k < tiles; k += THREADS) sum += parts[k].sum * expf(parts[k].top - base);
+    sum = wave_sum(sum);
+    if constexpr (THREADS > kWave) {
+        if (threadIdx.x % kWave == 0) lds[THREADS / kWave + wave] = sum;
+        __syncthreads();
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < THREADS / kWave; ++w) sum += lds[THREADS / kWave + w];
+    }
+    return base + logf(sum);
+}
+
 __global__ __launch_bounds__(256) void row_loss_kernel(const Part* parts, uint32_t tiles, const Plan* plan,
                                                        uint32_t first, uint32_t most, const uint32_t* rows,
                                                        const int32_t* row_targets, const float* target_scores,
-                                                       float* lse, float* row_loss)
+                                                       float* row_loss)
 {
-    const uint32_t row = blockIdx.x * 4 + threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const uint32_t row = blockIdx.x * 4 + threadIdx.x / kWave;
     if (row >= piece_rows(plan, first, most)) return;
-    const Part* mine = parts + static_cast<uint64_t>(row) * tiles;
-    float top = -INFINITY, sum = 0.0f;
-    for (uint32_t k = lane; k < tiles; k += kWave) top = fmaxf(top, mine[k].top);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const float base = top == -INFINITY ? 0.0f : top;
-    for (uint32_t k = lane; k < tiles; k += kWave) sum += mine[k].sum * expf(mine[k].top - base);
-    sum = wave_sum(sum);
-    if (lane != 0) return;
-    const float total = base + logf(sum);
-    const bool known = row_targets[first + row] >= 0;
-    lse[row] = known ? total : __builtin_nanf("");
-    row_loss[rows[first + row]] = known ? total - target_scores[row] : __builtin_nanf("");
+    const float lse = row_lse<kWave>(parts + static_cast<uint64_t>(row) * tiles, tiles, nullptr);
+    if (threadIdx.x % kWave == 0)
+        row_loss[rows[first + row]] =
+            row_targets[first + row] >= 0 ? lse - target_scores[row] : __builtin_nanf("");
 }
 
-__global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const uint32_t* rows, const Plan* plan,
-                                                    int mean, float* loss)
+// The sum of the rows' losses, in 64 bits and a fixed order, by one workgroup.
+template <uint32_t THREADS>
+__device__ void write_loss(const float* row_loss, const uint32_t* rows, const Plan* plan, int mean, float* loss)
 {
-    __shared__ double lds[16];
+    __shared__ double lds[THREADS / kWave];
+    const uint32_t count = plan->rows;
     double sum = 0.0;
-    for (uint32_t k = threadIdx.x; k < plan->rows; k += 1024) sum += static_cast<double>(row_loss[rows[k]]);
+#pragma unroll 4
+    for (uint32_t k = threadIdx.x; k < count; k += THREADS) sum += static_cast<double>(row_loss[rows[k]]);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
     if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = sum;
     __syncthreads();
     if (threadIdx.x != 0) return;
-    for (int w = 1; w < 16; ++w) sum += lds[w];
-    *loss = static_cast<float>(mean && plan->rows > 0 ? sum / plan->rows : sum);
+    for (uint32_t w = 1; w < THREADS / kWave; ++w) sum += lds[w];
+    *loss = static_cast<float>(mean && count > 0 ? sum / count : sum);
+}
+
+__global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const uint32_t* rows, const Plan* plan,
+                                                    int mean, float* loss)
+{
+    write_loss<1024>(row_loss, rows, plan, mean, loss);
 }
 
 // ---------------------------------------------------------------------------
 // D, in place of exp(s - m)
 // ---------------------------------------------------------------------------
+// Each workgroup joins its row's parts itself, a few KB out of the caches, rather
+// than wait for a launch that does it once.
 constexpr uint32_t kPerGroup = 4;                                // 16-byte vectors per thread
 
 template <typename T>
-__global__ __launch_bounds__(256) void softmax_grad_kernel(T* held, const Part* parts, const float* lse,
-                                                           const int32_t* row_targets, const Plan* plan,
-                                                           uint32_t first, uint32_t most, uint32_t width,
-                                                           uint32_t tiles)
+__global__ __launch_bounds__(256) void softmax_grad_kernel(ScoreArgs a, const uint32_t* rows, float* row_loss)
 {
-    const uint32_t row = blockIdx.y, rows = piece_rows(plan, first, most);
-    if (row >= round_up(rows, kTile)) return;
-    const uint32_t side = width / tiles;
-    T* mine = held + static_cast<uint64_t>(row) * width;
-    const int32_t target = row < rows ? row_targets[first + row] : -1;
-    const float total = row < rows ? lse[row] : 0.0f;
+    __shared__ float lds[8];
+    const uint32_t row = blockIdx.y, count = piece_rows(a.plan, a.first, a.most);
+    if (row >= round_up(count, kTile)) return;
+    const uint32_t side = a.columns / a.tiles;
+    const Part* parts = a.parts + static_cast<uint64_t>(row) * a.tiles;
+    T* mine = static_cast<T*>(a.held) + static_cast<uint64_t>(row) * a.columns;
+    int32_t target = -1;
+    float lse = 0.0f;
+    if (row < count) {
+        target = a.row_targets[a.first + row];
+        // a target that is none makes the row NaN
+        lse = target >= 0 ? row_lse<256>(parts, a.tiles, lds) : __builtin_nanf("");
+        if (blockIdx.x == 0 && threadIdx.x == 0)
+            row_loss[rows[a.first + row]] = target >= 0 ? lse - a.target_scores[row] : lse;
+    }
 #pragma unroll
     for (uint32_t k = 0; k < kPerGroup; ++k) {
         const uint32_t vec = (blockIdx.x * kPerGroup + k) * 256 + threadIdx.x;
-        if (vec * 8 >= width) return;
+        if (vec * 8 >= a.columns) return;
         float d[8] = {};
-        if (row < rows) {
-            load_vec<T>(mine, vec, width, d);
-            const float top = parts[static_cast<uint64_t>(row) * tiles + vec * 8 / side].top;
-            const float f = expf(top - total);
+        if (row < count) {
+            load_vec<T>(mine, vec, a.columns, d);
+            const float f = expf(parts[vec * 8 / side].top - lse);
 #pragma unroll
             for (uint32_t e = 0; e < 8; ++e)
                 d[e] = d[e] * f - (static_cast<int32_t>(vec * 8 + e) == target ? kHeld<T> : 0.0f);
         }
-        store_vec<T, 8>(mine, vec, width, d);
+        store_vec<T, 8>(mine, vec, a.columns, d);
     }
 }
 
@@ -500,9 +534,15 @@ __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void 
     });
 }
 
+// The last workgroup, after the piece's rows, writes the loss where it is known.
 template <typename T>
-__global__ __launch_bounds__(256) void join_grad_x_kernel(GradXArgs a, T* grad_x, uint64_t grad_x_stride)
+__global__ __launch_bounds__(256) void join_grad_x_kernel(GradXArgs a, T* grad_x, uint64_t grad_x_stride,
+                                                          const float* row_loss, int mean, float* loss)
 {
+    if (blockIdx.x == a.most) {
+        write_loss<256>(row_loss, a.rows, a.plan, mean, loss);
+        return;
+    }
     const uint32_t row = blockIdx.x, rows = piece_rows(a.plan, a.first, a.most);
     if (row >= rows) return;
     const uint32_t splits = *a.splits;
@@ -695,7 +735,7 @@ int side_of(uint64_t rows, uint64_t columns, uint64_t k, uint64_t max_splits)
 struct Layout {
     int score_side, grad_x_side, grad_w_side;
     uint64_t padded, columns, all, piece, pieces, max_splits;
-    uint64_t plan, splits, rows, row_targets, gathered, weight, parts, target_scores, lse, row_loss, held, partial, transposed, total, size;
+    uint64_t plan, splits, rows, row_targets, gathered, weight, parts, target_scores, row_loss, held, partial, transposed, total, size;
 
     explicit Layout(const la_linear_loss_t& c)
     {
@@ -730,7 +770,6 @@ struct Layout {
         weight = !copies_weight(c) ? 0 : take(c.vocab * padded * 2);
         parts = take(piece * (columns / score_side) * sizeof(Part));
         target_scores = take(piece * 4);
-        lse = take(piece * 4);
         row_loss = c.row_loss ? 0 : take(c.n * 4);
         held = c.grads ? take(piece * columns * 2) : 0;
         partial = c.grads ? take(max_splits * piece * c.hidden * 4) : 0;
@@ -750,13 +789,15 @@ template <typename T> int run_scores(const la_linear_loss_t& c, const Layout& l,
 }
 
 template <typename T, int SIDE>
-int run_grad_x(const Layout& l, GradXArgs a, T* grad_x, uint64_t grad_x_stride, hipStream_t st)
+int run_grad_x(const la_linear_loss_t& c, const Layout& l, GradXArgs a, const float* row_loss, hipStream_t st)
 {
     a.inners = ceil_div(a.hidden, SIDE);
     const int rc = launch(grad_x_kernel<T, SIDE>, dim3(tile::places(l.piece / SIDE * l.max_splits, a.inners)),
                           dim3(tile::kThreads), st, a);
     if (rc != LA_OK) return rc;
-    return launch(join_grad_x_kernel<T>, dim3(l.piece), dim3(256), st, a, grad_x, grad_x_stride);
+    const bool last = a.first + l.piece >= l.all;
+    return launch(join_grad_x_kernel<T>, dim3(l.piece + (last && c.loss ? 1 : 0)), dim3(256), st, a,
+                  static_cast<T*>(c.grad_x), c.grad_x_stride, row_loss, c.mean, c.loss);
 }
 
 template <typename T, typename W, int SIDE> int run_grad_weight(GradWeightArgs a, hipStream_t st)
@@ -776,7 +817,6 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
     T* gathered = reinterpret_cast<T*>(ws + l.gathered);
     Part* parts = reinterpret_cast<Part*>(ws + l.parts);
     float* target_scores = reinterpret_cast<float*>(ws + l.target_scores);
-    float* lse = reinterpret_cast<float*>(ws + l.lse);
     float* row_loss = c.row_loss ? c.row_loss : reinterpret_cast<float*>(ws + l.row_loss);
     T* held = c.grads ? reinterpret_cast<T*>(ws + l.held) : nullptr;
     T* grad_x = c.grads ? static_cast<T*>(c.grad_x) : nullptr;
@@ -806,20 +846,23 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
 
     for (uint64_t p = 0; p < l.pieces; ++p) {
         const uint32_t first = p * l.piece, most = l.piece;
-        rc = run_scores<T>(c, l, ScoreArgs{weight, x, plan, row_targets, parts, target_scores, held, first, most, vocab,
-                                           columns, tiles, static_cast<uint32_t>(l.padded / tile::kDepth)}, st);
+        const ScoreArgs scores{weight, x, plan, row_targets, parts, target_scores, held, first, most, vocab, columns,
+                               tiles, static_cast<uint32_t>(l.padded / tile::kDepth)};
+        rc = run_scores<T>(c, l, scores, st);
         if (rc != LA_OK) return rc;
-        rc = launch(row_loss_kernel, dim3(most / 4), dim3(256), st, parts, tiles, plan, first, most, rows, row_targets,
-                    target_scores, lse, row_loss);
-        if (rc != LA_OK) return rc;
-        if (!c.grads) continue;
-        rc = launch(softmax_grad_kernel<T>, dim3(ceil_div(columns, 8 * 256 * kPerGroup), most), dim3(256), st, held,
-                    parts, lse, row_targets, plan, first, most, columns, tiles);
+        if (!c.grads) {
+            rc = launch(row_loss_kernel, dim3(most / 4), dim3(256), st, parts, tiles, plan, first, most, rows,
+                        row_targets, target_scores, row_loss);
+            if (rc != LA_OK) return rc;
+            continue;
+        }
+        rc = launch(softmax_grad_kernel<T>, dim3(ceil_div(columns, 8 * 256 * kPerGroup), most), dim3(256), st, scores,
+                    rows, row_loss);
         if (rc != LA_OK) return rc;
         const GradXArgs gx{weight, d, plan, rows, reinterpret_cast<float*>(ws + l.partial), splits + p, first, most,
                            hidden, 0, static_cast<uint32_t>(columns / kPair)};
-        rc = l.grad_x_side == 128 ? run_grad_x<T, 128>(l, gx, grad_x, c.grad_x_stride, st)
-                                  : run_grad_x<T, 256>(l, gx, grad_x, c.grad_x_stride, st);
+        rc = l.grad_x_side == 128 ? run_grad_x<T, 128>(c, l, gx, row_loss, st)
+                                  : run_grad_x<T, 256>(c, l, gx, row_loss, st);
         if (rc != LA_OK) return rc;
         const tile::Matrix piece_x{gathered + first * l.padded, l.piece < l.all - first ? l.piece : l.all - first,
                                    l.padded, l.padded * 2};
@@ -837,7 +880,7 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
         rc = l.grad_w_side == 128 ? run_grad_weight<T, W, 128>(gw, st) : run_grad_weight<T, W, 256>(gw, st);
         if (rc != LA_OK) return rc;
     }
-    if (!c.loss) return LA_OK;
+    if (!c.loss || c.grads) return LA_OK;
     return launch(loss_kernel, dim3(1), dim3(1024), st, row_loss, rows, plan, c.mean, c.loss);
 }
 
