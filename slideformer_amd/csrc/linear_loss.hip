@@ -374,7 +374,7 @@ template <typename T, int OUTER> __global__ __launch_bounds__(256) void few_scor
     }
     reduce_scores<kTile>(a, blockIdx.x, 0, rows, wave, wave * 64, 0, sums, exchange);
     if (!a.held) return;
-    // the rows after these, up to a whole tile, are written as zeros with D
+    // the rows after these are written as zeros with D
 #pragma unroll
     for (int t = 0; t < OUTER; ++t) {
         T* held = static_cast<T*>(a.held) + static_cast<uint64_t>(t * 16 + lane % 16) * a.columns +
@@ -469,7 +469,9 @@ __global__ __launch_bounds__(256) void softmax_grad_kernel(ScoreArgs a, const ui
 {
     __shared__ float lds[8];
     const uint32_t row = blockIdx.y, count = piece_rows(a.plan, a.first, a.most);
-    if (row >= round_up(count, kTile)) return;
+    // rows past the last are zeros to the end of its pair of steps, as the matrix's gradient sums over rows; what
+    // lies beyond only reaches rows of the states' gradient that are not written
+    if (row >= round_up(count, 2 * tile::kDepth)) return;
     const uint32_t side = a.columns / a.tiles;
     const Part* parts = a.parts + static_cast<uint64_t>(row) * a.tiles;
     T* mine = static_cast<T*>(a.held) + static_cast<uint64_t>(row) * a.columns;
