@@ -59,12 +59,12 @@ __device__ __forceinline__ uint32_t round_up(uint32_t x, uint32_t to) { return (
 // which tiles, how many runs of k
 // ---------------------------------------------------------------------------
 // About how long a product of `tiles` tiles over `steps` steps of k takes in `splits`
-// runs of k, in us.  The chip holds 256 tiles of 256 x 256 at a time, or 512 of
+// runs of k, in us.  The chip holds 256 tiles of 256 x 256 at a time, or 768 of
 // 128 x 128, so they run in rounds; those of the larger ones end together.  A round
 // costs its steps and a start and an end; the partial sums of a split product are
 // written and read once more.  The constants are from products of 1000 to 3072
 // rows, 20000 to 128256 columns and 768 to 4096 k: of 256, 0.86 us a step and 12 us
-// a round; of 128, 0.53 to 0.78 us (two on a compute unit) and 5.5 us.
+// a round; of 128, about 0.9 us (three on a compute unit) and 6.5 us.
 __host__ __device__ __forceinline__ float product_us(int side, uint32_t tiles, uint32_t steps, uint32_t splits,
                                                      float partial_bytes)
 {
@@ -72,7 +72,7 @@ __host__ __device__ __forceinline__ float product_us(int side, uint32_t tiles, u
     const float all = static_cast<float>(tiles) * static_cast<float>(splits);
     const float join = static_cast<float>(splits) * partial_bytes * (2.0f / 4.0e6f);
     if (side == 256) return ceilf(all / 256.0f) * (0.86f * k + 12.0f) + join;
-    return fmaxf(1.0f, all / 512.0f) * (0.65f * k + 5.5f) + join;
+    return fmaxf(1.0f, all / 768.0f) * (0.9f * k + 6.5f) + join;
 }
 
 constexpr uint32_t kMostSplits = 64;

@@ -15,12 +15,13 @@
 //                64 KB of LDS reads and 32 KB of writes (768 cycles at 128 bytes each), so
 //                LDS stays behind the matrix cores; with eight waves of 128 x 64 the reads
 //                alone would take as long as the products.
-//   SIDE 128     two workgroups on a compute unit, each in the other's pauses: a
-//                product with few tiles or few steps is made of starts and ends.
+//   SIDE 128     three workgroups on a compute unit, each in the others' pauses: a
+//                product with few tiles or few steps is made of starts and ends.  Two,
+//                with a step more in LDS, took 1024 x 50257 x 768 370 us instead of 348.
 // What a wave multiplies in one step it reads from LDS during the step before,
 // instruction by instruction between the products, so that neither waits for the
-// other.  Operands go from memory into LDS without passing registers, four steps
-// ahead.  The LDS image is permuted so that no read has bank conflicts; since the
+// other.  Operands go from memory into LDS without passing registers, three or four
+// steps ahead.  The LDS image is permuted so that no read has bank conflicts; since the
 // loads write LDS linearly, the permutation is applied to the addresses that they read:
 //   by rows      [SIDE][32]: 16-byte chunk c of row r is at chunk c ^ (r / 2 % 4), so 8
 //                lanes that read one chunk column of 8 rows hit all 128 bytes of banks;
@@ -37,19 +38,19 @@
 namespace tile {
 
 constexpr int kDepth = 32;          // k per step
-constexpr int kAhead = 4;           // steps in LDS
 constexpr int kThreads = 256;
 
 template <int SIDE> struct Sizes {
     static constexpr int kPanelBytes = SIDE * kDepth * 2;   // one operand's share of a step
     static constexpr int kStepBytes = 2 * kPanelBytes;
+    static constexpr int kAhead = SIDE == 256 ? 4 : 3;      // steps in LDS
     static constexpr int kLdsBytes = kAhead * kStepBytes;
     static constexpr int kLoads = kPanelBytes / 4096;       // of a lane, for a panel
     static constexpr int kWave = SIDE / 2;                  // side of a wave's quarter
     static constexpr int kParts = kWave / 16;               // its fragments
     static constexpr int kRow = kWave + 4;                  // distance of rows that are handed out
     static constexpr int kHandOutBytes = 4 * 32 * kRow * 4;
-    static constexpr int kResident = SIDE == 256 ? 1 : 2;   // workgroups on a compute unit
+    static constexpr int kResident = SIDE == 256 ? 1 : 3;   // workgroups on a compute unit
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -222,18 +223,18 @@ template <typename T, int SIDE, bool INNER_ROWS, bool OUTER_ROWS> struct Product
     uint32_t place;                 // of this wave's loads in a panel
 
     // One step: multiplies `now`, reads the fragments of the next step into `then`,
-    // and loads the step kAhead from here over this one, whose reads are over.
+    // and loads the step Z::kAhead from here over this one, whose reads are over.
     __device__ __forceinline__ void step(uint32_t at, const Step<SIDE>& now, Step<SIDE>& then, Sums<SIDE>& sums)
     {
         // in groups of four products: reads in the first half, loads in the second
         constexpr int kGroups = Z::kParts * Z::kParts / 4, kHalf = kGroups / 2;
         constexpr int kReads = Z::kParts / kHalf, kLoads = 2 * Z::kLoads / kHalf;
         // the next step's loads have arrived: only those of two steps more are in flight
-        arrive<(kAhead - 2) * 2 * Z::kLoads>();
-        const lds_char* from = lds + (at + 1) % kAhead * Z::kStepBytes;
+        arrive<(Z::kAhead - 2) * 2 * Z::kLoads>();
+        const lds_char* from = lds + (at + 1) % Z::kAhead * Z::kStepBytes;
         const uint32_t to =
             __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) +
-                                           at % kAhead * Z::kStepBytes + place);
+                                           at % Z::kAhead * Z::kStepBytes + place);
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
             if (g < kHalf) {
@@ -243,8 +244,8 @@ template <typename T, int SIDE, bool INNER_ROWS, bool OUTER_ROWS> struct Product
                     then[1][g * kReads + k] = read_outer.read(from + Z::kPanelBytes, g * kReads + k);
                 }
             }
-            if (g == kHalf - 1) load_inner.turn(at + kAhead);
-            if (g == kHalf + kHalf / 4) load_outer.turn(at + kAhead);
+            if (g == kHalf - 1) load_inner.turn(at + Z::kAhead);
+            if (g == kHalf + kHalf / 4) load_outer.turn(at + Z::kAhead);
             if (g >= kHalf) {
 #pragma unroll
                 for (int k = (g - kHalf) * kLoads; k < (g - kHalf + 1) * kLoads; ++k) {
@@ -276,7 +277,7 @@ template <typename T, int SIDE, bool INNER_ROWS, bool OUTER_ROWS> struct Product
             for (int t = 0; t < Z::kParts; ++t) sums[s][t] = f32x4{0, 0, 0, 0};
         if (steps == 0) return;
 #pragma unroll
-        for (int ahead = 0; ahead < kAhead; ++ahead) {
+        for (int ahead = 0; ahead < Z::kAhead; ++ahead) {
             const uint32_t to = __builtin_amdgcn_readfirstlane(
                 static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + ahead * Z::kStepBytes + place);
             load_inner.turn(ahead);
@@ -286,7 +287,7 @@ template <typename T, int SIDE, bool INNER_ROWS, bool OUTER_ROWS> struct Product
 #pragma unroll
             for (int n = 0; n < Z::kLoads; ++n) load_outer.load(to + Z::kPanelBytes, n);
         }
-        arrive<(kAhead - 1) * 2 * Z::kLoads>();
+        arrive<(Z::kAhead - 1) * 2 * Z::kLoads>();
         Step<SIDE> even, odd;
 #pragma unroll
         for (int n = 0; n < Z::kParts; ++n) {

@@ -295,19 +295,19 @@ def _loss_inputs(device, n, hidden, vocab, dtype, ignored, seed=0, gap=0, offset
 
 
 class _Exact:
-    """Loss and gradients in 64 bits on the CPU, with bounds on what the kernels' roundings may do."""
+    """Loss and gradients in 64 bits on `where`, with bounds on what the kernels' roundings may do."""
 
-    def __init__(self, x, weight, targets, mean=True, scale=1.0):
+    def __init__(self, x, weight, targets, mean=True, scale=1.0, where="cpu"):
         u = U[x.dtype]
-        self.device, self.dtype = x.device, x.dtype
-        keep = (targets != IGNORE).cpu()
-        x, w, t = x.double().cpu(), weight.double().cpu(), targets.cpu()
+        self.where, self.dtype = where, x.dtype
+        keep = (targets != IGNORE).to(where)
+        x, w, t = x.double().to(where), weight.double().to(where), targets.to(where)
         x = torch.where(keep[:, None], x, torch.zeros_like(x))
         rows, at = torch.nonzero(keep).flatten(), t[keep]
         s = x[rows] @ w.t()
         lse = torch.logsumexp(s, 1)
-        losses = torch.zeros(t.numel(), dtype=torch.float64)
-        losses[rows] = lse - s[torch.arange(rows.numel()), at]
+        losses = torch.zeros(t.numel(), dtype=torch.float64, device=where)
+        losses[rows] = lse - s[torch.arange(rows.numel(), device=where), at]
         # a score is an fp32 sum of hidden products; a few more roundings for exp and the sums over the vocabulary
         sizes = x[rows].abs() @ w.abs().t()
         score = (x.shape[1] + 64) * U32 * (sizes.amax(1) if rows.numel() else sizes.new_zeros(0))
@@ -320,7 +320,7 @@ class _Exact:
         self.loss_bound = self.row_bounds.sum() / count + 4 * U32 * self.loss.abs() + 1e-30
         p = torch.exp(s - lse[:, None])
         hot = torch.zeros_like(p)
-        hot[torch.arange(rows.numel()), at] = 1
+        hot[torch.arange(rows.numel(), device=where), at] = 1
         f = scale / count
         # D: exp(s - m) rounded, its factor, D rounded; fp16 holds them times 2^13, steps of 2^-24 at the least
         d_off = p * (u + 4 * score[:, None] + 16 * U32) + (p + hot) * u + (2.0 ** -36 if self.dtype == F16 else 0)
@@ -335,11 +335,11 @@ class _Exact:
         self.grad_w_off = ((d_off + (p + hot) * chain).t() @ x[rows].abs()) * abs(f) * 1.1
 
     def check(self, loss, grad_x, grad_weight, before=None):
-        _within(loss.cpu(), self.loss, self.loss_bound, "loss")
-        _within(grad_x.cpu(), self.grad_x, self.grad_x_bound, "grad_x")
-        want = self.grad_w + (0 if before is None else before.double().cpu())
+        _within(loss.to(self.where), self.loss, self.loss_bound, "loss")
+        _within(grad_x.to(self.where), self.grad_x, self.grad_x_bound, "grad_x")
+        want = self.grad_w + (0 if before is None else before.double().to(self.where))
         bound = self.grad_w_off + (U[grad_weight.dtype] + 4 * U32) * want.abs() + TINY[grad_weight.dtype]
-        _within(grad_weight.cpu(), want, bound, "grad_weight")
+        _within(grad_weight.to(self.where), want, bound, "grad_weight")
 
 
 LOSS_SIZES = [
@@ -369,6 +369,18 @@ def test_linear_cross_entropy_grad(hip_device, n, hidden, vocab, dtype, ignored)
     e.check(*got)
     again = ops.linear_cross_entropy_grad(x, weight, targets)
     assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("dtype,ignored", [(BF16, 0.0), (F16, 0.03)])
+def test_linear_cross_entropy_grad_of_a_batch(hip_device, dtype, ignored):
+    """Large enough that all three products take the larger tiles, and the states' gradient is split."""
+    x, weight, targets = _loss_inputs(hip_device, 2040, 2048, 32700, dtype, ignored)
+    e = _Exact(x, weight, targets, where=hip_device)
+    got = ops.linear_cross_entropy_grad(x, weight, targets)
+    e.check(*got)
+    in_pieces = ops.linear_cross_entropy_grad(x, weight, targets, piece_bytes=1 << 26)
+    e.check(*in_pieces)
+    _within(ops.linear_cross_entropy(x, weight, targets, reduction="none"), e.row_losses, e.row_bounds + 1e-30)
 
 
 @pytest.mark.parametrize("n,ignored", [(1030, 0.1), (1030, 0.8), (600, 0.0), (1030, 1.0)])
