@@ -550,17 +550,23 @@ __global__ __launch_bounds__(256) void join_grad_x_kernel(GradXArgs a, T* grad_x
     const uint32_t splits = *a.splits;
     const float factor = a.plan->factor;
     T* out = grad_x + a.rows[a.first + row] * grad_x_stride;
-    for (uint32_t vec = threadIdx.x; vec * 4 < a.hidden; vec += 256) {
-        float sum[4] = {};
+    for (uint32_t vec = threadIdx.x; vec * 8 < a.hidden; vec += 256) {
+        float sum[8] = {};
+#pragma unroll 4
         for (uint32_t k = 0; k < splits; ++k) {
-            float v[4];
-            load_vec<float>(a.partial + (static_cast<uint64_t>(k) * a.most + row) * a.hidden, vec, a.hidden, v);
+            const float* partial = a.partial + (static_cast<uint64_t>(k) * a.most + row) * a.hidden;
+            float lo[4], hi[4];
+            load_vec<float>(partial, vec * 2, a.hidden, lo);
+            load_vec<float>(partial, vec * 2 + 1, a.hidden, hi);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] += v[e];
+            for (int e = 0; e < 4; ++e) {
+                sum[e] += lo[e];
+                sum[4 + e] += hi[e];
+            }
         }
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e)
-            if (vec * 4 + e < a.hidden) out[vec * 4 + e] = Elem<T>::from_f32(sum[e] * factor);
+        for (int e = 0; e < 8; ++e) sum[e] *= factor;
+        store_vec<T, 8>(out, vec, a.hidden, sum);
     }
 }
 

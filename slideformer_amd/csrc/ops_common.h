@@ -14,12 +14,10 @@
 namespace {
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 // The target runs with unaligned access on: a 16-byte access needs the
 // alignment of an element only, so rows of odd length and views at odd offsets
 // take the same instructions.
 typedef u32x4_t u32x4_any __attribute__((aligned(2)));
-typedef u32x2_t u32x2_any __attribute__((aligned(1)));
 
 // E elements of one 16-byte access, as fp32
 template <typename T> struct Elem;
