@@ -27,7 +27,8 @@ template <typename I> __device__ __forceinline__ uint64_t token_at(const I* toke
 // lookup
 // ---------------------------------------------------------------------------
 // A wave takes kLookup 16-byte vectors per lane of one row, all loaded before
-// the first is stored.
+// the first is stored.  8192 tokens of 128256 x 4096 bf16: 20.2 us, 6.6 TB/s; one
+// token: 2.9 us, a launch and two loads that depend on each other.
 constexpr int kLookup = 4;
 
 template <typename T, typename I>
@@ -119,6 +120,8 @@ __global__ __launch_bounds__(256) void rank_kernel(const I* tokens, uint32_t n, 
     }
 }
 
+// 16 lanes a token: the searches of its chunks run beside each other, ten loads
+// deep each.  8192 tokens: 5.1 us, which is their latency.
 __global__ __launch_bounds__(256) void merge_kernel(const uint32_t* keys, const uint32_t* places, uint32_t n,
                                                     uint32_t* sorted, uint32_t* sorted_places, uint8_t* marks)
 {
@@ -262,7 +265,8 @@ template <typename T, typename O> __global__ __launch_bounds__(256, 8) void run_
 }
 
 // A workgroup joins the run that starts in block `unit / slices` and goes on.  Its
-// waves take turns of kFlight partials and their sums are added in order.
+// waves take turns of kFlight partials and their sums are added in order.  8192
+// tokens of 128256 x 4096 with a most frequent one of 490: 14.4 us, latency.
 template <typename T, typename O> __global__ __launch_bounds__(256) void join_runs_kernel(SumArgs a)
 {
     constexpr int E = Elem<T>::kCount;

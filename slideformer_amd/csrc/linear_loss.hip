@@ -87,9 +87,7 @@ struct SplitArgs {
     uint32_t pieces, most, hidden, steps, side, max_splits;
 };
 
-constexpr uint32_t kFewRows = 64;                                // up to so many, a call is bound by the vocabulary matrix
-
-// One workgroup lists the rows whose target is not `ignore`, in order.
+// One workgroup (the list is in order, and 8192 targets are one trip: 5 us) lists the rows whose target is not `ignore`, in order.
 constexpr uint32_t kListed = 8;                                  // targets per thread and trip
 
 __global__ __launch_bounds__(1024) void list_rows_kernel(const int64_t* targets, uint32_t n, int64_t ignore,
@@ -157,22 +155,17 @@ __global__ __launch_bounds__(1024) void list_rows_kernel(const int64_t* targets,
     }
 }
 
+// Bound by memory and small: 14 us for 4096 x 4096 beside products of milliseconds.
 // Workgroup b < rows: row b of the gathered X, zeros after the last trained row and
 // after the row's end; the others zero what an ignored row answers.
 template <typename T>
 __global__ __launch_bounds__(256) void gather_kernel(const T* x, uint64_t x_stride, uint32_t hidden, uint32_t padded,
                                                      const uint32_t* rows, const Plan* plan, T* gathered,
                                                      uint32_t gathered_rows, const int64_t* targets, int64_t ignore,
-                                                     float* row_loss, T* grad_x, uint64_t grad_x_stride,
-                                                     T* transposed)
+                                                     float* row_loss, T* grad_x, uint64_t grad_x_stride)
 {
     if (blockIdx.x < gathered_rows) {
         const uint32_t row = blockIdx.x, count = plan->rows;
-        // few rows with gradients: X^T too, [padded][kFewRows]
-        if (transposed && row < kFewRows)
-            for (uint32_t h = threadIdx.x; h < padded; h += 256)
-                transposed[static_cast<uint64_t>(h) * kFewRows + row] =
-                    row < count && h < hidden ? x[rows[row] * x_stride + h] : Elem<T>::from_f32(0.0f);
         if (row >= round_up(count, kTile)) return;
         T* to = gathered + static_cast<uint64_t>(row) * padded;
         for (uint32_t vec = threadIdx.x; vec * 8 < padded; vec += 256) {
@@ -192,6 +185,7 @@ __global__ __launch_bounds__(256) void gather_kernel(const T* x, uint64_t x_stri
 }
 
 // A vocabulary matrix whose rows are not whole, aligned stages of k: a padded copy.
+// 32003 x 1023: 28 us, 4.7 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void pad_kernel(const T* weight, uint64_t stride, uint32_t hidden, uint32_t padded,
                                                   T* to)
@@ -296,6 +290,10 @@ __device__ __forceinline__ void reduce_scores(const ScoreArgs& a, uint32_t inner
         }
 }
 
+// s = X W^T by tiles, reduced where they are: 3072 x 128256 x 4096 in 2.78 ms, 1.16 PFLOP/s
+// with the softmax's part and 790 MB of exp(s - m) written; bound by the matrix
+// cores at the clock that power leaves (1.9 GHz, 55 % of cycles busy) and a start
+// and an end per tile, a sixth of it at k = 4096.
 template <typename T, int SIDE>
 __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void scores_kernel(ScoreArgs a)
 {
@@ -320,50 +318,49 @@ __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void 
     });
 }
 
-// The same for at most 16 * OUTER rows: the time is that of reading the vocabulary
+// The same for at most kFewRows rows: the time is that of reading the vocabulary
 // matrix, which goes from memory to registers in the order that the matrix
-// instructions take it, 64 of its rows a wave; the states come from the caches.
-// Rows of any alignment and width are read where they lie.  13 rows of
-// 128256 x 4096: 232 us (4.5 TB/s), with tiles of 256 rows 300 us.
-template <typename T, int OUTER> __global__ __launch_bounds__(256) void few_scores_kernel(ScoreArgs a)
+// instructions take it, 16 * INNER of its rows a wave; the states come from the caches.
+// Rows of any alignment and width are read where they lie.  13 rows of 128256 x
+// 4096: 241 us (4.4 TB/s), the call 250, with tiles of 128 261; of 60001 x 1023, which
+// tiles need a padded copy of, the call 71 us and 102.  From 17 rows on tiles are as
+// fast or faster (40 rows of 128256 x 4096: 268 us, four fragments of rows here 343).
+constexpr uint32_t kFewRows = 16;
+
+template <typename T, int INNER> __global__ __launch_bounds__(256) void few_scores_kernel(ScoreArgs a)
 {
-    __shared__ Exchange<4, 16 * OUTER> exchange;
+    constexpr int SIDE = 64 * INNER;
+    __shared__ Exchange<4, kFewRows> exchange;
     const uint32_t rows = piece_rows(a.plan, a.first, a.most);
     if (rows == 0) return;
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const uint32_t width = a.weight.width, steps = a.steps;
-    const T* weight[4];
-    const T* x[OUTER];
+    const T* weight[INNER];
 #pragma unroll
-    for (uint32_t s = 0; s < 4; ++s) {
-        const uint32_t row = blockIdx.x * kTile + wave * 64 + s * 16 + lane % 16;
+    for (uint32_t s = 0; s < INNER; ++s) {
+        const uint32_t row = blockIdx.x * SIDE + wave * (16 * INNER) + s * 16 + lane % 16;
         weight[s] = reinterpret_cast<const T*>(static_cast<const char*>(a.weight.data) +
                                                (row < a.vocab ? row : a.vocab - 1) * a.weight.stride);
     }
-#pragma unroll
-    for (uint32_t t = 0; t < OUTER; ++t)
-        x[t] = static_cast<const T*>(a.x.data) + (a.first + t * 16 + lane % 16) * (a.x.stride / 2);
-    f32x4 sums[4][OUTER] = {};
-    u32x4_t w[2][2][4], v[2][2][OUTER];                              // [buffer][step of the pair]
+    const T* x = static_cast<const T*>(a.x.data) + (a.first + lane % 16) * (a.x.stride / 2);
+    f32x4 sums[INNER][1] = {};
+    u32x4_t w[2][2][INNER], v[2][2];                                 // [buffer][step of the pair]
     const auto load = [&](int b, uint32_t step) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t vec = (step + h) * 4 + lane / 16;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) w[b][h][s] = load_raw<T>(weight[s], vec, width);
-#pragma unroll
-            for (int t = 0; t < OUTER; ++t) v[b][h][t] = *reinterpret_cast<const u32x4_t*>(x[t] + vec * 8);
+            for (int s = 0; s < INNER; ++s) w[b][h][s] = load_raw<T>(weight[s], vec, width);
+            v[b][h] = *reinterpret_cast<const u32x4_t*>(x + vec * 8);
         }
     };
     const auto multiply = [&](int b) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int t = 0; t < OUTER; ++t)
-                    sums[s][t] = tile::product_of<T>(__builtin_bit_cast(tile::s16x8, w[b][h][s]),
-                                                     __builtin_bit_cast(tile::s16x8, v[b][h][t]), sums[s][t]);
+            for (int s = 0; s < INNER; ++s)
+                sums[s][0] = tile::product_of<T>(__builtin_bit_cast(tile::s16x8, w[b][h][s]),
+                                                 __builtin_bit_cast(tile::s16x8, v[b][h]), sums[s][0]);
     };
     load(0, 0);
     for (uint32_t step = 0; step < steps; step += 4) {              // steps come in pairs
@@ -372,21 +369,18 @@ template <typename T, int OUTER> __global__ __launch_bounds__(256) void few_scor
         if (step + 4 < steps) load(0, step + 4);
         if (step + 2 < steps) multiply(1);
     }
-    reduce_scores<kTile>(a, blockIdx.x, 0, rows, wave, wave * 64, 0, sums, exchange);
+    reduce_scores<SIDE>(a, blockIdx.x, 0, rows, wave, wave * (16 * INNER), 0, sums, exchange);
     if (!a.held) return;
     // the rows after these are written as zeros with D
+    T* held = static_cast<T*>(a.held) + static_cast<uint64_t>(lane % 16) * a.columns + blockIdx.x * SIDE +
+              wave * (16 * INNER) + lane / 16 * 4;
 #pragma unroll
-    for (int t = 0; t < OUTER; ++t) {
-        T* held = static_cast<T*>(a.held) + static_cast<uint64_t>(t * 16 + lane % 16) * a.columns +
-                  blockIdx.x * kTile + wave * 64 + lane / 16 * 4;
+    for (int s = 0; s < INNER; ++s) {
+        typedef T v4 __attribute__((ext_vector_type(4)));
+        v4 e;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            typedef T v4 __attribute__((ext_vector_type(4)));
-            v4 e;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) e[r] = static_cast<T>(sums[s][t][r] * kHeld<T>);
-            *reinterpret_cast<v4*>(held + s * 16) = e;
-        }
+        for (int r = 0; r < 4; ++r) e[r] = static_cast<T>(sums[s][0][r] * kHeld<T>);
+        *reinterpret_cast<v4*>(held + s * 16) = e;
     }
 }
 
@@ -461,7 +455,8 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const
 // D, in place of exp(s - m)
 // ---------------------------------------------------------------------------
 // Each workgroup joins its row's parts itself, a few KB out of the caches, rather
-// than wait for a launch that does it once.
+// than wait for a launch that does it once.  3072 x 128256: 309 us, 5.1 TB/s, bound by
+// memory.
 constexpr uint32_t kPerGroup = 4;                                // 16-byte vectors per thread
 
 template <typename T>
@@ -512,6 +507,8 @@ struct GradXArgs {
     uint32_t first, most, hidden, inners, pairs;               // pairs of steps
 };
 
+// D W, W by columns.  3072 x 4096 over k = 128256 in four runs: 2.42 ms, 1.34 PFLOP/s,
+// the matrix cores busy 63 % of cycles at 1.9 GHz.
 template <typename T, int SIDE>
 __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void grad_x_kernel(GradXArgs a)
 {
@@ -580,6 +577,8 @@ struct GradWeightArgs {
     int accumulate;
 };
 
+// D^T X, both by columns.  128256 x 4096 over 3072 rows: 2.85 ms, 1.13 PFLOP/s; k is
+// 96 steps, so starts and ends of tiles take an eighth, and 1 GB is written.
 template <typename T, typename W, int SIDE>
 __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void grad_weight_kernel(GradWeightArgs a)
 {
@@ -617,84 +616,6 @@ __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void 
                 if (vec * 8 + k < a.hidden) v[k] += Elem<W>::to_f32(out[vec * 8 + k]);
         store_vec<W, 8>(out, vec, a.hidden, v);
     });
-}
-
-// The same for at most kFewRows rows, all of whose k fits two steps: the time is that
-// of writing the gradient.  A wave holds the D of 64 columns in registers, as the
-// matrix instructions take it, and goes along the hidden dimension with X^T out of
-// the caches.  Row m of a fragment of X^T is hidden element 16 (m / 4) + 4 s + m % 4,
-// s counting four fragments, so that a lane ends up with 16 neighbouring elements
-// of a row.  13 rows of 128256 x 4096: 260 us, with tiles of 128 354 us;
-// without the next chunk's loads before this one's stores 400 us.
-template <typename T, typename W>
-__global__ __launch_bounds__(256) void few_grad_weight_kernel(GradWeightArgs a, const T* transposed, uint32_t runs)
-{
-    using Z = tile::Sizes<kTile>;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * Z::kPanelBytes];
-    const uint32_t columns = blockIdx.x / runs * kTile, run = blockIdx.x % runs;
-    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const bool some = a.plan->rows > 0;
-    const float factor = a.plan->factor;
-    tile::Operand<kTile, false> load;
-    tile::Fragments<kTile, false> read;
-    load.init(a.held, columns, 0, some ? 2 : 0);
-    read.init(wave * 64);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        load.turn(half);
-        const uint32_t to = __builtin_amdgcn_readfirstlane(
-            static_cast<uint32_t>(reinterpret_cast<uintptr_t>((tile::lds_char*)lds)) + half * Z::kPanelBytes +
-            wave * 1024);
-#pragma unroll
-        for (int n = 0; n < Z::kLoads; ++n) load.load(to, n);
-    }
-    tile::arrive<0>();
-    tile::s16x8 d[2][4];
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) d[half][t] = read.read((tile::lds_char*)lds + half * Z::kPanelBytes, t);
-
-    const uint32_t chunks = ceil_div(a.hidden, 64u);
-    const T* x = transposed + (lane % 16 / 4 * 8 + lane % 4) * kFewRows + lane / 16 * 8;
-    const uint32_t end = chunks * (run + 1) / runs;
-    tile::s16x8 next[2][4];
-    const auto fetch = [&](uint32_t chunk) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-                next[half][s] = *reinterpret_cast<const tile::s16x8*>(x + (chunk * 64 + s / 2 * 32 + s % 2 * 4) * kFewRows + half * 32);
-    };
-    fetch(chunks * run / runs);
-    for (uint32_t chunk = chunks * run / runs; chunk < end; ++chunk) {
-        f32x4 sums[4][4] = {};
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) sums[s][t] = tile::product_of<T>(next[half][s], d[half][t], sums[s][t]);
-        // before this chunk's stores: a load after them would wait for them
-        fetch(chunk + 1 < end ? chunk + 1 : chunk);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const uint32_t row = columns + wave * 64 + t * 16 + lane % 16;
-            if (row >= a.vocab) continue;
-            W* out = static_cast<W*>(a.grad_weight) + row * a.stride;
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-                const uint32_t vec = chunk * 8 + part * 4 + lane / 16;
-                float v[8];
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) {
-                    v[k] = sums[part * 2 + k / 4][t][k % 4] * factor;
-                    if (a.accumulate && vec * 8 + k < a.hidden) v[k] += Elem<W>::to_f32(out[vec * 8 + k]);
-                }
-                store_vec<W, 8>(out, vec, a.hidden, v);
-            }
-        }
-    }
 }
 
 // ---------------------------------------------------------------------------
@@ -743,7 +664,7 @@ int side_of(uint64_t rows, uint64_t columns, uint64_t k, uint64_t max_splits)
 struct Layout {
     int score_side, grad_x_side, grad_w_side;
     uint64_t padded, columns, all, piece, pieces, max_splits;
-    uint64_t plan, splits, rows, row_targets, gathered, weight, parts, target_scores, row_loss, held, partial, transposed, total, size;
+    uint64_t plan, splits, rows, row_targets, gathered, weight, parts, target_scores, row_loss, held, partial, total, size;
 
     explicit Layout(const la_linear_loss_t& c)
     {
@@ -761,7 +682,8 @@ struct Layout {
         if (max_splits > kMostSplits) max_splits = kMostSplits;
         if (max_splits == 0) max_splits = 1;
         const uint64_t rows_of_piece = c.n < piece ? c.n : piece;
-        score_side = c.n <= kFewRows ? kTile : side_of(rows_of_piece, c.vocab, c.hidden, 1);
+        // few rows: workgroups of 256 of the matrix's rows where they fill the chip, else of 128
+        score_side = c.n <= kFewRows ? (columns / kTile >= 256 ? 256 : 128) : side_of(rows_of_piece, c.vocab, c.hidden, 1);
         grad_x_side = side_of(rows_of_piece, c.hidden, c.vocab, max_splits);
         grad_w_side = side_of(c.vocab, c.hidden, rows_of_piece, 1);
         uint64_t at = 0;
@@ -781,7 +703,6 @@ struct Layout {
         row_loss = c.row_loss ? 0 : take(c.n * 4);
         held = c.grads ? take(piece * columns * 2) : 0;
         partial = c.grads ? take(max_splits * piece * c.hidden * 4) : 0;
-        transposed = c.grads && c.n <= kFewRows ? take(kFewRows * padded * 2) : 0;
         total = c.grads && pieces > 1 ? take(c.vocab * c.hidden * 4) : 0;
         size = at;
     }
@@ -789,8 +710,9 @@ struct Layout {
 
 template <typename T> int run_scores(const la_linear_loss_t& c, const Layout& l, const ScoreArgs& a, hipStream_t st)
 {
-    if (c.n <= 16) return launch(few_scores_kernel<T, 1>, dim3(a.tiles), dim3(256), st, a);
-    if (c.n <= kFewRows) return launch(few_scores_kernel<T, 4>, dim3(a.tiles), dim3(256), st, a);
+    if (c.n <= kFewRows)
+        return l.score_side == 256 ? launch(few_scores_kernel<T, 4>, dim3(a.tiles), dim3(256), st, a)
+                                   : launch(few_scores_kernel<T, 2>, dim3(a.tiles), dim3(256), st, a);
     const dim3 grid(tile::places(l.piece / l.score_side, a.tiles)), block(tile::kThreads);
     return l.score_side == 128 ? launch(scores_kernel<T, 128>, grid, block, st, a)
                                : launch(scores_kernel<T, 256>, grid, block, st, a);
@@ -828,7 +750,6 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
     float* row_loss = c.row_loss ? c.row_loss : reinterpret_cast<float*>(ws + l.row_loss);
     T* held = c.grads ? reinterpret_cast<T*>(ws + l.held) : nullptr;
     T* grad_x = c.grads ? static_cast<T*>(c.grad_x) : nullptr;
-    T* transposed = c.grads && c.n <= kFewRows ? reinterpret_cast<T*>(ws + l.transposed) : nullptr;
 
     int rc = launch(list_rows_kernel, dim3(1), dim3(1024), st, c.targets, c.n, c.ignore_index, c.vocab, c.mean,
                     c.grad_scale, kHeld<T>, rows, row_targets, plan,
@@ -838,7 +759,7 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
                               static_cast<uint32_t>(l.max_splits)});
     if (rc != LA_OK) return rc;
     rc = launch(gather_kernel<T>, dim3(l.all + c.n), dim3(256), st, static_cast<const T*>(c.x), c.x_stride, c.hidden,
-                l.padded, rows, plan, gathered, l.all, c.targets, c.ignore_index, row_loss, grad_x, c.grad_x_stride, transposed);
+                l.padded, rows, plan, gathered, l.all, c.targets, c.ignore_index, row_loss, grad_x, c.grad_x_stride);
     if (rc != LA_OK) return rc;
     tile::Matrix weight{c.weight, c.vocab, c.hidden, c.weight_stride * 2};
     if (copies_weight(c)) {
@@ -877,14 +798,6 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
         const GradWeightArgs gw{piece_x, d, plan, c.grad_weight,
                                 l.pieces > 1 ? reinterpret_cast<float*>(ws + l.total) : nullptr, c.grad_weight_stride,
                                 first, most, vocab, hidden, 0, 0, c.accumulate};
-        if (transposed) {
-            // runs along the hidden dimension: enough workgroups to fill the chip
-            const uint32_t chunks = ceil_div(hidden, 64u), groups = columns / kTile;
-            const uint32_t wanted = ceil_div(2048u, groups), runs = wanted < chunks ? wanted : chunks;
-            rc = launch(few_grad_weight_kernel<T, W>, dim3(groups * runs), dim3(256), st, gw, transposed, runs);
-            if (rc != LA_OK) return rc;
-            continue;
-        }
         rc = l.grad_w_side == 128 ? run_grad_weight<T, W, 128>(gw, st) : run_grad_weight<T, W, 256>(gw, st);
         if (rc != LA_OK) return rc;
     }
