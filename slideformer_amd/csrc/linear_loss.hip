@@ -322,7 +322,7 @@ __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void 
 // matrix, which goes from memory to registers in the order that the matrix
 // instructions take it, 16 * INNER of its rows a wave; the states come from the caches.
 // Rows of any alignment and width are read where they lie.  13 rows of 128256 x
-// 4096: 241 us (4.4 TB/s), the call 250, with tiles of 128 261; of 60001 x 1023, which
+// 4096: the call 238 us, 4.7 TB/s in this, with tiles of 128 261; of 60001 x 1023, which
 // tiles need a padded copy of, the call 71 us and 102.  From 17 rows on tiles are as
 // fast or faster (40 rows of 128256 x 4096: 268 us, four fragments of rows here 343).
 constexpr uint32_t kFewRows = 16;
@@ -343,12 +343,17 @@ template <typename T, int INNER> __global__ __launch_bounds__(256) void few_scor
                                                (row < a.vocab ? row : a.vocab - 1) * a.weight.stride);
     }
     const T* x = static_cast<const T*>(a.x.data) + (a.first + lane % 16) * (a.x.stride / 2);
+    // workgroups begin at different k: rows a power of two apart would otherwise all
+    // be read from the same few memory channels at a time (251 -> 223 us for one row of
+    // 128256 x 4096)
+    const uint32_t skew = blockIdx.x * 10 % (steps / 2) * 2;
     f32x4 sums[INNER][1] = {};
     u32x4_t w[2][2][INNER], v[2][2];                                 // [buffer][step of the pair]
     const auto load = [&](int b, uint32_t step) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t vec = (step + h) * 4 + lane / 16;
+            const uint32_t at = step + h + skew;
+            const uint32_t vec = (at < steps ? at : at - steps) * 4 + lane / 16;
 #pragma unroll
             for (int s = 0; s < INNER; ++s) w[b][h][s] = load_raw<T>(weight[s], vec, width);
             v[b][h] = *reinterpret_cast<const u32x4_t*>(x + vec * 8);

@@ -39,6 +39,7 @@ namespace tile {
 
 constexpr int kDepth = 32;          // k per step
 constexpr int kThreads = 256;
+constexpr uint32_t kXcds = 8;       // consecutive workgroups go to different ones in turn
 
 template <int SIDE> struct Sizes {
     static constexpr int kPanelBytes = SIDE * kDepth * 2;   // one operand's share of a step
@@ -99,12 +100,18 @@ template <int SIDE, bool BY_ROWS> struct Operand {
     uint64_t at;                    // the next step's corner in memory
     uint64_t left;                  // bytes from there to the matrix's end
     uint64_t stride;                // bytes from step to step
+    uint64_t back;                  // and from the last to the first
+    uint32_t wanted;                // steps in all
     uint32_t steps;                 // with data to read
+    uint32_t k;                     // the next step's place among them
     uint32_t offset[kLoads];        // of this lane's loads
     u32x4_t rsrc;
 
-    __device__ void init(const Matrix& m, uint64_t tile_at, uint64_t k_at, uint32_t wanted)
+    // The product begins at step `begin` and goes round: see Product::run.
+    __device__ void init(const Matrix& m, uint64_t tile_at, uint64_t k_at, uint32_t all, uint32_t begin)
     {
+        wanted = all;
+        k = begin;
         const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x % 64;
         const uint64_t from = BY_ROWS ? tile_at * m.stride + k_at * 2 : k_at * m.stride + tile_at * 2;
         at = reinterpret_cast<uint64_t>(m.data) + from;
@@ -123,21 +130,27 @@ template <int SIDE, bool BY_ROWS> struct Operand {
 #pragma unroll
             for (uint32_t n = 0; n < kLoads; ++n) {
                 constexpr uint32_t kLanes = SIDE / 8;       // to a row
-                const uint32_t k = (n * 4 + wave) * (64 / kLanes) + lane / kLanes;
-                const uint32_t f = (k & 3) | (k >> 3 & 1) << 2;
-                offset[n] = k * static_cast<uint32_t>(m.stride) + (((lane % kLanes / 2) ^ f) * 2 + lane % 2) * 16;
+                const uint32_t row = (n * 4 + wave) * (64 / kLanes) + lane / kLanes;
+                const uint32_t f = (row & 3) | (row >> 3 & 1) << 2;
+                offset[n] = row * static_cast<uint32_t>(m.stride) + (((lane % kLanes / 2) ^ f) * 2 + lane % 2) * 16;
             }
         }
+        back = stride - stride * wanted;
+        at += stride * k;
+        left -= stride * k;
     }
 
-    // Turns to step `step`, the one after the last; one without data reads zeros.
-    __device__ __forceinline__ void turn(uint32_t step)
+    // Turns to the next step, the `turned`-th; one without data reads zeros.
+    __device__ __forceinline__ void turn(uint32_t turned)
     {
         const uint32_t low = static_cast<uint32_t>(left), high = static_cast<uint32_t>(left >> 32);
         rsrc = u32x4_t{static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32),
-                       step < steps ? (high ? 0xffffffffu : low) : 0u, 0x00020000u};
-        at += stride;
-        left -= stride;
+                       turned < wanted && k < steps ? (high ? 0xffffffffu : low) : 0u, 0x00020000u};
+        ++k;
+        const uint64_t by = k == wanted ? back : stride;
+        k = k == wanted ? 0 : k;
+        at += by;
+        left -= by;
     }
 
     // Load `n` of the step, to this wave's place `lds`; returns at once.  Written in
@@ -265,17 +278,22 @@ template <typename T, int SIDE, bool INNER_ROWS, bool OUTER_ROWS> struct Product
     __device__ __forceinline__ void run(const Matrix& inner, uint64_t inner_at, const Matrix& outer, uint64_t outer_at,
                                         uint64_t k_at, uint32_t steps, char* shared, Sums<SIDE>& sums)
     {
-        lds = (lds_char*)shared;
-        place = threadIdx.x / 64 * 1024;
-        load_inner.init(inner, inner_at, k_at, steps);
-        load_outer.init(outer, outer_at, k_at, steps);
-        read_inner.init(wave_inner<SIDE>());
-        read_outer.init(wave_outer<SIDE>());
 #pragma unroll
         for (int s = 0; s < Z::kParts; ++s)
 #pragma unroll
             for (int t = 0; t < Z::kParts; ++t) sums[s][t] = f32x4{0, 0, 0, 0};
         if (steps == 0) return;
+        lds = (lds_char*)shared;
+        place = threadIdx.x / 64 * 1024;
+        // Each XCD begins at an eighth of k of its own: rows a power of two apart would
+        // otherwise all be read from the same few memory channels at a time (200 x 128256 x
+        // 4096, forward: 327 -> 274 us; where operands come from the caches it makes no
+        // difference).  Within an XCD, whose tiles share operands, all go together.
+        const uint32_t begin = blockIdx.x % kXcds * steps / kXcds;
+        load_inner.init(inner, inner_at, k_at, steps, begin);
+        load_outer.init(outer, outer_at, k_at, steps, begin);
+        read_inner.init(wave_inner<SIDE>());
+        read_outer.init(wave_outer<SIDE>());
 #pragma unroll
         for (int ahead = 0; ahead < Z::kAhead; ++ahead) {
             const uint32_t to = __builtin_amdgcn_readfirstlane(
@@ -350,7 +368,6 @@ __device__ __forceinline__ void by_rows(const Sums<SIDE>& sums, char* shared, co
 // The tile that workgroup `id` of a launch computes.  Consecutive workgroups go
 // to different XCDs in turn; each XCD takes a run of consecutive tiles, in bands of
 // `kBand` outer tiles, so that what runs on it together shares operands in its L2.
-constexpr uint32_t kXcds = 8;
 constexpr uint32_t kBand = 4;
 
 struct Place {
