@@ -290,7 +290,7 @@ __device__ __forceinline__ void reduce_scores(const ScoreArgs& a, uint32_t inner
         }
 }
 
-// s = X W^T by tiles, reduced where they are: 3072 x 128256 x 4096 in 2.78 ms, 1.16 PFLOP/s
+// s = X W^T by tiles, reduced where they are: 3072 x 128256 x 4096 in 2.76 ms, 1.17 PFLOP/s
 // with the softmax's part and 790 MB of exp(s - m) written; bound by the matrix
 // cores at the clock that power leaves (1.9 GHz, 55 % of cycles busy) and a start
 // and an end per tile, a sixth of it at k = 4096.
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void 
 // matrix, which goes from memory to registers in the order that the matrix
 // instructions take it, 16 * INNER of its rows a wave; the states come from the caches.
 // Rows of any alignment and width are read where they lie.  13 rows of 128256 x
-// 4096: the call 238 us, 4.7 TB/s in this, with tiles of 128 261; of 60001 x 1023, which
+// 4096: 207 us (5.1 TB/s), the call 220; of 60001 x 1023, which
 // tiles need a padded copy of, the call 71 us and 102.  From 17 rows on tiles are as
 // fast or faster (40 rows of 128256 x 4096: 268 us, four fragments of rows here 343).
 constexpr uint32_t kFewRows = 16;
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const
 // D, in place of exp(s - m)
 // ---------------------------------------------------------------------------
 // Each workgroup joins its row's parts itself, a few KB out of the caches, rather
-// than wait for a launch that does it once.  3072 x 128256: 309 us, 5.1 TB/s, bound by
+// than wait for a launch that does it once.  3072 x 128256: 305 us, 5.2 TB/s, bound by
 // memory.
 constexpr uint32_t kPerGroup = 4;                                // 16-byte vectors per thread
 
@@ -512,7 +512,7 @@ struct GradXArgs {
     uint32_t first, most, hidden, inners, pairs;               // pairs of steps
 };
 
-// D W, W by columns.  3072 x 4096 over k = 128256 in four runs: 2.42 ms, 1.34 PFLOP/s,
+// D W, W by columns.  3072 x 4096 over k = 128256 in four runs: 2.50 ms, 1.29 PFLOP/s,
 // the matrix cores busy 63 % of cycles at 1.9 GHz.
 template <typename T, int SIDE>
 __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void grad_x_kernel(GradXArgs a)

@@ -17,7 +17,7 @@
 //                alone would take as long as the products.
 //   SIDE 128     three workgroups on a compute unit, each in the others' pauses: a
 //                product with few tiles or few steps is made of starts and ends.  Two,
-//                with a step more in LDS, took 1024 x 50257 x 768 370 us instead of 348.
+//                with a step more in LDS, took 1024 x 50257 x 768 369 us instead of 342.
 // What a wave multiplies in one step it reads from LDS during the step before,
 // instruction by instruction between the products, so that neither waits for the
 // other.  Operands go from memory into LDS without passing registers, three or four
