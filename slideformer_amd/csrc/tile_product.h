@@ -34,10 +34,10 @@
 #define SLIDEFORMER_AMD_TILE_PRODUCT_H
 
 #include "ops_common.h"
+#include "tile_range.h"
 
 namespace tile {
 
-constexpr int kDepth = 32;          // k per step
 constexpr int kThreads = 256;
 constexpr uint32_t kXcds = 8;       // consecutive workgroups go to different ones in turn
 
@@ -97,60 +97,26 @@ struct Matrix {
 // One operand's share of a workgroup's work.  BY_ROWS: see above.
 template <int SIDE, bool BY_ROWS> struct Operand {
     static constexpr uint32_t kLoads = Sizes<SIDE>::kLoads;
-    uint64_t at;                    // the next step's corner in memory
-    uint64_t left;                  // bytes from there to the matrix's end
-    uint64_t stride;                // bytes from step to step
-    uint64_t back;                  // and from the last to the first
-    uint32_t wanted;                // steps in all
-    uint32_t steps;                 // with data to read
-    uint32_t k;                     // the next step's place among them
+    Walk walk;                      // in addresses
     uint32_t offset[kLoads];        // of this lane's loads
     u32x4_t rsrc;
 
     // The product begins at step `begin` and goes round: see Product::run.
     __device__ void init(const Matrix& m, uint64_t tile_at, uint64_t k_at, uint32_t all, uint32_t begin)
     {
-        wanted = all;
-        k = begin;
-        const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-        const uint64_t from = BY_ROWS ? tile_at * m.stride + k_at * 2 : k_at * m.stride + tile_at * 2;
-        at = reinterpret_cast<uint64_t>(m.data) + from;
-        left = (m.count - 1) * m.stride + m.width * 2 - from;
-        if constexpr (BY_ROWS) {
-            stride = kDepth * 2;
-            steps = wanted;
+        walk.init(BY_ROWS, m.count, m.width, m.stride, tile_at, k_at, all, begin);
+        walk.at += reinterpret_cast<uint64_t>(m.data);
 #pragma unroll
-            for (uint32_t n = 0; n < kLoads; ++n)
-                offset[n] = (n * 64 + wave * 16 + lane / 4) * static_cast<uint32_t>(m.stride) +
-                            ((lane % 4) ^ (lane / 8 % 4)) * 16;
-        } else {
-            stride = kDepth * m.stride;
-            const uint64_t there = m.count > k_at ? (m.count - k_at + kDepth - 1) / kDepth : 0;
-            steps = there < wanted ? static_cast<uint32_t>(there) : wanted;
-#pragma unroll
-            for (uint32_t n = 0; n < kLoads; ++n) {
-                constexpr uint32_t kLanes = SIDE / 8;       // to a row
-                const uint32_t row = (n * 4 + wave) * (64 / kLanes) + lane / kLanes;
-                const uint32_t f = (row & 3) | (row >> 3 & 1) << 2;
-                offset[n] = row * static_cast<uint32_t>(m.stride) + (((lane % kLanes / 2) ^ f) * 2 + lane % 2) * 16;
-            }
-        }
-        back = stride - stride * wanted;
-        at += stride * k;
-        left -= stride * k;
+        for (uint32_t n = 0; n < kLoads; ++n)
+            offset[n] = load_offset(SIDE, BY_ROWS, n, threadIdx.x / 64, threadIdx.x % 64, static_cast<uint32_t>(m.stride));
     }
 
     // Turns to the next step, the `turned`-th; one without data reads zeros.
     __device__ __forceinline__ void turn(uint32_t turned)
     {
-        const uint32_t low = static_cast<uint32_t>(left), high = static_cast<uint32_t>(left >> 32);
-        rsrc = u32x4_t{static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32),
-                       turned < wanted && k < steps ? (high ? 0xffffffffu : low) : 0u, 0x00020000u};
-        ++k;
-        const uint64_t by = k == wanted ? back : stride;
-        k = k == wanted ? 0 : k;
-        at += by;
-        left -= by;
+        rsrc = u32x4_t{static_cast<uint32_t>(walk.at), static_cast<uint32_t>(walk.at >> 32), walk.range(turned),
+                       0x00020000u};
+        walk.turn();
     }
 
     // Load `n` of the step, to this wave's place `lds`; returns at once.  Written in
