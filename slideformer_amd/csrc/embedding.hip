@@ -321,49 +321,99 @@ template <typename T, typename O> __global__ __launch_bounds__(256) void join_ru
     write_row<O, E>(static_cast<O*>(a.weight), key, a.weight_stride, vec, hidden, a.scale, a.accumulate, sum);
 }
 
-// Up to kFewTokens tokens need no sorting: a wave a row of the matrix, each looks
-// through all of them for its own.  One launch for four: 7 tokens of 23587 x 1600
-// fp32 28 us, sorted 34 us; 250 of 2000 x 512 7.5 and 17 us.
+// Up to kFewTokens tokens need no sorting: each wave looks through all of them.  The
+// first `groups` workgroups have one for each token and slice of its row, which sums
+// all rows of the token's where it is its first occurrence: wave k those among tokens
+// 64 k to 64 k + 63, in order, kTogether of them in flight at a time; the waves' sums are
+// added in order too.  The other workgroups have a wave for each row of the
+// matrix, which clears it where no token is its own.  One launch for four: 7
+// tokens of 23587 x 1600 fp32 27 us, sorted 34; 250 of 2000 x 512 5.4 and 13 us; 256 equal
+// ones of 1000 x 4096 bf16 10 and 16 us (340 by one wave, a row after the other).
 constexpr uint32_t kFewTokens = 256;
+constexpr int kTogether = 16;
 
-template <typename T, typename O, typename I>
-__global__ __launch_bounds__(256) void few_tokens_kernel(const I* tokens, uint32_t n, int64_t padding, const T* grad,
-                                                         uint64_t grad_stride, O* weight, uint64_t vocab,
-                                                         uint32_t hidden, uint64_t weight_stride, float scale)
+// Which of the tokens are `row`, as bits; returns whether any is.
+template <typename I>
+__device__ __forceinline__ bool find(const I* tokens, uint32_t n, uint64_t row, uint64_t (&mine)[kFewTokens / kWave])
 {
-    constexpr int E = Elem<T>::kCount;
-    const uint64_t row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / kWave);
-    if (row >= vocab) return;
-    const uint32_t lane = threadIdx.x % kWave;
-    uint64_t mine[kFewTokens / kWave], any = 0;
+    uint64_t any = 0;
 #pragma unroll
     for (uint32_t k = 0; k < kFewTokens / kWave; ++k) {
         mine[k] = 0;
         if (k * kWave < n) {
-            const uint32_t at = k * kWave + lane;
+            const uint32_t at = k * kWave + threadIdx.x % kWave;
             mine[k] = __ballot(at < n && token_at(tokens, at < n ? at : 0) == row);
         }
         any |= mine[k];
     }
-    O* to = weight + row * weight_stride;
-    if (!any || row == static_cast<uint64_t>(padding)) {
-        clear_row(to, hidden);
+    return any != 0;
+}
+
+template <typename T, typename O, typename I>
+__global__ __launch_bounds__(256) void few_tokens_kernel(const I* tokens, uint32_t n, int64_t padding, const T* grad,
+                                                         uint64_t grad_stride, O* weight, uint64_t vocab,
+                                                         uint32_t hidden, uint64_t weight_stride, float scale,
+                                                         uint32_t slices, uint32_t groups)
+{
+    constexpr int E = Elem<T>::kCount;
+    uint64_t mine[kFewTokens / kWave];
+    if (blockIdx.x >= groups) {
+        const uint64_t row = __builtin_amdgcn_readfirstlane((blockIdx.x - groups) * 4 + threadIdx.x / kWave);
+        if (row < vocab && (!find(tokens, n, row, mine) || row == static_cast<uint64_t>(padding)))
+            clear_row(weight + row * weight_stride, hidden);
         return;
     }
-    for (uint32_t vec = lane; vec * E < hidden; vec += kWave) {
-        float sum[E] = {};
+    __shared__ float lds[kFewTokens / kWave][E][kWave];
+    const uint32_t own = blockIdx.x / slices, lane = threadIdx.x % kWave;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t vec = blockIdx.x % slices * kWave + lane;
+    const uint64_t row = token_at(tokens, own);
+    if (row >= vocab || row == static_cast<uint64_t>(padding)) return;
+    find(tokens, n, row, mine);
+    uint32_t first = kFewTokens, waves = 0;                         // that have rows of this token
 #pragma unroll
-        for (uint32_t k = 0; k < kFewTokens / kWave; ++k)
-            for (uint64_t left = mine[k]; left; left &= left - 1) {
-                float x[E];
-                load_vec<T>(grad + (k * kWave + __builtin_ctzll(left)) * grad_stride, vec, hidden, x);
+    for (uint32_t k = 0; k < kFewTokens / kWave; ++k)
+        if (mine[k]) {
+            if (first == kFewTokens) first = k * kWave + __builtin_ctzll(mine[k]);
+            ++waves;
+        }
+    if (first != own) return;                                       // the whole workgroup
+    uint64_t left = 0;
 #pragma unroll
-                for (int e = 0; e < E; ++e) sum[e] += x[e];
+    for (uint32_t k = 0; k < kFewTokens / kWave; ++k)
+        if (k == wave) left = mine[k];
+    float sum[E] = {};
+    while (left) {
+        u32x4_t x[kTogether];
+        const int count = __builtin_popcountll(left);
+#pragma unroll
+        for (int f = 0; f < kTogether; ++f)
+            if (f < count) {
+                x[f] = load_raw<T>(grad + (wave * kWave + __builtin_ctzll(left)) * grad_stride, vec, hidden);
+                left &= left - 1;
             }
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] *= scale;
-        store_vec<O, E>(to, vec, hidden, sum);
+        for (int f = 0; f < kTogether; ++f)
+            if (f < count) {
+                float g[E];
+                Elem<T>::unpack(x[f], g);
+#pragma unroll
+                for (int e = 0; e < E; ++e) sum[e] += g[e];
+            }
     }
+    if (waves > 1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) lds[wave][e][lane] = sum[e];
+        __syncthreads();
+        if (wave == own / kWave)
+            for (uint32_t k = wave + 1; k < kFewTokens / kWave; ++k)
+#pragma unroll
+                for (int e = 0; e < E; ++e) sum[e] += lds[k][e][lane];
+    }
+    if (wave != own / kWave || vec * E >= hidden) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] *= scale;
+    store_vec<O, E>(weight + row * weight_stride, vec, hidden, sum);
 }
 
 // ---------------------------------------------------------------------------
@@ -442,11 +492,12 @@ template <typename I> int sort(const GradCall& c, const Workspace& w)
 
 template <typename T, typename O, typename I> int few_tokens(const GradCall& c)
 {
-    const uint64_t grid = ceil_div(c.vocab, 4);
-    if (grid > kMaxGrid) return LA_EINVAL;
-    return launch(few_tokens_kernel<T, O, I>, dim3(grid), dim3(256), c.st, static_cast<const I*>(c.tokens), c.n,
-                  c.padding, static_cast<const T*>(c.grad), c.grad_stride, static_cast<O*>(c.weight), c.vocab, c.hidden,
-                  c.weight_stride, c.scale);
+    const uint64_t slices = ceil_div(c.hidden, kWave * Elem<T>::kCount);
+    const uint64_t groups = c.n * slices, clear = ceil_div(c.vocab, 4);
+    if (groups + clear > kMaxGrid) return LA_EINVAL;
+    return launch(few_tokens_kernel<T, O, I>, dim3(groups + clear), dim3(256), c.st, static_cast<const I*>(c.tokens),
+                  c.n, c.padding, static_cast<const T*>(c.grad), c.grad_stride, static_cast<O*>(c.weight), c.vocab,
+                  c.hidden, c.weight_stride, c.scale, slices, groups);
 }
 
 template <typename T, typename O> int grad(const GradCall& c)
