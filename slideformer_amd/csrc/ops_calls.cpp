@@ -15,6 +15,7 @@
 
 #include <Python.h>
 
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ops/empty.h>
@@ -105,6 +106,14 @@ PyObject* none()
     Py_RETURN_NONE;
 }
 
+// The Python error of the exception in flight, torch's own types among them (what an
+// allocation raises where memory runs out).
+PyObject* failed()
+{
+    torch::translate_exception_to_python(std::current_exception());
+    return nullptr;
+}
+
 PyObject* code(int rc) { return PyLong_FromLong(rc); }
 
 PyObject* wrap(const at::Tensor& t) { return THPVariable_Wrap(t); }
@@ -159,9 +168,8 @@ try {
                      stream);
     Py_END_ALLOW_THREADS
     return rc ? code(rc) : wrap(out);
-} catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+} catch (const std::exception&) {
+    return failed();
 }
 
 // embedding_grad(tokens, grad_out, grad_weight, scale, padding_idx, accumulate, device, stream)
@@ -193,9 +201,8 @@ try {
                           static_cast<float>(scale), padding, accumulate, ws, bytes, stream);
     Py_END_ALLOW_THREADS
     return rc ? code(rc) : again(a[2]);
-} catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+} catch (const std::exception&) {
+    return failed();
 }
 
 // rms_norm(x, weight, eps, residual, device, stream) and
@@ -235,17 +242,15 @@ PyObject* norm(PyObject* const* a, bool eight, bool float8, PyObject* device, Py
 PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t count)
 try {
     return count == 6 ? norm(a, false, false, a[4], a[5]) : none();
-} catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+} catch (const std::exception&) {
+    return failed();
 }
 
 PyObject* rms_norm_8bit(PyObject*, PyObject* const* a, Py_ssize_t count)
 try {
     return count == 7 ? norm(a, true, PyObject_IsTrue(a[4]), a[5], a[6]) : none();
-} catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+} catch (const std::exception&) {
+    return failed();
 }
 
 // rms_norm_grad(grad_out, summed, rstd, weight, grad_summed, grad_weight, accumulate, device, stream)
@@ -284,9 +289,8 @@ try {
     Py_END_ALLOW_THREADS
     if (rc) return code(rc);
     return tuple({wrap(grad_x), fresh ? wrap(grad_weight) : again(a[5])});
-} catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+} catch (const std::exception&) {
+    return failed();
 }
 
 // bind(addresses of the six functions above, in the order of their pointers)
