@@ -81,11 +81,19 @@ constexpr uint32_t kMostSplits = 64;
 // the trained rows
 // ---------------------------------------------------------------------------
 // What the states' gradient needs decided once the rows are known: in how many runs
-// of k each piece is taken.
+// of k each piece is taken, whose partial sums have `room` floats.
 struct SplitArgs {
     uint32_t* splits;               // [pieces], null without gradients
+    uint64_t room;
     uint32_t pieces, most, hidden, steps, side, max_splits;
 };
+
+// How many runs of k `rows` rows may take.
+__host__ __device__ __forceinline__ uint32_t runs_in(uint64_t room, uint64_t rows, uint64_t hidden, uint32_t max_splits)
+{
+    const uint64_t fit = rows > 0 ? room / (rows * hidden) : max_splits;
+    return fit < max_splits ? static_cast<uint32_t>(fit) : max_splits;
+}
 
 // One workgroup (the list is in order, and 8192 targets are one trip: 5 us) lists the rows whose target is not `ignore`, in order.
 constexpr uint32_t kListed = 8;                                  // targets per thread and trip
@@ -138,7 +146,7 @@ __global__ __launch_bounds__(1024) void list_rows_kernel(const int64_t* targets,
         const uint32_t first = p * split.most;
         const uint32_t piece = done <= first ? 0 : done - first < split.most ? done - first : split.most;
         const uint32_t tiles = ceil_div(piece, split.side) * ceil_div(split.hidden, split.side);
-        float least = lane < split.max_splits
+        float least = lane < runs_in(split.room, piece, split.hidden, split.max_splits)
                           ? product_us(split.side, tiles, split.steps, lane + 1, 4.0f * piece * split.hidden)
                           : 3.0e38f;
         uint32_t best = lane + 1;
@@ -507,7 +515,7 @@ struct GradXArgs {
     tile::Matrix weight, held;
     const Plan* plan;
     const uint32_t* rows;
-    float* partial;                 // [splits][rows of the piece][hidden]
+    float* partial;                 // [splits][trained rows of the piece][hidden]
     const uint32_t* splits;         // runs of k of this piece
     uint32_t first, most, hidden, inners, pairs;               // pairs of steps
 };
@@ -530,7 +538,7 @@ __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void 
     tile::Sums<SIDE> sums;
     tile::product<T, SIDE, false, true>(a.weight, at.inner * SIDE, a.held, outer * SIDE,
                                         static_cast<uint64_t>(from) * tile::kDepth, to - from, lds, sums);
-    float* partial = a.partial + (static_cast<uint64_t>(split) * a.most + outer * SIDE) * a.hidden;
+    float* partial = a.partial + (static_cast<uint64_t>(split) * rows + outer * SIDE) * a.hidden;
     tile::by_rows<SIDE>(sums, lds, [&](uint32_t row, uint32_t inner, const float(&v)[8]) {
         if (outer * SIDE + row < rows)
             store_vec<float, 8>(partial + static_cast<uint64_t>(row) * a.hidden, (at.inner * SIDE + inner) / 8,
@@ -556,7 +564,7 @@ __global__ __launch_bounds__(256) void join_grad_x_kernel(GradXArgs a, T* grad_x
         float sum[8] = {};
 #pragma unroll 4
         for (uint32_t k = 0; k < splits; ++k) {
-            const float* partial = a.partial + (static_cast<uint64_t>(k) * a.most + row) * a.hidden;
+            const float* partial = a.partial + (static_cast<uint64_t>(k) * rows + row) * a.hidden;
             float lo[4], hi[4];
             load_vec<float>(partial, vec * 2, a.hidden, lo);
             load_vec<float>(partial, vec * 2 + 1, a.hidden, hi);
@@ -668,7 +676,7 @@ int side_of(uint64_t rows, uint64_t columns, uint64_t k, uint64_t max_splits)
 // Sizes and the workspace's parts (offsets in bytes).
 struct Layout {
     int score_side, grad_x_side, grad_w_side;
-    uint64_t padded, columns, all, piece, pieces, max_splits;
+    uint64_t padded, columns, all, piece, pieces, max_splits, room;
     uint64_t plan, splits, rows, row_targets, gathered, weight, parts, target_scores, row_loss, held, partial, total, size;
 
     explicit Layout(const la_linear_loss_t& c)
@@ -680,16 +688,21 @@ struct Layout {
         if (piece > kMostRows) piece = kMostRows;
         if (piece == 0 || piece > all) piece = all;
         pieces = ceil_div(all, piece);
-        // partial sums of the states' gradient take at most the memory of a piece's D, or 64 MiB
-        const uint64_t partials = piece * columns * 2 > (64u << 20) ? piece * columns * 2 : 64u << 20;
-        max_splits = partials / (piece * c.hidden * 4);
+        // As many runs of k as would take the memory of a piece's D, or the 64 MiB of one round of large tiles, if
+        // all its rows were trained.  Their partial sums have half of that, of one run at the least: the full
+        // rows' tiles fill the chip in few runs, and fewer rows have room for more.
+        const uint64_t one = piece * c.hidden, most = piece * columns / 2;
+        max_splits = (most > (16u << 20) ? most : 16u << 20) / one;
         if (max_splits > columns / kTile) max_splits = columns / kTile;
         if (max_splits > kMostSplits) max_splits = kMostSplits;
         if (max_splits == 0) max_splits = 1;
+        room = most / 2 > (16u << 20) ? most / 2 : 16u << 20;
+        if (room > max_splits * one) room = max_splits * one;
+        if (room < one) room = one;
         const uint64_t rows_of_piece = c.n < piece ? c.n : piece;
         // few rows: workgroups of 256 of the matrix's rows where they fill the chip, else of 128
         score_side = c.n <= kFewRows ? (columns / kTile >= 256 ? 256 : 128) : side_of(rows_of_piece, c.vocab, c.hidden, 1);
-        grad_x_side = side_of(rows_of_piece, c.hidden, c.vocab, max_splits);
+        grad_x_side = side_of(rows_of_piece, c.hidden, c.vocab, runs_in(room, rows_of_piece, c.hidden, max_splits));
         grad_w_side = side_of(c.vocab, c.hidden, rows_of_piece, 1);
         uint64_t at = 0;
         const auto take = [&](uint64_t bytes) {
@@ -707,7 +720,7 @@ struct Layout {
         target_scores = take(piece * 4);
         row_loss = c.row_loss ? 0 : take(c.n * 4);
         held = c.grads ? take(piece * columns * 2) : 0;
-        partial = c.grads ? take(max_splits * piece * c.hidden * 4) : 0;
+        partial = c.grads ? take(room * 4) : 0;
         total = c.grads && pieces > 1 ? take(c.vocab * c.hidden * 4) : 0;
         size = at;
     }
@@ -727,8 +740,11 @@ template <typename T, int SIDE>
 int run_grad_x(const la_linear_loss_t& c, const Layout& l, GradXArgs a, const float* row_loss, hipStream_t st)
 {
     a.inners = ceil_div(a.hidden, SIDE);
-    const int rc = launch(grad_x_kernel<T, SIDE>, dim3(tile::places(l.piece / SIDE * l.max_splits, a.inners)),
-                          dim3(tile::kThreads), st, a);
+    // rows in whole tiles times runs: rows times runs are bounded by the partial sums' room, each run's last tile is partial
+    uint64_t outers = l.room / (a.hidden * static_cast<uint64_t>(SIDE)) + l.max_splits;
+    if (outers > l.piece / SIDE * l.max_splits) outers = l.piece / SIDE * l.max_splits;
+    const int rc =
+        launch(grad_x_kernel<T, SIDE>, dim3(tile::places(outers, a.inners)), dim3(tile::kThreads), st, a);
     if (rc != LA_OK) return rc;
     const bool last = a.first + l.piece >= l.all;
     return launch(join_grad_x_kernel<T>, dim3(l.piece + (last && c.loss ? 1 : 0)), dim3(256), st, a,
@@ -758,7 +774,7 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
 
     int rc = launch(list_rows_kernel, dim3(1), dim3(1024), st, c.targets, c.n, c.ignore_index, c.vocab, c.mean,
                     c.grad_scale, kHeld<T>, rows, row_targets, plan,
-                    SplitArgs{c.grads ? splits : nullptr, static_cast<uint32_t>(l.pieces),
+                    SplitArgs{c.grads ? splits : nullptr, l.room, static_cast<uint32_t>(l.pieces),
                               static_cast<uint32_t>(l.piece), static_cast<uint32_t>(c.hidden),
                               static_cast<uint32_t>(l.columns / tile::kDepth), static_cast<uint32_t>(l.grad_x_side),
                               static_cast<uint32_t>(l.max_splits)});

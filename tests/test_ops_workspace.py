@@ -1,0 +1,39 @@
+"""How much memory the loss with gradients takes beside its operands, and what it is made of.
+Sizes come from the library; nothing is launched."""
+from __future__ import annotations
+
+import ctypes
+
+from slideformer_amd import _lib, _ops_lib
+
+MIB = 1 << 20
+
+
+def _bytes(n, vocab, hidden, piece_bytes, grad_weight=_lib.LA_BF16):
+    """The workspace of a call as linear_cross_entropy_grad makes it."""
+    call = _ops_lib.LaLinearLoss(
+        dtype=_lib.LA_BF16, n=n, hidden=hidden, x_stride=hidden, weight=256, vocab=vocab, weight_stride=hidden,
+        grads=1, grad_x_stride=hidden, grad_weight_dtype=grad_weight, grad_weight_stride=hidden,
+        piece_rows=min(max(256, piece_bytes // (2 * vocab) // 256 * 256), 1 << 22))
+    return _ops_lib.load().la_linear_loss_workspace(ctypes.byref(call))
+
+
+def _up(x, to):
+    return -(-x // to) * to
+
+
+def _parts(n, vocab, hidden, rows):
+    """(softmax of `rows` rows in 16 bits, what all of a call's other buffers but the partial and running sums take
+    at most: the gathered states, a part of each row for 128 columns at the least, and lists)."""
+    columns = _up(vocab, 256)
+    return rows * columns * 2, _up(n, 256) * (_up(hidden, 64) * 2 + 32) + rows * (columns // 128 * 8 + 8) + MIB
+
+
+def test_partial_sums_take_half_of_the_softmax():
+    """The sums of the states' gradient over runs of k: at most half of the softmax in 16 bits, or 64 MiB, or one
+    run."""
+    for n, vocab, hidden in ((4096, 128256, 4096), (2048, 128256, 8192), (1024, 50257, 768), (4096, 32000, 4096),
+                             (4096, 1000, 4096), (300, 700, 64)):
+        softmax, others = _parts(n, vocab, hidden, _up(n, 256))
+        sums = max(softmax // 2, 64 * MIB, _up(n, 256) * hidden * 4)
+        assert _bytes(n, vocab, hidden, 1 << 40) <= softmax + sums + others, (n, vocab, hidden)
