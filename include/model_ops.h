@@ -97,7 +97,7 @@ int la_rms_norm_grad(int dtype, const void* grad_out, uint64_t grad_out_stride, 
  * The scores are never held as a whole: without gradients a tile of them at a
  * time, with gradients the softmax of piece_rows rows at a time (rounded up to a
  * multiple of 256; 0: of all).  Where that takes more than one piece, grad_weight is summed
- * in fp32 in the workspace.
+ * in fp32: where it lies if it is of fp32, else in the workspace.
  * workspace: la_linear_loss_workspace(call) bytes, 256-byte aligned.
  */
 typedef struct {

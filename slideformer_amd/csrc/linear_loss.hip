@@ -584,7 +584,8 @@ struct GradWeightArgs {
     tile::Matrix x, held;
     const Plan* plan;
     void* grad_weight;
-    float* total;                   // [vocab][hidden] where the rows take more than one piece, else null
+    float* total;                   // [vocab][hidden] where the rows take more than one piece and
+                                    // grad_weight cannot hold their sum, being of 16 bits; else null
     uint64_t stride;
     uint32_t first, most, vocab, hidden, inners, outers;
     int accumulate;
@@ -603,6 +604,7 @@ __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void 
     tile::Sums<SIDE> sums;
     tile::product<T, SIDE, false, false>(a.x, at.inner * SIDE, a.held, at.outer * SIDE, 0,
                                          ceil_div(rows, 2 * tile::kDepth) * 2, lds, sums);
+    constexpr bool kHoldsSum = __is_same(W, float);                  // over the pieces, without a buffer beside it
     const bool last = a.first + rows >= a.plan->rows;
     const float factor = a.plan->factor;
     tile::by_rows<SIDE>(sums, lds, [&](uint32_t outer, uint32_t inner, const float(&sum)[8]) {
@@ -611,19 +613,21 @@ __global__ __launch_bounds__(tile::kThreads, tile::Sizes<SIDE>::kResident) void 
         float v[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = sum[k];
-        float* total = a.total + static_cast<uint64_t>(row) * a.hidden;
-        if (a.first > 0)
+        if constexpr (!kHoldsSum) {
+            float* total = a.total + static_cast<uint64_t>(row) * a.hidden;
+            if (a.first > 0)
 #pragma unroll
-            for (uint32_t k = 0; k < 8; ++k)
-                if (vec * 8 + k < a.hidden) v[k] += total[vec * 8 + k];
-        if (!last) {
-            store_vec<float, 8>(total, vec, a.hidden, v);
-            return;
+                for (uint32_t k = 0; k < 8; ++k)
+                    if (vec * 8 + k < a.hidden) v[k] += total[vec * 8 + k];
+            if (!last) {
+                store_vec<float, 8>(total, vec, a.hidden, v);
+                return;
+            }
         }
         W* out = static_cast<W*>(a.grad_weight) + row * a.stride;
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] *= factor;
-        if (a.accumulate)
+        if (a.accumulate || (kHoldsSum && a.first > 0))
 #pragma unroll
             for (uint32_t k = 0; k < 8; ++k)
                 if (vec * 8 + k < a.hidden) v[k] += Elem<W>::to_f32(out[vec * 8 + k]);
@@ -721,7 +725,7 @@ struct Layout {
         row_loss = c.row_loss ? 0 : take(c.n * 4);
         held = c.grads ? take(piece * columns * 2) : 0;
         partial = c.grads ? take(room * 4) : 0;
-        total = c.grads && pieces > 1 ? take(c.vocab * c.hidden * 4) : 0;
+        total = c.grads && pieces > 1 && c.grad_weight_dtype != LA_F32 ? take(c.vocab * c.hidden * 4) : 0;
         size = at;
     }
 };
@@ -817,7 +821,7 @@ template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, h
         const tile::Matrix piece_x{gathered + first * l.padded, l.piece < l.all - first ? l.piece : l.all - first,
                                    l.padded, l.padded * 2};
         const GradWeightArgs gw{piece_x, d, plan, c.grad_weight,
-                                l.pieces > 1 ? reinterpret_cast<float*>(ws + l.total) : nullptr, c.grad_weight_stride,
+                                l.total ? reinterpret_cast<float*>(ws + l.total) : nullptr, c.grad_weight_stride,
                                 first, most, vocab, hidden, 0, 0, c.accumulate};
         rc = l.grad_w_side == 128 ? run_grad_weight<T, W, 128>(gw, st) : run_grad_weight<T, W, 256>(gw, st);
         if (rc != LA_OK) return rc;

@@ -37,3 +37,10 @@ def test_partial_sums_take_half_of_the_softmax():
         softmax, others = _parts(n, vocab, hidden, _up(n, 256))
         sums = max(softmax // 2, 64 * MIB, _up(n, 256) * hidden * 4)
         assert _bytes(n, vocab, hidden, 1 << 40) <= softmax + sums + others, (n, vocab, hidden)
+
+
+def test_an_fp32_gradient_is_its_own_sum_over_pieces():
+    """A grad_weight in fp32 holds the sum over the pieces itself: no second matrix beside it."""
+    n, vocab, hidden = 8192, 128256, 4096
+    softmax, others = _parts(n, vocab, hidden, 1024)
+    assert _bytes(n, vocab, hidden, 1024 * 2 * vocab, _lib.LA_F32) <= softmax * 3 // 2 + others
