@@ -94,10 +94,12 @@ int la_rms_norm_grad(int dtype, const void* grad_out, uint64_t grad_out_stride, 
  * With grads != 0 also grad_x = d loss / d x and grad_weight = (accumulate ?
  * grad_weight : 0) + d loss / d weight, both times *grad_scale (nullable: 1).
  * dtype (of x, weight, grad_x): LA_BF16 or LA_F16; grad_weight: that type or LA_F32.
- * The scores are never held as a whole: without gradients a tile of them at a
- * time, with gradients the softmax of piece_rows rows at a time (rounded up to a
- * multiple of 256; 0: of all).  Where that takes more than one piece, grad_weight is summed
- * in fp32: where it lies if it is of fp32, else in the workspace.
+ * Without gradients a tile of scores is held at a time.  With gradients the
+ * softmax of piece_rows rows is held in 16 bits at a time (rounded up to a multiple of
+ * 256; 0: of all), and up to half as much again or 64 MiB of partial sums of
+ * grad_x.  Where the rows take more than one piece, grad_weight is summed in
+ * fp32: where it lies if it is of fp32, else in the workspace; where that would take more
+ * memory than the softmax of all rows, all rows are one piece.
  * workspace: la_linear_loss_workspace(call) bytes, 256-byte aligned.
  */
 typedef struct {

@@ -1,5 +1,6 @@
 // slideformer_amd: softmax cross entropy of hidden states against a vocabulary
-// matrix, with its gradients, without the scores ever being held (gfx950, wave64).
+// matrix, with its gradients (gfx950, wave64).  The loss holds one tile of scores at a
+// time; with gradients the softmax of a piece of the rows is held, in 16 bits.
 //
 //   s = X W^T,  loss_i = log(sum_v exp(s_iv)) - s_i,t(i),
 //   D_iv = exp(s_iv) / sum_v exp(s_iv) - [v = t(i)],  dX = D W,  dW = D^T X.
@@ -683,12 +684,12 @@ struct Layout {
     uint64_t padded, columns, all, piece, pieces, max_splits, room;
     uint64_t plan, splits, rows, row_targets, gathered, weight, parts, target_scores, row_loss, held, partial, total, size;
 
-    explicit Layout(const la_linear_loss_t& c)
+    Layout(const la_linear_loss_t& c, uint64_t piece_rows)
     {
         padded = ceil_div(c.hidden, kPair) * kPair;
         columns = ceil_div(c.vocab, kTile) * kTile;
         all = c.n > 0 ? ceil_div(c.n, kTile) * kTile : kTile;     // no rows: one empty piece, which clears grad_weight
-        piece = ceil_div(c.grads ? c.piece_rows : kForwardRows, kTile) * kTile;
+        piece = ceil_div(piece_rows, kTile) * kTile;
         if (piece > kMostRows) piece = kMostRows;
         if (piece == 0 || piece > all) piece = all;
         pieces = ceil_div(all, piece);
@@ -730,6 +731,16 @@ struct Layout {
     }
 };
 
+// The sum over pieces, where grad_weight cannot hold it, can take more than the pieces
+// save: all rows are one piece where that takes no more memory.
+Layout layout_of(const la_linear_loss_t& c)
+{
+    const Layout asked(c, c.grads ? c.piece_rows : kForwardRows);
+    if (asked.total == 0 || asked.all > kMostRows) return asked;
+    const Layout whole(c, asked.all);
+    return whole.size <= asked.size ? whole : asked;
+}
+
 template <typename T> int run_scores(const la_linear_loss_t& c, const Layout& l, const ScoreArgs& a, hipStream_t st)
 {
     if (c.n <= kFewRows)
@@ -764,7 +775,7 @@ template <typename T, typename W, int SIDE> int run_grad_weight(GradWeightArgs a
 
 template <typename T, typename W> int run(const la_linear_loss_t& c, char* ws, hipStream_t st)
 {
-    const Layout l(c);
+    const Layout l = layout_of(c);
     Plan* plan = reinterpret_cast<Plan*>(ws + l.plan);
     uint32_t* splits = reinterpret_cast<uint32_t*>(ws + l.splits);
     uint32_t* rows = reinterpret_cast<uint32_t*>(ws + l.rows);
@@ -838,7 +849,7 @@ extern "C" {
 
 uint64_t la_linear_loss_workspace(const la_linear_loss_t* call)
 {
-    return call && sizes_ok(*call) ? Layout(*call).size : 0;
+    return call && sizes_ok(*call) ? layout_of(*call).size : 0;
 }
 
 int la_linear_loss(const la_linear_loss_t* call, void* workspace, uint64_t workspace_bytes, la_stream_t stream)
@@ -858,7 +869,7 @@ int la_linear_loss(const la_linear_loss_t* call, void* workspace, uint64_t works
         if (rc == LA_OK) rc = check_matrix(c.grad_weight, c.grad_weight_dtype, c.hidden, c.grad_weight_stride);
         if (rc == LA_OK && c.grad_scale) rc = check_matrix(c.grad_scale, LA_F32, 1, 1);
     }
-    if (rc == LA_OK) rc = check_workspace(workspace, workspace_bytes, Layout(c).size, 256);
+    if (rc == LA_OK) rc = check_workspace(workspace, workspace_bytes, layout_of(c).size, 256);
     if (rc != LA_OK) return rc;
     if (!reachable(workspace) || !reachable(c.weight) || (c.n > 0 && (!reachable(c.x) || !reachable(c.targets))) ||
         !reachable(c.loss) || !reachable(c.row_loss) ||

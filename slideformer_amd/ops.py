@@ -5,7 +5,8 @@ steps: the embedding matrix, the norms, and the vocabulary matrix with the loss.
 
 ``embedding`` / ``embedding_grad``            rows of a matrix by token, and the matrix's gradient
 ``rms_norm`` / ``rms_norm_8bit`` / ``rms_norm_grad``   the residual's addition and the norm over it
-``linear_cross_entropy`` / ``linear_cross_entropy_grad``  the loss, without the scores ever being held
+``linear_cross_entropy`` / ``linear_cross_entropy_grad``  the loss, a tile of scores at a time; with its gradients,
+                                              a piece of the rows' softmax at a time
 
 Gradients are explicit calls, as a layer-by-layer runtime makes them: each writes
 into the tensor that the optimizer reads, a slice of a flat grad buffer for
@@ -38,7 +39,7 @@ _TOKEN = {torch.int32: _ops_lib.LA_I32, torch.int64: _ops_lib.LA_I64}
 _EIGHT = {torch.int8: _ops_lib.LA_I8, torch.float8_e4m3fn: _ops_lib.LA_F8E4M3}
 
 # How much memory linear_cross_entropy_grad takes by default for the softmax of the
-# rows it works on at a time: 1 GiB, 4096 rows of a 128256-token vocabulary.
+# rows it works on at a time, in 16 bits: 1 GiB, 4096 rows of a 128256-token vocabulary.
 PIECE_BYTES = 1 << 30
 
 
@@ -357,8 +358,12 @@ def linear_cross_entropy_grad(x: torch.Tensor, weight: torch.Tensor, targets: to
     both gradients, not the loss (a loss scale, or one over the micro-batches).
     ``grad_weight``: the matrix to write (weight's type or float32; new by default), added to
     with ``accumulate``.  ``piece_bytes``: about how much memory the softmax of the rows in
-    work may take (at least 256 rows); where not all rows fit, grad_weight is summed over the
-    pieces in fp32, which takes 4 bytes an element and two passes over it a piece."""
+    work may take, in 16 bits (at least 256 rows).  Beside it the call takes up to half as much
+    again (or 64 MiB, or hidden fp32 values for each of these rows, if that is more) for partial
+    sums of grad_x, and a copy of the trained rows of x.  Where not all rows fit, grad_weight is
+    summed over the pieces in fp32, two passes over it a piece: in place if it is of float32, else in
+    a buffer of 4 bytes an element.  Where that buffer takes more than the pieces save, all
+    rows are worked on at once, so a smaller ``piece_bytes`` never takes more memory."""
     device, call = _loss_call(x, weight, targets, ignore_index, reduction, ("mean", "sum"))
     vocab, hidden = weight.shape
     if grad_weight is not None:

@@ -44,3 +44,19 @@ def test_an_fp32_gradient_is_its_own_sum_over_pieces():
     n, vocab, hidden = 8192, 128256, 4096
     softmax, others = _parts(n, vocab, hidden, 1024)
     assert _bytes(n, vocab, hidden, 1024 * 2 * vocab, _lib.LA_F32) <= softmax * 3 // 2 + others
+
+
+def test_smaller_pieces_never_take_more_memory():
+    for n, vocab, hidden in ((4096, 128256, 4096), (8192, 128256, 4096), (16384, 128256, 4096), (32768, 32000, 4096),
+                             (8192, 50257, 768), (60000, 32000, 1024), (1000, 1000, 64)):
+        for grad_weight in (_lib.LA_BF16, _lib.LA_F32):
+            sizes = [_bytes(n, vocab, hidden, b << 20, grad_weight) for b in (1 << 20, 4096, 2048, 1024, 512, 128, 16, 1)]
+            assert all(a >= b for a, b in zip(sizes, sizes[1:])), (n, vocab, hidden, sizes)
+        # and eight pieces or more do take less than all rows' scores in 16 bits, where the matrix is small beside them
+        if vocab * hidden * 4 * 3 < n * vocab * 2 and n * vocab * 2 > 8 * (128 << 20):
+            assert _bytes(n, vocab, hidden, 128 << 20) < n * vocab * 2, (n, vocab, hidden)
+
+
+def test_a_piece_more_does_not_cost_a_matrix():
+    """One row more than a piece of the default size holds, of 128256 x 4096 in bf16."""
+    assert _bytes(4097, 128256, 4096, 1 << 30) < 1.1 * _bytes(4096, 128256, 4096, 1 << 30)
