@@ -21,6 +21,12 @@ def no_memory(hip_device):
         torch.cuda.synchronize()
         torch.cuda.empty_cache()
         torch.cuda.set_per_process_memory_fraction(torch.cuda.memory_reserved(hip_device) / total, hip_device)
+        held = []                                            # what is free between other tensors
+        try:
+            while True:
+                held.append(torch.empty(1 << 24, dtype=torch.uint8, device=hip_device))
+        except torch.OutOfMemoryError:
+            return held
 
     yield limit
     torch.cuda.set_per_process_memory_fraction(1.0, hip_device)
@@ -43,9 +49,10 @@ def test_out_of_memory_is_torchs_error(hip_device, no_memory, name, stream):
             "rms_norm_grad": lambda: ops.rms_norm_grad(x, x, rstd, weight[0], stream=side),
             "linear_cross_entropy": lambda: ops.linear_cross_entropy(x, weight, tokens, stream=side),
             "linear_cross_entropy_grad": lambda: ops.linear_cross_entropy_grad(x, weight, tokens, stream=side)}[name]
-    no_memory()
+    held = no_memory()                                       # less than 16 MiB is left in one place
     with pytest.raises(torch.OutOfMemoryError):
         call()
+    del held
     torch.cuda.set_per_process_memory_fraction(1.0, hip_device)
     call()
     torch.cuda.synchronize()
