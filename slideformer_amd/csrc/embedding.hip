@@ -121,7 +121,9 @@ __global__ __launch_bounds__(256) void rank_kernel(const I* tokens, uint32_t n, 
 }
 
 // 16 lanes a token: the searches of its chunks run beside each other, ten loads
-// deep each.  8192 tokens: 5.1 us, which is their latency.
+// deep each.  8192 tokens: 5 us, which is their latency.  There are n / 1024 searches a
+// token, so a batch of many chunks pays for their square: the whole gradient of 50257 x 256
+// takes 47 us for 32768 tokens and 324 for 131072, where torch's index_add takes 69 and 175.
 __global__ __launch_bounds__(256) void merge_kernel(const uint32_t* keys, const uint32_t* places, uint32_t n,
                                                     uint32_t* sorted, uint32_t* sorted_places, uint8_t* marks)
 {
@@ -266,7 +268,9 @@ template <typename T, typename O> __global__ __launch_bounds__(256, 8) void run_
 
 // A workgroup joins the run that starts in block `unit / slices` and goes on.  Its
 // waves take turns of kFlight partials and their sums are added in order.  8192
-// tokens of 128256 x 4096 with a most frequent one of 490: 14.4 us, latency.
+// tokens of 128256 x 4096 with a most frequent one of 490: 14.3 us, latency; 8192 equal
+// tokens of 50257 x 256, 1024 partials one workgroup joins: 168 us for the whole call,
+// 26 where tokens differ.
 template <typename T, typename O> __global__ __launch_bounds__(256) void join_runs_kernel(SumArgs a)
 {
     constexpr int E = Elem<T>::kCount;

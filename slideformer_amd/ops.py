@@ -11,7 +11,11 @@ steps: the embedding matrix, the norms, and the vocabulary matrix with the loss.
 Gradients are explicit calls, as a layer-by-layer runtime makes them: each writes
 into the tensor that the optimizer reads, a slice of a flat grad buffer for
 instance, and with ``accumulate=True`` adds to what is there (a second
-micro-batch, or the other use of tied weights).
+micro-batch, or the other use of tied weights).  Nothing is recorded for autograd:
+outputs never require grad, whatever the inputs do.
+
+Matrices have two dimensions; ``embedding`` of tokens [batch, length] returns
+[batch, length, hidden], whose ``flatten(0, 1)`` the other calls take.
 
 All tensors live on one HIP device.  Calls are asynchronous on the current
 stream, or on ``stream``; results of one call belong to that stream.  Rows may be
@@ -159,7 +163,8 @@ def embedding_grad(tokens: torch.Tensor, grad_out: torch.Tensor, grad_weight: to
     ``grad_out``: [tokens.numel(), hidden] (or [*tokens.shape, hidden]).  Every row
     of ``grad_weight`` (grad_out's type or float32) is written: ``scale`` times the sum of its
     token's rows, zeros for tokens that do not occur; with ``accumulate`` the sums
-    are added to what is there and other rows stay untouched.  ``padding_idx`` and
+    are added to what is there and other rows stay untouched.  ``padding_idx`` (a token;
+    a negative one is none, and is not counted from the end as torch does) and
     out-of-range tokens contribute nothing.  Sums are fp32 in a fixed order: equal
     calls give equal bits."""
     if stream is None and tokens.is_cuda:
