@@ -96,7 +96,7 @@ int la_rms_norm_grad(int dtype, const void* grad_out, uint64_t grad_out_stride, 
  * dtype (of x, weight, grad_x): LA_BF16 or LA_F16; grad_weight: that type or LA_F32.
  * Without gradients a tile of scores is held at a time.  With gradients the
  * softmax of piece_rows rows is held in 16 bits at a time (rounded up to a multiple of
- * 256; 0: of all), and up to half as much again or 64 MiB of partial sums of
+ * 256; 0: of all; of 32768 at most), and up to half as much again or 64 MiB of partial sums of
  * grad_x.  Where the rows take more than one piece, grad_weight is summed in
  * fp32: where it lies if it is of fp32, else in the workspace; where that would take more
  * memory than the softmax of all rows, all rows are one piece.

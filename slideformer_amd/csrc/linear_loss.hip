@@ -690,8 +690,8 @@ struct Layout {
         columns = ceil_div(c.vocab, kTile) * kTile;
         all = c.n > 0 ? ceil_div(c.n, kTile) * kTile : kTile;     // no rows: one empty piece, which clears grad_weight
         piece = ceil_div(piece_rows, kTile) * kTile;
-        if (piece > kMostRows) piece = kMostRows;
         if (piece == 0 || piece > all) piece = all;
+        if (piece > kMostRows) piece = kMostRows;
         pieces = ceil_div(all, piece);
         // As many runs of k as would take the memory of a piece's D, or the 64 MiB of one round of large tiles, if
         // all its rows were trained.  Their partial sums have half of that, of one run at the least: the full

@@ -2,12 +2,13 @@
 against 64 bits on the device."""
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
-from slideformer_amd import ops
+from slideformer_amd import _lib, _ops_lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +72,34 @@ def test_pieces_of_a_batch(hip_device, dtype, w_dtype, n, hidden, vocab, ignored
     sizes = want_w.abs() + w_off / U[dtype] + (before.double().abs() if accumulate else 0)
     w_bound = w_off + U[w_dtype] * want_w.abs() + (pieces + 4) * U32 * sizes + TINY[w_dtype]
     assert not bool(((grad_weight.double() - want_w).abs() > w_bound).any()) and not bool(grad_weight.isnan().any())
+
+
+def test_all_rows_through_the_c_abi(hip_device):
+    """piece_rows 0: all rows, of which a launch takes 32768 at a time; the same bits as asked for in such pieces."""
+    n, hidden, vocab = 70001, 64, 300
+    gen = torch.Generator(device=hip_device).manual_seed(4)
+    x = torch.randn(n, hidden, generator=gen, device=hip_device).to(BF16)
+    weight = torch.randn(vocab, hidden, generator=gen, device=hip_device).to(BF16)
+    targets = torch.randint(0, vocab, (n,), generator=gen, device=hip_device)
+    lib, results = _ops_lib.load(), []
+    for piece_rows in (0, 32768):
+        loss = torch.empty((), device=hip_device)
+        grad_x, grad_weight = torch.empty_like(x), torch.empty_like(weight)
+        call = _ops_lib.LaLinearLoss(
+            dtype=_lib.LA_BF16, x=x.data_ptr(), n=n, hidden=hidden, x_stride=hidden, weight=weight.data_ptr(),
+            vocab=vocab, weight_stride=hidden, targets=targets.data_ptr(), ignore_index=IGNORE, mean=1,
+            loss=loss.data_ptr(), grads=1, grad_x=grad_x.data_ptr(), grad_x_stride=hidden,
+            grad_weight_dtype=_lib.LA_BF16, grad_weight=grad_weight.data_ptr(), grad_weight_stride=hidden,
+            piece_rows=piece_rows)
+        size = lib.la_linear_loss_workspace(ctypes.byref(call))
+        work = torch.empty(size, dtype=torch.uint8, device=hip_device)
+        stream = torch.cuda.current_stream(hip_device).cuda_stream
+        assert lib.la_linear_loss(ctypes.byref(call), work.data_ptr(), size, stream) == _lib.LA_OK
+        torch.cuda.synchronize()
+        results.append((loss, grad_x, grad_weight))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    want, bound, want_x, x_bound, want_w, w_off = _exact(x, weight, targets, 1.0)
+    assert float((results[0][0].double() - want).abs()) <= float(bound)
+    assert not bool(((results[0][1].double() - want_x).abs() > x_bound).any())
+    w_bound = w_off + U[BF16] * want_w.abs() + 8 * U32 * (want_w.abs() + w_off / U[BF16]) + TINY[BF16]
+    assert not bool(((results[0][2].double() - want_w).abs() > w_bound).any())

@@ -60,3 +60,15 @@ def test_smaller_pieces_never_take_more_memory():
 def test_a_piece_more_does_not_cost_a_matrix():
     """One row more than a piece of the default size holds, of 128256 x 4096 in bf16."""
     assert _bytes(4097, 128256, 4096, 1 << 30) < 1.1 * _bytes(4096, 128256, 4096, 1 << 30)
+
+
+def test_all_rows_at_once_are_as_many_as_a_launch_takes():
+    """piece_rows 0 asks for all rows: pieces of 32768 where there are more."""
+    def size(n, piece_rows):
+        call = _ops_lib.LaLinearLoss(
+            dtype=_lib.LA_BF16, n=n, hidden=64, x_stride=64, weight=256, vocab=300, weight_stride=64, grads=1,
+            grad_x_stride=64, grad_weight_dtype=_lib.LA_BF16, grad_weight_stride=64, piece_rows=piece_rows)
+        return _ops_lib.load().la_linear_loss_workspace(ctypes.byref(call))
+
+    for n in (1, 256, 32768, 32769, 65536, 100000, 1 << 22):
+        assert size(n, 0) == size(n, 32768), n
