@@ -1,8 +1,9 @@
 /*
- * slideformer_amd -- C-ABI of the operators at a language model's two ends on
- * MI355X (gfx950): embedding lookup and its gradient, the root-mean-square norm
- * with the residual's addition and its gradient, and softmax cross entropy over
- * a vocabulary matrix with its gradients.
+ * slideformer_amd -- C-ABI of a language model's operators on MI355X (gfx950):
+ * embedding lookup and its gradient, the root-mean-square norm with the residual's
+ * addition and its gradient, the norm and rotation of query and key heads, attention,
+ * both with their gradients, and softmax cross entropy over a vocabulary matrix
+ * with its gradients.
  *
  * Plain pointers and sizes only; no torch types.  The caller owns every buffer
  * and every workspace; the library allocates nothing and keeps no state.
@@ -25,7 +26,7 @@
 extern "C" {
 #endif
 
-#define LA_OPS_ABI_VERSION 1
+#define LA_OPS_ABI_VERSION 2
 
 /* element types of token ids, and of 8-bit outputs */
 #define LA_I32 16
@@ -126,6 +127,107 @@ typedef struct {
 
 uint64_t la_linear_loss_workspace(const la_linear_loss_t* call);
 int la_linear_loss(const la_linear_loss_t* call, void* workspace, uint64_t workspace_bytes, la_stream_t stream);
+
+/*
+ * Heads of 16-bit elements: element e of head h of row r of batch b is at
+ * b * batch_stride + r * row_stride + h * head_stride + e, in elements.
+ */
+typedef struct {
+    const void* data;
+    uint64_t batch_stride, row_stride, head_stride;
+} la_heads_t;
+
+/*
+ * Softmax attention: for every query row, out = sum_j exp(scale q k_j - lse) v_j over the
+ * keys j that it sees, lse = log sum_j exp(scale q k_j).  `heads` query heads share
+ * `kv_heads` key heads, heads / kv_heads beside each other each.
+ * Sequences: without `starts`, `batch` of them of `rows` queries and `key_rows` keys each, of
+ * which the first lengths[b] and key_lengths[b] are there (null: all).  With `starts`
+ * (batch + 1 indices that do not decrease) they lie one after the other: queries of sequence b are the
+ * rows starts[b] .. starts[b + 1] of `rows` in all, keys those of key_starts (null: starts) of
+ * `key_rows` in all; batch strides are not used.  Indices (index_dtype LA_I32 or LA_I64) are
+ * read on the device and made to lie within the rows there are.
+ * causal: query i of n sees the keys up to i + m - n of m, the last query the last
+ * key; window (with causal; 0: none): only the last `window` of these.
+ * A row that sees no key has out 0 and lse -inf; so has a row of no sequence.  What lies
+ * beyond a sequence's keys is never looked at, whatever it holds.
+ * dtype (of all heads): LA_BF16 or LA_F16; dim at most 128; scale above 0.
+ * lse: fp32 [batch][rows][heads], or [rows][heads].
+ * workspace: la_attention_workspace(call) bytes, 256-byte aligned: partial results where
+ * the keys of few rows are shared out among workgroups, and copies of what does not lie
+ * in whole 16-byte chunks.  Sums are fp32 in a fixed order.
+ */
+typedef struct {
+    int dtype;
+    uint64_t batch, rows, key_rows, heads, kv_heads, dim;
+    la_heads_t q, k, v, out;
+    float* lse;
+    int index_dtype;
+    const void* starts;
+    const void* key_starts;
+    const void* lengths;
+    const void* key_lengths;
+    int causal;
+    uint64_t window;
+    float scale;
+    la_heads_t grad_out, grad_q, grad_k, grad_v; /* la_attention_grad alone */
+    int keep_rest;
+} la_attention_t;
+
+uint64_t la_attention_workspace(const la_attention_t* call);
+int la_attention(const la_attention_t* call, void* workspace, uint64_t workspace_bytes, la_stream_t stream);
+
+/*
+ * The gradients of la_attention towards q, k and v from that of out, grad_out, and from its results out
+ * and lse: P = exp(scale q k - lse), dP = grad_out v, dS = P (dP - sum(grad_out out)),
+ *   grad_q = scale dS k,  grad_k = scale dS^T q,  grad_v = P^T grad_out,
+ * those of key heads summed over the query heads that share them.  Rows beyond a sequence's length or in no
+ * sequence have gradient 0, or with keep_rest != 0 stay as they were.  Nothing is added atomically.
+ * workspace: la_attention_grad_workspace(call) bytes, 256-byte aligned.
+ */
+uint64_t la_attention_grad_workspace(const la_attention_t* call);
+int la_attention_grad(const la_attention_t* call, void* workspace, uint64_t workspace_bytes, la_stream_t stream);
+
+/*
+ * For every row of heads q and k [n][heads or kv_heads][dim] of type dtype (LA_F32, LA_BF16 or LA_F16):
+ * y = x / sqrt(mean(x^2) + eps) * weight over dim (a null weight: y = x), then the first `rotated` elements in
+ * pairs (a, b) -> (a cos - b sin, b cos + a sin), pair j by cos and sin [position][j] of fp32 tables with
+ * `positions` rows of rotated / 2; in fp32, rounded once.  Pairs are elements (j, j + rotated / 2), or with
+ * interleaved != 0 (2 j, 2 j + 1).  Row i has position at[i] (int32 or int64), or i where `at` is null; one outside
+ * the tables makes the rotated elements of its row NaN.  Results may be written over their inputs.
+ */
+typedef struct {
+    int dtype;
+    uint64_t n, heads, kv_heads, dim, rotated;
+    la_heads_t q, k, q_out, k_out;          /* batch strides are not used */
+    const void* q_weight;                   /* dim of dtype, nullable */
+    const void* k_weight;
+    float eps;
+    const float* cos;
+    const float* sin;
+    uint64_t positions;
+    int at_dtype;
+    const void* at;                         /* n, nullable */
+    int interleaved;
+    /* la_qk_norm_rotary_grad alone */
+    la_heads_t grad_q, grad_k;
+    int weight_grad_dtype;
+    void* grad_q_weight;
+    void* grad_k_weight;
+    int accumulate;
+} la_rotary_t;
+
+int la_qk_norm_rotary(const la_rotary_t* call, la_stream_t stream);
+
+/*
+ * The gradients of la_qk_norm_rotary from those of its results, grad_q and grad_k: towards x, into q_out and
+ * k_out (which may be grad_q and grad_k), and towards the weights that there are, into grad_q_weight and
+ * grad_k_weight (dtype or LA_F32), added to with accumulate != 0.  q and k are its inputs; without weights they are
+ * not read and may be null.  Sums are fp32 in a fixed order.
+ * workspace: la_qk_norm_rotary_grad_workspace(call) bytes, 16-byte aligned.
+ */
+uint64_t la_qk_norm_rotary_grad_workspace(const la_rotary_t* call);
+int la_qk_norm_rotary_grad(const la_rotary_t* call, void* workspace, uint64_t workspace_bytes, la_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -21,7 +21,7 @@ LIB_PATH = os.path.join(os.path.dirname(_lib.LIB_PATH), "libslideformer_amd_ops.
 CALLS_PATH = os.path.join(os.path.dirname(LIB_PATH), "_ops_calls.so")
 
 # LA_OPS_ABI_VERSION of include/model_ops.h that these bindings declare
-ABI_VERSION = 1
+ABI_VERSION = 2
 
 LA_I32, LA_I64, LA_I8, LA_F8E4M3 = 16, 17, 18, 19
 
@@ -36,6 +36,13 @@ EXPORTED = (
     "la_rms_norm_grad",
     "la_linear_loss_workspace",
     "la_linear_loss",
+    "la_attention_workspace",
+    "la_attention",
+    "la_attention_grad_workspace",
+    "la_attention_grad",
+    "la_qk_norm_rotary",
+    "la_qk_norm_rotary_grad_workspace",
+    "la_qk_norm_rotary_grad",
 )
 
 
@@ -68,6 +75,81 @@ class LaLinearLoss(ctypes.Structure):
     ]
 
 
+class LaHeads(ctypes.Structure):
+    """Mirror of ``la_heads_t``."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("batch_stride", ctypes.c_uint64),
+        ("row_stride", ctypes.c_uint64),
+        ("head_stride", ctypes.c_uint64),
+    ]
+
+
+class LaAttention(ctypes.Structure):
+    """Mirror of ``la_attention_t``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int),
+        ("batch", ctypes.c_uint64),
+        ("rows", ctypes.c_uint64),
+        ("key_rows", ctypes.c_uint64),
+        ("heads", ctypes.c_uint64),
+        ("kv_heads", ctypes.c_uint64),
+        ("dim", ctypes.c_uint64),
+        ("q", LaHeads),
+        ("k", LaHeads),
+        ("v", LaHeads),
+        ("out", LaHeads),
+        ("lse", ctypes.c_void_p),
+        ("index_dtype", ctypes.c_int),
+        ("starts", ctypes.c_void_p),
+        ("key_starts", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("key_lengths", ctypes.c_void_p),
+        ("causal", ctypes.c_int),
+        ("window", ctypes.c_uint64),
+        ("scale", ctypes.c_float),
+        ("grad_out", LaHeads),
+        ("grad_q", LaHeads),
+        ("grad_k", LaHeads),
+        ("grad_v", LaHeads),
+        ("keep_rest", ctypes.c_int),
+    ]
+
+
+class LaRotary(ctypes.Structure):
+    """Mirror of ``la_rotary_t``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int),
+        ("n", ctypes.c_uint64),
+        ("heads", ctypes.c_uint64),
+        ("kv_heads", ctypes.c_uint64),
+        ("dim", ctypes.c_uint64),
+        ("rotated", ctypes.c_uint64),
+        ("q", LaHeads),
+        ("k", LaHeads),
+        ("q_out", LaHeads),
+        ("k_out", LaHeads),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("eps", ctypes.c_float),
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+        ("positions", ctypes.c_uint64),
+        ("at_dtype", ctypes.c_int),
+        ("at", ctypes.c_void_p),
+        ("interleaved", ctypes.c_int),
+        ("grad_q", LaHeads),
+        ("grad_k", LaHeads),
+        ("weight_grad_dtype", ctypes.c_int),
+        ("grad_q_weight", ctypes.c_void_p),
+        ("grad_k_weight", ctypes.c_void_p),
+        ("accumulate", ctypes.c_int),
+    ]
+
+
 _lock = threading.Lock()
 _loaded = None
 
@@ -94,6 +176,18 @@ def _declare(L):
     L.la_linear_loss_workspace.restype = u64
     L.la_linear_loss.argtypes = [call, P, u64, P]
     L.la_linear_loss.restype = i
+    attention, rotary = ctypes.POINTER(LaAttention), ctypes.POINTER(LaRotary)
+    for name in ("la_attention", "la_attention_grad"):
+        getattr(L, name + "_workspace").argtypes = [attention]
+        getattr(L, name + "_workspace").restype = u64
+        getattr(L, name).argtypes = [attention, P, u64, P]
+        getattr(L, name).restype = i
+    L.la_qk_norm_rotary.argtypes = [rotary, P]
+    L.la_qk_norm_rotary.restype = i
+    L.la_qk_norm_rotary_grad_workspace.argtypes = [rotary]
+    L.la_qk_norm_rotary_grad_workspace.restype = u64
+    L.la_qk_norm_rotary_grad.argtypes = [rotary, P, u64, P]
+    L.la_qk_norm_rotary_grad.restype = i
     return L
 
 

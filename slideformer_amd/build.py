@@ -79,11 +79,12 @@ SMALL_GRID_LIB = os.path.join(LIB_DIR, "libslideformer_amd_smallgrid.so")
 SMALL_GRID_DEFINES = {"LA_MAX_GRID": 64, "LA_NORM_MAX_GRID": 2, "LA_NORM_ONE": 16384, "LA_NORM_RUNS": 4096}
 
 
-# The operators at a model's two ends (include/model_ops.h), a library of their own:
+# A model's operators (include/model_ops.h), a library of their own:
 # a process that only steps an optimizer does not load them.
 OPS_LIB = os.path.join(LIB_DIR, "libslideformer_amd_ops.so")
 OPS_SOURCES = [os.path.join(CSRC, "embedding.hip"), os.path.join(CSRC, "rms_norm.hip"),
-               os.path.join(CSRC, "linear_loss.hip")]
+               os.path.join(CSRC, "linear_loss.hip"), os.path.join(CSRC, "qk_norm_rotary.hip"),
+               os.path.join(CSRC, "attention.hip"), os.path.join(CSRC, "attention_grad.hip")]
 
 
 # The update kernel's memory-ceiling probes (csrc/stream_probe.hip: its exact

@@ -1,0 +1,566 @@
+// slideformer_amd: softmax attention over packed or padded sequences, with query
+// heads that share key heads (gfx950, wave64).
+//
+// For a query row q of a sequence with keys k_j and values v_j that it sees:
+// s_j = scale q k_j, lse = log sum exp s_j, out = sum exp(s_j - lse) v_j.  One pass over the keys
+// with the running maximum m, the running sum l of exp(s_j - m), and the running sum of
+// exp(s_j - m) v_j, which both shrink by exp(m - m') when the maximum grows to m'.
+//
+// The query heads of one key head are rows beside each other, (token, head) in the order
+// in which they lie in memory: a tile of keys is loaded once for all of them, and a single new
+// token with eight query heads is eight rows.
+//
+// Scores are S^T = K Q^T, so a lane holds scores of one row (see attention_tile.h); rounded
+// to 16 bits they are the second operand of out^T += V^T P^T.  The sum l is that of
+// the unrounded values.
+#include "attention_tile.h"
+
+#include <algorithm>
+
+namespace {
+
+using namespace att;
+
+constexpr uint32_t kMostParts = 64;                      // the join has a lane for each
+
+struct ForwardArgs {
+    Heads q, k, v, out;
+    float* lse;                     // [rows][heads]
+    float* partial;                 // of each part: [part][row][D], then lse in base 2: [part][row]
+    Sequences seq;
+    uint32_t heads, kv_heads, dim;  // dim: of the result
+    uint32_t read_dim;              // of q, k, v: a multiple of 8
+    float scale;
+    uint32_t parts, part_tiles;     // the keys' tiles are shared out in runs of part_tiles
+    uint32_t rows_all;              // flat rows of the result, over all heads
+    int aligned;                    // rows of the result may be written 16 bytes at a time
+};
+
+// The running state of 32 rows in a wave: of row l % 32 a lane has the elements 32 d + 8 (i / 4) + 4 (l / 32) + i % 4.
+template <int D> struct State {
+    f32x16 out[D / 32];
+    float top;                      // the maximum that `sum` and `out` are relative to, in units of scores
+    float sum;                      // over this half's keys
+    __device__ __forceinline__ void init()
+    {
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) out[d] = zeros();
+        top = -INFINITY;
+        sum = 0.0f;
+    }
+};
+
+// How far, in powers of two, scores may pass the maximum before sums are brought
+// to the new one: a row's values stay below 2^8 times what they would be, which costs no
+// precision, and after the first tiles hardly any tile touches `out`.
+constexpr float kSlack = 8.0f;
+
+// Takes KEYS keys (32 or 64) of a tile in: their scores are in `s`, masked ones -inf.
+template <typename T, int D, int KEYS>
+__device__ __forceinline__ void take(State<D>& st, f32x16 (&s)[KEYS / 32], const lds_char* v, const Fragments<D>& f,
+                                     float factor)
+{
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < KEYS / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+    top = both_max(top);
+    if (__any(top > st.top + kSlack / factor || (st.top == -INFINITY && top > -INFINITY))) {
+        const float now = fmaxf(top, st.top);
+        const float shrink = now == st.top ? 1.0f : exp2_of((st.top - now) * factor);
+        st.top = now;
+        st.sum *= shrink;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) st.out[d] *= shrink;
+    }
+    // rows that have seen nothing yet: 0, and exp2(-inf) below
+    const float from = st.top == -INFINITY ? 0.0f : -st.top * factor;
+    float sum = 0.0f;
+#pragma unroll
+    for (int b = 0; b < KEYS / 32; ++b) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = exp2_of(__builtin_fmaf(s[b][i], factor, from));
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) sum += (s[b][i] + s[b][i + 1]) + (s[b][i + 2] + s[b][i + 3]);
+    }
+    st.sum += sum;
+#pragma unroll
+    for (int b = 0; b < KEYS / 32; ++b)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const s16x8 p = rounded<T>(s[b], half);
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) st.out[d] = mfma<T>(f.columns(v, d, b * 2 + half), p, st.out[d]);
+        }
+}
+
+template <typename T, int D, int KEYS>
+__device__ __forceinline__ void scores(f32x16 (&s)[KEYS / 32], const s16x8 (&q)[D / 16], const lds_char* k,
+                                       const Fragments<D>& f)
+{
+#pragma unroll
+    for (int b = 0; b < KEYS / 32; ++b) {
+        s[b] = zeros();
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) s[b] = mfma<T>(f.rows(k, e, b), q[e], s[b]);
+    }
+}
+
+// Scores of keys outside the row's [lo, hi) become -inf, whatever they were.
+template <int KEYS>
+__device__ __forceinline__ void mask(f32x16 (&s)[KEYS / 32], int32_t first_key, const Seen& row)
+{
+    const int32_t half = static_cast<int32_t>(threadIdx.x % kWave / 32) * 4;
+    const uint32_t from = static_cast<uint32_t>(row.lo - first_key - half);
+    const uint32_t count = row.hi > row.lo ? static_cast<uint32_t>(row.hi - row.lo) : 0u;
+#pragma unroll
+    for (int b = 0; b < KEYS / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t key = b * 32 + i / 4 * 8 + i % 4;
+            s[b][i] = key - from < count ? s[b][i] : -INFINITY;
+        }
+}
+
+// Eight elements of a row from either half of the lanes' four: lane l gets elements 16 j + 8 (l / 32) .. + 7 of
+// its row, j = 0, 1 of the 32 that `x` has.
+__device__ __forceinline__ void neighbours(const f32x16& x, int j, float (&v)[8])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const Halves h = halves(__float_as_uint(x[j * 8 + i]), __float_as_uint(x[j * 8 + 4 + i]));
+        v[i] = __uint_as_float(h.lo);
+        v[4 + i] = __uint_as_float(h.hi);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_eight(char* row, uint32_t at, uint32_t dim, bool aligned, const float (&v)[8])
+{
+    T* to = reinterpret_cast<T*>(row) + at;
+    if (aligned && at + 8 <= dim) {
+        *reinterpret_cast<u32x4_t*>(to) = Elem<T>::pack(v);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+            if (at + i < dim) to[i] = Elem<T>::from_f32(v[i]);
+    }
+}
+
+// The wave's 32 rows, rows `first` of the piece on, to the result or to this part's partial one.
+template <typename T, int D>
+__device__ __forceinline__ void finish(const ForwardArgs& a, const Piece& p, uint32_t kv_head, uint32_t part, uint32_t row,
+                                       State<D>& st)
+{
+    const uint32_t half = threadIdx.x % kWave / 32;
+    const uint32_t token = row / a.seq.group, head = kv_head * a.seq.group + row % a.seq.group;
+    const float sum = both_sum(st.sum);
+    // a row that sees nothing: zeros, and -inf
+    const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const bool there = token < p.stored;
+    const uint64_t flat = (static_cast<uint64_t>(p.batch) * a.seq.rows + p.first + token) * a.heads + head;
+    if (a.parts > 1) {
+        const uint64_t at = static_cast<uint64_t>(part) * a.rows_all + flat;
+        float* to = a.partial + at * D;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const float v[4] = {st.out[d][i] * scale, st.out[d][i + 1] * scale, st.out[d][i + 2] * scale,
+                                    st.out[d][i + 3] * scale};
+                if (there) *reinterpret_cast<u32x4_t*>(to + d * 32 + i * 2 + half * 4) = Elem<float>::pack(v);
+            }
+        if (there && half == 0)
+            a.partial[static_cast<uint64_t>(a.parts) * a.rows_all * D + at] =
+                sum == 0.0f ? -INFINITY : st.top * a.scale * kLog2E + __builtin_amdgcn_logf(sum);
+        return;
+    }
+    char* to = const_cast<char*>(a.out.at(p.batch, p.first + token, head));
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float v[8];
+            neighbours(st.out[d], j, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= scale;
+            if (there) store_eight<T>(to, d * 32 + j * 16 + half * 8, a.dim, a.aligned, v);
+        }
+    if (there && half == 0) a.lse[flat] = sum == 0.0f ? -INFINITY : st.top * a.scale + __builtin_amdgcn_logf(sum) * kLn2;
+}
+
+// This lane's row as the second operand of the scores: elements 16 k + 8 (l / 32) .. + 7.
+template <int D>
+__device__ __forceinline__ void load_row(s16x8 (&q)[D / 16], const char* row, bool there, uint32_t dim)
+{
+    const uint32_t half = threadIdx.x % kWave / 32;
+#pragma unroll
+    for (uint32_t k = 0; k < D / 16; ++k) {
+        u32x4_t u = {0, 0, 0, 0};
+        if (there && k * 16 + half * 8 < dim) u = *reinterpret_cast<const u32x4_t*>(row + (k * 16 + half * 8) * 2);
+        q[k] = __builtin_bit_cast(s16x8, u);
+    }
+    // the loads are over before others begin that are counted by hand
+#pragma unroll
+    for (uint32_t k = 0; k < D / 16; ++k) asm volatile("" : "+v"(q[k]));
+}
+
+// 128 rows to a workgroup, 32 to a wave; all waves go over the same tiles of 64 keys, two of which are
+// in LDS: one in work, the next on its way.
+template <typename T, int D> __global__ __launch_bounds__(256, 2) void attention_kernel(ForwardArgs a)
+{
+    constexpr uint32_t kBytes = Tile<D>::kBytes;
+    __shared__ __attribute__((aligned(1024))) char shared[4 * kBytes];
+    const uint32_t kv_head = blockIdx.x % a.kv_heads, part = blockIdx.y;
+    Piece p = locate(a.seq, blockIdx.x / a.kv_heads, false, a.seq.group, 128);
+    if (!p.valid) return;
+    {
+        // the last rows of a causal sequence see the most keys: they begin
+        const uint32_t tiles = ceil_div(p.stored * a.seq.group, 128u);
+        p.tile = tiles - 1 - p.tile;
+    }
+    const uint32_t wave = uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+    const uint32_t group = a.seq.group;
+    const uint32_t row = p.tile * 128 + wave * 32 + lane % 32;
+    const uint32_t token = row / group;
+    const Seen mine = seen(a.seq, p, token);
+
+    s16x8 q[D / 16];
+    load_row<D>(q, a.q.at(p.batch, p.first + token, kv_head * group + row % group), token < p.length, a.read_dim);
+
+    // the keys that the workgroup's rows see, and this wave's
+    const uint32_t last_row = p.length * group;          // one past
+    const auto range = [&](uint32_t row_from, uint32_t row_to) {
+        row_to = row_to < last_row ? row_to : last_row;
+        if (row_from >= row_to) return Seen{0, 0};
+        return Seen{seen(a.seq, p, row_from / group).lo, seen(a.seq, p, (row_to - 1) / group).hi};
+    };
+    const Seen all = range(p.tile * 128, p.tile * 128 + 128);
+    const uint32_t wave_row = p.tile * 128 + wave * 32;
+    const Seen own = range(wave_row, wave_row + 32);
+    // and those that all of them see
+    const bool full = wave_row + 32 <= last_row;
+    const Seen common = full ? Seen{seen(a.seq, p, (wave_row + 31) / group).lo, seen(a.seq, p, wave_row / group).hi}
+                             : Seen{0, 0};
+    int32_t tile = all.lo / static_cast<int32_t>(kTileRows);
+    int32_t end = all.hi > 0 ? (all.hi + static_cast<int32_t>(kTileRows) - 1) / static_cast<int32_t>(kTileRows) : 0;
+    if (a.parts > 1) {
+        const int32_t from = static_cast<int32_t>(part * a.part_tiles), to = from + static_cast<int32_t>(a.part_tiles);
+        tile = tile > from ? tile : from;
+        end = end < to || part + 1 == a.parts ? end : to;
+    }
+
+    State<D> st;
+    st.init();
+    if (tile < end) {
+        const Rows keys{reinterpret_cast<uint64_t>(a.k.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
+        const Rows values{reinterpret_cast<uint64_t>(a.v.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
+        Loader<D, kTileRows, 4> load_k, load_v;
+        load_k.init(wave, static_cast<uint32_t>(a.k.row), a.read_dim);
+        load_v.init(wave, static_cast<uint32_t>(a.v.row), a.read_dim);
+        Fragments<D> f;
+        f.init();
+        lds_char* lds = (lds_char*)shared;
+        const uint32_t place = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + wave * 1024;
+        const float factor = a.scale * kLog2E;
+        load_k.load(keys, tile * kTileRows, place);
+        load_v.load(values, tile * kTileRows, place + kBytes);
+        uint32_t buffer = 0;
+        for (; tile < end; ++tile, buffer ^= 2 * kBytes) {
+            arrive<0>();
+            if (tile + 1 < end) {
+                load_k.load(keys, (tile + 1) * kTileRows, place + (buffer ^ 2 * kBytes));
+                load_v.load(values, (tile + 1) * kTileRows, place + (buffer ^ 2 * kBytes) + kBytes);
+            }
+            const int32_t first_key = tile * static_cast<int32_t>(kTileRows);
+            if (first_key < own.hi && first_key + static_cast<int32_t>(kTileRows) > own.lo) {
+                const lds_char* k = lds + buffer;
+                f32x16 s[2];
+                scores<T, D, 64>(s, q, k, f);
+                if (first_key < common.lo || first_key + static_cast<int32_t>(kTileRows) > common.hi)
+                    mask<64>(s, first_key, mine);
+                take<T, D, 64>(st, s, k + kBytes, f, factor);
+            }
+        }
+    }
+    finish<T, D>(a, p, kv_head, part, row, st);
+}
+
+// At most 32 rows to a workgroup (a single new token's heads): its waves take the same rows and different keys, each
+// with tiles of its own in LDS and without waiting for the others, and join at the end.
+template <typename T, int D> __global__ __launch_bounds__(256, 1) void few_rows_kernel(ForwardArgs a)
+{
+    constexpr uint32_t kKeys = 32, kBytes = Tile<D>::kBytes / 2, kAhead = 2;
+    constexpr uint32_t kOwn = 2 * kAhead * kBytes;       // a wave's share of LDS
+    __shared__ __attribute__((aligned(1024))) char shared[4 * kOwn];
+    __shared__ float tops[4][32], sums[4][32];
+    const uint32_t kv_head = blockIdx.x % a.kv_heads, part = blockIdx.y;
+    const Piece p = locate(a.seq, blockIdx.x / a.kv_heads, false, a.seq.group, 32);
+    if (!p.valid) return;
+    const uint32_t wave = uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+    const uint32_t group = a.seq.group;
+    const uint32_t row = p.tile * 32 + lane % 32;
+    const uint32_t token = row / group;
+    const Seen mine = seen(a.seq, p, token);
+
+    const uint32_t last_row = p.length * group, row_from = p.tile * 32;
+    const uint32_t row_to = row_from + 32 < last_row ? row_from + 32 : last_row;
+    Seen all{0, 0}, common{0, 0};
+    if (row_from < row_to) {
+        const Seen first = seen(a.seq, p, row_from / group), last = seen(a.seq, p, (row_to - 1) / group);
+        all = {first.lo, last.hi};
+        common = {last.lo, first.hi};
+    }
+    int32_t tile = all.lo / static_cast<int32_t>(kKeys);
+    int32_t end = all.hi > 0 ? (all.hi + static_cast<int32_t>(kKeys) - 1) / static_cast<int32_t>(kKeys) : 0;
+    if (a.parts > 1) {
+        const int32_t from = static_cast<int32_t>(part * a.part_tiles), to = from + static_cast<int32_t>(a.part_tiles);
+        tile = tile > from ? tile : from;
+        end = end < to || part + 1 == a.parts ? end : to;
+    }
+
+    State<D> st;
+    st.init();
+    lds_char* lds = (lds_char*)shared;
+    if (tile < end) {
+        s16x8 q[D / 16];
+        load_row<D>(q, a.q.at(p.batch, p.first + token, kv_head * group + row % group), token < p.length, a.read_dim);
+        const Rows keys{reinterpret_cast<uint64_t>(a.k.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
+        const Rows values{reinterpret_cast<uint64_t>(a.v.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
+        Loader<D, kKeys, 1> load_k, load_v;
+        load_k.init(0, static_cast<uint32_t>(a.k.row), a.read_dim);
+        load_v.init(0, static_cast<uint32_t>(a.v.row), a.read_dim);
+        Fragments<D> f;
+        f.init();
+        const lds_char* own = lds + wave * kOwn;
+        const uint32_t place = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(own));
+        const float factor = a.scale * kLog2E;
+        const int32_t mine_from = tile + static_cast<int32_t>(wave);
+        load_k.load(keys, mine_from * kKeys, place);
+        load_v.load(values, mine_from * kKeys, place + kBytes);
+        uint32_t buffer = 0;
+        for (int32_t t = mine_from; t < end; t += 4, buffer ^= 2 * kBytes) {
+            // a tile past the end reads nothing: its zeros are waited for like any other's
+            load_k.load(keys, (t + 4) * kKeys, place + (buffer ^ 2 * kBytes));
+            load_v.load(values, (t + 4) * kKeys, place + (buffer ^ 2 * kBytes) + kBytes);
+            arrived<2 * Loader<D, kKeys, 1>::kLoads>();
+            const int32_t first_key = t * static_cast<int32_t>(kKeys);
+            const lds_char* k = own + buffer;
+            f32x16 s[1];
+            scores<T, D, 32>(s, q, k, f);
+            if (first_key < common.lo || first_key + static_cast<int32_t>(kKeys) > common.hi)
+                mask<32>(s, first_key, mine);
+            take<T, D, 32>(st, s, k + kBytes, f, factor);
+            // what was read is read before the next loads write over it
+            arrived<2 * Loader<D, kKeys, 1>::kLoads>();
+        }
+        arrived<0>();
+    }
+    // the waves' states, each shrunk to the largest of their maxima, added in the order of the waves
+    st.sum = both_sum(st.sum);
+    if (lane < 32) tops[wave][lane] = st.top, sums[wave][lane] = st.sum;
+    __syncthreads();
+    const uint32_t r = lane % 32;
+    float top = tops[0][r];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, tops[w][r]);
+    const float factor = a.scale * kLog2E;
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+        sum += tops[w][r] == -INFINITY ? sums[w][r] : sums[w][r] * exp2_of((tops[w][r] - top) * factor);
+    const float shrink = st.top == -INFINITY ? 1.0f : exp2_of((st.top - top) * factor);
+    constexpr uint32_t kRow = D + 4;                     // keeps 32 rows' accesses in different banks
+    float* mine_out = reinterpret_cast<float*>(shared) + wave * 32 * kRow;
+    static_assert(4 * 32 * kRow * 4 <= 4 * kOwn, "the states fit the tiles' place");
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const float v[4] = {st.out[d][i] * shrink, st.out[d][i + 1] * shrink, st.out[d][i + 2] * shrink,
+                                st.out[d][i + 3] * shrink};
+            *reinterpret_cast<u32x4_t*>(mine_out + r * kRow + d * 32 + i * 2 + lane / 32 * 4) = Elem<float>::pack(v);
+        }
+    __syncthreads();
+    // eight lanes to a row
+    const uint32_t out_row = threadIdx.x / 8, at = threadIdx.x % 8;
+    const uint32_t piece_row = p.tile * 32 + out_row, out_token = piece_row / group;
+    const uint32_t head = kv_head * group + piece_row % group;
+    // from lanes of rows that may not be there: before any lane leaves
+    const float row_sum = __shfl(sum, static_cast<int>(out_row % 32)), row_top = __shfl(top, static_cast<int>(out_row % 32));
+    if (out_token >= p.stored) return;
+    const float scale = row_sum == 0.0f ? 0.0f : 1.0f / row_sum;
+    const uint64_t flat = (static_cast<uint64_t>(p.batch) * a.seq.rows + p.first + out_token) * a.heads + head;
+    char* to = const_cast<char*>(a.out.at(p.batch, p.first + out_token, head));
+    float* part_to = a.partial + (static_cast<uint64_t>(part) * a.rows_all + flat) * D;
+#pragma unroll
+    for (uint32_t e = at * 8; e < D; e += 64) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float* from = reinterpret_cast<const float*>(shared) + out_row * kRow + e + i;
+            v[i] = ((from[0] + from[32 * kRow]) + (from[64 * kRow] + from[96 * kRow])) * scale;
+        }
+        if (a.parts > 1) store_vec<float, 8>(part_to, e / 8, D, v);
+        else store_eight<T>(to, e, a.dim, a.aligned, v);
+    }
+    if (at == 0) {
+        if (a.parts > 1)
+            a.partial[static_cast<uint64_t>(a.parts) * a.rows_all * D + static_cast<uint64_t>(part) * a.rows_all + flat] =
+                row_sum == 0.0f ? -INFINITY : row_top * factor + __builtin_amdgcn_logf(row_sum);
+        else
+            a.lse[flat] = row_sum == 0.0f ? -INFINITY : row_top * a.scale + __builtin_amdgcn_logf(row_sum) * kLn2;
+    }
+}
+
+// The parts' results of one row into one: a wave to a row, eight elements to a lane, the lanes beside each other in
+// turn on the parts.
+template <typename T, int D> __global__ __launch_bounds__(256) void join_kernel(ForwardArgs a)
+{
+    constexpr uint32_t kLanes = D / 8, kSide = kWave / kLanes;
+    __shared__ float shares[4][kMostParts];
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint32_t flat = blockIdx.x * 4 + uniform(threadIdx.x / kWave);
+    if (flat >= a.rows_all) return;
+    const float* lses = a.partial + static_cast<uint64_t>(a.parts) * a.rows_all * D + flat;
+    const float lse = lane < a.parts ? lses[static_cast<uint64_t>(lane) * a.rows_all] : -INFINITY;
+    float top = lse;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float share = lse == -INFINITY ? 0.0f : exp2_of(lse - top);
+    const float sum = wave_sum(share);
+    shares[threadIdx.x / kWave][lane] = share;
+    __builtin_amdgcn_wave_barrier();                     // read by this wave alone, whose accesses stay in order
+    float v[8] = {};
+#pragma unroll 4
+    for (uint32_t part = lane / kLanes; part < a.parts; part += kSide) {
+        const float w = shares[threadIdx.x / kWave][part];
+        const float* from = a.partial + (static_cast<uint64_t>(part) * a.rows_all + flat) * D;
+        float lo[4], hi[4];
+        load_vec<float>(from, lane % kLanes * 2, D, lo);
+        load_vec<float>(from, lane % kLanes * 2 + 1, D, hi);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = __builtin_fmaf(w, lo[i], v[i]);
+            v[4 + i] = __builtin_fmaf(w, hi[i], v[4 + i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (uint32_t d = kLanes; d < kWave; d <<= 1) v[i] += __shfl_xor(v[i], static_cast<int>(d));
+    const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= scale;
+    const uint32_t head = flat % a.heads, row = flat / a.heads;
+    char* to = const_cast<char*>(a.out.at(row / a.seq.rows, row % a.seq.rows, head));
+    if (lane < kLanes) store_eight<T>(to, lane * 8, a.dim, a.aligned, v);
+    if (lane == 0) a.lse[flat] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+constexpr uint64_t kFill = 512;                          // workgroups that fill the card, two on a compute unit
+
+struct Plan {
+    bool few;                                            // rows of a sequence fit a workgroup of few_rows_kernel
+    uint64_t parts, part_tiles;
+    uint64_t pieces;
+    uint32_t padded;                                     // the kernels' D
+    uint64_t partial_bytes;
+};
+
+Plan plan_of(const la_attention_t& c)
+{
+    Plan p{};
+    const Sequences s = sequences_of(c);
+    const uint64_t group = c.heads / c.kv_heads;
+    p.padded = c.dim <= 64 ? 64 : 128;
+    // Packed queries are of few rows if they are on average; longer ones among them are more pieces.
+    const uint64_t rows = s.starts ? ceil_div(c.rows, c.batch) : c.rows;
+    p.few = rows * group <= 32;
+    p.pieces = pieces(s, false, group, p.few ? 32 : 128);
+    const uint64_t tile = p.few ? 32 : kTileRows;
+    // Keys are shared out where there are too few pieces to fill the card, in parts of 512 keys at least: less
+    // is over before the join begins.
+    const uint64_t keys = s.starts ? ceil_div(c.key_rows, c.batch) : c.key_rows;
+    const uint64_t tiles = ceil_div(keys, tile);
+    const uint64_t wanted = ceil_div(kFill, std::max<uint64_t>(1, p.pieces * c.kv_heads));
+    p.parts = std::max<uint64_t>(1, std::min({wanted, tiles / (512 / tile), uint64_t{kMostParts}}));
+    p.part_tiles = ceil_div(std::max<uint64_t>(1, tiles), p.parts);
+    p.parts = std::max<uint64_t>(1, ceil_div(tiles, p.part_tiles));
+    p.partial_bytes = p.parts > 1 ? p.parts * flat_rows(c) * c.heads * (p.padded + 1) * sizeof(float) : 0;
+    p.partial_bytes = ceil_div(p.partial_bytes, 256) * 256;
+    return p;
+}
+
+template <typename T, int D> int run(const Plan& p, const ForwardArgs& a, hipStream_t stream)
+{
+    const dim3 grid(static_cast<uint32_t>(p.pieces * a.kv_heads), static_cast<uint32_t>(p.parts));
+    int rc = p.few ? launch(few_rows_kernel<T, D>, grid, dim3(256), stream, a)
+                   : launch(attention_kernel<T, D>, grid, dim3(256), stream, a);
+    if (rc == LA_OK && p.parts > 1)
+        rc = launch(join_kernel<T, D>, dim3(ceil_div(a.rows_all, 4u)), dim3(256), stream, a);
+    return rc;
+}
+
+template <typename T> int run(const Plan& p, const ForwardArgs& a, hipStream_t stream)
+{
+    return p.padded == 64 ? run<T, 64>(p, a, stream) : run<T, 128>(p, a, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t la_attention_workspace(const la_attention_t* call)
+{
+    if (check_call(call) != LA_OK || flat_rows(*call) == 0) return 0;
+    const Plan p = plan_of(*call);
+    return p.partial_bytes + packed_bytes(*call, call->q, true) + packed_bytes(*call, call->k, false) +
+           packed_bytes(*call, call->v, false);
+}
+
+int la_attention(const la_attention_t* call, void* workspace, uint64_t workspace_bytes, la_stream_t stream)
+{
+    int rc = check_call(call);
+    if (rc != LA_OK) return rc;
+    const la_attention_t& c = *call;
+    if (flat_rows(c) == 0) return LA_OK;
+    if (!there(c.q) || !there(c.out) || !c.lse || reinterpret_cast<uintptr_t>(c.lse) % 4 ||
+        (flat_keys(c) > 0 && (!there(c.k) || !there(c.v))))
+        return LA_EINVAL;
+    const Plan p = plan_of(c);
+    rc = check_workspace(workspace, workspace_bytes, la_attention_workspace(call), 256);
+    if (rc != LA_OK) return rc;
+    if (p.pieces * c.kv_heads >> 31) return LA_EINVAL;
+    if (!reachable(c.q.data) || !reachable(c.k.data) || !reachable(c.v.data) || !reachable(c.out.data) ||
+        !reachable(c.lse) || !indices_reachable(c) || (la_attention_workspace(call) && !reachable(workspace)))
+        return LA_EFAULT;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    ForwardArgs a{};
+    a.partial = reinterpret_cast<float*>(ws);
+    ws += p.partial_bytes;
+    rc = heads_of(c, c.q, true, a.q, ws, st);
+    if (rc == LA_OK) rc = heads_of(c, c.k, false, a.k, ws, st);
+    if (rc == LA_OK) rc = heads_of(c, c.v, false, a.v, ws, st);
+    if (rc != LA_OK) return rc;
+    a.out = plain(c.out);
+    a.lse = c.lse;
+    a.seq = sequences_of(c);
+    a.heads = static_cast<uint32_t>(c.heads);
+    a.kv_heads = static_cast<uint32_t>(c.kv_heads);
+    a.dim = static_cast<uint32_t>(c.dim);
+    a.read_dim = ceil_div(a.dim, 8u) * 8;
+    a.scale = c.scale;
+    a.parts = static_cast<uint32_t>(p.parts);
+    a.part_tiles = static_cast<uint32_t>(p.part_tiles);
+    a.rows_all = static_cast<uint32_t>(flat_rows(c) * c.heads);
+    a.aligned = in_chunks(c, c.out, true);
+    return c.dtype == LA_BF16 ? run<__bf16>(p, a, st) : run<_Float16>(p, a, st);
+}
+
+}  // extern "C"

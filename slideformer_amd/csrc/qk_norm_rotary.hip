@@ -1,0 +1,553 @@
+// slideformer_amd: the root-mean-square norm of every query and key head and the
+// position rotation after it, in one pass, and its gradient (gfx950, wave64).
+//
+// Forward, per head of a token: r = 1 / sqrt(mean(x^2) + eps), y = x r w, then each pair
+// (a, b) of the rotated elements becomes (a cos - b sin, b cos + a sin).
+// Gradient: with g the pairs of dy turned back, (a cos + b sin, b cos - a sin), and u = x r,
+// dx = r (g w - u mean(g w u)), dw = sum over all heads and tokens of g u.
+//
+// Bound by memory, or for few tokens by latency.  A head is 256 bytes: eight lanes with
+// two 16-byte accesses each in 16-bit types, whose elements are pairs of one another, so a
+// head's sum needs three exchanges and the rotation none.  A wave stays on one token,
+// whose row of the tables it reads once for all heads it takes.
+#include "ops_common.h"
+
+#include <algorithm>
+
+namespace {
+
+constexpr uint32_t kWave = 64;
+
+struct HeadRows {
+    char* data;
+    uint64_t row, head;             // distances in bytes
+};
+
+struct RotaryArgs {
+    HeadRows q, k, q_out, k_out, grad_q, grad_k;
+    const void *q_weight, *k_weight;
+    const float *cos, *sin;
+    const void* at;
+    uint64_t positions;
+    float* partial;                 // of each workgroup: the sums for both weights, [2][dim]
+    uint32_t n, heads, all, dim, rotated;
+    uint32_t lanes;                 // to a head: a power of two
+    uint32_t chunks;                // waves that share a token's heads
+    int wide;
+    float eps;
+};
+
+// Two of a head's 16-byte vectors, a lane's share of it.
+struct Slot {
+    uint32_t first[2];              // their first elements
+    uint32_t count[2];              // how many of them there are
+    uint32_t pair, pairs;           // the pairs that they make up; 0 pairs: elements that are not rotated
+};
+
+template <bool INTERLEAVED, uint32_t V> __device__ __forceinline__ Slot slot_of(uint32_t s, uint32_t dim, uint32_t rotated)
+{
+    const uint32_t pairs = rotated / 2, turning = ceil_div(pairs, V);
+    Slot t;
+    t.pair = s * V;
+    t.pairs = s < turning ? (pairs - s * V < V ? pairs - s * V : V) : 0u;
+    if (!INTERLEAVED && s < turning) {
+        t.first[0] = s * V;
+        t.first[1] = pairs + s * V;
+        t.count[0] = t.count[1] = t.pairs;
+        return t;
+    }
+    const uint32_t from = s < turning ? s * 2 * V : rotated + (s - turning) * 2 * V;
+    const uint32_t end = s < turning ? rotated : dim;
+    const uint32_t left = from < end ? end - from : 0;
+    t.first[0] = from;
+    t.first[1] = from + V;
+    t.count[0] = left < V ? left : V;
+    t.count[1] = left <= V ? 0 : left - V < V ? left - V : V;
+    return t;
+}
+
+inline uint32_t slots(uint32_t dim, uint32_t rotated, uint32_t v)
+{
+    return ceil_div(rotated / 2, v) + ceil_div(dim - rotated, 2 * v);
+}
+
+template <typename T> __device__ __forceinline__ u32x4_t load_some(const T* from, uint32_t count)
+{
+    constexpr uint32_t V = Elem<T>::kCount;
+    if (count == V) return *reinterpret_cast<const u32x4_any*>(from);
+    T x[V];
+#pragma unroll
+    for (uint32_t i = 0; i < V; ++i) x[i] = i < count ? from[i] : Elem<T>::from_f32(0.0f);
+    return __builtin_bit_cast(u32x4_t, x);
+}
+
+template <typename T> __device__ __forceinline__ void store_some(T* to, uint32_t count, const float (&x)[Elem<T>::kCount])
+{
+    constexpr uint32_t V = Elem<T>::kCount;
+    if (count == V) {
+        *reinterpret_cast<u32x4_any*>(to) = Elem<T>::pack(x);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i)
+            if (i < count) to[i] = Elem<T>::from_f32(x[i]);
+    }
+}
+
+// Partners i of a lane's pairs in its two vectors: (0, i), (1, i), or neighbours.
+template <bool INTERLEAVED, int V> struct Pair {
+    __device__ static constexpr int vec(int i, int side) { return INTERLEAVED ? (2 * i + side) / V : side; }
+    __device__ static constexpr int element(int i, int side) { return INTERLEAVED ? (2 * i + side) % V : i; }
+};
+
+template <bool INTERLEAVED, int V, bool BACK>
+__device__ __forceinline__ void rotate(float (&x)[2][V], const Slot& t, const float (&cos)[V], const float (&sin)[V])
+{
+    using P = Pair<INTERLEAVED, V>;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        float &a = x[P::vec(i, 0)][P::element(i, 0)], &b = x[P::vec(i, 1)][P::element(i, 1)];
+        const float s = BACK ? -sin[i] : sin[i];
+        const float turned_a = __builtin_fmaf(a, cos[i], -(b * s)), turned_b = __builtin_fmaf(b, cos[i], a * s);
+        a = t.pairs ? turned_a : a;
+        b = t.pairs ? turned_b : b;
+    }
+}
+
+// A token's row of both tables, this lane's pairs of it; NaN for a position outside them.
+template <int V>
+__device__ __forceinline__ void angles(const RotaryArgs& a, uint32_t token, const Slot& t, float (&cos)[V], float (&sin)[V])
+{
+    int64_t at = token;
+    if (a.at) at = a.wide ? static_cast<const int64_t*>(a.at)[token] : static_cast<const int32_t*>(a.at)[token];
+    const bool good = at >= 0 && static_cast<uint64_t>(at) < a.positions;
+    const uint64_t row = (good ? static_cast<uint64_t>(at) : 0) * (a.rotated / 2) + t.pair;
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+        const uint32_t count = t.pairs > static_cast<uint32_t>(i) ? t.pairs - i : 0;
+        float c[4], s[4];
+        Elem<float>::unpack(load_some<float>(a.cos + row + i, good ? (count < 4 ? count : 4) : 0), c);
+        Elem<float>::unpack(load_some<float>(a.sin + row + i, good ? (count < 4 ? count : 4) : 0), s);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            cos[i + k] = good ? c[k] : NAN;
+            sin[i + k] = good ? s[k] : NAN;
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void weights(const void* weight, const Slot& t, float (&w)[2][Elem<T>::kCount])
+{
+    constexpr int V = Elem<T>::kCount;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (weight) {
+            Elem<T>::unpack(load_some<T>(static_cast<const T*>(weight) + t.first[h], t.count[h]), w[h]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[h][i] = 1.0f;
+        }
+    }
+}
+
+__device__ __forceinline__ float chosen(bool first, float a, float b) { return first ? a : b; }
+
+template <int CONTROL> __device__ __forceinline__ float moved(float x)
+{
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CONTROL, 0xf, 0xf, true));
+}
+
+// The sum over a head's lanes, in each of them.  Up to 16 lanes the exchanges are operands of the sums.
+__device__ __forceinline__ float head_sum(float x, uint32_t lanes)
+{
+    if (lanes > 1) x += moved<0xb1>(x);                  // lane ^ 1
+    if (lanes > 2) x += moved<0x4e>(x);                  // lane ^ 2
+    if (lanes > 4) x += moved<0x141>(x);                 // 7 - lane of eight
+    if (lanes > 8) x += moved<0x140>(x);                 // 15 - lane of sixteen
+    if (lanes > 16) x += __shfl_xor(x, 16);
+    if (lanes > 32) x += __shfl_xor(x, 32);
+    return x;
+}
+
+template <typename T> __device__ __forceinline__ T* head_at(const HeadRows& q, const HeadRows& k, const RotaryArgs& a,
+                                                            uint32_t token, uint32_t head)
+{
+    char* const of_q = q.data + static_cast<uint64_t>(token) * q.row + static_cast<uint64_t>(head) * q.head;
+    char* const of_k = k.data + static_cast<uint64_t>(token) * k.row + (static_cast<uint64_t>(head) - a.heads) * k.head;
+    return reinterpret_cast<T*>(head < a.heads ? of_q : of_k);
+}
+
+// One wave takes U heads for each of its groups of lanes, all loads first.
+// 8192 tokens of 40 heads of 128 in bf16: see the operator's table of times.
+template <typename T, bool INTERLEAVED, int U> __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a)
+{
+    constexpr int V = Elem<T>::kCount;
+    const uint32_t lane = threadIdx.x % kWave, groups = kWave / a.lanes;
+    const uint64_t item = blockIdx.x * 4ull + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (item >= static_cast<uint64_t>(a.n) * a.chunks) return;
+    const uint32_t token = static_cast<uint32_t>(item / a.chunks);
+    const uint32_t first = static_cast<uint32_t>(item % a.chunks) * groups * U + lane / a.lanes;
+    const Slot t = slot_of<INTERLEAVED, V>(lane % a.lanes, a.dim, a.rotated);
+    u32x4_t raw[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t head = first + u * groups;
+        const bool there = head < a.all;
+        const T* from = head_at<T>(a.q, a.k, a, token, there ? head : 0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) raw[u][h] = load_some<T>(from + t.first[h], there ? t.count[h] : 0);
+    }
+    float cos[V], sin[V], w[2][2][V];
+    angles<V>(a, token, t, cos, sin);
+    weights<T>(a.q_weight, t, w[0]);
+    weights<T>(a.k_weight, t, w[1]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t head = first + u * groups;
+        const bool query = head < a.heads;
+        float x[2][V];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) Elem<T>::unpack(raw[u][h], x[h]);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum = __builtin_fmaf(x[1][i], x[1][i], __builtin_fmaf(x[0][i], x[0][i], sum));
+        sum = head_sum(sum, a.lanes);
+        if (query ? a.q_weight != nullptr : a.k_weight != nullptr) {
+            const float r = 1.0f / sqrtf(sum / static_cast<float>(a.dim) + a.eps);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[h][i] = x[h][i] * r * chosen(query, w[0][h][i], w[1][h][i]);
+        }
+        rotate<INTERLEAVED, V, false>(x, t, cos, sin);
+        if (head < a.all) {
+            T* to = head_at<T>(a.q_out, a.k_out, a, token, head);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) store_some<T>(to + t.first[h], t.count[h], x[h]);
+        }
+    }
+}
+
+// A wave goes over items like those above and keeps the sums for the weights in registers; a workgroup's are
+// added in the order of its waves, the workgroups' by join_kernel.
+template <typename T, bool INTERLEAVED, int U> __global__ __launch_bounds__(256) void rotary_grad_kernel(RotaryArgs a)
+{
+    constexpr int V = Elem<T>::kCount;
+    __shared__ float sums[4][2][kWave][2][V];
+    const uint32_t lane = threadIdx.x % kWave, groups = kWave / a.lanes;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const Slot t = slot_of<INTERLEAVED, V>(lane % a.lanes, a.dim, a.rotated);
+    float w[2][2][V], dw[2][2][V] = {};
+    weights<T>(a.q_weight, t, w[0]);
+    weights<T>(a.k_weight, t, w[1]);
+    const uint64_t items = static_cast<uint64_t>(a.n) * a.chunks;
+    for (uint64_t item = blockIdx.x * 4ull + wave; item < items; item += gridDim.x * 4ull) {
+        const uint32_t token = static_cast<uint32_t>(item / a.chunks);
+        const uint32_t first = static_cast<uint32_t>(item % a.chunks) * groups * U + lane / a.lanes;
+        u32x4_t raw_g[U][2], raw_x[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t head = first + u * groups;
+            const bool there = head < a.all, normed = head < a.heads ? a.q_weight != nullptr : a.k_weight != nullptr;
+            const T* g = head_at<T>(a.grad_q, a.grad_k, a, token, there ? head : 0);
+            const T* x = head_at<T>(a.q, a.k, a, token, there ? head : 0);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                raw_g[u][h] = load_some<T>(g + t.first[h], there ? t.count[h] : 0);
+                raw_x[u][h] = load_some<T>(x + t.first[h], there && normed ? t.count[h] : 0);
+            }
+        }
+        float cos[V], sin[V];
+        angles<V>(a, token, t, cos, sin);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t head = first + u * groups;
+            const bool query = head < a.heads, there = head < a.all;
+            float g[2][V], x[2][V];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                Elem<T>::unpack(raw_g[u][h], g[h]);
+                Elem<T>::unpack(raw_x[u][h], x[h]);
+            }
+            rotate<INTERLEAVED, V, true>(g, t, cos, sin);
+            float squares = 0.0f, products = 0.0f;
+            float gw[2][V];
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    gw[h][i] = g[h][i] * chosen(query, w[0][h][i], w[1][h][i]);
+                    squares = __builtin_fmaf(x[h][i], x[h][i], squares);
+                    products = __builtin_fmaf(gw[h][i], x[h][i], products);
+                }
+            squares = head_sum(squares, a.lanes);
+            products = head_sum(products, a.lanes);
+            if (query ? a.q_weight != nullptr : a.k_weight != nullptr) {
+                const float r = 1.0f / sqrtf(squares / static_cast<float>(a.dim) + a.eps);
+                const float mean = products * r / static_cast<float>(a.dim);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float unit = x[h][i] * r, share = there ? g[h][i] * unit : 0.0f;
+                        dw[0][h][i] += query ? share : 0.0f;
+                        dw[1][h][i] += query ? 0.0f : share;
+                        g[h][i] = r * __builtin_fmaf(-unit, mean, gw[h][i]);
+                    }
+            }
+            if (there) {
+                T* to = head_at<T>(a.q_out, a.k_out, a, token, head);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) store_some<T>(to + t.first[h], t.count[h], g[h]);
+            }
+        }
+    }
+    if (!a.partial) return;
+    for (uint32_t d = a.lanes; d < kWave; d <<= 1)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < V; ++i) dw[k][h][i] += __shfl_xor(dw[k][h][i], static_cast<int>(d));
+    if (lane < a.lanes)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < V; ++i) sums[wave][k][lane][h][i] = dw[k][h][i];
+    __syncthreads();
+    if (threadIdx.x >= 2 * a.lanes) return;
+    const uint32_t k = threadIdx.x / a.lanes, s = threadIdx.x % a.lanes;
+    const Slot to = slot_of<INTERLEAVED, V>(s, a.dim, a.rotated);
+    float* mine = a.partial + (static_cast<uint64_t>(blockIdx.x) * 2 + k) * a.dim;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i)
+            if (i < to.count[h])
+                mine[to.first[h] + i] = (sums[0][k][s][h][i] + sums[1][k][s][h][i]) + (sums[2][k][s][h][i] + sums[3][k][s][h][i]);
+}
+
+struct JoinArgs {
+    const float* partial;
+    void *q_weight, *k_weight;
+    uint32_t workers, dim;
+    int accumulate;
+};
+
+// Sixteen waves, 64 neighbouring sums to a workgroup: each takes a run of the workgroups' partial sums.
+template <typename W> __global__ __launch_bounds__(1024) void join_kernel(JoinArgs a)
+{
+    __shared__ float sums[16][kWave];
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const uint32_t at = blockIdx.x * kWave + lane;
+    const uint32_t run = ceil_div(a.workers, 16u), from = wave * run;
+    const uint32_t end = from + run < a.workers ? from + run : a.workers;
+    float sum = 0.0f;
+    if (at < 2 * a.dim)
+#pragma unroll 8
+        for (uint32_t k = from; k < end; ++k) sum += a.partial[static_cast<uint64_t>(k) * 2 * a.dim + at];
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave > 0 || at >= 2 * a.dim) return;
+    sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) sum += sums[k][lane];
+    W* to = static_cast<W*>(at < a.dim ? a.q_weight : a.k_weight);
+    if (!to) return;
+    to += at < a.dim ? at : at - a.dim;
+    *to = Elem<W>::from_f32(a.accumulate ? sum + Elem<W>::to_f32(*to) : sum);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+constexpr uint64_t kMostDim = 256;                       // 64 lanes of eight fp32
+constexpr uint64_t kMostWorkers = 512;                   // workgroups with partial sums
+
+bool reachable(const void* p) { return !p || la_ptr::device_accessible(p); }
+
+bool bad(const la_heads_t& h, int dtype)
+{
+    return !h.data || reinterpret_cast<uintptr_t>(h.data) % static_cast<uintptr_t>(dtype_bytes(dtype));
+}
+
+bool bad(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(dtype_bytes(dtype)); }
+
+HeadRows rows_of(const la_heads_t& h, int dtype)
+{
+    const uint64_t size = static_cast<uint64_t>(dtype_bytes(dtype));
+    return {static_cast<char*>(const_cast<void*>(h.data)), h.row_stride * size, h.head_stride * size};
+}
+
+int check_call(const la_rotary_t* call)
+{
+    if (!call) return LA_EINVAL;
+    const la_rotary_t& c = *call;
+    if (!is_float_dtype(c.dtype) || (c.at && c.at_dtype != LA_I32 && c.at_dtype != LA_I64)) return LA_EDTYPE;
+    constexpr uint64_t kMost = 1ull << 30;
+    if (c.dim == 0 || c.dim > kMostDim || c.rotated > c.dim || c.rotated % 2 || c.n > kMost || c.heads > kMost ||
+        c.kv_heads > kMost || (c.n > 0 && c.heads + c.kv_heads > kMost / c.n))
+        return LA_EINVAL;
+    if (c.n == 0 || c.heads + c.kv_heads == 0) return LA_OK;
+    if ((c.heads && bad(c.q_out, c.dtype)) || (c.kv_heads && bad(c.k_out, c.dtype)) || bad(c.q_weight, c.dtype) ||
+        bad(c.k_weight, c.dtype) || (c.at && bad(c.at, c.at_dtype)) || bad(c.cos, LA_F32) || bad(c.sin, LA_F32) ||
+        (c.rotated && (!c.cos || !c.sin)))
+        return LA_EINVAL;
+    return LA_OK;
+}
+
+int check_reach(const la_rotary_t& c)
+{
+    const void* all[] = {c.q.data, c.k.data, c.q_out.data, c.k_out.data, c.q_weight, c.k_weight, c.cos, c.sin, c.at};
+    for (const void* p : all)
+        if (!reachable(p)) return LA_EFAULT;
+    return LA_OK;
+}
+
+RotaryArgs args_of(const la_rotary_t& c)
+{
+    RotaryArgs a{};
+    a.q = rows_of(c.q, c.dtype);
+    a.k = rows_of(c.k, c.dtype);
+    a.q_out = rows_of(c.q_out, c.dtype);
+    a.k_out = rows_of(c.k_out, c.dtype);
+    a.q_weight = c.q_weight;
+    a.k_weight = c.k_weight;
+    a.cos = c.cos;
+    a.sin = c.sin;
+    a.at = c.at;
+    a.wide = c.at_dtype == LA_I64;
+    a.positions = c.positions;
+    a.n = static_cast<uint32_t>(c.n);
+    a.heads = static_cast<uint32_t>(c.heads);
+    a.all = static_cast<uint32_t>(c.heads + c.kv_heads);
+    a.dim = static_cast<uint32_t>(c.dim);
+    a.rotated = static_cast<uint32_t>(c.rotated);
+    a.eps = c.eps;
+    a.lanes = 1;
+    while (a.lanes < slots(a.dim, a.rotated, 16 / dtype_bytes(c.dtype))) a.lanes *= 2;
+    return a;
+}
+
+// Heads that a group of lanes takes at a time: up to `most`, as even as the token's heads allow; one
+// where there are too few tokens to fill the card otherwise.
+uint32_t heads_at_a_time(RotaryArgs& a, uint32_t most)
+{
+    const uint32_t each = ceil_div(a.all, kWave / a.lanes);
+    a.chunks = each;
+    if (static_cast<uint64_t>(a.n) * each <= 4096) return 1;
+    a.chunks = ceil_div(each, most);
+    const uint32_t u = ceil_div(each, a.chunks);
+    a.chunks = ceil_div(each, u);
+    return u;
+}
+
+template <typename T, bool INTERLEAVED> int forward(RotaryArgs& a, hipStream_t st)
+{
+    const uint32_t u = heads_at_a_time(a, 4);
+    const dim3 grid(static_cast<uint32_t>(ceil_div(static_cast<uint64_t>(a.n) * a.chunks, 4ull)));
+    switch (u) {
+    case 1: return launch(rotary_kernel<T, INTERLEAVED, 1>, grid, dim3(256), st, a);
+    case 2: return launch(rotary_kernel<T, INTERLEAVED, 2>, grid, dim3(256), st, a);
+    case 3: return launch(rotary_kernel<T, INTERLEAVED, 3>, grid, dim3(256), st, a);
+    default: return launch(rotary_kernel<T, INTERLEAVED, 4>, grid, dim3(256), st, a);
+    }
+}
+
+template <typename T> int forward(RotaryArgs& a, bool interleaved, hipStream_t st)
+{
+    return interleaved ? forward<T, true>(a, st) : forward<T, false>(a, st);
+}
+
+// Workgroups of a gradient's launch.
+uint64_t workers_of(const RotaryArgs& a)
+{
+    return std::min<uint64_t>(kMostWorkers, ceil_div(static_cast<uint64_t>(a.n) * a.chunks, 4ull));
+}
+
+template <typename T, bool INTERLEAVED> int backward(RotaryArgs& a, uint32_t u, hipStream_t st)
+{
+    const dim3 grid(static_cast<uint32_t>(workers_of(a)));
+    return u == 1 ? launch(rotary_grad_kernel<T, INTERLEAVED, 1>, grid, dim3(256), st, a)
+                  : launch(rotary_grad_kernel<T, INTERLEAVED, 2>, grid, dim3(256), st, a);
+}
+
+template <typename T> int backward(RotaryArgs& a, bool interleaved, uint32_t u, hipStream_t st)
+{
+    return interleaved ? backward<T, true>(a, u, st) : backward<T, false>(a, u, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int la_qk_norm_rotary(const la_rotary_t* call, la_stream_t stream)
+{
+    int rc = check_call(call);
+    if (rc != LA_OK) return rc;
+    const la_rotary_t& c = *call;
+    if (c.n == 0 || c.heads + c.kv_heads == 0) return LA_OK;
+    if ((c.heads && bad(c.q, c.dtype)) || (c.kv_heads && bad(c.k, c.dtype))) return LA_EINVAL;
+    rc = check_reach(c);
+    if (rc != LA_OK) return rc;
+    RotaryArgs a = args_of(c);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (c.dtype == LA_F32) return forward<float>(a, c.interleaved != 0, st);
+    return c.dtype == LA_BF16 ? forward<__bf16>(a, c.interleaved != 0, st) : forward<_Float16>(a, c.interleaved != 0, st);
+}
+
+uint64_t la_qk_norm_rotary_grad_workspace(const la_rotary_t* call)
+{
+    if (!call || call->dim > kMostDim || !(call->q_weight || call->k_weight)) return 0;
+    return kMostWorkers * 2 * call->dim * sizeof(float);
+}
+
+int la_qk_norm_rotary_grad(const la_rotary_t* call, void* workspace, uint64_t workspace_bytes, la_stream_t stream)
+{
+    int rc = check_call(call);
+    if (rc != LA_OK) return rc;
+    const la_rotary_t& c = *call;
+    const bool normed = c.q_weight || c.k_weight;
+    if (normed && c.weight_grad_dtype != c.dtype && c.weight_grad_dtype != LA_F32) return LA_EDTYPE;
+    if (normed && ((c.q_weight && (!c.grad_q_weight || bad(c.grad_q_weight, c.weight_grad_dtype))) ||
+                   (c.k_weight && (!c.grad_k_weight || bad(c.grad_k_weight, c.weight_grad_dtype)))))
+        return LA_EINVAL;
+    const bool any = c.n > 0 && c.heads + c.kv_heads > 0;
+    if (any && ((c.heads && (bad(c.grad_q, c.dtype) || (c.q_weight && bad(c.q, c.dtype)))) ||
+                (c.kv_heads && (bad(c.grad_k, c.dtype) || (c.k_weight && bad(c.k, c.dtype))))))
+        return LA_EINVAL;
+    rc = check_workspace(workspace, workspace_bytes, la_qk_norm_rotary_grad_workspace(call), 16);
+    if (rc != LA_OK) return rc;
+    if (any) rc = check_reach(c);
+    if (rc == LA_OK && (!reachable(c.grad_q_weight) || !reachable(c.grad_k_weight) || (normed && !reachable(workspace)) ||
+                        (any && (!reachable(c.grad_q.data) || !reachable(c.grad_k.data)))))
+        rc = LA_EFAULT;
+    if (rc != LA_OK) return rc;
+    RotaryArgs a = args_of(c);
+    a.grad_q = rows_of(c.grad_q, c.dtype);
+    a.grad_k = rows_of(c.grad_k, c.dtype);
+    a.partial = normed ? static_cast<float*>(workspace) : nullptr;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    uint64_t workers = 0;
+    if (any) {
+        const uint32_t u = heads_at_a_time(a, 2);
+        workers = workers_of(a);
+        const bool interleaved = c.interleaved != 0;
+        rc = c.dtype == LA_F32    ? backward<float>(a, interleaved, u, st)
+             : c.dtype == LA_BF16 ? backward<__bf16>(a, interleaved, u, st)
+                                  : backward<_Float16>(a, interleaved, u, st);
+        if (rc != LA_OK) return rc;
+    }
+    if (!normed) return LA_OK;
+    const JoinArgs j{a.partial, c.q_weight ? c.grad_q_weight : nullptr, c.k_weight ? c.grad_k_weight : nullptr,
+                     static_cast<uint32_t>(workers), a.dim, c.accumulate};
+    const dim3 grid(ceil_div(2 * a.dim, kWave));
+    return c.weight_grad_dtype == LA_F32    ? launch(join_kernel<float>, grid, dim3(1024), st, j)
+           : c.weight_grad_dtype == LA_BF16 ? launch(join_kernel<__bf16>, grid, dim3(1024), st, j)
+                                            : launch(join_kernel<_Float16>, grid, dim3(1024), st, j);
+}
+
+}  // extern "C"

@@ -1,10 +1,13 @@
-"""The operators at a language model's two ends, on MI355X.
+"""The operators of a language model, on MI355X.
 
-What lies outside the decoder layers of the model whose layers ``LayerAdam``
-steps: the embedding matrix, the norms, and the vocabulary matrix with the loss.
+What lies around the matrix products of the model whose layers ``LayerAdam`` steps: at
+its two ends the embedding matrix, the norms, and the vocabulary matrix with the loss;
+inside a decoder layer the attention.
 
 ``embedding`` / ``embedding_grad``            rows of a matrix by token, and the matrix's gradient
 ``rms_norm`` / ``rms_norm_8bit`` / ``rms_norm_grad``   the residual's addition and the norm over it
+``qk_norm_rotary`` / ``qk_norm_rotary_grad``  the norm of each query and key head, and the rotation by position
+``attention`` / ``attention_grad``            softmax attention over packed or padded sequences, or a cache
 ``linear_cross_entropy`` / ``linear_cross_entropy_grad``  the loss, a tile of scores at a time; with its gradients,
                                               a piece of the rows' softmax at a time
 
@@ -15,7 +18,10 @@ micro-batch, or the other use of tied weights).  Nothing is recorded for autogra
 outputs never require grad, whatever the inputs do.
 
 Matrices have two dimensions; ``embedding`` of tokens [batch, length] returns
-[batch, length, hidden], whose ``flatten(0, 1)`` the other calls take.
+[batch, length, hidden], whose ``flatten(0, 1)`` the other calls take.  Heads are the
+last two dimensions, [.., heads, dim]: a view of a projection's output
+(``qkv[:, :n].unflatten(1, (heads, dim))``), or in any order of memory in which a head's elements are
+contiguous.
 
 All tensors live on one HIP device.  Calls are asynchronous on the current
 stream, or on ``stream``; results of one call belong to that stream.  Rows may be
@@ -35,8 +41,9 @@ import torch
 from . import _lib, _ops_lib
 from .layer_adam import _on_device, _raw_current_stream, _stream_handle, _torch_stream
 
-__all__ = ["embedding", "embedding_grad", "rms_norm", "rms_norm_8bit", "rms_norm_grad", "linear_cross_entropy",
-           "linear_cross_entropy_grad", "PIECE_BYTES"]
+__all__ = ["embedding", "embedding_grad", "rms_norm", "rms_norm_8bit", "rms_norm_grad", "qk_norm_rotary",
+           "qk_norm_rotary_grad", "attention", "attention_grad", "linear_cross_entropy", "linear_cross_entropy_grad",
+           "PIECE_BYTES"]
 
 _FLOAT = {torch.float32: _lib.LA_F32, torch.bfloat16: _lib.LA_BF16, torch.float16: _lib.LA_F16}
 _TOKEN = {torch.int32: _ops_lib.LA_I32, torch.int64: _ops_lib.LA_I64}
@@ -299,6 +306,292 @@ def rms_norm_grad(grad_out: torch.Tensor, summed: torch.Tensor, rstd: torch.Tens
             grad_x.data_ptr(), hidden, _FLOAT[grad_weight.dtype], grad_weight.data_ptr(), int(accumulate),
             work.data_ptr(), size, s.handle), "la_rms_norm_grad")
     return grad_x, grad_weight
+
+
+# ---------------------------------------------------------------------------
+# heads
+# ---------------------------------------------------------------------------
+def _heads(t: torch.Tensor, name: str, device, dims: int, dtype=None, shape=None) -> "_ops_lib.LaHeads":
+    """Check [.., heads, dim] and describe where it lies."""
+    if t.device != device or not t.is_cuda:
+        raise RuntimeError(f"{name} on {t.device}, expected a HIP device"
+                           + (f" ({device})" if device.type == "cuda" else ""))
+    if t.dim() != dims:
+        raise RuntimeError(f"{name} must have {dims} dimensions, got {tuple(t.shape)}")
+    if shape is not None and t.shape != shape:
+        raise RuntimeError(f"size mismatch: {name} is {tuple(t.shape)}, expected {tuple(shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise RuntimeError(f"{name} is {t.dtype}, expected {dtype}")
+    if t.dtype not in _FLOAT:
+        raise RuntimeError(f"unsupported dtype of {name}: {t.dtype}")
+    strides = t.stride()
+    if t.numel() and t.shape[-1] > 1 and strides[-1] != 1:
+        raise RuntimeError(f"the heads of {name} must be contiguous")
+    return _ops_lib.LaHeads(data=t.data_ptr(), batch_stride=strides[0] if dims == 4 else 0, row_stride=strides[-3],
+                            head_stride=strides[-2])
+
+
+def _result(t: torch.Tensor, name: str, device, dims: int, dtype, shape) -> "_ops_lib.LaHeads":
+    """The same for a tensor to write: no two of its elements may be one."""
+    got = _heads(t, name, device, dims, dtype, shape)
+    span = t.shape[-1]
+    for stride, size in sorted((s, n) for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+        if t.numel() and stride < span:
+            raise RuntimeError(f"the heads of {name} overlap: strides {t.stride()}")
+        span = stride * (size - 1) + span
+    return got
+
+
+def _indices(t: Optional[torch.Tensor], name: str, device, size: int, dtype=None) -> Optional[int]:
+    if t is None:
+        return None
+    _vector(t, name, device, size, _TOKEN)
+    if dtype is not None and t.dtype != dtype:
+        raise RuntimeError(f"{name} is {t.dtype}, expected {dtype}")
+    return t.data_ptr()
+
+
+def _rotary_call(q, k, like_q, like_k, cos, sin, q_weight, k_weight, positions, eps, interleaved):
+    """The call without its results.  like_q, like_k: what the sizes are those of."""
+    device, dtype = like_q.device, like_q.dtype
+    of_q, of_k = _heads(like_q, "q", device, 3), _heads(like_k, "k", device, 3, dtype)
+    n, heads, dim = like_q.shape
+    if like_k.shape[0] != n or like_k.shape[2] != dim:
+        raise RuntimeError(f"size mismatch: k is {tuple(like_k.shape)}, expected ({n}, any, {dim})")
+    if dim > 256 or dim == 0:
+        raise RuntimeError(f"heads of {dim} elements are not supported (1 to 256)")
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        if t.device != device:
+            raise RuntimeError(f"{name} on {t.device}, expected {device}")
+        if t.dim() != 2 or t.shape != cos.shape or 2 * t.shape[1] > dim:
+            raise RuntimeError(f"size mismatch: {name} is {tuple(t.shape)}, expected two tables [positions, pairs] of at "
+                               f"most {dim // 2} pairs")
+        if t.dtype != torch.float32 or not t.is_contiguous():
+            raise RuntimeError(f"{name} must be a contiguous torch.float32 table, got {t.dtype}")
+    call = _ops_lib.LaRotary(
+        dtype=_FLOAT[dtype], n=n, heads=heads, kv_heads=like_k.shape[1], dim=dim, rotated=2 * cos.shape[1], eps=eps,
+        cos=cos.data_ptr(), sin=sin.data_ptr(), positions=cos.shape[0], interleaved=int(interleaved),
+        at=_indices(positions, "positions", device, n))
+    if positions is not None:
+        call.at_dtype = _TOKEN[positions.dtype]
+    for weight, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if weight is not None:
+            _vector(weight, name, device, dim, (dtype,))
+            setattr(call, name, weight.data_ptr())
+    if q is like_q:
+        call.q = of_q
+    elif q is not None:
+        call.q = _heads(q, "q", device, 3, dtype, like_q.shape)
+    if k is like_k:
+        call.k = of_k
+    elif k is not None:
+        call.k = _heads(k, "k", device, 3, dtype, like_k.shape)
+    return device, call, of_q, of_k
+
+
+def _rotary_out(call, out, q, k, device, s):
+    if out is None:
+        out = s.empty(q.shape, q.dtype), s.empty(k.shape, k.dtype)
+    call.q_out = _result(out[0], "out[0]", device, 3, q.dtype, q.shape)
+    call.k_out = _result(out[1], "out[1]", device, 3, q.dtype, k.shape)
+    return out
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
+                   q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                   positions: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                   out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                   stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The root-mean-square norm of every query and key head, then the rotation by position.
+
+    q: [n, heads, dim], k: [n, kv_heads, dim], of one type.  ``q_weight``, ``k_weight``: the
+    norms' scales [dim]; without one its heads are not normed.  ``cos``, ``sin``: fp32 tables
+    [positions, pairs]; the first ``2 * pairs`` elements of a head turn, (a, b) -> (a cos - b sin, b cos + a sin), pair
+    j of elements (j, j + pairs), or (2 j, 2 j + 1) if ``interleaved``.  ``positions``: int32 or int64
+    [n], row i of the tables for row i by default; one outside the tables makes the rotated elements NaN.
+    ``out``: the two tensors to write instead of new ones, q and k themselves for instance, or rows
+    of a cache.  All in fp32, rounded once."""
+    device, call, _, _ = _rotary_call(q, k, q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved)
+    lib = _ops_lib.load()
+    with _on_device(device), _Scratch(device, stream) as s:
+        out = _rotary_out(call, out, q, k, device, s)
+        _check(lib.la_qk_norm_rotary(ctypes.byref(call), s.handle), "la_qk_norm_rotary")
+    return out
+
+
+def qk_norm_rotary_grad(grad_q: torch.Tensor, grad_k: torch.Tensor, q: Optional[torch.Tensor],
+                        k: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, *,
+                        q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                        positions: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                        grad_q_weight: Optional[torch.Tensor] = None, grad_k_weight: Optional[torch.Tensor] = None,
+                        accumulate: bool = False, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None, stream=None):
+    """The gradients of ``qk_norm_rotary`` towards its q, k and weights, from those of its results.
+
+    q and k are its inputs (None will do for heads that are not normed).  ``out``: where the
+    gradients of q and k go, new tensors by default; ``grad_q`` and ``grad_k`` themselves may be written
+    over.  ``grad_q_weight``, ``grad_k_weight``: the tensors [dim] to write (of the weights' type or
+    float32, both of one; new by default), added to with ``accumulate``.  Returns ``(grad_q, grad_k,
+    grad_q_weight, grad_k_weight)``, None for a weight that there is not.  Sums are fp32 in a fixed order."""
+    for x, weight, name in ((q, q_weight, "q"), (k, k_weight, "k")):
+        if x is None and weight is not None:
+            raise RuntimeError(f"the gradient of a norm needs {name}, which was normed")
+    device, call, call_grad_q, call_grad_k = _rotary_call(q, k, grad_q, grad_k, cos, sin, q_weight, k_weight, positions,
+                                                          eps, interleaved)
+    call.grad_q, call.grad_k = call_grad_q, call_grad_k
+    grads = [grad_q_weight, grad_k_weight]
+    for g, weight, name in ((grad_q_weight, q_weight, "grad_q_weight"), (grad_k_weight, k_weight, "grad_k_weight")):
+        if g is not None:
+            if weight is None:
+                raise RuntimeError(f"{name} without its weight")
+            _vector(g, name, device, weight.numel(), (weight.dtype, torch.float32))
+        elif accumulate and weight is not None:
+            raise RuntimeError(f"accumulate needs a {name} to add to")
+    given = {g.dtype for g in grads if g is not None}
+    if len(given) > 1:
+        raise RuntimeError("grad_q_weight and grad_k_weight must be of one type")
+    kind = given.pop() if given else grad_q.dtype
+    lib = _ops_lib.load()
+    with _on_device(device), _Scratch(device, stream) as s:
+        out = _rotary_out(call, out, grad_q, grad_k, device, s)
+        for i, weight in enumerate((q_weight, k_weight)):
+            if weight is not None and grads[i] is None:
+                grads[i] = s.empty((weight.numel(),), kind)
+        call.weight_grad_dtype, call.accumulate = _FLOAT[kind], int(accumulate)
+        call.grad_q_weight, call.grad_k_weight = (None if g is None else g.data_ptr() for g in grads)
+        size = lib.la_qk_norm_rotary_grad_workspace(ctypes.byref(call))
+        work = s.workspace(size)
+        _check(lib.la_qk_norm_rotary_grad(ctypes.byref(call), work.data_ptr(), size, s.handle),
+               "la_qk_norm_rotary_grad")
+    return (*out, *grads)
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+def _attention_call(q, k, v, causal, window, scale, starts, key_starts, lengths, key_lengths):
+    device, dims = q.device, q.dim()
+    if dims not in (3, 4):
+        raise RuntimeError(f"q must have three dimensions (packed) or four (a batch), got {tuple(q.shape)}")
+    of_q = _heads(q, "q", device, dims)
+    of_k = _heads(k, "k", device, dims, q.dtype)
+    of_v = _heads(v, "v", device, dims, q.dtype, k.shape)
+    if q.dtype == torch.float32:
+        raise RuntimeError("unsupported dtype of q: torch.float32 (bfloat16 or float16)")
+    rows, heads, dim = q.shape[-3:]
+    key_rows, kv_heads = k.shape[-3:-1]
+    if k.shape[-1] != dim or dims == 4 and k.shape[0] != q.shape[0]:
+        raise RuntimeError(f"size mismatch: k is {tuple(k.shape)}, expected "
+                           f"({f'{q.shape[0]}, ' if dims == 4 else ''}any, any, {dim})")
+    if kv_heads == 0 or heads == 0 or heads % kv_heads:
+        raise RuntimeError(f"{heads} query heads cannot share {kv_heads} key heads evenly")
+    if dim == 0 or dim > 128:
+        raise RuntimeError(f"heads of {dim} elements are not supported (1 to 128)")
+    if window is not None and (window < 1 or not causal):
+        raise RuntimeError(f"window must be at least 1 and goes with causal, got {window}")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < float("inf"):
+        raise RuntimeError(f"scale must be above 0 and finite, got {scale}")
+    call = _ops_lib.LaAttention(dtype=_FLOAT[q.dtype], rows=rows, key_rows=key_rows, heads=heads, kv_heads=kv_heads,
+                                dim=dim, q=of_q, k=of_k, v=of_v, causal=int(bool(causal)), window=window or 0, scale=scale)
+    if dims == 3:
+        if starts is None:
+            raise RuntimeError("packed sequences need starts")
+        if lengths is not None or key_lengths is not None:
+            raise RuntimeError("lengths go with a batch (four dimensions); packed sequences have starts")
+        if starts.numel() < 2:
+            raise RuntimeError("starts must have an element more than there are sequences, and at least two")
+        if key_starts is None and rows != key_rows:
+            raise RuntimeError(f"size mismatch: {rows} queries and {key_rows} keys need key_starts")
+        call.batch = starts.numel() - 1
+        first = starts
+        call.starts = _indices(starts, "starts", device, starts.numel())
+        call.key_starts = _indices(key_starts, "key_starts", device, starts.numel(), starts.dtype)
+    else:
+        if starts is not None or key_starts is not None:
+            raise RuntimeError("starts go with packed sequences (three dimensions); a batch has lengths")
+        if key_lengths is None and lengths is not None:
+            if rows != key_rows:
+                raise RuntimeError(f"size mismatch: lengths of {rows} queries with {key_rows} keys need key_lengths")
+            key_lengths = lengths
+        call.batch = q.shape[0]
+        first = lengths if lengths is not None else key_lengths
+        call.lengths = _indices(lengths, "lengths", device, q.shape[0])
+        call.key_lengths = _indices(key_lengths, "key_lengths", device, q.shape[0],
+                                    None if lengths is None else lengths.dtype)
+    if first is not None:
+        call.index_dtype = _TOKEN[first.dtype]
+    return device, call
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = True, window: Optional[int] = None,
+              scale: Optional[float] = None, starts: Optional[torch.Tensor] = None,
+              key_starts: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+              key_lengths: Optional[torch.Tensor] = None, stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Softmax attention: ``(out, lse)``, out like q and the fp32 log-sum-exp of every row's scores.
+
+    A batch: q [batch, length, heads, dim], k and v [batch, key_length, kv_heads, dim], of which sequence b
+    has the first ``lengths[b]`` queries and ``key_lengths[b]`` keys (all without them; ``key_lengths`` are ``lengths``
+    by default).  A step of generation is a batch of length 1 against a cache with ``key_lengths``.
+    Packed sequences: q [n, heads, dim], k and v [m, kv_heads, dim], sequence b the rows ``starts[b]`` to
+    ``starts[b + 1]``, its keys by ``key_starts`` (``starts`` by default); indices do not decrease.
+    All indices are int32 or int64 on the device, of one type.
+
+    heads may be a multiple of kv_heads: neighbouring query heads share a key head.  dim is at most
+    128; bfloat16 or float16.  ``causal``: a sequence's last query sees its last key, each query before it one key
+    less; ``window``: of these only the last ``window``.  ``scale``: ``dim ** -0.5`` by default.
+
+    A row that sees no key, or is of no sequence, has out 0 and lse -inf.  Keys and values beyond a
+    sequence's are not looked at, whatever they hold; one that is NaN or infinite inside a sequence may also reach
+    rows that do not see it, as it does in a product with a probability of 0.  Statistics and sums are fp32,
+    in a fixed order; probabilities are rounded to the operands' 16 bits."""
+    device, call = _attention_call(q, k, v, causal, window, scale, starts, key_starts, lengths, key_lengths)
+    lib = _ops_lib.load()
+    with _on_device(device), _Scratch(device, stream) as s:
+        out = s.empty(q.shape, q.dtype)
+        lse = s.empty(q.shape[:-1], torch.float32)
+        if out.numel() == 0:
+            return out, lse
+        call.out, call.lse = _heads(out, "out", device, q.dim()), lse.data_ptr()
+        size = lib.la_attention_workspace(ctypes.byref(call))
+        work = s.workspace(size)
+        _check(lib.la_attention(ctypes.byref(call), work.data_ptr(), size, s.handle), "la_attention")
+    return out, lse
+
+
+def attention_grad(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                   lse: torch.Tensor, *, causal: bool = True, window: Optional[int] = None,
+                   scale: Optional[float] = None, starts: Optional[torch.Tensor] = None,
+                   key_starts: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                   key_lengths: Optional[torch.Tensor] = None,
+                   grads: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None,
+                   stream=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The gradients of ``attention`` towards q, k and v, from that of its out.
+
+    ``out`` and ``lse`` are its results, the other arguments those that it had.  Probabilities are computed
+    again.  ``grads``: the three tensors to write, like q, k and v (parts of one projection's gradient,
+    for instance); rows of no sequence stay as they were in them.  Without it they are new, and zero there.
+    The gradients of a key head are sums over the query heads that share it.  Sums are fp32 in a fixed
+    order: equal calls give equal bits."""
+    device, call = _attention_call(q, k, v, causal, window, scale, starts, key_starts, lengths, key_lengths)
+    dims = q.dim()
+    call.grad_out = _heads(grad_out, "grad_out", device, dims, q.dtype, q.shape)
+    call.out = _heads(out, "out", device, dims, q.dtype, q.shape)
+    _vector(lse, "lse", device, q.numel() // q.shape[-1], (torch.float32,))
+    call.lse = lse.data_ptr()
+    if grads is not None:
+        call.keep_rest = 1
+    lib = _ops_lib.load()
+    with _on_device(device), _Scratch(device, stream) as s:
+        if grads is None:
+            grads = tuple(s.empty(t.shape, t.dtype) for t in (q, k, v))
+        call.grad_q, call.grad_k, call.grad_v = (_result(g, name, device, dims, q.dtype, t.shape) for g, t, name in
+                                                 zip(grads, (q, k, v), ("grad_q", "grad_k", "grad_v")))
+        if q.numel() == 0 and k.numel() == 0:
+            return grads
+        size = lib.la_attention_grad_workspace(ctypes.byref(call))
+        work = s.workspace(size)
+        _check(lib.la_attention_grad(ctypes.byref(call), work.data_ptr(), size, s.handle), "la_attention_grad")
+    return grads
 
 
 # ---------------------------------------------------------------------------
