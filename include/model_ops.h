@@ -152,7 +152,6 @@ typedef struct {
  * A row that sees no key has out 0 and lse -inf; so has a row of no sequence.  What lies
  * beyond a sequence's keys is never looked at, whatever it holds.
  * dtype (of all heads): LA_BF16 or LA_F16; dim at most 128; scale above 0.
- * lse: fp32 [batch][rows][heads], or [rows][heads].
  * workspace: la_attention_workspace(call) bytes, 256-byte aligned: partial results where
  * the keys of few rows are shared out among workgroups, and copies of what does not lie
  * in whole 16-byte chunks.  Sums are fp32 in a fixed order.
@@ -161,7 +160,7 @@ typedef struct {
     int dtype;
     uint64_t batch, rows, key_rows, heads, kv_heads, dim;
     la_heads_t q, k, v, out;
-    float* lse;
+    la_heads_t lse;           /* of fp32, one to a head */
     int index_dtype;
     const void* starts;
     const void* key_starts;

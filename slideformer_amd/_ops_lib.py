@@ -101,7 +101,7 @@ class LaAttention(ctypes.Structure):
         ("k", LaHeads),
         ("v", LaHeads),
         ("out", LaHeads),
-        ("lse", ctypes.c_void_p),
+        ("lse", LaHeads),
         ("index_dtype", ctypes.c_int),
         ("starts", ctypes.c_void_p),
         ("key_starts", ctypes.c_void_p),

@@ -24,8 +24,7 @@ using namespace att;
 constexpr uint32_t kMostParts = 64;                      // the join has a lane for each
 
 struct ForwardArgs {
-    Heads q, k, v, out;
-    float* lse;                     // [rows][heads]
+    Heads q, k, v, out, lse;
     float* partial;                 // of each part: [part][row][D], then lse in base 2: [part][row]
     Sequences seq;
     uint32_t heads, kv_heads, dim;  // dim: of the result
@@ -148,6 +147,8 @@ __device__ __forceinline__ void store_eight(char* row, uint32_t at, uint32_t dim
     }
 }
 
+__device__ __forceinline__ void put(const char* to, float x) { *reinterpret_cast<float*>(const_cast<char*>(to)) = x; }
+
 // The wave's 32 rows, rows `first` of the piece on, to the result or to this part's partial one.
 template <typename T, int D>
 __device__ __forceinline__ void finish(const ForwardArgs& a, const Piece& p, uint32_t kv_head, uint32_t part, uint32_t row,
@@ -187,7 +188,9 @@ __device__ __forceinline__ void finish(const ForwardArgs& a, const Piece& p, uin
             for (int i = 0; i < 8; ++i) v[i] *= scale;
             if (there) store_eight<T>(to, d * 32 + j * 16 + half * 8, a.dim, a.aligned, v);
         }
-    if (there && half == 0) a.lse[flat] = sum == 0.0f ? -INFINITY : st.top * a.scale + __builtin_amdgcn_logf(sum) * kLn2;
+    if (there && half == 0)
+        put(a.lse.at(p.batch, p.first + token, head),
+            sum == 0.0f ? -INFINITY : st.top * a.scale + __builtin_amdgcn_logf(sum) * kLn2);
 }
 
 // This lane's row as the second operand of the scores: elements 16 k + 8 (l / 32) .. + 7.
@@ -410,7 +413,8 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void few_rows_
             a.partial[static_cast<uint64_t>(a.parts) * a.rows_all * D + static_cast<uint64_t>(part) * a.rows_all + flat] =
                 row_sum == 0.0f ? -INFINITY : row_top * factor + __builtin_amdgcn_logf(row_sum);
         else
-            a.lse[flat] = row_sum == 0.0f ? -INFINITY : row_top * a.scale + __builtin_amdgcn_logf(row_sum) * kLn2;
+            put(a.lse.at(p.batch, p.first + out_token, head),
+                row_sum == 0.0f ? -INFINITY : row_top * a.scale + __builtin_amdgcn_logf(row_sum) * kLn2);
     }
 }
 
@@ -456,7 +460,9 @@ template <typename T, int D> __global__ __launch_bounds__(256) void join_kernel(
     const uint32_t head = flat % a.heads, row = flat / a.heads;
     char* to = const_cast<char*>(a.out.at(row / a.seq.rows, row % a.seq.rows, head));
     if (lane < kLanes) store_eight<T>(to, lane * 8, a.dim, a.aligned, v);
-    if (lane == 0) a.lse[flat] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (lane == 0)
+        put(a.lse.at(row / a.seq.rows, row % a.seq.rows, head),
+            sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2);
 }
 
 // ---------------------------------------------------------------------------
@@ -529,7 +535,7 @@ int la_attention(const la_attention_t* call, void* workspace, uint64_t workspace
     if (rc != LA_OK) return rc;
     const la_attention_t& c = *call;
     if (flat_rows(c) == 0) return LA_OK;
-    if (!there(c.q) || !there(c.out) || !c.lse || reinterpret_cast<uintptr_t>(c.lse) % 4 ||
+    if (!there(c.q) || !there(c.out) || !there_fp32(c.lse) ||
         (flat_keys(c) > 0 && (!there(c.k) || !there(c.v))))
         return LA_EINVAL;
     const Plan p = plan_of(c);
@@ -537,7 +543,7 @@ int la_attention(const la_attention_t* call, void* workspace, uint64_t workspace
     if (rc != LA_OK) return rc;
     if (p.pieces * c.kv_heads >> 31) return LA_EINVAL;
     if (!reachable(c.q.data) || !reachable(c.k.data) || !reachable(c.v.data) || !reachable(c.out.data) ||
-        !reachable(c.lse) || !indices_reachable(c) || (la_attention_workspace(call) && !reachable(workspace)))
+        !reachable(c.lse.data) || !indices_reachable(c) || (la_attention_workspace(call) && !reachable(workspace)))
         return LA_EFAULT;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
@@ -549,7 +555,7 @@ int la_attention(const la_attention_t* call, void* workspace, uint64_t workspace
     if (rc == LA_OK) rc = heads_of(c, c.v, false, a.v, ws, st);
     if (rc != LA_OK) return rc;
     a.out = plain(c.out);
-    a.lse = c.lse;
+    a.lse = plain(c.lse, 4);
     a.seq = sequences_of(c);
     a.heads = static_cast<uint32_t>(c.heads);
     a.kv_heads = static_cast<uint32_t>(c.kv_heads);

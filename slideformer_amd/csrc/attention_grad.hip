@@ -25,10 +25,9 @@ namespace {
 using namespace att;
 
 struct GradArgs {
-    Heads q, k, v, out, grad_out;
+    Heads q, k, v, out, grad_out, lse;
     Heads grad_q, grad_k, grad_v;
-    const float* lse;
-    float *lse2, *delta;            // [heads][flat rows]: lse in base 2, and delta, by grad_q_kernel
+    float *less, *delta;            // [heads][flat rows], by grad_q_kernel: minus lse in base 2, and delta
     Sequences seq;
     uint32_t heads, kv_heads, dim, read_dim;
     uint32_t rows_all;              // flat rows
@@ -37,19 +36,29 @@ struct GradArgs {
     int keep_rest;
 };
 
+// Waits until what wrote these sums has, and what reads them may: longer than any matrix instruction needs.
+template <int N> __device__ __forceinline__ void settle(f32x16 (&x)[N])
+{
+#pragma unroll
+    for (int n = 0; n < N; ++n) asm volatile("" : "+a"(x[n]));
+    asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15");
+#pragma unroll
+    for (int n = 0; n < N; ++n) asm volatile("" : "+a"(x[n]));
+}
+
 // dS in the operands' 16 bits.  bfloat16 has fp32's range.  fp16 has not: what a wave rounds is brought near the
 // top of its range by a power of two for each column, which shrinks when a larger value comes, and its
 // sums with it; P, at most 1, by a fixed one.
 template <typename T> struct Range {
     static constexpr float kP = 0.0f;
     __device__ __forceinline__ float factor() const { return 1.0f; }
-    template <int N> __device__ __forceinline__ void fit(f32x16&, f32x16 (&)[N]) {}
+    template <bool SETTLE, int N> __device__ __forceinline__ void fit(f32x16&, f32x16 (&)[N]) {}
 };
 template <> struct Range<_Float16> {
     static constexpr float kP = 14.0f;                   // P is held times 2^14
     float up = 0x1p60f;
     __device__ __forceinline__ float factor() const { return up; }
-    template <int N> __device__ __forceinline__ void fit(f32x16& x, f32x16 (&sums)[N])
+    template <bool SETTLE, int N> __device__ __forceinline__ void fit(f32x16& x, f32x16 (&sums)[N])
     {
         float most = 0.0f;
 #pragma unroll
@@ -64,8 +73,10 @@ template <> struct Range<_Float16> {
             const float now = most * up > 32768.0f && most < INFINITY ? __builtin_ldexpf(1.0f, e) : up;
             const float shrink = now / up;
             up = now;
+            if constexpr (SETTLE) settle(sums);
 #pragma unroll
             for (int n = 0; n < N; ++n) sums[n] *= shrink;
+            if constexpr (SETTLE) settle(sums);
         }
         x *= up;
     }
@@ -171,10 +182,10 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_q_ke
         for (int i = 0; i < 16; ++i) found = c / 8 * 4 + c % 4 == static_cast<uint32_t>(i) ? x[i] : found;
         const Halves h = halves(__float_as_uint(found), __float_as_uint(found));
         delta = __uint_as_float(c / 4 % 2 ? h.hi : h.lo);
-        lse2 = there ? a.lse[flat * a.heads + head] * kLog2E : 0.0f;
+        lse2 = there ? *reinterpret_cast<const float*>(a.lse.at(p.batch, p.first + token, head)) * kLog2E : 0.0f;
         if (there && lane < 32) {
             const uint64_t at = static_cast<uint64_t>(head) * a.rows_all + flat;
-            a.lse2[at] = lse2;
+            a.less[at] = Range<T>::kP - lse2;
             a.delta[at] = delta;
         }
         asm volatile("" : "+v"(lse2));
@@ -231,7 +242,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_q_ke
                 for (int i = 0; i < 16; ++i)
                     d[i] = exp2_of(__builtin_fmaf(s[i], factor, -lse2)) * (d[i] - delta);
                 if (partly) hide(d, first_key + b * 32, mine);
-                scaled.fit(d, sums);
+                scaled.template fit<false>(d, sums);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const s16x8 ds = rounded<T>(d, half);
@@ -246,13 +257,183 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_q_ke
                     a.dim, a.q_aligned);
 }
 
-// 128 keys to a workgroup, 32 to a wave; all waves go over the same tiles of 64 rows of one query
-// head after the other.
-template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_kv_kernel(GradArgs a)
+// The products of grad_kv_kernel, in assembly: the sums stay in accumulation registers, and so do a wave's own
+// keys and values; left to itself the compiler moves them to and fro.  It adds no wait states
+// to these.  Their first operands come from LDS and need none, P and dS are settled before the sums begin, and
+// scores are read no sooner than a phase later.
+template <typename T> __device__ __forceinline__ void add_product(f32x16& c, const s16x8& a, const s16x8& b);
+template <> __device__ __forceinline__ void add_product<__bf16>(f32x16& c, const s16x8& a, const s16x8& b)
 {
-    constexpr uint32_t kBytes = Tile<D>::kBytes;
-    constexpr uint32_t kRowValues = kTileRows * 4;       // bytes of a tile's lse, and of its delta
-    __shared__ __attribute__((aligned(1024))) char shared[4 * kBytes + 4 * 4 * kRowValues];
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+template <> __device__ __forceinline__ void add_product<_Float16>(f32x16& c, const s16x8& a, const s16x8& b)
+{
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+template <typename T> __device__ __forceinline__ void score(f32x16& c, const s16x8& a, const s16x8& b, bool first);
+template <> __device__ __forceinline__ void score<__bf16>(f32x16& c, const s16x8& a, const s16x8& b, bool first)
+{
+    if (first) asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "a"(b));
+    else asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "a"(b));
+}
+template <> __device__ __forceinline__ void score<_Float16>(f32x16& c, const s16x8& a, const s16x8& b, bool first)
+{
+    if (first) asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "a"(b));
+    else asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "a"(b));
+}
+
+template <int N> struct Number {
+    static constexpr int value = N;
+};
+
+// A wave's 32 keys and what it goes through, 32 rows at a time:
+//   products   the scores S and dP of the next rows (2 D / 16 matrix instructions), between which
+//   values     P and dS of these rows are made of theirs;
+//   sums       dV and dK of these rows (4 D / 32 matrix instructions).
+// So the matrix cores have work while exponentials are taken, though a SIMD has one wave.
+template <typename T, int D> struct Keys {
+    static constexpr uint32_t kBytes = Tile<D>::kBytes;
+    static constexpr uint32_t kRowValues = kTileRows * 4;    // bytes of a tile's lse, and of its delta
+    static constexpr uint32_t kBuffer = 2 * kBytes + 4 * 2 * kRowValues;     // Q, dO, and a copy of these for each wave
+    static constexpr int kSteps = D / 16, kParts = D / 32;
+    static constexpr int kEach = 16 / (2 * kSteps);          // values made beside a product
+    f32x16 sums_k[kParts], sums_v[kParts];
+    s16x8 k[kSteps], v[kSteps];
+    Range<T> scaled;
+    // Buffers come in two pairs.  What is read of the one in a pair is known beforehand; after a pair the places are
+    // moved to the other one, those of the scores, which run ahead, before those of the sums.
+    Fragments<D> f;
+    const lds_char* values;
+    const lds_char* lds;
+    uint32_t rows_on, columns_on;   // to the other pair
+    float factor;
+
+    struct Scores {
+        f32x16 s, d;
+    };
+
+    // Of the tile in buffer BUF: fragment m of block B for the scores, S's and dP's in turn,
+    template <int BUF, int B> __device__ __forceinline__ s16x8 row_fragment(int m) const
+    {
+        return f.rows(lds + BUF * kBuffer + m % 2 * kBytes, m / 2, B);
+    }
+    // and for the sums: dV's, then dK's.
+    template <int BUF, int B> __device__ __forceinline__ s16x8 column_fragment(int m) const
+    {
+        return f.columns(lds + BUF * kBuffer + (m < 2 * kParts ? kBytes : 0), m % kParts, B * 2 + m / kParts % 2);
+    }
+
+    // Scores alone, of block 0 of the first tile.
+    __device__ __forceinline__ void begin(Scores& x)
+    {
+#pragma unroll
+        for (int m = 0; m < 2 * kSteps; ++m) {
+            const s16x8 a = row_fragment<0, 0>(m);
+            if (m % 2) score<T>(x.d, a, v[m / 2], m < 2);
+            else score<T>(x.s, a, k[m / 2], m < 2);
+        }
+        asm volatile("s_nop 15\n\ts_nop 15");
+    }
+
+    // What a block begins with, read from LDS while the one before ends.
+    static constexpr int kAhead = 4;
+    struct Begin {
+        s16x8 rows[kAhead];
+        f32x4 less[4], delta[4];
+    };
+    template <int BUF, int B> __device__ __forceinline__ void read_values(Begin& x) const
+    {
+        const lds_char* at = values + BUF * kBuffer + B * 128;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x.less[i] = *reinterpret_cast<const lds_f32x4*>(at + i * 32);
+            x.delta[i] = *reinterpret_cast<const lds_f32x4*>(at + kRowValues + i * 32);
+        }
+    }
+    template <int BUF, int B> __device__ __forceinline__ void read_rows(Begin& x) const
+    {
+#pragma unroll
+        for (int m = 0; m < kAhead; ++m) x.rows[m] = row_fragment<BUF, B>(m);
+    }
+
+    __device__ __forceinline__ void move_rows()
+    {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) f.row_at[k] += rows_on;
+        values += static_cast<int32_t>(rows_on);
+        rows_on = -rows_on;
+    }
+    __device__ __forceinline__ void move_columns()
+    {
+#pragma unroll
+        for (int d = 0; d < kParts; ++d)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) f.column_at[d][k] += columns_on;
+        columns_on = -columns_on;
+    }
+
+    // Block B of the tile in buffer BUF of a pair, whose scores are in `now`; the next block's into `then`.  `between` is called
+    // before the sums, beside which `beside` is called 4 * kParts times.
+    template <int BUF, int B, typename Between, typename Beside>
+    __device__ __forceinline__ void block(Scores& now, Scores& then, Begin& begin, int32_t first_row, const Seen& mine,
+                                          bool partly, const Between& between, const Beside& beside)
+    {
+        constexpr int kNext = B ? 1 - BUF : BUF, kAfter = 1 - BUF;
+        s16x8 rows[2 * kSteps], columns[4 * kParts];
+#pragma unroll
+        for (int m = 0; m < kAhead; ++m) rows[m] = begin.rows[m];
+#pragma unroll
+        for (int m = 0; m < 2 * kSteps; ++m) {
+            if (m % 2 == 0)
+#pragma unroll
+                for (int n = m + kAhead; n < m + kAhead + 2; ++n) {
+                    if (n < 2 * kSteps) rows[n] = row_fragment<kNext, 1 - B>(n);
+                    else columns[n - 2 * kSteps] = column_fragment<BUF, B>(n - 2 * kSteps);
+                }
+            if (m % 2) score<T>(then.d, rows[m], v[m / 2], m < 2);
+            else score<T>(then.s, rows[m], k[m / 2], m < 2);
+#pragma unroll
+            for (int i = m * kEach; i < (m + 1) * kEach; ++i) {
+                now.s[i] = exp2_of(__builtin_fmaf(now.s[i], factor, begin.less[i / 4][i % 4]));
+                now.d[i] = now.s[i] * (now.d[i] - begin.delta[i / 4][i % 4]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (partly) {
+            hide(now.s, first_row + B * 32, mine);
+            hide(now.d, first_row + B * 32, mine);
+        }
+        scaled.template fit<true>(now.d, sums_k);
+        between();
+        s16x8 p[2] = {rounded<T>(now.s, 0), rounded<T>(now.s, 1)}, ds[2] = {rounded<T>(now.d, 0), rounded<T>(now.d, 1)};
+        asm volatile("s_nop 1" : "+v"(p[0]), "+v"(p[1]), "+v"(ds[0]), "+v"(ds[1]));
+#pragma unroll
+        for (int m = 0; m < 4 * kParts; ++m) {
+            if (m % 2 == 0 && m + kAhead < 4 * kParts) {
+                columns[m + kAhead] = column_fragment<BUF, B>(m + kAhead);
+                columns[m + kAhead + 1] = column_fragment<BUF, B>(m + kAhead + 1);
+            }
+            if (m + kAhead == 4 * kParts) {
+                read_values<kNext, 1 - B>(begin);
+                if (BUF == 1 && B == 0) move_rows();
+                read_rows<kAfter, B>(begin);
+            }
+            if (m < 2 * kParts) add_product<T>(sums_v[m % kParts], columns[m], p[m / kParts]);
+            else add_product<T>(sums_k[m % kParts], columns[m], ds[m / kParts - 2]);
+            beside(m);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (BUF == 1 && B == 1) move_columns();
+    }
+};
+
+// 128 keys to a workgroup, 32 to a wave; all waves go over the same tiles of 64 rows of one query
+// head after the other.  Four tiles are in LDS: one whose sums are made, one whose scores are, two on their way.
+template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_kernel(GradArgs a)
+{
+    using Mine = Keys<T, D>;
+    constexpr uint32_t kBytes = Mine::kBytes, kRowValues = Mine::kRowValues, kBuffer = Mine::kBuffer;
+    __shared__ __attribute__((aligned(1024))) char shared[4 * kBuffer];
     const uint32_t kv_head = blockIdx.x % a.kv_heads;
     const Piece p = locate(a.seq, blockIdx.x / a.kv_heads, true, 1, 128);
     if (!p.valid) return;
@@ -262,7 +443,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_kv_k
     const bool there = key < p.keys;
     const int32_t shift = static_cast<int32_t>(p.keys) - static_cast<int32_t>(p.length);
 
-    // the queries that see keys [from, to): those of row `from` .. where causal
+    // the queries that see keys [from, to)
     const auto rows_of = [&](uint32_t from, uint32_t to) {
         Seen r{0, static_cast<int32_t>(p.length)};
         if (!a.seq.causal) return r;
@@ -277,99 +458,106 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_kv_k
     const uint32_t first = p.tile * 128, wave_first = first + wave * 32;
     const uint32_t past = first + 128 < p.keys ? first + 128 : p.keys;
     const Seen all = p.rest ? Seen{0, 0} : rows_of(first, past);
-    const Seen own = rows_of(wave_first, wave_first + 32);
     const Seen common{rows_of(wave_first + 31, wave_first + 32).lo, rows_of(wave_first, wave_first + 1).hi};
     const int32_t tile_from = all.lo / static_cast<int32_t>(kTileRows);
     const int32_t tile_to = all.hi > 0 ? (all.hi + static_cast<int32_t>(kTileRows) - 1) / static_cast<int32_t>(kTileRows) : 0;
 
-    f32x16 sums_k[D / 32], sums_v[D / 32];
+    Mine w;
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d) sums_k[d] = sums_v[d] = zeros();
-    Range<T> scaled;
+    for (int d = 0; d < D / 32; ++d) w.sums_k[d] = w.sums_v[d] = zeros();
     if (tile_from < tile_to) {
-        s16x8 k[D / 16], v[D / 16];
-        load_row<D>(k, a.k.at(p.batch, p.key_first + key, kv_head), there, a.read_dim);
-        load_row<D>(v, a.v.at(p.batch, p.key_first + key, kv_head), there, a.read_dim);
+        load_row<D>(w.k, a.k.at(p.batch, p.key_first + key, kv_head), there, a.read_dim);
+        load_row<D>(w.v, a.v.at(p.batch, p.key_first + key, kv_head), there, a.read_dim);
+#pragma unroll
+        for (int m = 0; m < D / 16; ++m) asm volatile("" : "+a"(w.k[m]), "+a"(w.v[m]));
+        w.factor = a.scale * kLog2E;
         Loader<D, kTileRows, 4> load_q, load_g;
         load_q.init(wave, static_cast<uint32_t>(a.q.row), a.read_dim);
         load_g.init(wave, static_cast<uint32_t>(a.grad_out.row), a.read_dim);
-        Fragments<D> f;
-        f.init();
-        lds_char* lds = (lds_char*)shared;
-        const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
-        const uint32_t place = base + wave * 1024;
-        const uint32_t values = 4 * kBytes + wave * 4 * kRowValues;      // this wave's own copy
-        const float factor = a.scale * kLog2E;
-        const auto load = [&](uint32_t head, int32_t tile, uint32_t buffer) {
-            const Rows queries{reinterpret_cast<uint64_t>(a.q.at(p.batch, p.first, head)), static_cast<int32_t>(p.length)};
-            const Rows grads{reinterpret_cast<uint64_t>(a.grad_out.at(p.batch, p.first, head)),
-                             static_cast<int32_t>(p.length)};
-            load_q.load(queries, tile * kTileRows, place + buffer * 2 * kBytes);
-            load_g.load(grads, tile * kTileRows, place + buffer * 2 * kBytes + kBytes);
-            const uint64_t at = static_cast<uint64_t>(head) * a.rows_all + static_cast<uint64_t>(p.batch) * a.seq.rows + p.first;
-            const int32_t left = static_cast<int32_t>(p.length) - tile * static_cast<int32_t>(kTileRows);
-            const uint32_t bytes = left <= 0 ? 0u : left < static_cast<int32_t>(kTileRows) ? left * 4u : kRowValues;
-            load_values(reinterpret_cast<uint64_t>(a.lse2 + at + tile * kTileRows), bytes,
-                        base + values + buffer * 2 * kRowValues);
-            load_values(reinterpret_cast<uint64_t>(a.delta + at + tile * kTileRows), bytes,
-                        base + values + buffer * 2 * kRowValues + kRowValues);
+        w.lds = (lds_char*)shared;
+        const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(w.lds));
+        const uint32_t values = 2 * kBytes + wave * 2 * kRowValues;
+        w.f.init();
+        w.values = w.lds + values + lane / 32 * 16;
+        w.rows_on = w.columns_on = 2 * kBuffer;
+        // the tile that is loaded next: tiles of a head, then the next head's; past the last nothing
+        uint32_t load_head = kv_head * group, load_to = 0;
+        const uint32_t head_end = load_head + group;
+        int32_t load_tile = tile_from;
+        u32x4_t rsrc_q, rsrc_g;
+        uint64_t values_at;
+        uint32_t values_bytes;
+        // In parts, to go between products: where the tile lies, and its loads.
+        constexpr int kEach = Loader<D, kTileRows, 4>::kLoads, kLoads = 2 * kEach + 2;   // of a wave, for a tile
+        const auto turn = [&] {
+            const int32_t from = load_tile * static_cast<int32_t>(kTileRows);
+            const int32_t left = load_head < head_end ? static_cast<int32_t>(p.length) - from : 0;
+            const uint64_t row = static_cast<uint64_t>(p.first) + from;
+            rsrc_q = load_q.descriptor(reinterpret_cast<uint64_t>(a.q.at(p.batch, row, load_head)), left);
+            rsrc_g = load_g.descriptor(reinterpret_cast<uint64_t>(a.grad_out.at(p.batch, row, load_head)), left);
+            values_at = (static_cast<uint64_t>(load_head) * a.rows_all + static_cast<uint64_t>(p.batch) * a.seq.rows + row) * 4;
+            values_bytes = left <= 0 ? 0u : left < static_cast<int32_t>(kTileRows) ? left * 4u : kRowValues;
+            if (++load_tile == tile_to) load_tile = tile_from, ++load_head;
         };
-        uint32_t head = kv_head * group, buffer = 0;
-        const uint32_t head_end = head + group;
-        load(head, tile_from, 0);
-        for (int32_t tile = tile_from; head < head_end; buffer ^= 1) {
-            arrive<0>();
-            int32_t next = tile + 1;
-            uint32_t next_head = head;
-            if (next == tile_to) next = tile_from, ++next_head;
-            if (next_head < head_end) load(next_head, next, buffer ^ 1);
-            const lds_char *qs = lds + buffer * 2 * kBytes, *gs = qs + kBytes;
-            const lds_char* rows = lds + values + buffer * 2 * kRowValues;
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int32_t first_row = tile * static_cast<int32_t>(kTileRows) + b * 32;
-                if (first_row >= own.hi || first_row + 32 <= own.lo) continue;
-                f32x16 s = product<T, D>(qs, k, f, b);
-                f32x16 d = product<T, D>(gs, v, f, b);
-                const uint32_t half = lane / 32 * 16;
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const f32x4 lse2 = *reinterpret_cast<const lds_f32x4*>(rows + b * 128 + i * 8 + half);
-                    const f32x4 delta = *reinterpret_cast<const lds_f32x4*>(rows + kRowValues + b * 128 + i * 8 + half);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[i + e] = exp2_of(__builtin_fmaf(s[i + e], factor, Range<T>::kP - lse2[e]));
-                        d[i + e] = s[i + e] * (d[i + e] - delta[e]);
-                    }
-                }
-                if (first_row < common.lo || first_row + 32 > common.hi) {
-                    hide(s, first_row, mine);
-                    hide(d, first_row, mine);
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const s16x8 p16 = rounded<T>(s, h);
-#pragma unroll
-                    for (int e = 0; e < D / 32; ++e) sums_v[e] = mfma<T>(f.columns(gs, e, b * 2 + h), p16, sums_v[e]);
-                }
-                scaled.fit(d, sums_k);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const s16x8 ds = rounded<T>(d, h);
-#pragma unroll
-                    for (int e = 0; e < D / 32; ++e) sums_k[e] = mfma<T>(f.columns(qs, e, b * 2 + h), ds, sums_k[e]);
-                }
+        const auto load_part = [&](int n) {
+            if (n < kEach) load_q.load(rsrc_q, n, base + load_to + wave * 1024);
+            else if (n < 2 * kEach) load_g.load(rsrc_g, n - kEach, base + load_to + wave * 1024 + kBytes);
+            else if (n == 2 * kEach)
+                load_values(reinterpret_cast<uint64_t>(a.less) + values_at, values_bytes, base + load_to + values);
+            else if (n == 2 * kEach + 1) {
+                load_values(reinterpret_cast<uint64_t>(a.delta) + values_at, values_bytes, base + load_to + values + kRowValues);
+                load_to = load_to == 3 * kBuffer ? 0 : load_to + kBuffer;
             }
-            tile = next;
-            head = next_head;
+        };
+        const int32_t count = (tile_to - tile_from) * static_cast<int32_t>(group);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            turn();
+#pragma unroll
+            for (int k = 0; k < kLoads; ++k) load_part(k);
         }
+        arrive<2 * kLoads>();
+        typename Mine::Scores even, odd;
+        typename Mine::Begin begin;
+        w.begin(even);
+        w.template read_rows<0, 1>(begin);
+        w.template read_values<0, 0>(begin);
+        int32_t tile = tile_from;
+        // One tile, in buffer kBuf of a pair.
+        const auto step = [&](auto buffer) {
+            constexpr int kBuf = decltype(buffer)::value;
+            const int32_t first_row = tile * static_cast<int32_t>(kTileRows);
+            const bool partly = first_row < common.lo || first_row + static_cast<int32_t>(kTileRows) > common.hi;
+            constexpr int kSums = 4 * (D / 32), kPerSum = (kLoads + kSums - 3) / (kSums - 2);
+            w.template block<kBuf, 0>(
+                even, odd, begin, first_row, mine, partly,
+                // the next tile is there, and all waves have done with the one before this
+                [&] { arrive<kLoads>(); },
+                [&](int m) {
+                    if (m == 0) turn();
+#pragma unroll
+                    for (int n = 0; n < kPerSum; ++n)
+                        if (m > 0 && (m - 1) * kPerSum + n < kLoads) load_part((m - 1) * kPerSum + n);
+                });
+            w.template block<kBuf, 1>(odd, even, begin, first_row, mine, partly, [] {}, [](int) {});
+            if (++tile == tile_to) tile = tile_from;
+        };
+        // where there is an odd number of tiles, one of zeros follows
+        for (int32_t t = 0; t < count; t += 2) {
+            step(Number<0>{});
+            step(Number<1>{});
+        }
+        // loads into LDS that nobody reads are over before the workgroup is
+        arrive<0>();
     }
+    settle(w.sums_k);
+    settle(w.sums_v);
     constexpr float kShrinkP = Range<T>::kP == 0.0f ? 1.0f : 0x1p-14f;
     const bool stored = key < (a.keep_rest ? (p.rest ? 0u : p.keys) : p.key_stored);
-    store_row<T, D>(const_cast<char*>(a.grad_v.at(p.batch, p.key_first + key, kv_head)), sums_v, kShrinkP, stored, a.dim,
+    store_row<T, D>(const_cast<char*>(a.grad_v.at(p.batch, p.key_first + key, kv_head)), w.sums_v, kShrinkP, stored, a.dim,
                     a.v_aligned);
-    store_row<T, D>(const_cast<char*>(a.grad_k.at(p.batch, p.key_first + key, kv_head)), sums_k,
-                    a.scale * kShrinkP / scaled.factor(), stored, a.dim, a.k_aligned);
+    store_row<T, D>(const_cast<char*>(a.grad_k.at(p.batch, p.key_first + key, kv_head)), w.sums_k,
+                    a.scale * kShrinkP / w.scaled.factor(), stored, a.dim, a.k_aligned);
 }
 
 // ---------------------------------------------------------------------------
@@ -411,8 +599,8 @@ int la_attention_grad(const la_attention_t* call, void* workspace, uint64_t work
     if (rc != LA_OK) return rc;
     const la_attention_t& c = *call;
     const bool rows = flat_rows(c) > 0, keys = flat_keys(c) > 0;
-    if ((rows && (!there(c.q) || !there(c.out) || !there(c.grad_out) || !there(c.grad_q) || !c.lse ||
-                  reinterpret_cast<uintptr_t>(c.lse) % 4)) ||
+    if ((rows && (!there(c.q) || !there(c.out) || !there(c.grad_out) || !there(c.grad_q) ||
+                  !there_fp32(c.lse))) ||
         (keys && (!there(c.k) || !there(c.v) || !there(c.grad_k) || !there(c.grad_v))))
         return LA_EINVAL;
     rc = check_workspace(workspace, workspace_bytes, la_attention_grad_workspace(call), 256);
@@ -420,14 +608,14 @@ int la_attention_grad(const la_attention_t* call, void* workspace, uint64_t work
     const Sequences s = sequences_of(c);
     if (pieces(s, false, s.group, 128) * c.kv_heads >> 31 || pieces(s, true, 1, 128) * c.kv_heads >> 31) return LA_EINVAL;
     for (const void* p : {c.q.data, c.k.data, c.v.data, c.out.data, c.grad_out.data, c.grad_q.data, c.grad_k.data,
-                          c.grad_v.data, static_cast<const void*>(c.lse)})
+                          c.grad_v.data, c.lse.data})
         if (!reachable(p)) return LA_EFAULT;
     if (!indices_reachable(c) || !reachable(workspace)) return LA_EFAULT;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
     GradArgs a{};
-    a.lse = c.lse;
-    a.lse2 = reinterpret_cast<float*>(ws);
+    a.lse = plain(c.lse, 4);
+    a.less = reinterpret_cast<float*>(ws);
     a.delta = reinterpret_cast<float*>(ws + row_values_bytes(c));
     ws += 2 * row_values_bytes(c);
     rc = heads_of(c, c.q, true, a.q, ws, st);

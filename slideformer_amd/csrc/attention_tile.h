@@ -140,23 +140,38 @@ template <int D, uint32_t ROWS, uint32_t WAVES> struct Loader {
         }
     }
 
-    // Row `first` of `m` on into `lds`, the place of this wave's first 1024 bytes; returns at once.
+    // The descriptor of `count` rows (up to ROWS) from `at` on.
+    __device__ __forceinline__ u32x4_t descriptor(uint64_t at, int32_t count) const
+    {
+        const uint32_t rows = count <= 0 ? 0u : count < static_cast<int32_t>(ROWS) ? static_cast<uint32_t>(count) : ROWS;
+        return {uniform(static_cast<uint32_t>(at)), uniform(static_cast<uint32_t>(at >> 32)) & 0xffffu,
+                uniform(rows ? (rows - 1) * stride + width : 0u), 0x00020000u};
+    }
+
+    // Load n into `lds`, the place of this wave's first 1024 bytes; returns at once.
     // Written in assembly, which takes no result in a register: the compiler would
     // wait for every load in flight before any read of LDS.  The loops wait themselves.
-    // The wait states before a load are for the descriptor, which vector instructions may have written.
-    __device__ __forceinline__ void load(const Rows& m, int32_t first, uint32_t lds) const
+    // The wait states before the first load are for the descriptor, which vector instructions may have written.
+    __device__ __forceinline__ void load(const u32x4_t& rsrc, uint32_t n, uint32_t lds) const
     {
-        const int32_t left = m.rows - first;
-        const uint32_t count = left <= 0 ? 0u : left < static_cast<int32_t>(ROWS) ? static_cast<uint32_t>(left) : ROWS;
-        const uint64_t at = m.at + static_cast<uint64_t>(first < 0 ? 0 : first) * stride;
-        const u32x4_t rsrc = {uniform(static_cast<uint32_t>(at)), uniform(static_cast<uint32_t>(at >> 32)) & 0xffffu,
-                              uniform(count ? (count - 1) * stride + width : 0u), 0x00020000u};
-#pragma unroll
-        for (uint32_t n = 0; n < kLoads; ++n)
+        if (n == 0)
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :
+                         : "s"(uniform(lds)), "v"(offset[n]), "s"(rsrc)
+                         : "m0");
+        else
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
                          : "s"(uniform(lds + n * WAVES * 1024)), "v"(offset[n]), "s"(rsrc)
                          : "m0");
+    }
+
+    // Row `first` of `m` on.
+    __device__ __forceinline__ void load(const Rows& m, int32_t first, uint32_t lds) const
+    {
+        const u32x4_t rsrc = descriptor(m.at + static_cast<uint64_t>(first < 0 ? 0 : first) * stride, m.rows - first);
+#pragma unroll
+        for (uint32_t n = 0; n < kLoads; ++n) load(rsrc, n, lds);
     }
 };
 
@@ -393,6 +408,8 @@ inline bool reachable(const void* p) { return !p || la_ptr::device_accessible(p)
 
 inline bool there(const la_heads_t& h) { return h.data && reinterpret_cast<uintptr_t>(h.data) % 2 == 0; }
 
+inline bool there_fp32(const la_heads_t& h) { return h.data && reinterpret_cast<uintptr_t>(h.data) % 4 == 0; }
+
 inline uint64_t sets(const la_attention_t& c) { return c.starts ? 1 : c.batch; }
 inline uint64_t flat_rows(const la_attention_t& c) { return sets(c) * c.rows; }
 inline uint64_t flat_keys(const la_attention_t& c) { return sets(c) * c.key_rows; }
@@ -416,9 +433,9 @@ inline uint64_t packed_bytes(const la_attention_t& c, const la_heads_t& h, bool 
     return ceil_div(rows * (queries ? c.heads : c.kv_heads) * ceil_div(c.dim, 8ull) * 16, 256ull) * 256;
 }
 
-inline Heads plain(const la_heads_t& h)
+inline Heads plain(const la_heads_t& h, uint64_t size = 2)
 {
-    return {static_cast<const char*>(h.data), h.batch_stride * 2, h.row_stride * 2, h.head_stride * 2};
+    return {static_cast<const char*>(h.data), h.batch_stride * size, h.row_stride * size, h.head_stride * size};
 }
 
 // `h` as the kernels read it; where it has to be copied, to `space`, which moves on.

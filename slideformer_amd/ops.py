@@ -342,6 +342,19 @@ def _result(t: torch.Tensor, name: str, device, dims: int, dtype, shape) -> "_op
     return got
 
 
+def _row_values(t: torch.Tensor, name: str, device, like: torch.Tensor) -> "_ops_lib.LaHeads":
+    """fp32 values for every head of every row of `like`, in any order of memory."""
+    if t.device != device:
+        raise RuntimeError(f"{name} on {t.device}, expected {device}")
+    if t.shape != like.shape[:-1]:
+        raise RuntimeError(f"size mismatch: {name} is {tuple(t.shape)}, expected {tuple(like.shape[:-1])}")
+    if t.dtype != torch.float32:
+        raise RuntimeError(f"{name} is {t.dtype}, expected torch.float32")
+    strides = t.stride()
+    return _ops_lib.LaHeads(data=t.data_ptr(), batch_stride=strides[0] if t.dim() == 3 else 0, row_stride=strides[-2],
+                            head_stride=strides[-1])
+
+
 def _indices(t: Optional[torch.Tensor], name: str, device, size: int, dtype=None) -> Optional[int]:
     if t is None:
         return None
@@ -551,7 +564,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
         lse = s.empty(q.shape[:-1], torch.float32)
         if out.numel() == 0:
             return out, lse
-        call.out, call.lse = _heads(out, "out", device, q.dim()), lse.data_ptr()
+        call.out, call.lse = _heads(out, "out", device, q.dim()), _row_values(lse, "lse", device, q)
         size = lib.la_attention_workspace(ctypes.byref(call))
         work = s.workspace(size)
         _check(lib.la_attention(ctypes.byref(call), work.data_ptr(), size, s.handle), "la_attention")
@@ -567,7 +580,7 @@ def attention_grad(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                    stream=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The gradients of ``attention`` towards q, k and v, from that of its out.
 
-    ``out`` and ``lse`` are its results, the other arguments those that it had.  Probabilities are computed
+    ``out`` and ``lse`` are its results (lse in any order of memory), the other arguments those that it had.  Probabilities are computed
     again.  ``grads``: the three tensors to write, like q, k and v (parts of one projection's gradient,
     for instance); rows of no sequence stay as they were in them.  Without it they are new, and zero there.
     The gradients of a key head are sums over the query heads that share it.  Sums are fp32 in a fixed
@@ -576,8 +589,7 @@ def attention_grad(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     dims = q.dim()
     call.grad_out = _heads(grad_out, "grad_out", device, dims, q.dtype, q.shape)
     call.out = _heads(out, "out", device, dims, q.dtype, q.shape)
-    _vector(lse, "lse", device, q.numel() // q.shape[-1], (torch.float32,))
-    call.lse = lse.data_ptr()
+    call.lse = _row_values(lse, "lse", device, q)
     if grads is not None:
         call.keep_rest = 1
     lib = _ops_lib.load()

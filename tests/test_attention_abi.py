@@ -44,9 +44,9 @@ def _heads(data=HP, **strides):
 
 
 def _attention(**changed):
-    fields = dict(dtype=BF16, batch=2, rows=4, key_rows=4, heads=2, kv_heads=1, dim=64, lse=HP, causal=1, scale=0.125,
+    fields = dict(dtype=BF16, batch=2, rows=4, key_rows=4, heads=2, kv_heads=1, dim=64, causal=1, scale=0.125,
                   index_dtype=I32)
-    fields.update({name: _heads() for name in ("q", "k", "v", "out", "grad_out", "grad_q", "grad_k", "grad_v")})
+    fields.update({name: _heads() for name in ("q", "k", "v", "out", "lse", "grad_out", "grad_q", "grad_k", "grad_v")})
     fields.update(changed)
     return _ops_lib.LaAttention(**fields)
 
@@ -78,8 +78,8 @@ def _attention(**changed):
     (dict(q=_heads(HP + 1)), EINVAL),
     (dict(k=_heads(None)), EINVAL),
     (dict(out=_heads(HP + 1)), EINVAL),
-    (dict(lse=None), EINVAL),
-    (dict(lse=HP + 2), EINVAL),
+    (dict(lse=_heads(None)), EINVAL),
+    (dict(lse=_heads(HP + 2)), EINVAL),
     (dict(), EFAULT),                                        # host memory
     (dict(starts=HP, key_starts=HP, key_rows=9), EFAULT),
 ])
@@ -126,7 +126,7 @@ def test_attention_workspaces():
 def test_attention_of_nothing():
     L = _ops_lib.load()
     none = _heads(None)
-    call = _attention(rows=0, q=none, out=none, lse=None)
+    call = _attention(rows=0, q=none, out=none, lse=none)
     assert L.la_attention(ctypes.byref(call), None, 0, None) == OK
 
 
