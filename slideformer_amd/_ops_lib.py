@@ -229,6 +229,8 @@ def calls():
                 spec.loader.exec_module(module)
                 module.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
                     L.la_embedding, L.la_embedding_grad_workspace, L.la_embedding_grad, L.la_rms_norm,
-                    L.la_rms_norm_grad_workspace, L.la_rms_norm_grad)))
+                    L.la_rms_norm_grad_workspace, L.la_rms_norm_grad, L.la_qk_norm_rotary,
+                    L.la_qk_norm_rotary_grad_workspace, L.la_qk_norm_rotary_grad, L.la_attention_workspace,
+                    L.la_attention, L.la_attention_grad_workspace, L.la_attention_grad)))
                 _calls = module
     return _calls

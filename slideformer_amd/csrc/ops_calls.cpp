@@ -20,6 +20,7 @@
 
 #include <ATen/ops/empty.h>
 
+#include <cmath>
 #include <cstdint>
 #include <exception>
 
@@ -33,6 +34,13 @@ decltype(&la_embedding_grad) p_embedding_grad = nullptr;
 decltype(&la_rms_norm) p_rms_norm = nullptr;
 decltype(&la_rms_norm_grad_workspace) p_rms_norm_grad_workspace = nullptr;
 decltype(&la_rms_norm_grad) p_rms_norm_grad = nullptr;
+decltype(&la_qk_norm_rotary) p_rotary = nullptr;
+decltype(&la_qk_norm_rotary_grad_workspace) p_rotary_grad_workspace = nullptr;
+decltype(&la_qk_norm_rotary_grad) p_rotary_grad = nullptr;
+decltype(&la_attention_workspace) p_attention_workspace = nullptr;
+decltype(&la_attention) p_attention = nullptr;
+decltype(&la_attention_grad_workspace) p_attention_grad_workspace = nullptr;
+decltype(&la_attention_grad) p_attention_grad = nullptr;
 
 int code_of(at::ScalarType t)
 {
@@ -293,15 +301,270 @@ try {
     return failed();
 }
 
-// bind(addresses of the six functions above, in the order of their pointers)
+// Heads [.., heads, dim] of `dims` dimensions with contiguous elements, none of them empty.
+const at::Tensor* heads(PyObject* o, int64_t dev, int64_t dims, la_heads_t& h)
+{
+    const at::Tensor* t = plain(o, dev);
+    if (!t || t->dim() != dims || t->numel() == 0 || (t->size(-1) > 1 && t->stride(-1) != 1)) return nullptr;
+    h = {t->data_ptr(), dims == 4 ? static_cast<uint64_t>(t->stride(0)) : 0, static_cast<uint64_t>(t->stride(-3)),
+         static_cast<uint64_t>(t->stride(-2))};
+    return t;
+}
+
+const at::Tensor* heads_like(PyObject* o, int64_t dev, const at::Tensor& like, la_heads_t& h)
+{
+    const at::Tensor* t = heads(o, dev, like.dim(), h);
+    return t && t->sizes() == like.sizes() && t->scalar_type() == like.scalar_type() ? t : nullptr;
+}
+
+la_heads_t fresh_heads(const at::Tensor& t)
+{
+    return {t.data_ptr(), t.dim() == 4 ? static_cast<uint64_t>(t.stride(0)) : 0, static_cast<uint64_t>(t.stride(-3)),
+            static_cast<uint64_t>(t.stride(-2))};
+}
+
+// None, or a vector of `size` indices.
+bool indices(PyObject* o, int64_t dev, int64_t size, const at::Tensor*& t)
+{
+    t = nullptr;
+    if (o == Py_None) return true;
+    t = vector(o, dev, size);
+    return t && (t->scalar_type() == at::kInt || t->scalar_type() == at::kLong);
+}
+
+void* data_of(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
+
+// What both calls of the rotation check alike: tables, weights, positions; `of_q` and `of_k` have their sizes.
+bool rotary_call(PyObject* const* a, int64_t dev, const at::Tensor& of_q, const at::Tensor& of_k, la_rotary_t& c)
+{
+    const at::Tensor *cos = plain(a[0], dev), *sin = plain(a[1], dev), *at = nullptr;
+    c.dtype = code_of(of_q.scalar_type());
+    c.n = of_q.size(0);
+    c.heads = of_q.size(1);
+    c.kv_heads = of_k.size(1);
+    c.dim = of_q.size(2);
+    if (c.dtype < 0 || c.dtype > LA_F16 || of_k.scalar_type() != of_q.scalar_type() || of_k.size(0) != of_q.size(0) ||
+        of_k.size(2) != of_q.size(2) || c.dim > 256 || !cos || !sin || cos->dim() != 2 || sin->sizes() != cos->sizes() ||
+        cos->scalar_type() != at::kFloat || sin->scalar_type() != at::kFloat || !cos->is_contiguous() ||
+        !sin->is_contiguous() || 2 * cos->size(1) > of_q.size(2) || cos->numel() == 0 || !indices(a[4], dev, of_q.size(0), at))
+        return false;
+    const void** weights[] = {&c.q_weight, &c.k_weight};
+    for (int k = 0; k < 2; ++k) {
+        if (a[2 + k] == Py_None) continue;
+        const at::Tensor* w = vector(a[2 + k], dev, of_q.size(2));
+        if (!w || w->scalar_type() != of_q.scalar_type()) return false;
+        *weights[k] = w->data_ptr();
+    }
+    c.cos = static_cast<const float*>(cos->data_ptr());
+    c.sin = static_cast<const float*>(sin->data_ptr());
+    c.rotated = 2 * cos->size(1);
+    c.positions = cos->size(0);
+    c.at = data_of(at);
+    if (at) c.at_dtype = code_of(at->scalar_type());
+    c.eps = static_cast<float>(PyFloat_AsDouble(a[5]));
+    c.interleaved = PyObject_IsTrue(a[6]);
+    return true;
+}
+
+// qk_norm_rotary(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved, device, stream)
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t count)
+try {
+    if (count != 11) return none();
+    const int64_t dev = PyLong_AsLongLong(a[9]);
+    void* stream = PyLong_AsVoidPtr(a[10]);
+    la_rotary_t c{};
+    const at::Tensor *q = heads(a[0], dev, 3, c.q), *k = heads(a[1], dev, 3, c.k);
+    if (!q || !k || !rotary_call(a + 2, dev, *q, *k, c) || PyErr_Occurred()) {
+        PyErr_Clear();
+        return none();
+    }
+    const at::Tensor q_out = empty(q->sizes(), q->scalar_type(), dev), k_out = empty(k->sizes(), k->scalar_type(), dev);
+    c.q_out = fresh_heads(q_out);
+    c.k_out = fresh_heads(k_out);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_rotary(&c, stream);
+    Py_END_ALLOW_THREADS
+    return rc ? code(rc) : tuple({wrap(q_out), wrap(k_out)});
+} catch (const std::exception&) {
+    return failed();
+}
+
+// qk_norm_rotary_grad(grad_q, grad_k, q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved, device, stream):
+// the call whose results are all new, of heads that are both normed or both not
+PyObject* rotary_grad(PyObject*, PyObject* const* a, Py_ssize_t count)
+try {
+    if (count != 13) return none();
+    const int64_t dev = PyLong_AsLongLong(a[11]);
+    void* stream = PyLong_AsVoidPtr(a[12]);
+    la_rotary_t c{};
+    const at::Tensor *gq = heads(a[0], dev, 3, c.grad_q), *gk = heads(a[1], dev, 3, c.grad_k);
+    if (!gq || !gk || !rotary_call(a + 4, dev, *gq, *gk, c) || PyErr_Occurred() || !c.q_weight != !c.k_weight ||
+        (c.q_weight && (!heads_like(a[2], dev, *gq, c.q) || !heads_like(a[3], dev, *gk, c.k)))) {
+        PyErr_Clear();
+        return none();
+    }
+    const at::ScalarType type = gq->scalar_type();
+    const at::Tensor q_out = empty(gq->sizes(), type, dev), k_out = empty(gk->sizes(), type, dev);
+    c.q_out = fresh_heads(q_out);
+    c.k_out = fresh_heads(k_out);
+    at::Tensor wq, wk, work;
+    const uint64_t bytes = p_rotary_grad_workspace(&c);
+    c.weight_grad_dtype = c.dtype;
+    if (c.q_weight) {
+        wq = empty({gq->size(2)}, type, dev);
+        wk = empty({gq->size(2)}, type, dev);
+        work = empty({static_cast<int64_t>(bytes)}, at::kByte, dev);
+        c.grad_q_weight = wq.data_ptr();
+        c.grad_k_weight = wk.data_ptr();
+    }
+    void* ws = c.q_weight ? work.data_ptr() : nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_rotary_grad(&c, ws, bytes, stream);
+    Py_END_ALLOW_THREADS
+    if (rc) return code(rc);
+    return tuple({wrap(q_out), wrap(k_out), c.q_weight ? wrap(wq) : again(Py_None), c.q_weight ? wrap(wk) : again(Py_None)});
+} catch (const std::exception&) {
+    return failed();
+}
+
+// What both calls of attention check alike: (q, k, v), and from `a` on (causal, window or 0, scale or None, starts,
+// key_starts, lengths, key_lengths).
+bool attention_call(PyObject* const* qkv, PyObject* const* a, int64_t dev, la_attention_t& c, const at::Tensor* (&t)[3])
+{
+    const at::Tensor* of_q = plain(qkv[0], dev);
+    if (!of_q || (of_q->dim() != 3 && of_q->dim() != 4)) return false;
+    const int64_t dims = of_q->dim();
+    t[0] = heads(qkv[0], dev, dims, c.q);
+    t[1] = heads(qkv[1], dev, dims, c.k);
+    if (!t[0] || !t[1]) return false;
+    t[2] = heads_like(qkv[2], dev, *t[1], c.v);
+    const at::Tensor &q = *t[0], &k = *t[1];
+    if (!t[2] || k.scalar_type() != q.scalar_type()) return false;
+    c.dtype = code_of(q.scalar_type());
+    c.rows = q.size(-3);
+    c.heads = q.size(-2);
+    c.dim = q.size(-1);
+    c.key_rows = k.size(-3);
+    c.kv_heads = k.size(-2);
+    c.causal = PyObject_IsTrue(a[0]);
+    c.window = PyLong_AsUnsignedLongLong(a[1]);
+    c.scale = static_cast<float>(a[2] == Py_None ? 1.0 / std::sqrt(static_cast<double>(c.dim)) : PyFloat_AsDouble(a[2]));
+    if ((c.dtype != LA_BF16 && c.dtype != LA_F16) || k.size(-1) != q.size(-1) || c.dim > 128 || c.heads % c.kv_heads ||
+        (c.window && !c.causal) || !(c.scale > 0.0f) || !std::isfinite(c.scale))
+        return false;
+    const at::Tensor *starts, *key_starts, *lengths, *key_lengths, *first;
+    if (dims == 3) {
+        const at::Tensor* given = plain(a[3], dev);
+        if (!given || given->numel() < 2 || a[5] != Py_None || a[6] != Py_None ||
+            !indices(a[3], dev, given->numel(), starts) || !indices(a[4], dev, given->numel(), key_starts) ||
+            (!key_starts && c.rows != c.key_rows) || (key_starts && key_starts->scalar_type() != starts->scalar_type()))
+            return false;
+        c.batch = given->numel() - 1;
+        c.starts = data_of(starts);
+        c.key_starts = data_of(key_starts);
+        first = starts;
+    } else {
+        if (a[3] != Py_None || a[4] != Py_None || k.size(0) != q.size(0) || !indices(a[5], dev, q.size(0), lengths) ||
+            !indices(a[6], dev, q.size(0), key_lengths))
+            return false;
+        if (lengths && !key_lengths) {
+            if (c.rows != c.key_rows) return false;
+            key_lengths = lengths;
+        }
+        if (lengths && lengths->scalar_type() != key_lengths->scalar_type()) return false;
+        c.batch = q.size(0);
+        c.lengths = data_of(lengths);
+        c.key_lengths = data_of(key_lengths);
+        first = key_lengths;
+    }
+    if (first) c.index_dtype = code_of(first->scalar_type());
+    return true;
+}
+
+// The values of one fp32 for each head.
+bool row_values(PyObject* o, int64_t dev, const at::Tensor& q, la_heads_t& h)
+{
+    const at::Tensor* t = plain(o, dev);
+    if (!t || t->dim() != q.dim() - 1 || t->sizes() != q.sizes().slice(0, q.dim() - 1) || t->scalar_type() != at::kFloat)
+        return false;
+    h = {t->data_ptr(), t->dim() == 3 ? static_cast<uint64_t>(t->stride(0)) : 0, static_cast<uint64_t>(t->stride(-2)),
+         static_cast<uint64_t>(t->stride(-1))};
+    return true;
+}
+
+// attention(q, k, v, causal, window, scale, starts, key_starts, lengths, key_lengths, device, stream)
+PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t count)
+try {
+    if (count != 12) return none();
+    const int64_t dev = PyLong_AsLongLong(a[10]);
+    void* stream = PyLong_AsVoidPtr(a[11]);
+    la_attention_t c{};
+    const at::Tensor* t[3];
+    if (!attention_call(a, a + 3, dev, c, t) || PyErr_Occurred()) {
+        PyErr_Clear();
+        return none();
+    }
+    const at::Tensor& q = *t[0];
+    const at::Tensor out = empty(q.sizes(), q.scalar_type(), dev);
+    const at::Tensor lse = empty(q.sizes().slice(0, q.dim() - 1), at::kFloat, dev);
+    c.out = fresh_heads(out);
+    c.lse = {lse.data_ptr(), q.dim() == 4 ? c.rows * c.heads : 0, c.heads, 1};
+    const uint64_t bytes = p_attention_workspace(&c);
+    at::Tensor work;
+    if (bytes) work = empty({static_cast<int64_t>(bytes)}, at::kByte, dev);
+    void* ws = bytes ? work.data_ptr() : nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_attention(&c, ws, bytes, stream);
+    Py_END_ALLOW_THREADS
+    return rc ? code(rc) : tuple({wrap(out), wrap(lse)});
+} catch (const std::exception&) {
+    return failed();
+}
+
+// attention_grad(grad_out, q, k, v, out, lse, causal, window, scale, starts, key_starts, lengths, key_lengths, device,
+// stream): the call whose results are new
+PyObject* attention_grad(PyObject*, PyObject* const* a, Py_ssize_t count)
+try {
+    if (count != 15) return none();
+    const int64_t dev = PyLong_AsLongLong(a[13]);
+    void* stream = PyLong_AsVoidPtr(a[14]);
+    la_attention_t c{};
+    const at::Tensor* t[3];
+    if (!attention_call(a + 1, a + 6, dev, c, t) || PyErr_Occurred() || !heads_like(a[0], dev, *t[0], c.grad_out) ||
+        !heads_like(a[4], dev, *t[0], c.out) || !row_values(a[5], dev, *t[0], c.lse)) {
+        PyErr_Clear();
+        return none();
+    }
+    at::Tensor grads[3];
+    for (int k = 0; k < 3; ++k) grads[k] = empty(t[k]->sizes(), t[k]->scalar_type(), dev);
+    c.grad_q = fresh_heads(grads[0]);
+    c.grad_k = fresh_heads(grads[1]);
+    c.grad_v = fresh_heads(grads[2]);
+    const uint64_t bytes = p_attention_grad_workspace(&c);
+    const at::Tensor work = empty({static_cast<int64_t>(bytes) + 1}, at::kByte, dev);
+    void* ws = work.data_ptr();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_attention_grad(&c, ws, bytes, stream);
+    Py_END_ALLOW_THREADS
+    return rc ? code(rc) : tuple({wrap(grads[0]), wrap(grads[1]), wrap(grads[2])});
+} catch (const std::exception&) {
+    return failed();
+}
+
+// bind(addresses of the functions above, in the order of their pointers)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count)
 {
-    if (count != 6) {
-        PyErr_SetString(PyExc_TypeError, "bind takes six addresses");
+    constexpr Py_ssize_t kCount = 13;
+    if (count != kCount) {
+        PyErr_SetString(PyExc_TypeError, "bind takes thirteen addresses");
         return nullptr;
     }
-    void* at[6];
-    for (int k = 0; k < 6; ++k) at[k] = PyLong_AsVoidPtr(a[k]);
+    void* at[kCount];
+    for (Py_ssize_t k = 0; k < kCount; ++k) at[k] = PyLong_AsVoidPtr(a[k]);
     if (PyErr_Occurred()) return nullptr;
     p_embedding = reinterpret_cast<decltype(p_embedding)>(at[0]);
     p_embedding_grad_workspace = reinterpret_cast<decltype(p_embedding_grad_workspace)>(at[1]);
@@ -309,6 +572,13 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count)
     p_rms_norm = reinterpret_cast<decltype(p_rms_norm)>(at[3]);
     p_rms_norm_grad_workspace = reinterpret_cast<decltype(p_rms_norm_grad_workspace)>(at[4]);
     p_rms_norm_grad = reinterpret_cast<decltype(p_rms_norm_grad)>(at[5]);
+    p_rotary = reinterpret_cast<decltype(p_rotary)>(at[6]);
+    p_rotary_grad_workspace = reinterpret_cast<decltype(p_rotary_grad_workspace)>(at[7]);
+    p_rotary_grad = reinterpret_cast<decltype(p_rotary_grad)>(at[8]);
+    p_attention_workspace = reinterpret_cast<decltype(p_attention_workspace)>(at[9]);
+    p_attention = reinterpret_cast<decltype(p_attention)>(at[10]);
+    p_attention_grad_workspace = reinterpret_cast<decltype(p_attention_grad_workspace)>(at[11]);
+    p_attention_grad = reinterpret_cast<decltype(p_attention_grad)>(at[12]);
     Py_RETURN_NONE;
 }
 
@@ -321,6 +591,10 @@ PyMethodDef methods[] = {
     {"rms_norm", FAST(rms_norm), nullptr},
     {"rms_norm_8bit", FAST(rms_norm_8bit), nullptr},
     {"rms_norm_grad", FAST(rms_norm_grad), nullptr},
+    {"qk_norm_rotary", FAST(rotary), nullptr},
+    {"qk_norm_rotary_grad", FAST(rotary_grad), nullptr},
+    {"attention", FAST(attention), nullptr},
+    {"attention_grad", FAST(attention_grad), nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

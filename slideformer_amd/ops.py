@@ -424,6 +424,10 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: tor
     [n], row i of the tables for row i by default; one outside the tables makes the rotated elements NaN.
     ``out``: the two tensors to write instead of new ones, q and k themselves for instance, or rows
     of a cache.  All in fp32, rounded once."""
+    if out is None and stream is None and q.is_cuda:
+        done = _ops_lib.calls().qk_norm_rotary(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved, *_here())
+        if done is not None:
+            return _got(done, "la_qk_norm_rotary")
     device, call, _, _ = _rotary_call(q, k, q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved)
     lib = _ops_lib.load()
     with _on_device(device), _Scratch(device, stream) as s:
@@ -445,6 +449,12 @@ def qk_norm_rotary_grad(grad_q: torch.Tensor, grad_k: torch.Tensor, q: Optional[
     over.  ``grad_q_weight``, ``grad_k_weight``: the tensors [dim] to write (of the weights' type or
     float32, both of one; new by default), added to with ``accumulate``.  Returns ``(grad_q, grad_k,
     grad_q_weight, grad_k_weight)``, None for a weight that there is not.  Sums are fp32 in a fixed order."""
+    if grad_q_weight is None and grad_k_weight is None and not accumulate and out is None and stream is None \
+            and grad_q.is_cuda:
+        done = _ops_lib.calls().qk_norm_rotary_grad(grad_q, grad_k, q, k, cos, sin, q_weight, k_weight, positions, eps,
+                                                    interleaved, *_here())
+        if done is not None:
+            return _got(done, "la_qk_norm_rotary_grad")
     for x, weight, name in ((q, q_weight, "q"), (k, k_weight, "k")):
         if x is None and weight is not None:
             raise RuntimeError(f"the gradient of a norm needs {name}, which was normed")
@@ -557,6 +567,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     sequence's are not looked at, whatever they hold; one that is NaN or infinite inside a sequence may also reach
     rows that do not see it, as it does in a product with a probability of 0.  Statistics and sums are fp32,
     in a fixed order; probabilities are rounded to the operands' 16 bits."""
+    if stream is None and q.is_cuda and (window is None or window > 0):
+        done = _ops_lib.calls().attention(q, k, v, causal, window or 0, scale, starts, key_starts, lengths, key_lengths,
+                                          *_here())
+        if done is not None:
+            return _got(done, "la_attention")
     device, call = _attention_call(q, k, v, causal, window, scale, starts, key_starts, lengths, key_lengths)
     lib = _ops_lib.load()
     with _on_device(device), _Scratch(device, stream) as s:
@@ -585,6 +600,11 @@ def attention_grad(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     for instance); rows of no sequence stay as they were in them.  Without it they are new, and zero there.
     The gradients of a key head are sums over the query heads that share it.  Sums are fp32 in a fixed
     order: equal calls give equal bits."""
+    if grads is None and stream is None and q.is_cuda and (window is None or window > 0):
+        done = _ops_lib.calls().attention_grad(grad_out, q, k, v, out, lse, causal, window or 0, scale, starts,
+                                               key_starts, lengths, key_lengths, *_here())
+        if done is not None:
+            return _got(done, "la_attention_grad")
     device, call = _attention_call(q, k, v, causal, window, scale, starts, key_starts, lengths, key_lengths)
     dims = q.dim()
     call.grad_out = _heads(grad_out, "grad_out", device, dims, q.dtype, q.shape)
