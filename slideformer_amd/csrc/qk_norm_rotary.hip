@@ -29,12 +29,13 @@ struct RotaryArgs {
     const float *cos, *sin;
     const void* at;
     uint64_t positions;
-    float* partial;                 // of each workgroup: the sums for both weights, [2][dim]
-    uint32_t n, heads, all, dim, rotated;
+    float* partial;                 // of each workgroup: the sums for its heads' weight, [dim]
+    uint32_t n, heads, kv_heads, dim, rotated;
     uint32_t lanes;                 // to a head: a power of two
-    uint32_t chunks;                // waves that share a token's heads
+    uint32_t chunks, kv_chunks;     // waves that share a token's query heads, and its key heads
+    uint32_t workers;               // workgroups of a gradient that take query heads; the others take key heads
     int wide;
-    float eps;
+    float eps, per_dim;
 };
 
 // Two of a head's 16-byte vectors, a lane's share of it.
@@ -71,20 +72,22 @@ inline uint32_t slots(uint32_t dim, uint32_t rotated, uint32_t v)
     return ceil_div(rotated / 2, v) + ceil_div(dim - rotated, 2 * v);
 }
 
-template <typename T> __device__ __forceinline__ u32x4_t load_some(const T* from, uint32_t count)
+// WHOLE: every lane of every head has two whole vectors, so that there are no branches between its loads.
+template <typename T, bool WHOLE = false> __device__ __forceinline__ u32x4_t load_some(const T* from, uint32_t count)
 {
     constexpr uint32_t V = Elem<T>::kCount;
-    if (count == V) return *reinterpret_cast<const u32x4_any*>(from);
+    if (WHOLE || count == V) return *reinterpret_cast<const u32x4_any*>(from);
     T x[V];
 #pragma unroll
     for (uint32_t i = 0; i < V; ++i) x[i] = i < count ? from[i] : Elem<T>::from_f32(0.0f);
     return __builtin_bit_cast(u32x4_t, x);
 }
 
-template <typename T> __device__ __forceinline__ void store_some(T* to, uint32_t count, const float (&x)[Elem<T>::kCount])
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void store_some(T* to, uint32_t count, const float (&x)[Elem<T>::kCount])
 {
     constexpr uint32_t V = Elem<T>::kCount;
-    if (count == V) {
+    if (WHOLE || count == V) {
         *reinterpret_cast<u32x4_any*>(to) = Elem<T>::pack(x);
     } else {
 #pragma unroll
@@ -114,7 +117,7 @@ __device__ __forceinline__ void rotate(float (&x)[2][V], const Slot& t, const fl
 }
 
 // A token's row of both tables, this lane's pairs of it; NaN for a position outside them.
-template <int V>
+template <int V, bool WHOLE>
 __device__ __forceinline__ void angles(const RotaryArgs& a, uint32_t token, const Slot& t, float (&cos)[V], float (&sin)[V])
 {
     int64_t at = token;
@@ -123,10 +126,13 @@ __device__ __forceinline__ void angles(const RotaryArgs& a, uint32_t token, cons
     const uint64_t row = (good ? static_cast<uint64_t>(at) : 0) * (a.rotated / 2) + t.pair;
 #pragma unroll
     for (int i = 0; i < V; i += 4) {
-        const uint32_t count = t.pairs > static_cast<uint32_t>(i) ? t.pairs - i : 0;
-        float c[4], s[4];
-        Elem<float>::unpack(load_some<float>(a.cos + row + i, good ? (count < 4 ? count : 4) : 0), c);
-        Elem<float>::unpack(load_some<float>(a.sin + row + i, good ? (count < 4 ? count : 4) : 0), s);
+        const uint32_t left = t.pairs > static_cast<uint32_t>(i) ? t.pairs - i : 0, count = left < 4 ? left : 4;
+        float c[4] = {}, s[4] = {};
+        // where every lane is whole, one whose elements do not turn has no pairs, else as many as elements in a vector
+        if (a.positions && (!WHOLE || t.pairs)) {
+            Elem<float>::unpack(load_some<float, WHOLE>(a.cos + row + i, count), c);
+            Elem<float>::unpack(load_some<float, WHOLE>(a.sin + row + i, count), s);
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             cos[i + k] = good ? c[k] : NAN;
@@ -150,8 +156,6 @@ __device__ __forceinline__ void weights(const void* weight, const Slot& t, float
     }
 }
 
-__device__ __forceinline__ float chosen(bool first, float a, float b) { return first ? a : b; }
-
 template <int CONTROL> __device__ __forceinline__ float moved(float x)
 {
     return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CONTROL, 0xf, 0xf, true));
@@ -169,203 +173,222 @@ __device__ __forceinline__ float head_sum(float x, uint32_t lanes)
     return x;
 }
 
-template <typename T> __device__ __forceinline__ T* head_at(const HeadRows& q, const HeadRows& k, const RotaryArgs& a,
-                                                            uint32_t token, uint32_t head)
+template <typename T> __device__ __forceinline__ T* head_at(const HeadRows& r, uint32_t token, uint32_t head)
 {
-    char* const of_q = q.data + static_cast<uint64_t>(token) * q.row + static_cast<uint64_t>(head) * q.head;
-    char* const of_k = k.data + static_cast<uint64_t>(token) * k.row + (static_cast<uint64_t>(head) - a.heads) * k.head;
-    return reinterpret_cast<T*>(head < a.heads ? of_q : of_k);
+    return reinterpret_cast<T*>(r.data + static_cast<uint64_t>(token) * r.row + static_cast<uint64_t>(head) * r.head);
 }
 
-// One wave takes U heads for each of its groups of lanes, all loads first.
-// 8192 tokens of 40 heads of 128 in bf16: see the operator's table of times.
-template <typename T, bool INTERLEAVED, int U> __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a)
+// One wave takes U query heads, or key heads, of a token for each of its groups of lanes, all loads first.
+// 8192 tokens of 32 and 8 heads of 128 in bf16: see the operator's table of times.
+template <typename T, bool INTERLEAVED, bool WHOLE, int U> __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a)
 {
     constexpr int V = Elem<T>::kCount;
     const uint32_t lane = threadIdx.x % kWave, groups = kWave / a.lanes;
-    const uint64_t item = blockIdx.x * 4ull + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    if (item >= static_cast<uint64_t>(a.n) * a.chunks) return;
-    const uint32_t token = static_cast<uint32_t>(item / a.chunks);
-    const uint32_t first = static_cast<uint32_t>(item % a.chunks) * groups * U + lane / a.lanes;
+    uint64_t item = blockIdx.x * 4ull + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const bool query = item < static_cast<uint64_t>(a.n) * a.chunks;
+    if (!query) item -= static_cast<uint64_t>(a.n) * a.chunks;
+    const uint32_t chunks = query ? a.chunks : a.kv_chunks, heads = query ? a.heads : a.kv_heads;
+    if (item >= static_cast<uint64_t>(a.n) * chunks) return;
+    const HeadRows from = query ? a.q : a.k, to = query ? a.q_out : a.k_out;
+    const void* weight = query ? a.q_weight : a.k_weight;
+    const uint32_t token = static_cast<uint32_t>(item / chunks);
+    const uint32_t first = static_cast<uint32_t>(item % chunks) * groups * U + lane / a.lanes;
     const Slot t = slot_of<INTERLEAVED, V>(lane % a.lanes, a.dim, a.rotated);
     u32x4_t raw[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint32_t head = first + u * groups;
-        const bool there = head < a.all;
-        const T* from = head_at<T>(a.q, a.k, a, token, there ? head : 0);
+        const bool there = head < heads;
+        const T* x = head_at<T>(from, token, there ? head : 0);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) raw[u][h] = load_some<T>(from + t.first[h], there ? t.count[h] : 0);
+        for (int h = 0; h < 2; ++h) {
+            raw[u][h] = u32x4_t{0, 0, 0, 0};
+            if (there) raw[u][h] = load_some<T, WHOLE>(x + t.first[h], t.count[h]);
+        }
     }
-    float cos[V], sin[V], w[2][2][V];
-    angles<V>(a, token, t, cos, sin);
-    weights<T>(a.q_weight, t, w[0]);
-    weights<T>(a.k_weight, t, w[1]);
+    float cos[V], sin[V], w[2][V];
+    angles<V, WHOLE>(a, token, t, cos, sin);
+    weights<T>(weight, t, w);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint32_t head = first + u * groups;
-        const bool query = head < a.heads;
         float x[2][V];
 #pragma unroll
         for (int h = 0; h < 2; ++h) Elem<T>::unpack(raw[u][h], x[h]);
-        float sum = 0.0f;
+        if (weight) {
+            float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum = __builtin_fmaf(x[1][i], x[1][i], __builtin_fmaf(x[0][i], x[0][i], sum));
-        sum = head_sum(sum, a.lanes);
-        if (query ? a.q_weight != nullptr : a.k_weight != nullptr) {
-            const float r = 1.0f / sqrtf(sum / static_cast<float>(a.dim) + a.eps);
+            for (int i = 0; i < V; ++i) sum = __builtin_fmaf(x[1][i], x[1][i], __builtin_fmaf(x[0][i], x[0][i], sum));
+            sum = head_sum(sum, a.lanes);
+            const float r = 1.0f / sqrtf(__builtin_fmaf(sum, a.per_dim, a.eps));
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < V; ++i) x[h][i] = x[h][i] * r * chosen(query, w[0][h][i], w[1][h][i]);
+                for (int i = 0; i < V; ++i) x[h][i] = x[h][i] * r * w[h][i];
         }
         rotate<INTERLEAVED, V, false>(x, t, cos, sin);
-        if (head < a.all) {
-            T* to = head_at<T>(a.q_out, a.k_out, a, token, head);
+        if (head < heads) {
+            T* out = head_at<T>(to, token, head);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) store_some<T>(to + t.first[h], t.count[h], x[h]);
+            for (int h = 0; h < 2; ++h) store_some<T, WHOLE>(out + t.first[h], t.count[h], x[h]);
         }
     }
 }
 
-// A wave goes over items like those above and keeps the sums for the weights in registers; a workgroup's are
-// added in the order of its waves, the workgroups' by join_kernel.
-template <typename T, bool INTERLEAVED, int U> __global__ __launch_bounds__(256) void rotary_grad_kernel(RotaryArgs a)
+// A wave goes over items like those above and keeps the sums for the weight in registers; a workgroup's are
+// added in the order of its waves, the workgroups' by join_kernel.  The next item is on its way while one is
+// computed.
+template <typename T, bool INTERLEAVED, bool WHOLE, int U> __global__ __launch_bounds__(256, 2) void rotary_grad_kernel(RotaryArgs a)
 {
     constexpr int V = Elem<T>::kCount;
-    __shared__ float sums[4][2][kWave][2][V];
+    __shared__ float sums[4][kWave][2][V];
     const uint32_t lane = threadIdx.x % kWave, groups = kWave / a.lanes;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const bool query = blockIdx.x < a.workers;
+    const uint32_t worker = query ? blockIdx.x : blockIdx.x - a.workers;
+    const uint32_t workers = query ? a.workers : gridDim.x - a.workers;
+    const uint32_t chunks = query ? a.chunks : a.kv_chunks, heads = query ? a.heads : a.kv_heads;
+    const HeadRows from_g = query ? a.grad_q : a.grad_k, from_x = query ? a.q : a.k, to = query ? a.q_out : a.k_out;
+    const void* weight = query ? a.q_weight : a.k_weight;
     const Slot t = slot_of<INTERLEAVED, V>(lane % a.lanes, a.dim, a.rotated);
-    float w[2][2][V], dw[2][2][V] = {};
-    weights<T>(a.q_weight, t, w[0]);
-    weights<T>(a.k_weight, t, w[1]);
-    const uint64_t items = static_cast<uint64_t>(a.n) * a.chunks;
-    for (uint64_t item = blockIdx.x * 4ull + wave; item < items; item += gridDim.x * 4ull) {
-        const uint32_t token = static_cast<uint32_t>(item / a.chunks);
-        const uint32_t first = static_cast<uint32_t>(item % a.chunks) * groups * U + lane / a.lanes;
-        u32x4_t raw_g[U][2], raw_x[U][2];
+    float w[2][V], dw[2][V] = {};
+    weights<T>(weight, t, w);
+    const uint64_t items = static_cast<uint64_t>(a.n) * chunks, stride = workers * 4ull;
+    struct Item {
+        u32x4_t g[U][2], x[U][2];
+        float cos[V], sin[V];
+        uint32_t token, first;
+    };
+    const auto load = [&](Item& d, uint64_t item) {
+        d.token = static_cast<uint32_t>(item / chunks);
+        d.first = static_cast<uint32_t>(item % chunks) * groups * U + lane / a.lanes;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t head = first + u * groups;
-            const bool there = head < a.all, normed = head < a.heads ? a.q_weight != nullptr : a.k_weight != nullptr;
-            const T* g = head_at<T>(a.grad_q, a.grad_k, a, token, there ? head : 0);
-            const T* x = head_at<T>(a.q, a.k, a, token, there ? head : 0);
+            const uint32_t head = d.first + u * groups;
+            const bool there = head < heads;
+            const T* g = head_at<T>(from_g, d.token, there ? head : 0);
+            const T* x = head_at<T>(from_x, d.token, there ? head : 0);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                raw_g[u][h] = load_some<T>(g + t.first[h], there ? t.count[h] : 0);
-                raw_x[u][h] = load_some<T>(x + t.first[h], there && normed ? t.count[h] : 0);
+                d.g[u][h] = d.x[u][h] = u32x4_t{0, 0, 0, 0};
+                if (there) d.g[u][h] = load_some<T, WHOLE>(g + t.first[h], t.count[h]);
+                if (there && weight) d.x[u][h] = load_some<T, WHOLE>(x + t.first[h], t.count[h]);
             }
         }
-        float cos[V], sin[V];
-        angles<V>(a, token, t, cos, sin);
+        angles<V, WHOLE>(a, d.token, t, d.cos, d.sin);
+    };
+    const auto compute = [&](const Item& d) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t head = first + u * groups;
-            const bool query = head < a.heads, there = head < a.all;
-            float g[2][V], x[2][V];
+            const uint32_t head = d.first + u * groups;
+            float g[2][V];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                Elem<T>::unpack(raw_g[u][h], g[h]);
-                Elem<T>::unpack(raw_x[u][h], x[h]);
-            }
-            rotate<INTERLEAVED, V, true>(g, t, cos, sin);
-            float squares = 0.0f, products = 0.0f;
-            float gw[2][V];
-#pragma unroll
-            for (int i = 0; i < V; ++i)
+            for (int h = 0; h < 2; ++h) Elem<T>::unpack(d.g[u][h], g[h]);
+            rotate<INTERLEAVED, V, true>(g, t, d.cos, d.sin);
+            if (weight) {
+                float x[2][V], squares = 0.0f, products = 0.0f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    gw[h][i] = g[h][i] * chosen(query, w[0][h][i], w[1][h][i]);
-                    squares = __builtin_fmaf(x[h][i], x[h][i], squares);
-                    products = __builtin_fmaf(gw[h][i], x[h][i], products);
+                    Elem<T>::unpack(d.x[u][h], x[h]);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        squares = __builtin_fmaf(x[h][i], x[h][i], squares);
+                        products = __builtin_fmaf(g[h][i] * w[h][i], x[h][i], products);
+                    }
                 }
-            squares = head_sum(squares, a.lanes);
-            products = head_sum(products, a.lanes);
-            if (query ? a.q_weight != nullptr : a.k_weight != nullptr) {
-                const float r = 1.0f / sqrtf(squares / static_cast<float>(a.dim) + a.eps);
-                const float mean = products * r / static_cast<float>(a.dim);
+                squares = head_sum(squares, a.lanes);
+                products = head_sum(products, a.lanes);
+                const float r = 1.0f / sqrtf(__builtin_fmaf(squares, a.per_dim, a.eps));
+                const float mean = products * r * a.per_dim;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        const float unit = x[h][i] * r, share = there ? g[h][i] * unit : 0.0f;
-                        dw[0][h][i] += query ? share : 0.0f;
-                        dw[1][h][i] += query ? 0.0f : share;
-                        g[h][i] = r * __builtin_fmaf(-unit, mean, gw[h][i]);
+                        // a head that is not there is all zeros, and adds none
+                        const float unit = x[h][i] * r;
+                        dw[h][i] = __builtin_fmaf(g[h][i], unit, dw[h][i]);
+                        g[h][i] = r * __builtin_fmaf(-unit, mean, g[h][i] * w[h][i]);
                     }
             }
-            if (there) {
-                T* to = head_at<T>(a.q_out, a.k_out, a, token, head);
+            if (head < heads) {
+                T* out = head_at<T>(to, d.token, head);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) store_some<T>(to + t.first[h], t.count[h], g[h]);
+                for (int h = 0; h < 2; ++h) store_some<T, WHOLE>(out + t.first[h], t.count[h], g[h]);
             }
         }
+    };
+    Item one, other;
+    uint64_t item = worker * 4ull + wave;
+    if (item < items) load(one, item);
+    while (item < items) {
+        if (item + stride < items) load(other, item + stride);
+        compute(one);
+        item += stride;
+        if (item >= items) break;
+        if (item + stride < items) load(one, item + stride);
+        compute(other);
+        item += stride;
     }
-    if (!a.partial) return;
+    if (!weight) return;
     for (uint32_t d = a.lanes; d < kWave; d <<= 1)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < V; ++i) dw[k][h][i] += __shfl_xor(dw[k][h][i], static_cast<int>(d));
+            for (int i = 0; i < V; ++i) dw[h][i] += __shfl_xor(dw[h][i], static_cast<int>(d));
     if (lane < a.lanes)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < V; ++i) sums[wave][k][lane][h][i] = dw[k][h][i];
+            for (int i = 0; i < V; ++i) sums[wave][lane][h][i] = dw[h][i];
     __syncthreads();
-    if (threadIdx.x >= 2 * a.lanes) return;
-    const uint32_t k = threadIdx.x / a.lanes, s = threadIdx.x % a.lanes;
-    const Slot to = slot_of<INTERLEAVED, V>(s, a.dim, a.rotated);
-    float* mine = a.partial + (static_cast<uint64_t>(blockIdx.x) * 2 + k) * a.dim;
+    if (threadIdx.x >= a.lanes) return;
+    float* mine = a.partial + static_cast<uint64_t>(blockIdx.x) * a.dim;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (uint32_t i = 0; i < V; ++i)
-            if (i < to.count[h])
-                mine[to.first[h] + i] = (sums[0][k][s][h][i] + sums[1][k][s][h][i]) + (sums[2][k][s][h][i] + sums[3][k][s][h][i]);
+            if (i < t.count[h])
+                mine[t.first[h] + i] = (sums[0][lane][h][i] + sums[1][lane][h][i]) + (sums[2][lane][h][i] + sums[3][lane][h][i]);
 }
 
 struct JoinArgs {
     const float* partial;
-    void *q_weight, *k_weight;
-    uint32_t workers, dim;
+    void* weight[2];
+    uint32_t first[2], workers[2];  // of the workgroups with query heads, and with key heads
+    uint32_t dim;
     int accumulate;
 };
 
-// Sixteen waves, 64 neighbouring sums to a workgroup: each takes a run of the workgroups' partial sums.
+// Sixteen waves, 64 neighbouring sums of one weight to a workgroup: each takes a run of the workgroups' partial sums.
 template <typename W> __global__ __launch_bounds__(1024) void join_kernel(JoinArgs a)
 {
     __shared__ float sums[16][kWave];
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const uint32_t at = blockIdx.x * kWave + lane;
-    const uint32_t run = ceil_div(a.workers, 16u), from = wave * run;
-    const uint32_t end = from + run < a.workers ? from + run : a.workers;
+    W* to = static_cast<W*>(blockIdx.y ? a.weight[1] : a.weight[0]);
+    if (!to) return;
+    const uint32_t workers = blockIdx.y ? a.workers[1] : a.workers[0];
+    const float* partial = a.partial + static_cast<uint64_t>(blockIdx.y ? a.first[1] : a.first[0]) * a.dim;
+    const uint32_t run = ceil_div(workers, 16u), from = wave * run;
+    const uint32_t end = from + run < workers ? from + run : workers;
     float sum = 0.0f;
-    if (at < 2 * a.dim)
-#pragma unroll 8
-        for (uint32_t k = from; k < end; ++k) sum += a.partial[static_cast<uint64_t>(k) * 2 * a.dim + at];
+    if (at < a.dim)
+#pragma unroll 16
+        for (uint32_t k = from; k < end; ++k) sum += partial[static_cast<uint64_t>(k) * a.dim + at];
     sums[wave][lane] = sum;
     __syncthreads();
-    if (wave > 0 || at >= 2 * a.dim) return;
+    if (wave > 0 || at >= a.dim) return;
     sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < 16; ++k) sum += sums[k][lane];
-    W* to = static_cast<W*>(at < a.dim ? a.q_weight : a.k_weight);
-    if (!to) return;
-    to += at < a.dim ? at : at - a.dim;
-    *to = Elem<W>::from_f32(a.accumulate ? sum + Elem<W>::to_f32(*to) : sum);
+    to[at] = Elem<W>::from_f32(a.accumulate ? sum + Elem<W>::to_f32(to[at]) : sum);
 }
 
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 constexpr uint64_t kMostDim = 256;                       // 64 lanes of eight fp32
-constexpr uint64_t kMostWorkers = 512;                   // workgroups with partial sums
+constexpr uint64_t kMostWorkers = 512;                   // workgroups with partial sums: two to a compute unit
 
 bool reachable(const void* p) { return !p || la_ptr::device_accessible(p); }
 
@@ -423,61 +446,77 @@ RotaryArgs args_of(const la_rotary_t& c)
     a.positions = c.positions;
     a.n = static_cast<uint32_t>(c.n);
     a.heads = static_cast<uint32_t>(c.heads);
-    a.all = static_cast<uint32_t>(c.heads + c.kv_heads);
+    a.kv_heads = static_cast<uint32_t>(c.kv_heads);
     a.dim = static_cast<uint32_t>(c.dim);
     a.rotated = static_cast<uint32_t>(c.rotated);
     a.eps = c.eps;
+    a.per_dim = 1.0f / static_cast<float>(c.dim);
     a.lanes = 1;
     while (a.lanes < slots(a.dim, a.rotated, 16 / dtype_bytes(c.dtype))) a.lanes *= 2;
     return a;
 }
 
-// Heads that a group of lanes takes at a time: up to `most`, as even as the token's heads allow; one
+// Heads that a group of lanes takes at a time: up to `most`, as even as the token's query heads allow; one
 // where there are too few tokens to fill the card otherwise.
 uint32_t heads_at_a_time(RotaryArgs& a, uint32_t most)
 {
-    const uint32_t each = ceil_div(a.all, kWave / a.lanes);
-    a.chunks = each;
-    if (static_cast<uint64_t>(a.n) * each <= 4096) return 1;
-    a.chunks = ceil_div(each, most);
-    const uint32_t u = ceil_div(each, a.chunks);
-    a.chunks = ceil_div(each, u);
+    const uint32_t groups = kWave / a.lanes, each = std::max(1u, ceil_div(a.heads, groups));
+    uint32_t u = ceil_div(each, ceil_div(each, most));
+    if (static_cast<uint64_t>(a.n) * each <= 4096) u = 1;
+    a.chunks = ceil_div(a.heads, groups * u);
+    a.kv_chunks = ceil_div(a.kv_heads, groups * u);
     return u;
 }
 
-template <typename T, bool INTERLEAVED> int forward(RotaryArgs& a, hipStream_t st)
+template <typename T, bool INTERLEAVED, bool WHOLE> int forward(RotaryArgs& a, hipStream_t st)
 {
     const uint32_t u = heads_at_a_time(a, 4);
-    const dim3 grid(static_cast<uint32_t>(ceil_div(static_cast<uint64_t>(a.n) * a.chunks, 4ull)));
+    const dim3 grid(static_cast<uint32_t>(ceil_div(static_cast<uint64_t>(a.n) * (a.chunks + a.kv_chunks), 4ull)));
     switch (u) {
-    case 1: return launch(rotary_kernel<T, INTERLEAVED, 1>, grid, dim3(256), st, a);
-    case 2: return launch(rotary_kernel<T, INTERLEAVED, 2>, grid, dim3(256), st, a);
-    case 3: return launch(rotary_kernel<T, INTERLEAVED, 3>, grid, dim3(256), st, a);
-    default: return launch(rotary_kernel<T, INTERLEAVED, 4>, grid, dim3(256), st, a);
+    case 1: return launch(rotary_kernel<T, INTERLEAVED, WHOLE, 1>, grid, dim3(256), st, a);
+    case 2: return launch(rotary_kernel<T, INTERLEAVED, WHOLE, 2>, grid, dim3(256), st, a);
+    case 3: return launch(rotary_kernel<T, INTERLEAVED, WHOLE, 3>, grid, dim3(256), st, a);
+    default: return launch(rotary_kernel<T, INTERLEAVED, WHOLE, 4>, grid, dim3(256), st, a);
     }
+}
+
+// Whether all lanes have two whole vectors.
+bool whole(const RotaryArgs& a, uint32_t v)
+{
+    return a.rotated / 2 % v == 0 && (a.dim - a.rotated) % (2 * v) == 0 && slots(a.dim, a.rotated, v) == a.lanes;
 }
 
 template <typename T> int forward(RotaryArgs& a, bool interleaved, hipStream_t st)
 {
-    return interleaved ? forward<T, true>(a, st) : forward<T, false>(a, st);
+    if (whole(a, Elem<T>::kCount)) return interleaved ? forward<T, true, true>(a, st) : forward<T, false, true>(a, st);
+    return interleaved ? forward<T, true, false>(a, st) : forward<T, false, false>(a, st);
 }
 
-// Workgroups of a gradient's launch.
-uint64_t workers_of(const RotaryArgs& a)
+// Workgroups of a gradient's launch: a.workers for the query heads, those returned for the key heads; in proportion to
+// their items, and at least one where there are such heads.
+uint32_t share_out(RotaryArgs& a)
 {
-    return std::min<uint64_t>(kMostWorkers, ceil_div(static_cast<uint64_t>(a.n) * a.chunks, 4ull));
+    const uint64_t q = ceil_div(static_cast<uint64_t>(a.n) * a.chunks, 4ull);
+    const uint64_t k = ceil_div(static_cast<uint64_t>(a.n) * a.kv_chunks, 4ull);
+    const uint64_t of_k = a.kv_chunks ? kMostWorkers * a.kv_chunks / (a.chunks + a.kv_chunks) : 0;
+    const uint64_t most_k = std::max<uint64_t>(1, std::min(of_k, kMostWorkers - 1));
+    a.workers = static_cast<uint32_t>(std::min(q, kMostWorkers - most_k));
+    return static_cast<uint32_t>(std::min(k, most_k));
 }
 
-template <typename T, bool INTERLEAVED> int backward(RotaryArgs& a, uint32_t u, hipStream_t st)
+template <typename T, bool INTERLEAVED, bool WHOLE>
+int backward(RotaryArgs& a, uint32_t u, uint32_t kv_workers, hipStream_t st)
 {
-    const dim3 grid(static_cast<uint32_t>(workers_of(a)));
-    return u == 1 ? launch(rotary_grad_kernel<T, INTERLEAVED, 1>, grid, dim3(256), st, a)
-                  : launch(rotary_grad_kernel<T, INTERLEAVED, 2>, grid, dim3(256), st, a);
+    const dim3 grid(a.workers + kv_workers);
+    return u == 1 ? launch(rotary_grad_kernel<T, INTERLEAVED, WHOLE, 1>, grid, dim3(256), st, a)
+                  : launch(rotary_grad_kernel<T, INTERLEAVED, WHOLE, 2>, grid, dim3(256), st, a);
 }
 
-template <typename T> int backward(RotaryArgs& a, bool interleaved, uint32_t u, hipStream_t st)
+template <typename T> int backward(RotaryArgs& a, bool interleaved, uint32_t u, uint32_t kv_workers, hipStream_t st)
 {
-    return interleaved ? backward<T, true>(a, u, st) : backward<T, false>(a, u, st);
+    if (whole(a, Elem<T>::kCount))
+        return interleaved ? backward<T, true, true>(a, u, kv_workers, st) : backward<T, false, true>(a, u, kv_workers, st);
+    return interleaved ? backward<T, true, false>(a, u, kv_workers, st) : backward<T, false, false>(a, u, kv_workers, st);
 }
 
 }  // namespace
@@ -502,7 +541,7 @@ int la_qk_norm_rotary(const la_rotary_t* call, la_stream_t stream)
 uint64_t la_qk_norm_rotary_grad_workspace(const la_rotary_t* call)
 {
     if (!call || call->dim > kMostDim || !(call->q_weight || call->k_weight)) return 0;
-    return kMostWorkers * 2 * call->dim * sizeof(float);
+    return kMostWorkers * call->dim * sizeof(float);
 }
 
 int la_qk_norm_rotary_grad(const la_rotary_t* call, void* workspace, uint64_t workspace_bytes, la_stream_t stream)
@@ -531,20 +570,20 @@ int la_qk_norm_rotary_grad(const la_rotary_t* call, void* workspace, uint64_t wo
     a.grad_k = rows_of(c.grad_k, c.dtype);
     a.partial = normed ? static_cast<float*>(workspace) : nullptr;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    uint64_t workers = 0;
+    uint32_t kv_workers = 0;
     if (any) {
         const uint32_t u = heads_at_a_time(a, 2);
-        workers = workers_of(a);
+        kv_workers = share_out(a);
         const bool interleaved = c.interleaved != 0;
-        rc = c.dtype == LA_F32    ? backward<float>(a, interleaved, u, st)
-             : c.dtype == LA_BF16 ? backward<__bf16>(a, interleaved, u, st)
-                                  : backward<_Float16>(a, interleaved, u, st);
+        rc = c.dtype == LA_F32    ? backward<float>(a, interleaved, u, kv_workers, st)
+             : c.dtype == LA_BF16 ? backward<__bf16>(a, interleaved, u, kv_workers, st)
+                                  : backward<_Float16>(a, interleaved, u, kv_workers, st);
         if (rc != LA_OK) return rc;
     }
     if (!normed) return LA_OK;
-    const JoinArgs j{a.partial, c.q_weight ? c.grad_q_weight : nullptr, c.k_weight ? c.grad_k_weight : nullptr,
-                     static_cast<uint32_t>(workers), a.dim, c.accumulate};
-    const dim3 grid(ceil_div(2 * a.dim, kWave));
+    const JoinArgs j{a.partial, {c.q_weight ? c.grad_q_weight : nullptr, c.k_weight ? c.grad_k_weight : nullptr},
+                     {0, a.workers}, {a.workers, kv_workers}, a.dim, c.accumulate};
+    const dim3 grid(ceil_div(a.dim, kWave), 2);
     return c.weight_grad_dtype == LA_F32    ? launch(join_kernel<float>, grid, dim3(1024), st, j)
            : c.weight_grad_dtype == LA_BF16 ? launch(join_kernel<__bf16>, grid, dim3(1024), st, j)
                                             : launch(join_kernel<_Float16>, grid, dim3(1024), st, j);
