@@ -229,9 +229,6 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void attention
     const uint32_t token = row / group;
     const Seen mine = seen(a.seq, p, token);
 
-    s16x8 q[D / 16];
-    load_row<D>(q, a.q.at(p.batch, p.first + token, kv_head * group + row % group), token < p.length, a.read_dim);
-
     // the keys that the workgroup's rows see, and this wave's
     const uint32_t last_row = p.length * group;          // one past
     const auto range = [&](uint32_t row_from, uint32_t row_to) {
@@ -269,6 +266,8 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void attention
         const float factor = a.scale * kLog2E;
         load_k.load(keys, tile * kTileRows, place);
         load_v.load(values, tile * kTileRows, place + kBytes);
+        s16x8 q[D / 16];
+        load_row<D>(q, a.q.at(p.batch, p.first + token, kv_head * group + row % group), token < p.length, a.read_dim);
         uint32_t buffer = 0;
         for (; tile < end; ++tile, buffer ^= 2 * kBytes) {
             arrive<0>();
@@ -291,13 +290,17 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void attention
 }
 
 // At most 32 rows to a workgroup (a single new token's heads): its waves take the same rows and different keys, each
-// with tiles of its own in LDS and without waiting for the others, and join at the end.
-template <typename T, int D> __global__ __launch_bounds__(256, 1) void few_rows_kernel(ForwardArgs a)
+// with tiles of its own in LDS and without waiting for the others, and join at the end.  Two waves, so that
+// two workgroups or more are on a compute unit and one's start and end are under the other's loads.
+// Bound by memory: a wave takes 0.8 us for 32 keys where loads do not bind.  With five tiles in a ring, four of them
+// on their way, one row over 65536 keys of eight heads took 47.9 us instead of 44.4, with four waves 46.5.
+constexpr uint32_t kFewWaves = 2;
+
+template <typename T, int D> __global__ __launch_bounds__(kFewWaves * 64, 1) void few_rows_kernel(ForwardArgs a)
 {
-    constexpr uint32_t kKeys = 32, kBytes = Tile<D>::kBytes / 2, kAhead = 2;
-    constexpr uint32_t kOwn = 2 * kAhead * kBytes;       // a wave's share of LDS
-    __shared__ __attribute__((aligned(1024))) char shared[4 * kOwn];
-    __shared__ float tops[4][32], sums[4][32];
+    constexpr uint32_t kKeys = 32, kBytes = Tile<D>::kBytes / 2;
+    constexpr uint32_t kOwn = 4 * kBytes;                // a wave's share of LDS: keys and values of two tiles
+    __shared__ __attribute__((aligned(1024))) char shared[kFewWaves * kOwn];
     const uint32_t kv_head = blockIdx.x % a.kv_heads, part = blockIdx.y;
     const Piece p = locate(a.seq, blockIdx.x / a.kv_heads, false, a.seq.group, 32);
     if (!p.valid) return;
@@ -327,8 +330,6 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void few_rows_
     st.init();
     lds_char* lds = (lds_char*)shared;
     if (tile < end) {
-        s16x8 q[D / 16];
-        load_row<D>(q, a.q.at(p.batch, p.first + token, kv_head * group + row % group), token < p.length, a.read_dim);
         const Rows keys{reinterpret_cast<uint64_t>(a.k.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
         const Rows values{reinterpret_cast<uint64_t>(a.v.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
         Loader<D, kKeys, 1> load_k, load_v;
@@ -339,19 +340,34 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void few_rows_
         const lds_char* own = lds + wave * kOwn;
         const uint32_t place = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(own));
         const float factor = a.scale * kLog2E;
+        // A wave's tiles, from one of them on and round: caches that lie a power of two apart would otherwise all be
+        // read from the same few memory channels at a time.
         const int32_t mine_from = tile + static_cast<int32_t>(wave);
-        load_k.load(keys, mine_from * kKeys, place);
-        load_v.load(values, mine_from * kKeys, place + kBytes);
+        const int32_t count = mine_from < end ? (end - mine_from + static_cast<int32_t>(kFewWaves) - 1) / static_cast<int32_t>(kFewWaves) : 0;
+        const uint32_t ids = gridDim.x * gridDim.y, id = blockIdx.x + blockIdx.y * gridDim.x;
+        int32_t at = static_cast<int32_t>(static_cast<uint64_t>(id) * static_cast<uint32_t>(count) / ids), load_at = at;
+        const auto first_of = [&](int32_t t) {
+            return (mine_from + t * static_cast<int32_t>(kFewWaves)) * static_cast<int32_t>(kKeys);
+        };
+        const auto turn = [&](int32_t& t) { t = t + 1 == count ? 0 : t + 1; };
+        const auto load = [&](uint32_t to) {
+            load_k.load(keys, first_of(load_at), place + to);
+            load_v.load(values, first_of(load_at), place + to + kBytes);
+            turn(load_at);
+        };
+        if (count > 0) load(0);
+        s16x8 q[D / 16];
+        load_row<D>(q, a.q.at(p.batch, p.first + token, kv_head * group + row % group), token < p.length, a.read_dim);
         uint32_t buffer = 0;
-        for (int32_t t = mine_from; t < end; t += 4, buffer ^= 2 * kBytes) {
-            // a tile past the end reads nothing: its zeros are waited for like any other's
-            load_k.load(keys, (t + 4) * kKeys, place + (buffer ^ 2 * kBytes));
-            load_v.load(values, (t + 4) * kKeys, place + (buffer ^ 2 * kBytes) + kBytes);
+        for (int32_t t = 0; t < count; ++t, buffer ^= 2 * kBytes) {
+            // after the last tile the first one is loaded again, and waited for like any other
+            load(buffer ^ 2 * kBytes);
             arrived<2 * Loader<D, kKeys, 1>::kLoads>();
-            const int32_t first_key = t * static_cast<int32_t>(kKeys);
             const lds_char* k = own + buffer;
             f32x16 s[1];
             scores<T, D, 32>(s, q, k, f);
+            const int32_t first_key = first_of(at);
+            turn(at);
             if (first_key < common.lo || first_key + static_cast<int32_t>(kKeys) > common.hi)
                 mask<32>(s, first_key, mine);
             take<T, D, 32>(st, s, k + kBytes, f, factor);
@@ -362,21 +378,24 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void few_rows_
     }
     // the waves' states, each shrunk to the largest of their maxima, added in the order of the waves
     st.sum = both_sum(st.sum);
+    __syncthreads();                                     // no tile is read any more
+    constexpr uint32_t kRow = D + 4;                     // keeps 32 rows' accesses in different banks
+    static_assert(kFewWaves * 32 * (kRow + 2) * 4 <= kFewWaves * kOwn, "the states fit the tiles' place");
+    float(*tops)[32] = reinterpret_cast<float(*)[32]>(shared + kFewWaves * 32 * kRow * 4);
+    float(*sums)[32] = tops + kFewWaves;
     if (lane < 32) tops[wave][lane] = st.top, sums[wave][lane] = st.sum;
     __syncthreads();
     const uint32_t r = lane % 32;
     float top = tops[0][r];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, tops[w][r]);
+    for (uint32_t w = 1; w < kFewWaves; ++w) top = fmaxf(top, tops[w][r]);
     const float factor = a.scale * kLog2E;
     float sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
+    for (uint32_t w = 0; w < kFewWaves; ++w)
         sum += tops[w][r] == -INFINITY ? sums[w][r] : sums[w][r] * exp2_of((tops[w][r] - top) * factor);
     const float shrink = st.top == -INFINITY ? 1.0f : exp2_of((st.top - top) * factor);
-    constexpr uint32_t kRow = D + 4;                     // keeps 32 rows' accesses in different banks
     float* mine_out = reinterpret_cast<float*>(shared) + wave * 32 * kRow;
-    static_assert(4 * 32 * kRow * 4 <= 4 * kOwn, "the states fit the tiles' place");
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -386,8 +405,8 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void few_rows_
             *reinterpret_cast<u32x4_t*>(mine_out + r * kRow + d * 32 + i * 2 + lane / 32 * 4) = Elem<float>::pack(v);
         }
     __syncthreads();
-    // eight lanes to a row
-    const uint32_t out_row = threadIdx.x / 8, at = threadIdx.x % 8;
+    // a row to 2 * kFewWaves lanes; the statistics are those of lane row % 32
+    const uint32_t out_row = threadIdx.x / (2 * kFewWaves), at = threadIdx.x % (2 * kFewWaves);
     const uint32_t piece_row = p.tile * 32 + out_row, out_token = piece_row / group;
     const uint32_t head = kv_head * group + piece_row % group;
     // from lanes of rows that may not be there: before any lane leaves
@@ -398,12 +417,15 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void few_rows_
     char* to = const_cast<char*>(a.out.at(p.batch, p.first + out_token, head));
     float* part_to = a.partial + (static_cast<uint64_t>(part) * a.rows_all + flat) * D;
 #pragma unroll
-    for (uint32_t e = at * 8; e < D; e += 64) {
+    for (uint32_t e = at * 8; e < D; e += 16 * kFewWaves) {
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float* from = reinterpret_cast<const float*>(shared) + out_row * kRow + e + i;
-            v[i] = ((from[0] + from[32 * kRow]) + (from[64 * kRow] + from[96 * kRow])) * scale;
+            v[i] = from[0];
+#pragma unroll
+            for (uint32_t w = 1; w < kFewWaves; ++w) v[i] += from[w * 32 * kRow];
+            v[i] *= scale;
         }
         if (a.parts > 1) store_vec<float, 8>(part_to, e / 8, D, v);
         else store_eight<T>(to, e, a.dim, a.aligned, v);
@@ -505,7 +527,7 @@ Plan plan_of(const la_attention_t& c)
 template <typename T, int D> int run(const Plan& p, const ForwardArgs& a, hipStream_t stream)
 {
     const dim3 grid(static_cast<uint32_t>(p.pieces * a.kv_heads), static_cast<uint32_t>(p.parts));
-    int rc = p.few ? launch(few_rows_kernel<T, D>, grid, dim3(256), stream, a)
+    int rc = p.few ? launch(few_rows_kernel<T, D>, grid, dim3(kFewWaves * 64), stream, a)
                    : launch(attention_kernel<T, D>, grid, dim3(256), stream, a);
     if (rc == LA_OK && p.parts > 1)
         rc = launch(join_kernel<T, D>, dim3(ceil_div(a.rows_all, 4u)), dim3(256), stream, a);
