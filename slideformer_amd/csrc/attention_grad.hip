@@ -282,6 +282,12 @@ template <> __device__ __forceinline__ void score<_Float16>(f32x16& c, const s16
     else asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "a"(b));
 }
 
+// One wait for four reads of LDS in place of one for each.
+__device__ __forceinline__ void wait_for(const s16x8& a, const s16x8& b, const s16x8& c, const s16x8& d)
+{
+    asm volatile("" : : "v"(a), "v"(b), "v"(c), "v"(d));
+}
+
 template <int N> struct Number {
     static constexpr int value = N;
 };
@@ -384,12 +390,14 @@ template <typename T, int D> struct Keys {
         for (int m = 0; m < kAhead; ++m) rows[m] = begin.rows[m];
 #pragma unroll
         for (int m = 0; m < 2 * kSteps; ++m) {
-            if (m % 2 == 0)
+            // four at a time, so that they are waited for once in four products
+            if (m % kAhead == 0)
 #pragma unroll
-                for (int n = m + kAhead; n < m + kAhead + 2; ++n) {
+                for (int n = m + kAhead; n < m + 2 * kAhead; ++n) {
                     if (n < 2 * kSteps) rows[n] = row_fragment<kNext, 1 - B>(n);
                     else columns[n - 2 * kSteps] = column_fragment<BUF, B>(n - 2 * kSteps);
                 }
+            if (m % kAhead == 0) wait_for(rows[m], rows[m + 1], rows[m + 2], rows[m + 3]);
             if (m % 2) score<T>(then.d, rows[m], v[m / 2], m < 2);
             else score<T>(then.s, rows[m], k[m / 2], m < 2);
 #pragma unroll
@@ -409,15 +417,15 @@ template <typename T, int D> struct Keys {
         asm volatile("s_nop 1" : "+v"(p[0]), "+v"(p[1]), "+v"(ds[0]), "+v"(ds[1]));
 #pragma unroll
         for (int m = 0; m < 4 * kParts; ++m) {
-            if (m % 2 == 0 && m + kAhead < 4 * kParts) {
-                columns[m + kAhead] = column_fragment<BUF, B>(m + kAhead);
-                columns[m + kAhead + 1] = column_fragment<BUF, B>(m + kAhead + 1);
-            }
+            if (m % kAhead == 0 && m + kAhead < 4 * kParts)
+#pragma unroll
+                for (int n = m + kAhead; n < m + 2 * kAhead; ++n) columns[n] = column_fragment<BUF, B>(n);
             if (m + kAhead == 4 * kParts) {
                 read_values<kNext, 1 - B>(begin);
                 if (BUF == 1 && B == 0) move_rows();
                 read_rows<kAfter, B>(begin);
             }
+            if (m % kAhead == 0) wait_for(columns[m], columns[m + 1], columns[m + 2], columns[m + 3]);
             if (m < 2 * kParts) add_product<T>(sums_v[m % kParts], columns[m], p[m / kParts]);
             else add_product<T>(sums_k[m % kParts], columns[m], ds[m / kParts - 2]);
             beside(m);
@@ -483,29 +491,38 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
         // the tile that is loaded next: tiles of a head, then the next head's; past the last nothing
         uint32_t load_head = kv_head * group, load_to = 0;
         const uint32_t head_end = load_head + group;
-        int32_t load_tile = tile_from;
+        int32_t load_tile = tile_from, left = 0;
         u32x4_t rsrc_q, rsrc_g;
-        uint64_t values_at;
+        uint64_t at_q = 0, at_g = 0, values_at = 0;
         uint32_t values_bytes;
+        const uint32_t step_q = kTileRows * load_q.stride, step_g = kTileRows * load_g.stride;
         // In parts, to go between products: where the tile lies, and its loads.
-        constexpr int kEach = Loader<D, kTileRows, 4>::kLoads, kLoads = 2 * kEach + 2;   // of a wave, for a tile
+        constexpr int kParts = 4, kLoads = 2 * Loader<D, kTileRows, 4>::kLoads + 2;      // of a wave, for a tile
         const auto turn = [&] {
-            const int32_t from = load_tile * static_cast<int32_t>(kTileRows);
-            const int32_t left = load_head < head_end ? static_cast<int32_t>(p.length) - from : 0;
-            const uint64_t row = static_cast<uint64_t>(p.first) + from;
-            rsrc_q = load_q.descriptor(reinterpret_cast<uint64_t>(a.q.at(p.batch, row, load_head)), left);
-            rsrc_g = load_g.descriptor(reinterpret_cast<uint64_t>(a.grad_out.at(p.batch, row, load_head)), left);
-            values_at = (static_cast<uint64_t>(load_head) * a.rows_all + static_cast<uint64_t>(p.batch) * a.seq.rows + row) * 4;
+            if (load_tile == tile_from) {
+                const int32_t from = load_tile * static_cast<int32_t>(kTileRows);
+                const uint64_t row = static_cast<uint64_t>(p.first) + from;
+                left = load_head < head_end ? static_cast<int32_t>(p.length) - from : 0;
+                at_q = uniform(reinterpret_cast<uint64_t>(a.q.at(p.batch, row, load_head)));
+                at_g = uniform(reinterpret_cast<uint64_t>(a.grad_out.at(p.batch, row, load_head)));
+                values_at = (static_cast<uint64_t>(load_head) * a.rows_all + static_cast<uint64_t>(p.batch) * a.seq.rows + row) * 4;
+            }
+            rsrc_q = load_q.descriptor(at_q, left);
+            rsrc_g = load_g.descriptor(at_g, left);
             values_bytes = left <= 0 ? 0u : left < static_cast<int32_t>(kTileRows) ? left * 4u : kRowValues;
+            at_q += step_q;
+            at_g += step_g;
+            left -= static_cast<int32_t>(kTileRows);
             if (++load_tile == tile_to) load_tile = tile_from, ++load_head;
         };
         const auto load_part = [&](int n) {
-            if (n < kEach) load_q.load(rsrc_q, n, base + load_to + wave * 1024);
-            else if (n < 2 * kEach) load_g.load(rsrc_g, n - kEach, base + load_to + wave * 1024 + kBytes);
-            else if (n == 2 * kEach)
+            if (n == 0) load_q.load(rsrc_q, base + load_to + wave * 1024);
+            if (n == 1) load_g.load(rsrc_g, base + load_to + wave * 1024 + kBytes);
+            if (n == 2)
                 load_values(reinterpret_cast<uint64_t>(a.less) + values_at, values_bytes, base + load_to + values);
-            else if (n == 2 * kEach + 1) {
+            if (n == 3) {
                 load_values(reinterpret_cast<uint64_t>(a.delta) + values_at, values_bytes, base + load_to + values + kRowValues);
+                values_at += kRowValues;
                 load_to = load_to == 3 * kBuffer ? 0 : load_to + kBuffer;
             }
         };
@@ -514,7 +531,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
         for (int n = 0; n < 3; ++n) {
             turn();
 #pragma unroll
-            for (int k = 0; k < kLoads; ++k) load_part(k);
+            for (int k = 0; k < kParts; ++k) load_part(k);
         }
         arrive<2 * kLoads>();
         typename Mine::Scores even, odd;
@@ -528,16 +545,13 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
             constexpr int kBuf = decltype(buffer)::value;
             const int32_t first_row = tile * static_cast<int32_t>(kTileRows);
             const bool partly = first_row < common.lo || first_row + static_cast<int32_t>(kTileRows) > common.hi;
-            constexpr int kSums = 4 * (D / 32), kPerSum = (kLoads + kSums - 3) / (kSums - 2);
             w.template block<kBuf, 0>(
                 even, odd, begin, first_row, mine, partly,
                 // the next tile is there, and all waves have done with the one before this
                 [&] { arrive<kLoads>(); },
                 [&](int m) {
                     if (m == 0) turn();
-#pragma unroll
-                    for (int n = 0; n < kPerSum; ++n)
-                        if (m > 0 && (m - 1) * kPerSum + n < kLoads) load_part((m - 1) * kPerSum + n);
+                    if (m > 0 && m <= kParts) load_part(m - 1);
                 });
             w.template block<kBuf, 1>(odd, even, begin, first_row, mine, partly, [] {}, [](int) {});
             if (++tile == tile_to) tile = tile_from;

@@ -148,30 +148,38 @@ template <int D, uint32_t ROWS, uint32_t WAVES> struct Loader {
                 uniform(rows ? (rows - 1) * stride + width : 0u), 0x00020000u};
     }
 
-    // Load n into `lds`, the place of this wave's first 1024 bytes; returns at once.
+    // The loads of such rows into `lds`, the place of this wave's first 1024 bytes; returns at once.
     // Written in assembly, which takes no result in a register: the compiler would
     // wait for every load in flight before any read of LDS.  The loops wait themselves.
     // The wait states before the first load are for the descriptor, which vector instructions may have written.
-    __device__ __forceinline__ void load(const u32x4_t& rsrc, uint32_t n, uint32_t lds) const
+    __device__ __forceinline__ void load(const u32x4_t& rsrc, uint32_t lds) const
     {
-        if (n == 0)
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+        if constexpr (kLoads == 2) {
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+                         "s_add_u32 m0, m0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
                          :
-                         : "s"(uniform(lds)), "v"(offset[n]), "s"(rsrc)
-                         : "m0");
-        else
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                         :
-                         : "s"(uniform(lds + n * WAVES * 1024)), "v"(offset[n]), "s"(rsrc)
-                         : "m0");
+                         : "s"(uniform(lds)), "v"(offset[0]), "v"(offset[1]), "s"(rsrc), "n"(WAVES * 1024)
+                         : "m0", "scc");
+        } else {
+            static_assert(kLoads % 4 == 0, "four loads at a time");
+#pragma unroll
+            for (uint32_t n = 0; n < kLoads; n += 4)
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
+                             "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %5, 0 offen lds\n\t"
+                             "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %5, 0 offen lds\n\t"
+                             "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %5, 0 offen lds"
+                             :
+                             : "s"(uniform(lds + n * WAVES * 1024)), "v"(offset[n]), "v"(offset[n + 1]), "v"(offset[n + 2]),
+                               "v"(offset[n + 3]), "s"(rsrc), "n"(WAVES * 1024)
+                             : "m0", "scc");
+        }
     }
 
     // Row `first` of `m` on.
     __device__ __forceinline__ void load(const Rows& m, int32_t first, uint32_t lds) const
     {
         const u32x4_t rsrc = descriptor(m.at + static_cast<uint64_t>(first < 0 ? 0 : first) * stride, m.rows - first);
-#pragma unroll
-        for (uint32_t n = 0; n < kLoads; ++n) load(rsrc, n, lds);
+        load(rsrc, lds);
     }
 };
 
