@@ -210,7 +210,11 @@ __device__ __forceinline__ void load_row(s16x8 (&q)[D / 16], const char* row, bo
 }
 
 // 128 rows to a workgroup, 32 to a wave; all waves go over the same tiles of 64 keys, two of which are
-// in LDS: one in work, the next on its way.
+// in LDS: one in work, the next on its way.  Two workgroups on a compute unit (four of D = 64), each in the
+// other's pauses.  8192 tokens, causal, 32 and 8 heads of 128 in bf16: 525 us, 1.05 PFLOP/s, the matrix cores busy 57 % of
+// the cycles.  Two variants took fewer cycles and no less time, as the clock sank with them (1.95 GHz
+// in a first launch, 1.6 to 1.7 under load): scores of the next tile between the exponentials of this
+// one (541), and eight waves that take turns at multiplying and at exponentials (530).
 template <typename T, int D> __global__ __launch_bounds__(256, 2) void attention_kernel(ForwardArgs a)
 {
     constexpr uint32_t kBytes = Tile<D>::kBytes;

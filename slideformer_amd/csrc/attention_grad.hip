@@ -95,6 +95,7 @@ __device__ __forceinline__ void hide(f32x16& x, int32_t first, const Seen& range
     }
 }
 
+// This lane's row as an operand: elements 16 k + 8 (l / 32) .. + 7.
 template <int D> __device__ __forceinline__ void load_row(s16x8 (&q)[D / 16], const char* row, bool there, uint32_t dim)
 {
     const uint32_t half = threadIdx.x % kWave / 32;
@@ -104,7 +105,10 @@ template <int D> __device__ __forceinline__ void load_row(s16x8 (&q)[D / 16], co
         if (there && k * 16 + half * 8 < dim) u = *reinterpret_cast<const u32x4_t*>(row + (k * 16 + half * 8) * 2);
         q[k] = __builtin_bit_cast(s16x8, u);
     }
-    // the loads are over before others begin that are counted by hand
+}
+// It is there: no load of it is in flight beside those that are counted by hand.
+template <int D> __device__ __forceinline__ void have_row(s16x8 (&q)[D / 16])
+{
 #pragma unroll
     for (uint32_t k = 0; k < D / 16; ++k) asm volatile("" : "+v"(q[k]));
 }
@@ -165,32 +169,6 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_q_ke
     const Seen mine = seen(a.seq, p, token);
     const uint64_t flat = static_cast<uint64_t>(p.batch) * a.seq.rows + p.first + token;
 
-    s16x8 q[D / 16], g[D / 16];
-    load_row<D>(q, a.q.at(p.batch, p.first + token, head), there, a.read_dim);
-    load_row<D>(g, a.grad_out.at(p.batch, p.first + token, head), there, a.read_dim);
-    float delta, lse2;
-    {
-        s16x8 o[D / 16];
-        load_row<D>(o, a.out.at(p.batch, p.first + token, head), there, a.read_dim);
-        f32x16 x = zeros();
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) x = mfma<T>(o[k], g[k], x);
-        // column c's own row: element 4 (c / 8) + c % 4 of the half of lanes c / 4 % 2
-        const uint32_t c = lane % 32;
-        float found = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) found = c / 8 * 4 + c % 4 == static_cast<uint32_t>(i) ? x[i] : found;
-        const Halves h = halves(__float_as_uint(found), __float_as_uint(found));
-        delta = __uint_as_float(c / 4 % 2 ? h.hi : h.lo);
-        lse2 = there ? *reinterpret_cast<const float*>(a.lse.at(p.batch, p.first + token, head)) * kLog2E : 0.0f;
-        if (there && lane < 32) {
-            const uint64_t at = static_cast<uint64_t>(head) * a.rows_all + flat;
-            a.less[at] = Range<T>::kP - lse2;
-            a.delta[at] = delta;
-        }
-        asm volatile("" : "+v"(lse2));
-    }
-
     const uint32_t last_row = p.length * group;
     const auto range = [&](uint32_t row_from, uint32_t row_to) {
         row_to = row_to < last_row ? row_to : last_row;
@@ -206,23 +184,54 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_q_ke
     int32_t tile = all.lo / static_cast<int32_t>(kTileRows);
     const int32_t end = all.hi > 0 ? (all.hi + static_cast<int32_t>(kTileRows) - 1) / static_cast<int32_t>(kTileRows) : 0;
 
+    // the first tile is on its way while this lane's row is fetched
+    const Rows keys{reinterpret_cast<uint64_t>(a.k.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
+    const Rows values{reinterpret_cast<uint64_t>(a.v.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
+    Loader<D, kTileRows, 4> load_k, load_v;
+    load_k.init(wave, static_cast<uint32_t>(a.k.row), a.read_dim);
+    load_v.init(wave, static_cast<uint32_t>(a.v.row), a.read_dim);
+    lds_char* lds = (lds_char*)shared;
+    const uint32_t place = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + wave * 1024;
+    if (tile < end) {
+        load_k.load(keys, tile * kTileRows, place);
+        load_v.load(values, tile * kTileRows, place + kBytes);
+    }
+    s16x8 q[D / 16], g[D / 16];
+    float delta, lse2;
+    {
+        s16x8 o[D / 16];
+        load_row<D>(g, a.grad_out.at(p.batch, p.first + token, head), there, a.read_dim);
+        load_row<D>(o, a.out.at(p.batch, p.first + token, head), there, a.read_dim);
+        load_row<D>(q, a.q.at(p.batch, p.first + token, head), there, a.read_dim);
+        lse2 = there ? *reinterpret_cast<const float*>(a.lse.at(p.batch, p.first + token, head)) * kLog2E : 0.0f;
+        f32x16 x = zeros();
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) x = mfma<T>(o[k], g[k], x);
+        // column c's own row: element 4 (c / 8) + c % 4 of the half of lanes c / 4 % 2
+        const uint32_t c = lane % 32;
+        float found = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) found = c / 8 * 4 + c % 4 == static_cast<uint32_t>(i) ? x[i] : found;
+        const Halves h = halves(__float_as_uint(found), __float_as_uint(found));
+        delta = __uint_as_float(c / 4 % 2 ? h.hi : h.lo);
+        if (there && lane < 32) {
+            const uint64_t at = static_cast<uint64_t>(head) * a.rows_all + flat;
+            a.less[at] = Range<T>::kP - lse2;
+            a.delta[at] = delta;
+        }
+        have_row<D>(q);
+        have_row<D>(g);
+        asm volatile("" : "+v"(lse2));
+    }
+
     f32x16 sums[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) sums[d] = zeros();
     Range<T> scaled;
     if (tile < end) {
-        const Rows keys{reinterpret_cast<uint64_t>(a.k.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
-        const Rows values{reinterpret_cast<uint64_t>(a.v.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
-        Loader<D, kTileRows, 4> load_k, load_v;
-        load_k.init(wave, static_cast<uint32_t>(a.k.row), a.read_dim);
-        load_v.init(wave, static_cast<uint32_t>(a.v.row), a.read_dim);
         Fragments<D> f;
         f.init();
-        lds_char* lds = (lds_char*)shared;
-        const uint32_t place = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + wave * 1024;
         const float factor = a.scale * kLog2E;
-        load_k.load(keys, tile * kTileRows, place);
-        load_v.load(values, tile * kTileRows, place + kBytes);
         uint32_t buffer = 0;
         for (; tile < end; ++tile, buffer ^= 2 * kBytes) {
             arrive<0>();
@@ -474,10 +483,6 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) w.sums_k[d] = w.sums_v[d] = zeros();
     if (tile_from < tile_to) {
-        load_row<D>(w.k, a.k.at(p.batch, p.key_first + key, kv_head), there, a.read_dim);
-        load_row<D>(w.v, a.v.at(p.batch, p.key_first + key, kv_head), there, a.read_dim);
-#pragma unroll
-        for (int m = 0; m < D / 16; ++m) asm volatile("" : "+a"(w.k[m]), "+a"(w.v[m]));
         w.factor = a.scale * kLog2E;
         Loader<D, kTileRows, 4> load_q, load_g;
         load_q.init(wave, static_cast<uint32_t>(a.q.row), a.read_dim);
@@ -533,6 +538,11 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
 #pragma unroll
             for (int k = 0; k < kParts; ++k) load_part(k);
         }
+        load_row<D>(w.k, a.k.at(p.batch, p.key_first + key, kv_head), there, a.read_dim);
+        load_row<D>(w.v, a.v.at(p.batch, p.key_first + key, kv_head), there, a.read_dim);
+#pragma unroll
+        for (int m = 0; m < D / 16; ++m) asm volatile("" : "+a"(w.k[m]), "+a"(w.v[m]));
+        // the first tile, and these rows, which were asked for later than all three
         arrive<2 * kLoads>();
         typename Mine::Scores even, odd;
         typename Mine::Begin begin;
