@@ -34,7 +34,49 @@ struct GradArgs {
     float scale;
     int q_aligned, k_aligned, v_aligned;
     int keep_rest;
+    uint32_t parts, chain;          // of grad_kv_kernel: see Span
+    float* partial;                 // [part][flat keys][kv_heads][k's and v's][D]
+    uint32_t keys_all;              // flat keys
 };
+
+// The rows that see keys [from, to) of a sequence, those of a workgroup in tiles of 64, of each of its query heads.
+// Where they are more than `chain` tiles, up to `parts` workgroups share them and add their sums in join_kv_kernel: a
+// launch takes as long as its longest chain of tiles.
+struct Span {
+    Seen rows;
+    int32_t tile_from, tiles;       // of one head
+    int32_t count;                  // of all heads
+    int32_t parts;
+};
+
+__device__ __forceinline__ Seen rows_of(const Sequences& s, const Piece& p, uint32_t from, uint32_t to)
+{
+    Seen r{0, static_cast<int32_t>(p.length)};
+    if (!s.causal) return r;
+    const int32_t shift = static_cast<int32_t>(p.keys) - static_cast<int32_t>(p.length);
+    r.lo = static_cast<int32_t>(from) - shift;
+    r.lo = r.lo < 0 ? 0 : r.lo;
+    const int32_t last = static_cast<int32_t>(to) - 1 - shift;           // sees key `to` - 1 as its last
+    if (s.window && last + static_cast<int64_t>(s.window) < r.hi) r.hi = last + static_cast<int32_t>(s.window);
+    return r;
+}
+
+template <int D> __device__ __forceinline__ Span span_of(const GradArgs& a, const Piece& p)
+{
+    const uint32_t first = p.tile * 128, past = first + 128 < p.keys ? first + 128 : p.keys;
+    Span s{};
+    s.rows = p.rest ? Seen{0, 0} : rows_of(a.seq, p, first, past);
+    s.tile_from = s.rows.lo / static_cast<int32_t>(kTileRows);
+    const int32_t to = s.rows.hi > 0 ? (s.rows.hi + static_cast<int32_t>(kTileRows) - 1) / static_cast<int32_t>(kTileRows) : 0;
+    s.tiles = to > s.tile_from ? to - s.tile_from : 0;
+    s.count = s.tiles * static_cast<int32_t>(a.seq.group);
+    s.parts = 1;
+    if (D == 128 && a.parts > 1 && s.count > static_cast<int32_t>(a.chain)) {
+        s.parts = (s.count + static_cast<int32_t>(a.chain) - 1) / static_cast<int32_t>(a.chain);
+        s.parts = s.parts < static_cast<int32_t>(a.parts) ? s.parts : static_cast<int32_t>(a.parts);
+    }
+    return s;
+}
 
 // Waits until what wrote these sums has, and what reads them may: longer than any matrix instruction needs.
 template <int N> __device__ __forceinline__ void settle(f32x16 (&x)[N])
@@ -63,9 +105,9 @@ template <> struct Range<_Float16> {
         float most = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) most = fmaxf(most, __builtin_fabsf(x[i]));
-        most = both_max(most);
         if (__any(most * up > 32768.0f)) {
             // to 2^10 .. 2^11: five doublings before it shrinks again
+            most = both_max(most);
             int e;
             (void)frexpf(most, &e);
             e = 11 - e;
@@ -458,31 +500,21 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
     const uint32_t group = a.seq.group;
     const uint32_t key = p.tile * 128 + wave * 32 + lane % 32;
     const bool there = key < p.keys;
-    const int32_t shift = static_cast<int32_t>(p.keys) - static_cast<int32_t>(p.length);
-
-    // the queries that see keys [from, to)
-    const auto rows_of = [&](uint32_t from, uint32_t to) {
-        Seen r{0, static_cast<int32_t>(p.length)};
-        if (!a.seq.causal) return r;
-        r.lo = static_cast<int32_t>(from) - shift;
-        r.lo = r.lo < 0 ? 0 : r.lo;
-        const int32_t last = static_cast<int32_t>(to) - 1 - shift;       // sees key `to` - 1 as its last
-        if (a.seq.window && last + static_cast<int64_t>(a.seq.window) < r.hi)
-            r.hi = last + static_cast<int32_t>(a.seq.window);
-        return r;
-    };
-    const Seen mine = rows_of(key, key + 1);
-    const uint32_t first = p.tile * 128, wave_first = first + wave * 32;
-    const uint32_t past = first + 128 < p.keys ? first + 128 : p.keys;
-    const Seen all = p.rest ? Seen{0, 0} : rows_of(first, past);
-    const Seen common{rows_of(wave_first + 31, wave_first + 32).lo, rows_of(wave_first, wave_first + 1).hi};
-    const int32_t tile_from = all.lo / static_cast<int32_t>(kTileRows);
-    const int32_t tile_to = all.hi > 0 ? (all.hi + static_cast<int32_t>(kTileRows) - 1) / static_cast<int32_t>(kTileRows) : 0;
+    const Span span = span_of<D>(a, p);
+    const int32_t part = static_cast<int32_t>(blockIdx.y);
+    if (part >= span.parts) return;
+    const int32_t tile_from = span.tile_from, tile_to = span.tile_from + span.tiles;
+    const int32_t begun = D == 128 ? static_cast<int32_t>(static_cast<int64_t>(span.count) * part / span.parts) : 0;
+    const int32_t count =
+        D == 128 ? static_cast<int32_t>(static_cast<int64_t>(span.count) * (part + 1) / span.parts) - begun : span.count;
+    const Seen mine = rows_of(a.seq, p, key, key + 1);
+    const uint32_t wave_first = p.tile * 128 + wave * 32;
+    const Seen common{rows_of(a.seq, p, wave_first + 31, wave_first + 32).lo, rows_of(a.seq, p, wave_first, wave_first + 1).hi};
 
     Mine w;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) w.sums_k[d] = w.sums_v[d] = zeros();
-    if (tile_from < tile_to) {
+    if (count > 0) {
         w.factor = a.scale * kLog2E;
         Loader<D, kTileRows, 4> load_q, load_g;
         load_q.init(wave, static_cast<uint32_t>(a.q.row), a.read_dim);
@@ -494,31 +526,39 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
         w.values = w.lds + values + lane / 32 * 16;
         w.rows_on = w.columns_on = 2 * kBuffer;
         // the tile that is loaded next: tiles of a head, then the next head's; past the last nothing
-        uint32_t load_head = kv_head * group, load_to = 0;
-        const uint32_t head_end = load_head + group;
-        int32_t load_tile = tile_from, left = 0;
+        uint32_t load_head = kv_head * group + begun / span.tiles, load_to = 0;
+        int32_t tile = tile_from + begun % span.tiles, load_tile = tile, loads = count, left = 0;
         u32x4_t rsrc_q, rsrc_g;
         uint64_t at_q = 0, at_g = 0, values_at = 0;
         uint32_t values_bytes;
         const uint32_t step_q = kTileRows * load_q.stride, step_g = kTileRows * load_g.stride;
         // In parts, to go between products: where the tile lies, and its loads.
         constexpr int kParts = 4, kLoads = 2 * Loader<D, kTileRows, 4>::kLoads + 2;      // of a wave, for a tile
+        const auto aim = [&] {
+            const int32_t from = load_tile * static_cast<int32_t>(kTileRows);
+            const uint64_t row = static_cast<uint64_t>(p.first) + from;
+            left = static_cast<int32_t>(p.length) - from;
+            at_q = uniform(reinterpret_cast<uint64_t>(a.q.at(p.batch, row, load_head)));
+            at_g = uniform(reinterpret_cast<uint64_t>(a.grad_out.at(p.batch, row, load_head)));
+            values_at = (static_cast<uint64_t>(load_head) * a.rows_all + static_cast<uint64_t>(p.batch) * a.seq.rows + row) * 4;
+        };
+        aim();
         const auto turn = [&] {
-            if (load_tile == tile_from) {
-                const int32_t from = load_tile * static_cast<int32_t>(kTileRows);
-                const uint64_t row = static_cast<uint64_t>(p.first) + from;
-                left = load_head < head_end ? static_cast<int32_t>(p.length) - from : 0;
-                at_q = uniform(reinterpret_cast<uint64_t>(a.q.at(p.batch, row, load_head)));
-                at_g = uniform(reinterpret_cast<uint64_t>(a.grad_out.at(p.batch, row, load_head)));
-                values_at = (static_cast<uint64_t>(load_head) * a.rows_all + static_cast<uint64_t>(p.batch) * a.seq.rows + row) * 4;
-            }
-            rsrc_q = load_q.descriptor(at_q, left);
-            rsrc_g = load_g.descriptor(at_g, left);
-            values_bytes = left <= 0 ? 0u : left < static_cast<int32_t>(kTileRows) ? left * 4u : kRowValues;
+            const int32_t rows = loads-- > 0 ? left : 0;
+            rsrc_q = load_q.descriptor(at_q, rows);
+            rsrc_g = load_g.descriptor(at_g, rows);
+            values_bytes = rows <= 0 ? 0u : rows < static_cast<int32_t>(kTileRows) ? rows * 4u : kRowValues;
+        };
+        const auto advance = [&] {
             at_q += step_q;
             at_g += step_g;
+            values_at += kRowValues;
             left -= static_cast<int32_t>(kTileRows);
-            if (++load_tile == tile_to) load_tile = tile_from, ++load_head;
+            if (++load_tile == tile_to) {
+                load_tile = tile_from;
+                ++load_head;
+                aim();
+            }
         };
         const auto load_part = [&](int n) {
             if (n == 0) load_q.load(rsrc_q, base + load_to + wave * 1024);
@@ -527,11 +567,10 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
                 load_values(reinterpret_cast<uint64_t>(a.less) + values_at, values_bytes, base + load_to + values);
             if (n == 3) {
                 load_values(reinterpret_cast<uint64_t>(a.delta) + values_at, values_bytes, base + load_to + values + kRowValues);
-                values_at += kRowValues;
                 load_to = load_to == 3 * kBuffer ? 0 : load_to + kBuffer;
+                advance();
             }
         };
-        const int32_t count = (tile_to - tile_from) * static_cast<int32_t>(group);
 #pragma unroll
         for (int n = 0; n < 3; ++n) {
             turn();
@@ -549,7 +588,6 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
         w.begin(even);
         w.template read_rows<0, 1>(begin);
         w.template read_values<0, 0>(begin);
-        int32_t tile = tile_from;
         // One tile, in buffer kBuf of a pair.
         const auto step = [&](auto buffer) {
             constexpr int kBuf = decltype(buffer)::value;
@@ -577,17 +615,105 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
     settle(w.sums_k);
     settle(w.sums_v);
     constexpr float kShrinkP = Range<T>::kP == 0.0f ? 1.0f : 0x1p-14f;
+    const float scale_k = a.scale * kShrinkP / w.scaled.factor();
+    if (D == 128 && span.parts > 1) {
+        float* to = a.partial + ((static_cast<uint64_t>(part) * a.keys_all + static_cast<uint64_t>(p.batch) * a.seq.key_rows +
+                                  p.key_first + key) * a.kv_heads + kv_head) * (2 * D);
+        if (!there) return;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                float x[4], y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = w.sums_k[d][i + e] * scale_k;
+                    y[e] = w.sums_v[d][i + e] * kShrinkP;
+                }
+                const uint32_t at = d * 32 + i * 2 + lane / 32 * 4;
+                *reinterpret_cast<u32x4_t*>(to + at) = Elem<float>::pack(x);
+                *reinterpret_cast<u32x4_t*>(to + D + at) = Elem<float>::pack(y);
+            }
+        return;
+    }
     const bool stored = key < (a.keep_rest ? (p.rest ? 0u : p.keys) : p.key_stored);
     store_row<T, D>(const_cast<char*>(a.grad_v.at(p.batch, p.key_first + key, kv_head)), w.sums_v, kShrinkP, stored, a.dim,
                     a.v_aligned);
-    store_row<T, D>(const_cast<char*>(a.grad_k.at(p.batch, p.key_first + key, kv_head)), w.sums_k,
-                    a.scale * kShrinkP / w.scaled.factor(), stored, a.dim, a.k_aligned);
+    store_row<T, D>(const_cast<char*>(a.grad_k.at(p.batch, p.key_first + key, kv_head)), w.sums_k, scale_k, stored, a.dim,
+                    a.k_aligned);
+}
+
+// The sums of keys whose rows several workgroups shared, in the order of the parts: eight elements to a lane.
+template <typename T, int D> __global__ __launch_bounds__(256) void join_kv_kernel(GradArgs a)
+{
+    const uint32_t kv_head = blockIdx.x % a.kv_heads;
+    const Piece p = locate(a.seq, blockIdx.x / a.kv_heads, true, 1, 128);
+    if (!p.valid) return;
+    const Span span = span_of<D>(a, p);
+    if (span.parts < 2) return;
+    // beyond a sequence's keys there are no sums; those rows get zeros, if anything
+    const uint32_t stored = a.keep_rest ? p.keys : p.key_stored;
+    for (uint32_t at = threadIdx.x; at < 128 * (2 * D / 8); at += 256) {
+        const uint32_t key = p.tile * 128 + at / (2 * D / 8), e = at % (2 * D / 8) * 8;
+        if (key >= stored) continue;
+        float v[8] = {};
+        if (key < p.keys)
+            for (int32_t part = 0; part < span.parts; ++part) {
+                const float* from = a.partial + ((static_cast<uint64_t>(part) * a.keys_all +
+                                                  static_cast<uint64_t>(p.batch) * a.seq.key_rows + p.key_first + key) *
+                                                     a.kv_heads + kv_head) * (2 * D) + e;
+                float lo[4], hi[4];
+                load_vec<float>(from, 0, 8, lo);
+                load_vec<float>(from, 1, 8, hi);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[i] += lo[i];
+                    v[4 + i] += hi[i];
+                }
+            }
+        const bool of_v = e >= D;
+        const Heads& to = of_v ? a.grad_v : a.grad_k;
+        T* out = reinterpret_cast<T*>(const_cast<char*>(to.at(p.batch, p.key_first + key, kv_head)));
+        const uint32_t first = e % D;
+        if ((of_v ? a.v_aligned : a.k_aligned) && first + 8 <= a.dim) {
+            *reinterpret_cast<u32x4_t*>(out + first) = Elem<T>::pack(v);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                if (first + i < a.dim) out[first + i] = Elem<T>::from_f32(v[i]);
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 uint64_t row_values_bytes(const la_attention_t& c) { return ceil_div(flat_rows(c) * c.heads * 4, 256ull) * 256; }
+
+// How the rows of keys are shared out, from what the host knows: sequences of average length, of which one may be as long
+// as all are.
+struct Parts {
+    uint64_t parts = 1, chain = 0, bytes = 0;
+};
+
+Parts parts_of(const la_attention_t& c)
+{
+    Parts p;
+    const uint64_t rows = c.starts ? ceil_div(c.rows, c.batch) : c.rows, keys = c.starts ? ceil_div(c.key_rows, c.batch) : c.key_rows;
+    const uint64_t group = c.heads / c.kv_heads, slots = c.dim <= 64 ? 512 : 256;       // workgroups at a time
+    const uint64_t most = c.window ? (128 + c.window) / kTileRows + 2 : ~0ull;          // tiles of a head that see 128 keys
+    const uint64_t tiles = ceil_div(rows, kTileRows), average = std::min(c.causal ? tiles / 2 + 1 : tiles, most);
+    const uint64_t ideal = c.batch * c.kv_heads * ceil_div(keys, 128) * group * average / slots;
+    const uint64_t longest = group * std::min<uint64_t>(ceil_div(c.rows, kTileRows), most);
+    const uint64_t workgroups = c.batch * c.kv_heads * ceil_div(keys, 128);
+    if (c.dim > 64 && longest > 24 && workgroups < slots) {
+        p.chain = std::max<uint64_t>(ideal, 16);
+        p.parts = std::min<uint64_t>(4, ceil_div(longest, p.chain));
+    }
+    if (p.parts > 1)
+        p.bytes = ceil_div(p.parts * flat_keys(c) * c.kv_heads * 2 * (c.dim <= 64 ? 64 : 128) * sizeof(float), 256ull) * 256;
+    return p;
+}
 
 template <typename T, int D> int run(const la_attention_t& c, const GradArgs& a, hipStream_t stream)
 {
@@ -596,7 +722,9 @@ template <typename T, int D> int run(const la_attention_t& c, const GradArgs& a,
     const uint64_t by_keys = pieces(a.seq, true, 1, 128) * c.kv_heads;
     if (flat_rows(c) > 0) rc = launch(grad_q_kernel<T, D>, dim3(static_cast<uint32_t>(by_rows)), dim3(256), stream, a);
     if (rc == LA_OK && flat_keys(c) > 0)
-        rc = launch(grad_kv_kernel<T, D>, dim3(static_cast<uint32_t>(by_keys)), dim3(256), stream, a);
+        rc = launch(grad_kv_kernel<T, D>, dim3(static_cast<uint32_t>(by_keys), a.parts), dim3(256), stream, a);
+    if (rc == LA_OK && flat_keys(c) > 0 && a.parts > 1)
+        rc = launch(join_kv_kernel<T, D>, dim3(static_cast<uint32_t>(by_keys)), dim3(256), stream, a);
     return rc;
 }
 
@@ -613,7 +741,7 @@ uint64_t la_attention_grad_workspace(const la_attention_t* call)
 {
     if (check_call(call) != LA_OK) return 0;
     const la_attention_t& c = *call;
-    return 2 * row_values_bytes(c) + packed_bytes(c, c.q, true) + packed_bytes(c, c.k, false) +
+    return 2 * row_values_bytes(c) + parts_of(c).bytes + packed_bytes(c, c.q, true) + packed_bytes(c, c.k, false) +
            packed_bytes(c, c.v, false) + packed_bytes(c, c.out, true) + packed_bytes(c, c.grad_out, true);
 }
 
@@ -642,6 +770,12 @@ int la_attention_grad(const la_attention_t* call, void* workspace, uint64_t work
     a.less = reinterpret_cast<float*>(ws);
     a.delta = reinterpret_cast<float*>(ws + row_values_bytes(c));
     ws += 2 * row_values_bytes(c);
+    const Parts parts = parts_of(c);
+    a.parts = static_cast<uint32_t>(parts.parts);
+    a.chain = static_cast<uint32_t>(parts.chain);
+    a.partial = reinterpret_cast<float*>(ws);
+    a.keys_all = static_cast<uint32_t>(flat_keys(c));
+    ws += parts.bytes;
     rc = heads_of(c, c.q, true, a.q, ws, st);
     if (rc == LA_OK) rc = heads_of(c, c.k, false, a.k, ws, st);
     if (rc == LA_OK) rc = heads_of(c, c.v, false, a.v, ws, st);
