@@ -243,6 +243,22 @@ def test_long_sequences(hip_device):
     Case(hip_device, F16, [1900, 2300], [1900, 2300], 2, 1, 64, packed=False).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("how", [dict(), dict(window=500), dict(causal=False), dict(packed=False, rows=1200, key_rows=1200)])
+def test_gradients_of_few_keys_with_many_rows(hip_device, dtype, how):
+    """Several workgroups share the rows that see a key, and add their sums at the end."""
+    lengths = [1100, 0, 40, 260]
+    case = Case(hip_device, dtype, lengths, lengths, 8, 1, 128, before=3, behind=150, **how)
+    case.all()
+    out, lse = case.run()
+    want = case.grad(out, lse)
+    given = tuple(torch.full_like(t, 3.0) for t in (case.q, case.k, case.v))
+    for g, w, mine in zip(case.grad(out, lse, grads=given), want, (case.mine, case.my_keys, case.my_keys)):
+        assert torch.equal(g[mine], w[mine]) and bool((g[~mine] == 3).all())
+    few = Case(hip_device, dtype, [1500], [70], 8, 1, 128, causal=False)
+    few.all()
+
+
 def _fused(t):
     """Heads as they lie in the rows of a wider matrix."""
     wide = torch.full((*t.shape[:-2], t.shape[-2] + 3, t.shape[-1]), NAN, dtype=t.dtype, device=t.device)
