@@ -38,61 +38,16 @@ struct ForwardArgs {
 // The running state of 32 rows in a wave: of row l % 32 a lane has the elements 32 d + 8 (i / 4) + 4 (l / 32) + i % 4.
 template <int D> struct State {
     f32x16 out[D / 32];
-    float top;                      // the maximum that `sum` and `out` are relative to, in units of scores
+    float top;                      // the score that `sum` and `out` are relative to: -inf until the row's first key
     float sum;                      // over this half's keys
-    __device__ __forceinline__ void init()
+    __device__ __forceinline__ void init(const Seen& row)
     {
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) out[d] = zeros();
-        top = -INFINITY;
+        top = row.hi > row.lo ? -INFINITY : 0.0f;        // one that sees nothing waits for no key
         sum = 0.0f;
     }
 };
-
-// How far, in powers of two, scores may pass the maximum before sums are brought
-// to the new one: a row's values stay below 2^8 times what they would be, which costs no
-// precision, and after the first tiles hardly any tile touches `out`.
-constexpr float kSlack = 8.0f;
-
-// Takes KEYS keys (32 or 64) of a tile in: their scores are in `s`, masked ones -inf.
-template <typename T, int D, int KEYS>
-__device__ __forceinline__ void take(State<D>& st, f32x16 (&s)[KEYS / 32], const lds_char* v, const Fragments<D>& f,
-                                     float factor)
-{
-    float top = s[0][0];
-#pragma unroll
-    for (int b = 0; b < KEYS / 32; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-    top = both_max(top);
-    if (__any(top > st.top + kSlack / factor || (st.top == -INFINITY && top > -INFINITY))) {
-        const float now = fmaxf(top, st.top);
-        const float shrink = now == st.top ? 1.0f : exp2_of((st.top - now) * factor);
-        st.top = now;
-        st.sum *= shrink;
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) st.out[d] *= shrink;
-    }
-    // rows that have seen nothing yet: 0, and exp2(-inf) below
-    const float from = st.top == -INFINITY ? 0.0f : -st.top * factor;
-    float sum = 0.0f;
-#pragma unroll
-    for (int b = 0; b < KEYS / 32; ++b) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][i] = exp2_of(__builtin_fmaf(s[b][i], factor, from));
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) sum += (s[b][i] + s[b][i + 1]) + (s[b][i + 2] + s[b][i + 3]);
-    }
-    st.sum += sum;
-#pragma unroll
-    for (int b = 0; b < KEYS / 32; ++b)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const s16x8 p = rounded<T>(s[b], half);
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d) st.out[d] = mfma<T>(f.columns(v, d, b * 2 + half), p, st.out[d]);
-        }
-}
 
 template <typename T, int D, int KEYS>
 __device__ __forceinline__ void scores(f32x16 (&s)[KEYS / 32], const s16x8 (&q)[D / 16], const lds_char* k,
@@ -119,6 +74,72 @@ __device__ __forceinline__ void mask(f32x16 (&s)[KEYS / 32], int32_t first_key, 
         for (int i = 0; i < 16; ++i) {
             const uint32_t key = b * 32 + i / 4 * 8 + i % 4;
             s[b][i] = key - from < count ? s[b][i] : -INFINITY;
+        }
+}
+
+// P of scores relative to st.top, in their place; returns the sum over this half's keys.
+template <int D, int KEYS>
+__device__ __forceinline__ float exponentials(const State<D>& st, f32x16 (&s)[KEYS / 32], float factor)
+{
+    // rows that have seen nothing yet: 0, and exp2(-inf) below
+    const float from = st.top == -INFINITY ? 0.0f : -st.top * factor;
+    float sum = 0.0f;
+#pragma unroll
+    for (int b = 0; b < KEYS / 32; ++b) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = exp2_of(__builtin_fmaf(s[b][i], factor, from));
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) sum += (s[b][i] + s[b][i + 1]) + (s[b][i + 2] + s[b][i + 3]);
+    }
+    return sum;
+}
+
+// Raises the rows' maxima to those of these scores, and brings the sums to them.
+template <int D, int KEYS>
+__device__ __forceinline__ void raise(State<D>& st, const f32x16 (&s)[KEYS / 32], float factor)
+{
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < KEYS / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+    top = fmaxf(both_max(top), st.top);
+    const float shrink = top == st.top ? 1.0f : exp2_of((st.top - top) * factor);
+    st.top = top;
+    st.sum *= shrink;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) st.out[d] *= shrink;
+}
+
+// Takes KEYS keys (32 or 64) of a tile in.  Exponentials need the maximum of no tile but a row's first: those of
+// later ones stay below kMost nearly always, and where a lane's sum of them is more, the scores are made again and
+// the maxima raised.  Looking for the maximum of every tile instead is 21 more vector instructions of about 165, which
+// bind heads of 64.
+constexpr float kMost = 4096.0f;                         // which float16 holds, and each of its terms
+
+template <typename T, int D, int KEYS>
+__device__ __forceinline__ void take(State<D>& st, const s16x8 (&q)[D / 16], const lds_char* k, const lds_char* v,
+                                     const Fragments<D>& f, float factor, bool partly, int32_t first_key, const Seen& row)
+{
+    f32x16 s[KEYS / 32];
+    scores<T, D, KEYS>(s, q, k, f);
+    if (partly) mask<KEYS>(s, first_key, row);
+    if (__any(st.top == -INFINITY)) raise<D, KEYS>(st, s, factor);
+    float sum = exponentials<D, KEYS>(st, s, factor);
+    if (__any(sum > kMost)) {
+        scores<T, D, KEYS>(s, q, k, f);
+        if (partly) mask<KEYS>(s, first_key, row);
+        raise<D, KEYS>(st, s, factor);
+        sum = exponentials<D, KEYS>(st, s, factor);
+    }
+    st.sum += sum;
+#pragma unroll
+    for (int b = 0; b < KEYS / 32; ++b)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const s16x8 p = rounded<T>(s[b], half);
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) st.out[d] = mfma<T>(f.columns(v, d, b * 2 + half), p, st.out[d]);
         }
 }
 
@@ -256,7 +277,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void attention
     }
 
     State<D> st;
-    st.init();
+    st.init(mine);
     if (tile < end) {
         const Rows keys{reinterpret_cast<uint64_t>(a.k.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
         const Rows values{reinterpret_cast<uint64_t>(a.v.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
@@ -282,11 +303,8 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void attention
             const int32_t first_key = tile * static_cast<int32_t>(kTileRows);
             if (first_key < own.hi && first_key + static_cast<int32_t>(kTileRows) > own.lo) {
                 const lds_char* k = lds + buffer;
-                f32x16 s[2];
-                scores<T, D, 64>(s, q, k, f);
-                if (first_key < common.lo || first_key + static_cast<int32_t>(kTileRows) > common.hi)
-                    mask<64>(s, first_key, mine);
-                take<T, D, 64>(st, s, k + kBytes, f, factor);
+                const bool partly = first_key < common.lo || first_key + static_cast<int32_t>(kTileRows) > common.hi;
+                take<T, D, 64>(st, q, k, k + kBytes, f, factor, partly, first_key, mine);
             }
         }
     }
@@ -331,7 +349,7 @@ template <typename T, int D> __global__ __launch_bounds__(kFewWaves * 64, 1) voi
     }
 
     State<D> st;
-    st.init();
+    st.init(mine);
     lds_char* lds = (lds_char*)shared;
     if (tile < end) {
         const Rows keys{reinterpret_cast<uint64_t>(a.k.at(p.batch, p.key_first, kv_head)), static_cast<int32_t>(p.keys)};
@@ -368,13 +386,10 @@ template <typename T, int D> __global__ __launch_bounds__(kFewWaves * 64, 1) voi
             load(buffer ^ 2 * kBytes);
             arrived<2 * Loader<D, kKeys, 1>::kLoads>();
             const lds_char* k = own + buffer;
-            f32x16 s[1];
-            scores<T, D, 32>(s, q, k, f);
             const int32_t first_key = first_of(at);
             turn(at);
-            if (first_key < common.lo || first_key + static_cast<int32_t>(kKeys) > common.hi)
-                mask<32>(s, first_key, mine);
-            take<T, D, 32>(st, s, k + kBytes, f, factor);
+            const bool partly = first_key < common.lo || first_key + static_cast<int32_t>(kKeys) > common.hi;
+            take<T, D, 32>(st, q, k, k + kBytes, f, factor, partly, first_key, mine);
             // what was read is read before the next loads write over it
             arrived<2 * Loader<D, kKeys, 1>::kLoads>();
         }
