@@ -530,12 +530,16 @@ Plan plan_of(const la_attention_t& c)
     p.few = rows * group <= 32;
     p.pieces = pieces(s, false, group, p.few ? 32 : 128);
     const uint64_t tile = p.few ? 32 : kTileRows;
-    // Keys are shared out where there are too few pieces to fill the card, in parts of 512 keys at least: less
-    // is over before the join begins.
+    // Keys are shared out where there are too few pieces to fill the card, in parts of 512 keys at least: less is over
+    // before the join begins.  What the join reads of many rows grows with their workgroups, and a part's own time with
+    // its keys, so a part has 8 keys for each workgroup too: 12 heads of 64, 4 x 1024 tokens (384 workgroups) take
+    // 43 us in two parts and 24 in one; 32/8 heads of 128, 128 rows of 8 sequences (256), 41 and 27 against 1024 keys
+    // and 317 and 332 against 16384; and one such sequence of 4096 (32) 23 in eight parts and 75 in one.
     const uint64_t keys = s.starts ? ceil_div(c.key_rows, c.batch) : c.key_rows;
-    const uint64_t tiles = ceil_div(keys, tile);
-    const uint64_t wanted = ceil_div(kFill, std::max<uint64_t>(1, p.pieces * c.kv_heads));
-    p.parts = std::max<uint64_t>(1, std::min({wanted, tiles / (512 / tile), uint64_t{kMostParts}}));
+    const uint64_t tiles = ceil_div(keys, tile), workgroups = std::max<uint64_t>(1, p.pieces * c.kv_heads);
+    const uint64_t wanted = p.few ? ceil_div(kFill, workgroups) : kFill / workgroups;
+    const uint64_t least = p.few ? 512 : std::max<uint64_t>(512, 8 * workgroups);
+    p.parts = std::max<uint64_t>(1, std::min({wanted, keys / least, uint64_t{kMostParts}}));
     p.part_tiles = ceil_div(std::max<uint64_t>(1, tiles), p.parts);
     p.parts = std::max<uint64_t>(1, ceil_div(tiles, p.part_tiles));
     p.partial_bytes = p.parts > 1 ? p.parts * flat_rows(c) * c.heads * (p.padded + 1) * sizeof(float) : 0;
