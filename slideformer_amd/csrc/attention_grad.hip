@@ -49,8 +49,10 @@ struct Span {
     int32_t parts;
 };
 
+// Those that see some of keys [from, to): none where the sequence has no such key.
 __device__ __forceinline__ Seen rows_of(const Sequences& s, const Piece& p, uint32_t from, uint32_t to)
 {
+    if (from >= p.keys) return {0, 0};
     Seen r{0, static_cast<int32_t>(p.length)};
     if (!s.causal) return r;
     const int32_t shift = static_cast<int32_t>(p.keys) - static_cast<int32_t>(p.length);
@@ -509,7 +511,9 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
         D == 128 ? static_cast<int32_t>(static_cast<int64_t>(span.count) * (part + 1) / span.parts) - begun : span.count;
     const Seen mine = rows_of(a.seq, p, key, key + 1);
     const uint32_t wave_first = p.tile * 128 + wave * 32;
-    const Seen common{rows_of(a.seq, p, wave_first + 31, wave_first + 32).lo, rows_of(a.seq, p, wave_first, wave_first + 1).hi};
+    const Seen common = wave_first + 32 <= p.keys ? Seen{rows_of(a.seq, p, wave_first + 31, wave_first + 32).lo,
+                                                         rows_of(a.seq, p, wave_first, wave_first + 1).hi}
+                                                  : Seen{0, 0};
 
     Mine w;
 #pragma unroll

@@ -188,6 +188,15 @@ def test_queries_and_keys_of_different_lengths(hip_device, dtype, dim, queries, 
     Case(hip_device, dtype, queries, keys, 4, 2, dim, causal=causal, window=window).all()
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [(BF16, 4, 2, 64), (F16, 8, 1, 128)])
+@pytest.mark.parametrize("causal,window", [(False, None), (True, None), (True, 30)])
+@pytest.mark.parametrize("queries,keys", [([5, 200, 64, 0], [100, 30, 0, 9]), ([700, 3], [2, 200])])
+def test_padded_keys_have_no_gradient(hip_device, dtype, heads, kv_heads, dim, causal, window, queries, keys):
+    """Whole tiles of them, and some beside a sequence's own keys."""
+    Case(hip_device, dtype, queries, keys, heads, kv_heads, dim, packed=False, causal=causal, window=window,
+         rows=max(queries) + 20, key_rows=300).all()
+
+
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
 @pytest.mark.parametrize("packed", [True, False])
 def test_rows_of_no_sequence(hip_device, index, packed):
