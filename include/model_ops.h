@@ -181,7 +181,8 @@ int la_attention(const la_attention_t* call, void* workspace, uint64_t workspace
  * and lse: P = exp(scale q k - lse), dP = grad_out v, dS = P (dP - sum(grad_out out)),
  *   grad_q = scale dS k,  grad_k = scale dS^T q,  grad_v = P^T grad_out,
  * those of key heads summed over the query heads that share them.  Rows beyond a sequence's length or in no
- * sequence have gradient 0, or with keep_rest != 0 stay as they were.  Nothing is added atomically.
+ * sequence have gradient 0, or with keep_rest != 0 stay as they were.  Nothing is added atomically.  The gradients
+ * may lie between one another, as parts of one projection's do, but not where the call reads.
  * workspace: la_attention_grad_workspace(call) bytes, 256-byte aligned.
  */
 uint64_t la_attention_grad_workspace(const la_attention_t* call);
@@ -193,7 +194,8 @@ int la_attention_grad(const la_attention_t* call, void* workspace, uint64_t work
  * pairs (a, b) -> (a cos - b sin, b cos + a sin), pair j by cos and sin [position][j] of fp32 tables with
  * `positions` rows of rotated / 2; in fp32, rounded once.  Pairs are elements (j, j + rotated / 2), or with
  * interleaved != 0 (2 j, 2 j + 1).  Row i has position at[i] (int32 or int64), or i where `at` is null; one outside
- * the tables makes the rotated elements of its row NaN.  Results may be written over their inputs.
+ * the tables makes the rotated elements of its row NaN.  Results may be written over their inputs, not over
+ * one another.
  */
 typedef struct {
     int dtype;

@@ -590,6 +590,10 @@ int la_attention(const la_attention_t* call, void* workspace, uint64_t workspace
     if (!reachable(c.q.data) || !reachable(c.k.data) || !reachable(c.v.data) || !reachable(c.out.data) ||
         !reachable(c.lse.data) || !indices_reachable(c) || (la_attention_workspace(call) && !reachable(workspace)))
         return LA_EFAULT;
+    const Extent written = extent(c, c.out, true);
+    if (!apart(written, extent(c, c.q, true)) || !apart(written, extent(c, c.k, false)) ||
+        !apart(written, extent(c, c.v, false)))
+        return LA_EINVAL;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
     ForwardArgs a{};

@@ -441,6 +441,19 @@ inline uint64_t packed_bytes(const la_attention_t& c, const la_heads_t& h, bool 
     return ceil_div(rows * (queries ? c.heads : c.kv_heads) * ceil_div(c.dim, 8ull) * 16, 256ull) * 256;
 }
 
+// The memory from the first to the last element of `h`.
+struct Extent {
+    uintptr_t from, to;
+};
+inline Extent extent(const la_attention_t& c, const la_heads_t& h, bool queries)
+{
+    const uint64_t rows = queries ? c.rows : c.key_rows, heads = queries ? c.heads : c.kv_heads;
+    const uintptr_t from = reinterpret_cast<uintptr_t>(h.data);
+    if (sets(c) * rows == 0) return {from, from};
+    return {from, from + 2 * ((sets(c) - 1) * h.batch_stride + (rows - 1) * h.row_stride + (heads - 1) * h.head_stride + c.dim)};
+}
+inline bool apart(const Extent& a, const Extent& b) { return a.from == a.to || b.from == b.to || a.to <= b.from || b.to <= a.from; }
+
 inline Heads plain(const la_heads_t& h, uint64_t size = 2)
 {
     return {static_cast<const char*>(h.data), h.batch_stride * size, h.row_stride * size, h.head_stride * size};

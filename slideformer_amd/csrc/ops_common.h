@@ -186,6 +186,7 @@ int launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t stream, A...
     return [&](P... args) {
         int k = 0;
         ((ptrs[k++] = &args), ...);
+        if (static_cast<uint64_t>(grid.x) * block.x >> 32) return static_cast<int>(LA_EINVAL);     // HIP counts threads in 32 bits
         const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, ptrs, 0, stream);
         return e == hipSuccess ? LA_OK : static_cast<int>(e);
     }(static_cast<P>(given)...);

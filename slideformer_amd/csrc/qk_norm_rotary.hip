@@ -434,6 +434,8 @@ int check_reach(const la_rotary_t& c)
     return LA_OK;
 }
 
+bool same_results(const la_rotary_t& c) { return c.n && c.heads && c.kv_heads && c.q_out.data == c.k_out.data; }
+
 RotaryArgs args_of(const la_rotary_t& c)
 {
     RotaryArgs a{};
@@ -535,6 +537,7 @@ int la_qk_norm_rotary(const la_rotary_t* call, la_stream_t stream)
     if (c.n == 0 || c.heads + c.kv_heads == 0) return LA_OK;
     if ((c.heads && bad(c.q, c.dtype)) || (c.kv_heads && bad(c.k, c.dtype))) return LA_EINVAL;
     rc = check_reach(c);
+    if (rc == LA_OK && same_results(c)) rc = LA_EINVAL;
     if (rc != LA_OK) return rc;
     RotaryArgs a = args_of(c);
     const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -568,6 +571,8 @@ int la_qk_norm_rotary_grad(const la_rotary_t* call, void* workspace, uint64_t wo
     if (rc == LA_OK && (!reachable(c.grad_q_weight) || !reachable(c.grad_k_weight) || (normed && !reachable(workspace)) ||
                         (any && (!reachable(c.grad_q.data) || !reachable(c.grad_k.data)))))
         rc = LA_EFAULT;
+    // each result is written by workgroups of its own, in no order
+    if (rc == LA_OK && (same_results(c) || (c.q_weight && c.k_weight && c.grad_q_weight == c.grad_k_weight))) rc = LA_EINVAL;
     if (rc != LA_OK) return rc;
     RotaryArgs a = args_of(c);
     a.grad_q = rows_of(c.grad_q, c.dtype);

@@ -216,6 +216,38 @@ def test_refusals_of_attention(hip_device, t):
             ops.attention_grad(**{**call, **how})
 
 
+@pytest.mark.parametrize("packed", [True, False])
+def test_gradients_do_not_go_where_the_call_reads(hip_device, t, packed):
+    """One kernel would write what the next reads.  Parts of one projection's gradient are fine, and so is
+    memory beside what is read."""
+    rows = (130,) if packed else (2, 65)
+    qkv, new = t(*rows, 8, 64), torch.zeros(*rows, 8, 64, dtype=torch.bfloat16, device=hip_device)
+    q, k, v = qkv[..., :4, :], qkv[..., 4:6, :], qkv[..., 6:, :]
+    how = dict(starts=torch.tensor([0, 60, 130], device=hip_device)) if packed else {}
+    out, lse = ops.attention(q, k, v, **how)
+    g = t(*rows, 4, 64)
+    want = ops.attention_grad(g, q, k, v, out, lse, **how)
+    parts = (new[..., :4, :], new[..., 4:6, :], new[..., 6:, :])
+    ops.attention_grad(g, q, k, v, out, lse, grads=parts, **how)
+    for a, b in zip(parts, want):
+        assert torch.equal(a, b)
+    for grads in ((q, k, v), (g, *parts[1:]), (out, *parts[1:]), (parts[0], k, parts[2]), (parts[0], parts[1], v),
+                  (parts[0], parts[1], parts[1])):
+        kept = [x.clone() for x in grads]
+        with pytest.raises(RuntimeError, match="la_attention_grad"):
+            ops.attention_grad(g, q, k, v, out, lse, grads=grads, **how)
+        assert all(torch.equal(a, b) for a, b in zip(grads, kept))
+    table, w, n = t(130, 32, dtype=torch.float32), t(64), 130
+    q, k = q.reshape(n, 4, 64).clone(), k.reshape(n, 2, 64).clone()
+    k4 = t(n, 4, 64)
+    with pytest.raises(RuntimeError, match="la_qk_norm_rotary"):
+        ops.qk_norm_rotary(q, k4, table, table, out=(k4, k4))
+    with pytest.raises(RuntimeError, match="la_qk_norm_rotary_grad"):
+        ops.qk_norm_rotary_grad(q, k4, q, k4, table, table, out=(q, q))
+    with pytest.raises(RuntimeError, match="la_qk_norm_rotary_grad"):
+        ops.qk_norm_rotary_grad(q, k, q, k, table, table, q_weight=w, k_weight=w, grad_q_weight=w, grad_k_weight=w)
+
+
 def test_refusals_of_the_rotation(hip_device, t):
     q, k, table = t(5, 4, 64), t(5, 2, 64), t(5, 32, dtype=torch.float32)
 
