@@ -338,7 +338,8 @@ template <typename T, int D> __global__ __launch_bounds__(kFewWaves * 64, 1) voi
     if (row_from < row_to) {
         const Seen first = seen(a.seq, p, row_from / group), last = seen(a.seq, p, (row_to - 1) / group);
         all = {first.lo, last.hi};
-        common = {last.lo, first.hi};
+        // those that all of them see: none where rows behind a sequence's are among what is written
+        if (row_to == row_from + 32 || row_to == p.stored * group) common = {last.lo, first.hi};
     }
     int32_t tile = all.lo / static_cast<int32_t>(kKeys);
     int32_t end = all.hi > 0 ? (all.hi + static_cast<int32_t>(kKeys) - 1) / static_cast<int32_t>(kKeys) : 0;

@@ -197,6 +197,15 @@ def test_padded_keys_have_no_gradient(hip_device, dtype, heads, kv_heads, dim, c
          rows=max(queries) + 20, key_rows=300).all()
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [(BF16, 2, 1, 64), (F16, 24, 8, 100), (BF16, 5, 5, 128)])
+@pytest.mark.parametrize("causal,window", [(False, None), (True, None), (True, 40)])
+@pytest.mark.parametrize("queries,keys,rows", [([1], [1300], 6), ([3, 1, 0, 2], [90, 300, 70, 1], 8), ([20], [200], 100)])
+def test_padded_queries_see_nothing(hip_device, dtype, heads, kv_heads, dim, causal, window, queries, keys, rows):
+    """Beside whole tiles of keys that the sequence's own queries see."""
+    Case(hip_device, dtype, queries, keys, heads, kv_heads, dim, packed=False, causal=causal, window=window, rows=rows,
+         key_rows=max(keys) + 30).all()
+
+
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
 @pytest.mark.parametrize("packed", [True, False])
 def test_rows_of_no_sequence(hip_device, index, packed):
