@@ -647,45 +647,45 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
                     a.k_aligned);
 }
 
-// The sums of keys whose rows several workgroups shared, in the order of the parts: eight elements to a lane.
+// The sums of keys whose rows several workgroups shared, in the order of the parts: eight elements to a lane.  A workgroup
+// takes 256 / (2 D / 8) of a piece's 128 keys, one round of loads: all 128 in one workgroup's rounds took 20 us.
 template <typename T, int D> __global__ __launch_bounds__(256) void join_kv_kernel(GradArgs a)
 {
+    constexpr uint32_t kChunks = 2 * D / 8;              // of a key's two rows
     const uint32_t kv_head = blockIdx.x % a.kv_heads;
     const Piece p = locate(a.seq, blockIdx.x / a.kv_heads, true, 1, 128);
     if (!p.valid) return;
     const Span span = span_of<D>(a, p);
     if (span.parts < 2) return;
+    const uint32_t key = p.tile * 128 + blockIdx.y * (256 / kChunks) + threadIdx.x / kChunks, e = threadIdx.x % kChunks * 8;
     // beyond a sequence's keys there are no sums; those rows get zeros, if anything
-    const uint32_t stored = a.keep_rest ? p.keys : p.key_stored;
-    for (uint32_t at = threadIdx.x; at < 128 * (2 * D / 8); at += 256) {
-        const uint32_t key = p.tile * 128 + at / (2 * D / 8), e = at % (2 * D / 8) * 8;
-        if (key >= stored) continue;
-        float v[8] = {};
-        if (key < p.keys)
-            for (int32_t part = 0; part < span.parts; ++part) {
-                const float* from = a.partial + ((static_cast<uint64_t>(part) * a.keys_all +
-                                                  static_cast<uint64_t>(p.batch) * a.seq.key_rows + p.key_first + key) *
-                                                     a.kv_heads + kv_head) * (2 * D) + e;
-                float lo[4], hi[4];
-                load_vec<float>(from, 0, 8, lo);
-                load_vec<float>(from, 1, 8, hi);
+    if (key >= (a.keep_rest ? p.keys : p.key_stored)) return;
+    float v[8] = {};
+    if (key < p.keys)
+#pragma unroll 4
+        for (int32_t part = 0; part < span.parts; ++part) {
+            const float* from = a.partial + ((static_cast<uint64_t>(part) * a.keys_all +
+                                              static_cast<uint64_t>(p.batch) * a.seq.key_rows + p.key_first + key) *
+                                                 a.kv_heads + kv_head) * (2 * D) + e;
+            float lo[4], hi[4];
+            load_vec<float>(from, 0, 8, lo);
+            load_vec<float>(from, 1, 8, hi);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[i] += lo[i];
-                    v[4 + i] += hi[i];
-                }
+            for (int i = 0; i < 4; ++i) {
+                v[i] += lo[i];
+                v[4 + i] += hi[i];
             }
-        const bool of_v = e >= D;
-        const Heads& to = of_v ? a.grad_v : a.grad_k;
-        T* out = reinterpret_cast<T*>(const_cast<char*>(to.at(p.batch, p.key_first + key, kv_head)));
-        const uint32_t first = e % D;
-        if ((of_v ? a.v_aligned : a.k_aligned) && first + 8 <= a.dim) {
-            *reinterpret_cast<u32x4_t*>(out + first) = Elem<T>::pack(v);
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i)
-                if (first + i < a.dim) out[first + i] = Elem<T>::from_f32(v[i]);
         }
+    const bool of_v = e >= D;
+    const Heads& to = of_v ? a.grad_v : a.grad_k;
+    T* out = reinterpret_cast<T*>(const_cast<char*>(to.at(p.batch, p.key_first + key, kv_head)));
+    const uint32_t first = e % D;
+    if ((of_v ? a.v_aligned : a.k_aligned) && first + 8 <= a.dim) {
+        *reinterpret_cast<u32x4_t*>(out + first) = Elem<T>::pack(v);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+            if (first + i < a.dim) out[first + i] = Elem<T>::from_f32(v[i]);
     }
 }
 
@@ -696,6 +696,8 @@ uint64_t row_values_bytes(const la_attention_t& c) { return ceil_div(flat_rows(c
 
 // How the rows of keys are shared out, from what the host knows: sequences of average length, of which one may be as long
 // as all are.
+constexpr uint64_t kFill = 256;                          // workgroups of D = 128 that the card takes at a time
+
 struct Parts {
     uint64_t parts = 1, chain = 0, bytes = 0;
 };
@@ -704,18 +706,24 @@ Parts parts_of(const la_attention_t& c)
 {
     Parts p;
     const uint64_t rows = c.starts ? ceil_div(c.rows, c.batch) : c.rows, keys = c.starts ? ceil_div(c.key_rows, c.batch) : c.key_rows;
-    const uint64_t group = c.heads / c.kv_heads, slots = c.dim <= 64 ? 512 : 256;       // workgroups at a time
+    const uint64_t group = c.heads / c.kv_heads, workgroups = c.batch * c.kv_heads * ceil_div(keys, 128);
     const uint64_t most = c.window ? (128 + c.window) / kTileRows + 2 : ~0ull;          // tiles of a head that see 128 keys
-    const uint64_t tiles = ceil_div(rows, kTileRows), average = std::min(c.causal ? tiles / 2 + 1 : tiles, most);
-    const uint64_t ideal = c.batch * c.kv_heads * ceil_div(keys, 128) * group * average / slots;
+    const uint64_t tiles = std::min(ceil_div(rows, kTileRows), most);
     const uint64_t longest = group * std::min<uint64_t>(ceil_div(c.rows, kTileRows), most);
-    const uint64_t workgroups = c.batch * c.kv_heads * ceil_div(keys, 128);
-    if (c.dim > 64 && longest > 24 && workgroups < slots) {
-        p.chain = std::max<uint64_t>(ideal, 16);
-        p.parts = std::min<uint64_t>(4, ceil_div(longest, p.chain));
+    if (c.dim > 64 && longest > 8 && workgroups < kFill) {
+        // No more parts than the card has room for.  Chains of full or windowed sequences are about as long as each other;
+        // causal ones are of all lengths up to the longest, and half a part is left over of each.
+        const bool alike = !c.causal || most == tiles;
+        const uint64_t chain = alike ? ceil_div(group * tiles, kFill / workgroups)
+                                     : ceil_div(workgroups * group * (tiles / 2 + 1), kFill - workgroups / 2);
+        // More than four only where the launch is resident at once if all have them: workgroups go to the compute
+        // units in turn, and wait behind long ones where others are free.
+        const uint64_t most_parts = std::min<uint64_t>(16, std::max<uint64_t>(4, kFill / workgroups));
+        p.chain = std::max({chain, ceil_div(group * tiles, most_parts), uint64_t{6}});
+        p.parts = std::min(most_parts, ceil_div(longest, p.chain));
     }
     if (p.parts > 1)
-        p.bytes = ceil_div(p.parts * flat_keys(c) * c.kv_heads * 2 * (c.dim <= 64 ? 64 : 128) * sizeof(float), 256ull) * 256;
+        p.bytes = ceil_div(p.parts * flat_keys(c) * c.kv_heads * 2 * 128 * sizeof(float), 256ull) * 256;
     return p;
 }
 
@@ -728,7 +736,7 @@ template <typename T, int D> int run(const la_attention_t& c, const GradArgs& a,
     if (rc == LA_OK && flat_keys(c) > 0)
         rc = launch(grad_kv_kernel<T, D>, dim3(static_cast<uint32_t>(by_keys), a.parts), dim3(256), stream, a);
     if (rc == LA_OK && flat_keys(c) > 0 && a.parts > 1)
-        rc = launch(join_kv_kernel<T, D>, dim3(static_cast<uint32_t>(by_keys)), dim3(256), stream, a);
+        rc = launch(join_kv_kernel<T, D>, dim3(static_cast<uint32_t>(by_keys), 128 / (256 / (2 * D / 8))), dim3(256), stream, a);
     return rc;
 }
 
