@@ -73,7 +73,7 @@ template <int D> __device__ __forceinline__ Span span_of(const GradArgs& a, cons
     s.tiles = to > s.tile_from ? to - s.tile_from : 0;
     s.count = s.tiles * static_cast<int32_t>(a.seq.group);
     s.parts = 1;
-    if (D == 128 && a.parts > 1 && s.count > static_cast<int32_t>(a.chain)) {
+    if (a.parts > 1 && s.count > static_cast<int32_t>(a.chain)) {
         s.parts = (s.count + static_cast<int32_t>(a.chain) - 1) / static_cast<int32_t>(a.chain);
         s.parts = s.parts < static_cast<int32_t>(a.parts) ? s.parts : static_cast<int32_t>(a.parts);
     }
@@ -506,9 +506,9 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
     const int32_t part = static_cast<int32_t>(blockIdx.y);
     if (part >= span.parts) return;
     const int32_t tile_from = span.tile_from, tile_to = span.tile_from + span.tiles;
-    const int32_t begun = D == 128 ? static_cast<int32_t>(static_cast<int64_t>(span.count) * part / span.parts) : 0;
+    const int32_t begun = static_cast<int32_t>(static_cast<int64_t>(span.count) * part / span.parts);
     const int32_t count =
-        D == 128 ? static_cast<int32_t>(static_cast<int64_t>(span.count) * (part + 1) / span.parts) - begun : span.count;
+        static_cast<int32_t>(static_cast<int64_t>(span.count) * (part + 1) / span.parts) - begun;
     const Seen mine = rows_of(a.seq, p, key, key + 1);
     const uint32_t wave_first = p.tile * 128 + wave * 32;
     const Seen common = wave_first + 32 <= p.keys ? Seen{rows_of(a.seq, p, wave_first + 31, wave_first + 32).lo,
@@ -620,7 +620,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
     settle(w.sums_v);
     constexpr float kShrinkP = Range<T>::kP == 0.0f ? 1.0f : 0x1p-14f;
     const float scale_k = a.scale * kShrinkP / w.scaled.factor();
-    if (D == 128 && span.parts > 1) {
+    if (span.parts > 1) {
         float* to = a.partial + ((static_cast<uint64_t>(part) * a.keys_all + static_cast<uint64_t>(p.batch) * a.seq.key_rows +
                                   p.key_first + key) * a.kv_heads + kv_head) * (2 * D);
         if (!there) return;
@@ -696,8 +696,6 @@ uint64_t row_values_bytes(const la_attention_t& c) { return ceil_div(flat_rows(c
 
 // How the rows of keys are shared out, from what the host knows: sequences of average length, of which one may be as long
 // as all are.
-constexpr uint64_t kFill = 256;                          // workgroups of D = 128 that the card takes at a time
-
 struct Parts {
     uint64_t parts = 1, chain = 0, bytes = 0;
 };
@@ -705,25 +703,31 @@ struct Parts {
 Parts parts_of(const la_attention_t& c)
 {
     Parts p;
-    const uint64_t rows = c.starts ? ceil_div(c.rows, c.batch) : c.rows, keys = c.starts ? ceil_div(c.key_rows, c.batch) : c.key_rows;
+    const uint64_t rows = c.starts ? ceil_div(c.rows, c.batch) : c.rows;
+    const uint64_t keys = c.starts ? ceil_div(c.key_rows, c.batch) : c.key_rows;
+    const uint64_t fill = c.dim <= 64 ? 512 : 256;       // workgroups that the card takes at a time
     const uint64_t group = c.heads / c.kv_heads, workgroups = c.batch * c.kv_heads * ceil_div(keys, 128);
     const uint64_t most = c.window ? (128 + c.window) / kTileRows + 2 : ~0ull;          // tiles of a head that see 128 keys
     const uint64_t tiles = std::min(ceil_div(rows, kTileRows), most);
     const uint64_t longest = group * std::min<uint64_t>(ceil_div(c.rows, kTileRows), most);
-    if (c.dim > 64 && longest > 8 && workgroups < kFill) {
-        // No more parts than the card has room for.  Chains of full or windowed sequences are about as long as each other;
-        // causal ones are of all lengths up to the longest, and half a part is left over of each.
+    if (longest > 8 && workgroups > 0 && workgroups < fill) {
+        // Without parts, and with: 16/2 heads of 64, 1 x 1024 tokens 160 and 43 us, of 128 1 x 2048 450 and 126; 16/4 heads
+        // of 64, 8 x 1024 130 and 114.  No more parts than the card has room for (32/8 heads of 128, 4 x 512: 72 us, and 90
+        // with chains of ten tiles), and none of fewer than six tiles, which take about as long as the join.  Chains of full
+        // or windowed sequences are about as long as each other; causal ones are of all lengths up to the longest, and
+        // half a part is left over of each.
         const bool alike = !c.causal || most == tiles;
-        const uint64_t chain = alike ? ceil_div(group * tiles, kFill / workgroups)
-                                     : ceil_div(workgroups * group * (tiles / 2 + 1), kFill - workgroups / 2);
+        const uint64_t chain = alike ? ceil_div(group * tiles, fill / workgroups)
+                                     : ceil_div(workgroups * group * (tiles / 2 + 1), fill - workgroups / 2);
         // More than four only where the launch is resident at once if all have them: workgroups go to the compute
-        // units in turn, and wait behind long ones where others are free.
-        const uint64_t most_parts = std::min<uint64_t>(16, std::max<uint64_t>(4, kFill / workgroups));
+        // units in turn, and wait behind long ones where others are free (32/8 heads of 128, 1 x 1024: 77 us, and 98 with
+        // eight; 16/2 heads 97 and 75).
+        const uint64_t most_parts = std::min<uint64_t>(16, std::max<uint64_t>(4, fill / workgroups));
         p.chain = std::max({chain, ceil_div(group * tiles, most_parts), uint64_t{6}});
         p.parts = std::min(most_parts, ceil_div(longest, p.chain));
     }
     if (p.parts > 1)
-        p.bytes = ceil_div(p.parts * flat_keys(c) * c.kv_heads * 2 * 128 * sizeof(float), 256ull) * 256;
+        p.bytes = ceil_div(p.parts * flat_keys(c) * c.kv_heads * 2 * (c.dim <= 64 ? 64 : 128) * sizeof(float), 256ull) * 256;
     return p;
 }
 

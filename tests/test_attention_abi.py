@@ -123,6 +123,19 @@ def test_attention_workspaces():
     assert L.la_attention(ctypes.byref(call), HP, parts - 1, None) == EINVAL
 
 
+@pytest.mark.parametrize("causal", [0, 1])
+@pytest.mark.parametrize("rows,key_rows", [(4096, 0), (0, 4096), (4096, 1), (1, 4096), (4096, 4096)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_workspaces_of_any_lengths(causal, rows, key_rows, dim):
+    """The rows' statistics, and partial results of keys; packed sequences that may all be empty among them."""
+    L = _ops_lib.load()
+    for packed in (dict(), dict(starts=HP, key_starts=HP, batch=1 << 20)):
+        call = _attention(causal=causal, rows=rows, key_rows=key_rows, dim=dim, **packed)
+        L.la_attention_workspace(ctypes.byref(call))
+        flat = rows * (1 if packed else 2)
+        assert L.la_attention_grad_workspace(ctypes.byref(call)) >= 2 * flat * 2 * 4
+
+
 def test_attention_of_nothing():
     L = _ops_lib.load()
     none = _heads(None)
