@@ -10,9 +10,11 @@
 // in which they lie in memory: a tile of keys is loaded once for all of them, and a single new
 // token with eight query heads is eight rows.
 //
-// Scores are S^T = K Q^T, so a lane holds scores of one row (see attention_tile.h); rounded
-// to 16 bits they are the second operand of out^T += V^T P^T.  The sum l is that of
-// the unrounded values.
+// Scores are S^T = K Q^T, so a lane holds scores of one row (see attention_tile.h); their exponentials, rounded
+// to the 16 bits that the matrix cores take, are the second operand of out^T += V^T P^T.  That rounding is the one
+// before the result's own: half a step for each probability, in no direction, so a row's result is off by less than
+// half a step of its largest terms (bf16: 2.2e-3 of all results where the rounding of exact ones is 1.6e-3).  The
+// sum l is that of the unrounded values, in fp32 like the maxima and the sums of products.
 #include "attention_tile.h"
 
 #include <algorithm>
@@ -233,7 +235,8 @@ __device__ __forceinline__ void load_row(s16x8 (&q)[D / 16], const char* row, bo
 // 128 rows to a workgroup, 32 to a wave; all waves go over the same tiles of 64 keys, two of which are
 // in LDS: one in work, the next on its way.  Two workgroups on a compute unit (four of D = 64), each in the
 // other's pauses.  8192 tokens, causal, 32 and 8 heads of 128 in bf16: 525 us, 1.05 PFLOP/s, the matrix cores busy 57 % of
-// the cycles.  Two variants took fewer cycles and no less time, as the clock sank with them (1.95 GHz
+// the cycles.  8 x 1024 tokens, causal, 12 heads of 64: 27 us, 0.49 PFLOP/s, matrix cores busy 31 %: with half the products
+// for each exponential the vector instructions bind, 15 to a product, and the launch is as long as its longest piece.  Two variants took fewer cycles and no less time, as the clock sank with them (1.95 GHz
 // in a first launch, 1.6 to 1.7 under load): scores of the next tile between the exponentials of this
 // one (541), and eight waves that take turns at multiplying and at exponentials (530).
 template <typename T, int D> __global__ __launch_bounds__(256, 2) void attention_kernel(ForwardArgs a)
@@ -314,7 +317,8 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void attention
 // At most 32 rows to a workgroup (a single new token's heads): its waves take the same rows and different keys, each
 // with tiles of its own in LDS and without waiting for the others, and join at the end.  Two waves, so that
 // two workgroups or more are on a compute unit and one's start and end are under the other's loads.
-// Bound by memory: a wave takes 0.8 us for 32 keys where loads do not bind.  With five tiles in a ring, four of them
+// Bound by memory: a wave takes 0.8 us for 32 keys where loads do not bind.  16 rows of 32/8 heads of 128 over caches
+// of 8192 filled to 5600 on average, 367 MB: 75 us, 4.9 TB/s; one row over 65536, 268 MB: 44.6 us, 6.0 TB/s.  With five tiles in a ring, four of them
 // on their way, one row over 65536 keys of eight heads took 47.9 us instead of 44.4, with four waves 46.5.
 constexpr uint32_t kFewWaves = 2;
 
@@ -460,8 +464,9 @@ template <typename T, int D> __global__ __launch_bounds__(kFewWaves * 64, 1) voi
     }
 }
 
-// The parts' results of one row into one: a wave to a row, eight elements to a lane, the lanes beside each other in
-// turn on the parts.
+// The parts' results of one row into one, each by its share exp(lse of the part - lse of all): a wave to a row, eight
+// elements to a lane, the lanes beside each other in turn on the parts.  All latency: 4.8 us for 32 rows of 64 parts,
+// as for 512 of 4, with the launch before it about 10 us of a step.  Partial results are fp32.
 template <typename T, int D> __global__ __launch_bounds__(256) void join_kernel(ForwardArgs a)
 {
     constexpr uint32_t kLanes = D / 8, kSide = kWave / kLanes;

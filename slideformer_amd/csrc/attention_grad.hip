@@ -16,6 +16,11 @@
 //
 // delta is the diagonal of O dO^T, by the matrix instructions that make dP of V and dO, in the
 // same order: a row that sees one key has O = V and exactly no dS.
+//
+// P and dS are rounded to the operands' 16 bits before the last three products, as the matrix cores take them, and
+// delta is that of the O that was given, itself rounded: bf16 gradients of q and k are 2.7e-3 off where rounding the exact
+// ones is 1.7e-3 off, fp16 3.5e-4 and 2.1e-4.  A delta from the sums of P dP would not have O's rounding, but would be
+// wrong with an lse over more keys than the call has.  Everything else is fp32.
 #include "attention_tile.h"
 
 #include <algorithm>
@@ -35,6 +40,8 @@ struct GradArgs {
     int q_aligned, k_aligned, v_aligned;
     int keep_rest;
     uint32_t parts, chain;          // of grad_kv_kernel: see Span
+    uint32_t pieces;                // of keys
+    int neighbours;                 // a piece's parts beside each other, not a part's pieces
     float* partial;                 // [part][flat keys][kv_heads][k's and v's][D]
     uint32_t keys_all;              // flat keys
 };
@@ -196,7 +203,10 @@ __device__ __forceinline__ void store_row(char* to, const f32x16 (&x)[D / 32], f
         }
 }
 
-// 128 rows to a workgroup, 32 to a wave, tiles of 64 keys as in the forward pass.
+// 128 rows to a workgroup, 32 to a wave, tiles of 64 keys as in the forward pass, and two workgroups on a compute unit.
+// 8192 tokens in five packed documents of 717 to 3588, 32/8 heads of 128 in bf16: 261 us, 0.89 PFLOP/s of its three
+// products; 8 x 1024 tokens, 12 heads of 64, 34 us.  The matrix cores are busy 51 and 35 % of the cycles: between a tile's
+// scores and its sums a wave has exponentials, and one other wave whose products could go on meanwhile.
 template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_q_kernel(GradArgs a)
 {
     constexpr uint32_t kBytes = Tile<D>::kBytes;
@@ -489,21 +499,28 @@ template <typename T, int D> struct Keys {
 };
 
 // 128 keys to a workgroup, 32 to a wave; all waves go over the same tiles of 64 rows of one query
-// head after the other.  Four tiles are in LDS: one whose sums are made, one whose scores are, two on their way.
+// head after the other.  Four tiles are in LDS: one whose sums are made, one whose scores are, two on their way.  One wave
+// on a SIMD (two of D = 64): both sums and both own operands of 128 keys take 360 registers.
+// 8192 tokens in five packed documents of 717 to 3588, 32/8 heads of 128 in bf16: 445 us, 0.69 PFLOP/s of its four
+// products; 8 x 1024 tokens, 12 heads of 64, 46 us.  The matrix cores are busy 51 and 35 % of the cycles, bound by issue
+// (a wave alone issues an instruction in 5.5 cycles, a product takes 32); and compute units have work 71 % of the first
+// case's time, for the longest document's first keys are the longest chain.  Two parts for each such piece took 10 % longer
+// with the card full: their rows no longer come from L2 together.
 template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_kernel(GradArgs a)
 {
     using Mine = Keys<T, D>;
     constexpr uint32_t kBytes = Mine::kBytes, kRowValues = Mine::kRowValues, kBuffer = Mine::kBuffer;
     __shared__ __attribute__((aligned(1024))) char shared[4 * kBuffer];
     const uint32_t kv_head = blockIdx.x % a.kv_heads;
-    const Piece p = locate(a.seq, blockIdx.x / a.kv_heads, true, 1, 128);
+    const uint32_t id = blockIdx.x / a.kv_heads;
+    const Piece p = locate(a.seq, a.neighbours ? id / a.parts : id % a.pieces, true, 1, 128);
     if (!p.valid) return;
     const uint32_t wave = uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     const uint32_t group = a.seq.group;
     const uint32_t key = p.tile * 128 + wave * 32 + lane % 32;
     const bool there = key < p.keys;
     const Span span = span_of<D>(a, p);
-    const int32_t part = static_cast<int32_t>(blockIdx.y);
+    const int32_t part = static_cast<int32_t>(a.neighbours ? id % a.parts : id / a.pieces);
     if (part >= span.parts) return;
     const int32_t tile_from = span.tile_from, tile_to = span.tile_from + span.tiles;
     const int32_t begun = static_cast<int32_t>(static_cast<int64_t>(span.count) * part / span.parts);
@@ -648,7 +665,8 @@ template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_k
 }
 
 // The sums of keys whose rows several workgroups shared, in the order of the parts: eight elements to a lane.  A workgroup
-// takes 256 / (2 D / 8) of a piece's 128 keys, one round of loads: all 128 in one workgroup's rounds took 20 us.
+// takes 256 / (2 D / 8) of a piece's 128 keys, one round of loads: 5.3 us for 70 pieces of up to three parts, where all 128
+// in one workgroup's rounds took 20.
 template <typename T, int D> __global__ __launch_bounds__(256) void join_kv_kernel(GradArgs a)
 {
     constexpr uint32_t kChunks = 2 * D / 8;              // of a key's two rows
@@ -698,6 +716,7 @@ uint64_t row_values_bytes(const la_attention_t& c) { return ceil_div(flat_rows(c
 // as all are.
 struct Parts {
     uint64_t parts = 1, chain = 0, bytes = 0;
+    bool neighbours = false;
 };
 
 Parts parts_of(const la_attention_t& c)
@@ -725,6 +744,10 @@ Parts parts_of(const la_attention_t& c)
         const uint64_t most_parts = std::min<uint64_t>(16, std::max<uint64_t>(4, fill / workgroups));
         p.chain = std::max({chain, ceil_div(group * tiles, most_parts), uint64_t{6}});
         p.parts = std::min(most_parts, ceil_div(longest, p.chain));
+        // Where not all are resident at once, long chains begin with all parts of the longest: 16/2 heads of 128, 1 x 8192
+        // tokens 1108 us, and 1358 with all first parts first; 32/8 heads, 1 x 2048 (chains of 45 tiles) 170 and 199, but
+        // 2 x 1024 (24) 110 and 100.
+        p.neighbours = workgroups * p.parts > fill && p.chain > 32;
     }
     if (p.parts > 1)
         p.bytes = ceil_div(p.parts * flat_keys(c) * c.kv_heads * 2 * (c.dim <= 64 ? 64 : 128) * sizeof(float), 256ull) * 256;
@@ -738,7 +761,7 @@ template <typename T, int D> int run(const la_attention_t& c, const GradArgs& a,
     const uint64_t by_keys = pieces(a.seq, true, 1, 128) * c.kv_heads;
     if (flat_rows(c) > 0) rc = launch(grad_q_kernel<T, D>, dim3(static_cast<uint32_t>(by_rows)), dim3(256), stream, a);
     if (rc == LA_OK && flat_keys(c) > 0)
-        rc = launch(grad_kv_kernel<T, D>, dim3(static_cast<uint32_t>(by_keys), a.parts), dim3(256), stream, a);
+        rc = launch(grad_kv_kernel<T, D>, dim3(static_cast<uint32_t>(by_keys * a.parts)), dim3(256), stream, a);
     if (rc == LA_OK && flat_keys(c) > 0 && a.parts > 1)
         rc = launch(join_kv_kernel<T, D>, dim3(static_cast<uint32_t>(by_keys), 128 / (256 / (2 * D / 8))), dim3(256), stream, a);
     return rc;
@@ -796,6 +819,8 @@ int la_attention_grad(const la_attention_t* call, void* workspace, uint64_t work
     const Parts parts = parts_of(c);
     a.parts = static_cast<uint32_t>(parts.parts);
     a.chain = static_cast<uint32_t>(parts.chain);
+    a.neighbours = parts.neighbours;
+    a.pieces = static_cast<uint32_t>(pieces(s, true, 1, 128));
     a.partial = reinterpret_cast<float*>(ws);
     a.keys_all = static_cast<uint32_t>(flat_keys(c));
     ws += parts.bytes;
