@@ -515,7 +515,8 @@ def _attention_call(q, k, v, causal, window, scale, starts, key_starts, lengths,
     if not 0 < scale < float("inf"):
         raise RuntimeError(f"scale must be above 0 and finite, got {scale}")
     call = _ops_lib.LaAttention(dtype=_FLOAT[q.dtype], rows=rows, key_rows=key_rows, heads=heads, kv_heads=kv_heads,
-                                dim=dim, q=of_q, k=of_k, v=of_v, causal=int(bool(causal)), window=window or 0, scale=scale)
+                                dim=dim, q=of_q, k=of_k, v=of_v, causal=int(bool(causal)), window=min(window or 0, 1 << 40),
+                                scale=scale)
     if dims == 3:
         if starts is None:
             raise RuntimeError("packed sequences need starts")

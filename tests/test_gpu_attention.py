@@ -432,6 +432,15 @@ def test_on_another_stream(hip_device):
         assert torch.equal(a, b)
 
 
+def test_windows_longer_than_any_sequence(hip_device):
+    case = Case(hip_device, BF16, [70], [70], 2, 1, 64)
+    want = case.run()
+    for window in (70, 1 << 32, 1 << 40, (1 << 64) + 1):
+        for side in (None, torch.cuda.current_stream()):
+            got = ops.attention(case.q, case.k, case.v, window=window, starts=case.where["starts"], stream=side)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_nothing_to_do(hip_device):
     empty = torch.empty(0, 4, 64, dtype=BF16, device=hip_device)
     keys = torch.ones(0, 2, 64, dtype=BF16, device=hip_device)
