@@ -115,8 +115,8 @@ def test_attention_workspaces():
     assert size(q=_heads(head=65)) == 2 * 4 * 2 * 64 * 2
     assert size(dim=60) == 2 * 4 * (2 + 1 + 1) * 64 * 2      # rounded up to a multiple of eight
     parts = size(rows=1, key_rows=8192)
-    assert parts % (2 * 2 * 65 * 4) < 256 and 2 <= parts // (2 * 2 * 65 * 4) <= 16
-    assert size(rows=1, key_rows=600) == 0
+    assert parts % (2 * 2 * 65 * 4) < 256 and 2 <= parts // (2 * 2 * 65 * 4) <= 64
+    assert size(rows=1, key_rows=300) == 0
     assert size(dtype=F32) == 0
     assert L.la_attention_workspace(None) == 0
     call = _attention(rows=1, key_rows=8192)
