@@ -536,23 +536,21 @@ Plan plan_of(const la_attention_t& c)
     p.few = rows * group <= 32;
     p.pieces = pieces(s, false, group, p.few ? 32 : 128);
     const uint64_t tile = p.few ? 32 : kTileRows;
-    // Keys are shared out where there are too few pieces to fill the card.
+    // Keys are shared out where there are too few pieces to fill the card: in parts of 512 keys and more for two
+    // workgroups on a compute unit, in shorter ones for one; what is left then is the start and the join.
+    //   One row, 8 heads of 128: 4096 keys 18.5 us in parts of 512 and 12.2 of 128, 16384 keys 20.4 in 32 parts and 21.7
+    //   in 64; four rows, 8192 keys, 33.8 in 16 and 36.6 in 8; 256 keys 10.2 in one part and 11.5 in two.
+    //   128 rows, 12 heads of 64, 1024 keys: 15.6 us in two parts and 12.7 in four; 512 keys 11.0 in one and 12.4 in two.
+    // What the join reads of many rows grows with the workgroups, and a part's own time with its keys, so a part of these
+    // has 8 keys for each workgroup too: 12 heads of 64, 4 x 1024 tokens (384 workgroups) take 43 us in two parts and 24
+    // in one; 32/8 heads of 128, 128 rows of 8 sequences (256), 41 and 27 against 1024 keys and 317 and 332 against
+    // 16384; and one such sequence of 4096 (32) 23 in eight parts and 75 in one.
     const uint64_t keys = s.starts ? ceil_div(c.key_rows, c.batch) : c.key_rows;
     const uint64_t tiles = ceil_div(keys, tile), workgroups = std::max<uint64_t>(1, p.pieces * c.kv_heads);
-    if (p.few) {
-        // Parts of 512 keys and more for two workgroups on a compute unit, shorter ones down to 128 for one; what is left
-        // is the start and the join (one row, 8 heads of 128: 4096 keys 18.5 us in parts of 512 and 12.2 of 128, 16384 20.4 in
-        // 32 parts and 21.7 in 64; four rows, 8192 keys, 33.8 in 16 and 36.6 in 8).  256 keys take 10.2 us in one part and
-        // 11.5 in two.
-        const uint64_t half = std::min(ceil_div(kFill / 2, workgroups), keys < 384 ? 1 : keys / 128);
-        p.parts = std::min(ceil_div(kFill, workgroups), std::max(keys / 512, half));
-    } else {
-        // Parts of 512 keys at least.  What the join reads grows with the workgroups, and a part's own time with its keys, so
-        // a part has 8 keys for each workgroup too: 12 heads of 64, 4 x 1024 tokens (384 workgroups) take 43 us in two
-        // parts and 24 in one; 32/8 heads of 128, 128 rows of 8 sequences (256), 41 and 27 against 1024 keys and 317 and
-        // 332 against 16384; and one such sequence of 4096 (32) 23 in eight parts and 75 in one.
-        p.parts = std::min(kFill / workgroups, keys / std::max<uint64_t>(512, 8 * workgroups));
-    }
+    const uint64_t joined = p.few ? 0 : 8 * workgroups, least = std::max<uint64_t>(p.few ? 128 : 256, joined);
+    const auto fill = [&](uint64_t of) { return p.few ? ceil_div(of, workgroups) : of / workgroups; };
+    const uint64_t shorter = std::min(fill(kFill / 2), keys < 3 * least ? 1 : keys / least);
+    p.parts = std::min(fill(kFill), std::max(shorter, keys / std::max<uint64_t>(512, joined)));
     p.parts = std::max<uint64_t>(1, std::min<uint64_t>(p.parts, kMostParts));
     p.part_tiles = ceil_div(std::max<uint64_t>(1, tiles), p.parts);
     p.parts = std::max<uint64_t>(1, ceil_div(tiles, p.part_tiles));
