@@ -18,7 +18,7 @@
 // same order: a row that sees one key has O = V and exactly no dS.
 //
 // P and dS are rounded to the operands' 16 bits before the last three products, as the matrix cores take them, and
-// delta is that of the O that was given, itself rounded: bf16 gradients of q and k are 2.7e-3 off where rounding the exact
+// delta, but for short sequences and windows, is that of the O that was given, itself rounded: bf16 gradients of q and k are 2.7e-3 off where rounding the exact
 // ones is 1.7e-3 off, fp16 3.5e-4 and 2.1e-4.  A delta from the sums of P dP would not have O's rounding, but would be
 // wrong with an lse over more keys than the call has.  Everything else is fp32.
 #include "attention_tile.h"
@@ -203,6 +203,12 @@ __device__ __forceinline__ void store_row(char* to, const f32x16 (&x)[D / 32], f
         }
 }
 
+// Workgroups that see no more tiles than these make delta from P and dP instead, in 32 bits, which takes as long again as
+// two of the three products: out is rounded, and where a row sees few keys dP - delta may be much smaller than
+// either.  Two tokens, two heads: grads were 0.22 off; windows of two or three keys 0.03.  With three tiles, those of 128
+// rows in windows of up to 64 keys, rows beyond have enough keys for 4e-3.
+constexpr int32_t kOwnTiles = 3;
+
 // 128 rows to a workgroup, 32 to a wave, tiles of 64 keys as in the forward pass, and two workgroups on a compute unit.
 // 8192 tokens in five packed documents of 717 to 3588, 32/8 heads of 128 in bf16: 261 us, 0.89 PFLOP/s of its three
 // products; 8 x 1024 tokens, 12 heads of 64, 34 us.  The matrix cores are busy 51 and 35 % of the cycles: between a tile's
@@ -268,14 +274,55 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_q_ke
         for (int i = 0; i < 16; ++i) found = c / 8 * 4 + c % 4 == static_cast<uint32_t>(i) ? x[i] : found;
         const Halves h = halves(__float_as_uint(found), __float_as_uint(found));
         delta = __uint_as_float(c / 4 % 2 ? h.hi : h.lo);
-        if (there && lane < 32) {
-            const uint64_t at = static_cast<uint64_t>(head) * a.rows_all + flat;
-            a.less[at] = Range<T>::kP - lse2;
-            a.delta[at] = delta;
-        }
         have_row<D>(q);
         have_row<D>(g);
         asm volatile("" : "+v"(lse2));
+    }
+    Fragments<D> f;
+    f.init();
+    const float factor = a.scale * kLog2E;
+    if (tile < end && end - tile <= kOwnTiles) {
+        // delta from P and dP themselves, in a pass of its own
+        float products = 0.0f, sum = 0.0f;
+        uint32_t buffer = 0;
+        for (int32_t t = tile; t < end; ++t, buffer ^= 2 * kBytes) {
+            arrive<0>();
+            if (t + 1 < end) {
+                load_k.load(keys, (t + 1) * kTileRows, place + (buffer ^ 2 * kBytes));
+                load_v.load(values, (t + 1) * kTileRows, place + (buffer ^ 2 * kBytes) + kBytes);
+            }
+            const int32_t first_key = t * static_cast<int32_t>(kTileRows);
+            const lds_char *k = lds + buffer, *v = k + kBytes;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                f32x16 s = product<T, D>(k, q, f, b);
+                f32x16 d = product<T, D>(v, g, f, b);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = exp2_of(__builtin_fmaf(s[i], factor, -lse2));
+                    d[i] *= s[i];
+                }
+                hide(s, first_key + b * 32, mine);
+                hide(d, first_key + b * 32, mine);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    sum += s[i];
+                    products += d[i];
+                }
+            }
+        }
+        sum = both_sum(sum);
+        products = both_sum(products);
+        // where keys are missing that lse covers, and where there is one, delta stays that of out
+        if (mine.hi - mine.lo > 1 && __builtin_fabsf(sum - 1.0f) < 0x1p-12f) delta = products / sum;
+        arrive<0>();                                     // all waves have read the tiles
+        load_k.load(keys, tile * kTileRows, place);
+        load_v.load(values, tile * kTileRows, place + kBytes);
+    }
+    if (there && lane < 32) {
+        const uint64_t at = static_cast<uint64_t>(head) * a.rows_all + flat;
+        a.less[at] = Range<T>::kP - lse2;
+        a.delta[at] = delta;
     }
 
     f32x16 sums[D / 32];
@@ -283,9 +330,6 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_q_ke
     for (int d = 0; d < D / 32; ++d) sums[d] = zeros();
     Range<T> scaled;
     if (tile < end) {
-        Fragments<D> f;
-        f.init();
-        const float factor = a.scale * kLog2E;
         uint32_t buffer = 0;
         for (; tile < end; ++tile, buffer ^= 2 * kBytes) {
             arrive<0>();

@@ -121,7 +121,7 @@ class Case:
             _within(lse[at].transpose(0, 1), want_lse,
                     worst[..., 0] + (n + 8) * U32 + want_lse.nan_to_num(neginf=0.0).abs() * 4 * U32, "lse")
 
-    def check_grads(self, grads, out, lse):
+    def check_grads(self, grads, out, lse, exact=False):
         """The formula with the out and lse that were given."""
         u, tiny = U[self.dtype], TINY[self.dtype]
         gq, gk, gv = grads
@@ -137,8 +137,15 @@ class Case:
             e = off + (s.masked_fill(~sees, 0).abs() + row_lse.abs()[..., None] + 2) * 4 * U32
             o = out[at].double().transpose(0, 1)
             dp, delta = g @ v.transpose(1, 2), (g * o).sum(2, keepdim=True)
+            # delta from out, or from P and dP where a row sees few keys: what lies between is out's rounding
+            own = (p * dp).sum(2, keepdim=True)
+            if exact:
+                delta, gap = own, (4 * e.amax(2, keepdim=True) if m else 0) * (p * dp.abs()).sum(2, keepdim=True) + \
+                    2 * (m + 8) * U32 * (p * dp.abs()).sum(2, keepdim=True)
+            else:
+                gap = (own - delta).abs() * (1 + 2.0 ** -12) + 2.0 ** -12 * own.abs()
             ds = p * (dp - delta)
-            dp_off = self.dim * U32 * (g.abs() @ v.abs().transpose(1, 2) + (g.abs() * o.abs()).sum(2, keepdim=True))
+            dp_off = self.dim * U32 * (g.abs() @ v.abs().transpose(1, 2) + (g.abs() * o.abs()).sum(2, keepdim=True)) + gap
             ds_off = ds.abs() * (u + e + 4 * U32) + p * (dp_off + 2 * U32 * (dp.abs() + delta.abs()))
             if self.dtype == F16 and ds.numel():
                 # held within a wave times a power of two that brings the largest to 2^10 at least
@@ -204,6 +211,32 @@ def test_padded_queries_see_nothing(hip_device, dtype, heads, kv_heads, dim, cau
     """Beside whole tiles of keys that the sequence's own queries see."""
     Case(hip_device, dtype, queries, keys, heads, kv_heads, dim, packed=False, causal=causal, window=window, rows=rows,
          key_rows=max(keys) + 30).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 1, 64), (3, 3, 128), (8, 1, 96)])
+@pytest.mark.parametrize("lengths,how", [([2], {}), ([3, 2, 6, 1], {}), ([60, 5], dict(causal=False)), ([500, 131], dict(window=2)),
+                                         ([400], dict(window=5)), ([300], dict(window=33))])
+def test_gradients_of_rows_that_see_few_keys(hip_device, dtype, heads, kv_heads, dim, lengths, how):
+    """dP - delta is small there beside both, and out's rounding is not: delta is that of P and dP."""
+    case = Case(hip_device, dtype, lengths, lengths, heads, kv_heads, dim, **how)
+    out, lse = case.run()
+    case.check_grads(case.grad(out, lse), out, lse, exact=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("keys", [10, 64, 300])
+def test_gradients_of_a_share_of_the_keys(hip_device, dtype, keys):
+    """With out and lse over all keys, calls over pieces of them give these pieces' gradients, and add up."""
+    case = Case(hip_device, dtype, [40], [2 * keys], 4, 2, 64, packed=False, causal=False)
+    out, lse = case.run()
+    gq, gk, gv = case.grad(out, lse)
+    halves = [ops.attention_grad(case.g, case.q, case.k[:, s].contiguous(), case.v[:, s].contiguous(), out, lse, causal=False)
+              for s in (slice(0, keys), slice(keys, 2 * keys))]
+    for whole, at in ((gk, 1), (gv, 2), (gq, 0)):
+        got = halves[0][0].double() + halves[1][0].double() if at == 0 else torch.cat([h[at] for h in halves], 1).double()
+        # delta is out's in the halves and may be its own in the whole: each element within out's rounding
+        assert float((got - whole.double()).norm() / whole.double().norm()) < 8 * U[dtype]
 
 
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
