@@ -206,7 +206,7 @@ __device__ __forceinline__ void store_row(char* to, const f32x16 (&x)[D / 32], f
 // Workgroups that see no more tiles than these make delta from P and dP instead, in 32 bits, which takes as long again as
 // two of the three products: out is rounded, and where a row sees few keys dP - delta may be much smaller than
 // either.  Two tokens, two heads: grads were 0.22 off; windows of two or three keys 0.03.  With three tiles, those of 128
-// rows in windows of up to 64 keys, rows beyond have enough keys for 4e-3.
+// rows in windows of up to 64 keys, what is beyond is at most 2.9e-3 off.
 constexpr int32_t kOwnTiles = 3;
 
 // 128 rows to a workgroup, 32 to a wave, tiles of 64 keys as in the forward pass, and two workgroups on a compute unit.
