@@ -302,13 +302,13 @@ template <typename T, bool INTERLEAVED, bool WHOLE, int U> __global__ __launch_b
                 }
                 squares = head_sum(squares, a.lanes);
                 products = head_sum(products, a.lanes);
-                const float r = 1.0f / sqrtf(__builtin_fmaf(squares, a.per_dim, a.eps));
+                // a head that is not there is all zeros, and adds none, whatever eps is
+                const float r = head < heads ? 1.0f / sqrtf(__builtin_fmaf(squares, a.per_dim, a.eps)) : 0.0f;
                 const float mean = products * r * a.per_dim;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        // a head that is not there is all zeros, and adds none
                         const float unit = x[h][i] * r;
                         dw[h][i] = __builtin_fmaf(g[h][i], unit, dw[h][i]);
                         g[h][i] = r * __builtin_fmaf(-unit, mean, g[h][i] * w[h][i]);

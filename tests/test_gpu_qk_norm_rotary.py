@@ -299,3 +299,14 @@ def test_on_another_stream_and_nothing_to_do(hip_device):
     base = torch.ones(64, dtype=BF16, device=hip_device)
     none.grad(grad_q_weight=base, grad_k_weight=base.clone(), accumulate=True)
     assert bool((base == 1).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n,heads,kv_heads,dim,rotated", [(1, 32, 8, 128, 128), (200, 8, 2, 128, 128), (37, 5, 1, 80, 40),
+                                                          (300, 32, 8, 128, 64), (3, 3, 1, 7, 2)])
+def test_gradients_without_an_epsilon(hip_device, monkeypatch, dtype, n, heads, kv_heads, dim, rotated):
+    """The formula is finite as long as no head is all zeros: lanes without a head add nothing to the scales' gradients."""
+    monkeypatch.setitem(globals(), "EPS", 0.0)
+    case = Case(hip_device, dtype, n, heads, kv_heads, dim, rotated)
+    case.check(case.run())
+    case.check_grads(case.grad())
