@@ -13,8 +13,9 @@
 // Scores are S^T = K Q^T, so a lane holds scores of one row (see attention_tile.h); their exponentials, rounded
 // to the 16 bits that the matrix cores take, are the second operand of out^T += V^T P^T.  That rounding is the one
 // before the result's own: half a step for each probability, in no direction, so a row's result is off by less than
-// half a step of its largest terms (bf16: 2.2e-3 of all results where the rounding of exact ones is 1.6e-3).  The
-// sum l is that of the unrounded values, in fp32 like the maxima and the sums of products.
+// half a step of its largest terms (bf16: 2.2e-3 of all results where the rounding of exact ones is 1.6e-3).  bf16 has
+// fp32's range.  fp16 has not: see Held.  The sum l is that of the unrounded values, in fp32 like the maxima and the sums
+// of products.
 #include "attention_tile.h"
 
 #include <algorithm>
@@ -37,11 +38,35 @@ struct ForwardArgs {
     int aligned;                    // rows of the result may be written 16 bytes at a time
 };
 
+// How P is held, relative to a row's reference st.top: times 2^kUp.  Exponentials need the maximum of no tile but a row's
+// first: those of later ones add up to less than kMost nearly always, and where they do not, the scores are made again and
+// the references raised.  Looking for the maximum of every tile instead is 21 more vector instructions of about 165, which
+// bind heads of 64.
+template <typename T> struct Held {
+    static constexpr bool kLowers = false;
+    static constexpr float kUp = 0.0f, kDown = 1.0f, kMost = 4096.0f;
+};
+// fp16 holds 2^-24 to 65504, and where one key is far above the others, as a text's first token often is, the others are
+// below that beside it: 65536 of them, 17.5 lower, were 3 % off together, where the first one's value is small.  So P is held
+// times 2^9, and where a tile's sum is less than kLeast, the reference is lowered to the tile's maximum, and `sum` and `out`,
+// in fp32, raised by as much; so are the wave's other rows whose sum is less than kLow, which would soon be next.  A
+// probability is then off by half a step, or by 2^-20 of its tile's sum.  Lowering ends with sums of kLowered and
+// more, beside which what is lower still is nothing in fp16 results; it is by 2^kStep at the most, so that sums of products
+// stay below 2^(kStep + 50) * 65504.
+// 8192 tokens, causal, 32 and 8 heads of 128: 562 us, and 553 with P held times 1 as bf16's; 8 x 1024, 12 heads of 64: 28.9
+// and 27.4; with a first key 17.5 above the others 563 and 29.5.
+template <> struct Held<_Float16> {
+    static constexpr bool kLowers = true;
+    static constexpr float kUp = 9.0f, kDown = 0x1p-9f, kMost = 65024.0f;    // 127 * 2^9; each term is below 65504
+    static constexpr float kLeast = 0x1p-5f, kLow = 0x1p5f;                  // 2^-14 and 2^-4 times 2^9
+    static constexpr float kLowered = 0x1p50f, kStep = 40.0f;
+};
+
 // The running state of 32 rows in a wave: of row l % 32 a lane has the elements 32 d + 8 (i / 4) + 4 (l / 32) + i % 4.
 template <int D> struct State {
-    f32x16 out[D / 32];
+    f32x16 out[D / 32];             // times 2^Held::kUp
     float top;                      // the score that `sum` and `out` are relative to: -inf until the row's first key
-    float sum;                      // over this half's keys
+    float sum;                      // over this half's keys, or, where Held::kLowers, all; times 2^Held::kUp
     __device__ __forceinline__ void init(const Seen& row)
     {
 #pragma unroll
@@ -79,12 +104,12 @@ __device__ __forceinline__ void mask(f32x16 (&s)[KEYS / 32], int32_t first_key, 
         }
 }
 
-// P of scores relative to st.top, in their place; returns the sum over this half's keys.
-template <int D, int KEYS>
+// P of scores relative to st.top, as it is held, in their place; returns its sum over this half's keys, or all.
+template <typename T, int D, int KEYS>
 __device__ __forceinline__ float exponentials(const State<D>& st, f32x16 (&s)[KEYS / 32], float factor)
 {
     // rows that have seen nothing yet: 0, and exp2(-inf) below
-    const float from = st.top == -INFINITY ? 0.0f : -st.top * factor;
+    const float from = st.top == -INFINITY ? 0.0f : __builtin_fmaf(-st.top, factor, Held<T>::kUp);
     float sum = 0.0f;
 #pragma unroll
     for (int b = 0; b < KEYS / 32; ++b) {
@@ -93,32 +118,39 @@ __device__ __forceinline__ float exponentials(const State<D>& st, f32x16 (&s)[KE
 #pragma unroll
         for (int i = 0; i < 16; i += 4) sum += (s[b][i] + s[b][i + 1]) + (s[b][i + 2] + s[b][i + 3]);
     }
-    return sum;
+    return Held<T>::kLowers ? both_sum(sum) : sum;
 }
 
-// Raises the rows' maxima to those of these scores, and brings the sums to them.
-template <int D, int KEYS>
-__device__ __forceinline__ void raise(State<D>& st, const f32x16 (&s)[KEYS / 32], float factor)
+// The sum over all keys, relative to st.top.
+template <typename T, int D> __device__ __forceinline__ float sum_of(const State<D>& st)
+{
+    return Held<T>::kLowers ? st.sum * Held<T>::kDown : both_sum(st.sum);
+}
+
+// Moves the rows' references to the maxima of these scores, up in any case, down where `lower` says so, and brings the
+// sums to them.
+template <typename T, int D, int KEYS>
+__device__ __forceinline__ void refer(State<D>& st, const f32x16 (&s)[KEYS / 32], float factor, bool lower)
 {
     float top = s[0][0];
 #pragma unroll
     for (int b = 0; b < KEYS / 32; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-    top = fmaxf(both_max(top), st.top);
-    const float shrink = top == st.top ? 1.0f : exp2_of((st.top - top) * factor);
+    top = both_max(top);
+    if constexpr (Held<T>::kLowers) {
+        top = fmaxf(top, lower ? st.top - Held<T>::kStep / factor : st.top);
+    } else {
+        top = fmaxf(top, st.top);
+    }
+    const float times = top == st.top ? 1.0f : exp2_of((st.top - top) * factor);
     st.top = top;
-    st.sum *= shrink;
+    st.sum *= times;
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d) st.out[d] *= shrink;
+    for (int d = 0; d < D / 32; ++d) st.out[d] *= times;
 }
 
-// Takes KEYS keys (32 or 64) of a tile in.  Exponentials need the maximum of no tile but a row's first: those of
-// later ones stay below kMost nearly always, and where a lane's sum of them is more, the scores are made again and
-// the maxima raised.  Looking for the maximum of every tile instead is 21 more vector instructions of about 165, which
-// bind heads of 64.
-constexpr float kMost = 4096.0f;                         // which float16 holds, and each of its terms
-
+// Takes KEYS keys (32 or 64) of a tile in.
 template <typename T, int D, int KEYS>
 __device__ __forceinline__ void take(State<D>& st, const s16x8 (&q)[D / 16], const lds_char* k, const lds_char* v,
                                      const Fragments<D>& f, float factor, bool partly, int32_t first_key, const Seen& row)
@@ -126,13 +158,26 @@ __device__ __forceinline__ void take(State<D>& st, const s16x8 (&q)[D / 16], con
     f32x16 s[KEYS / 32];
     scores<T, D, KEYS>(s, q, k, f);
     if (partly) mask<KEYS>(s, first_key, row);
-    if (__any(st.top == -INFINITY)) raise<D, KEYS>(st, s, factor);
-    float sum = exponentials<D, KEYS>(st, s, factor);
-    if (__any(sum > kMost)) {
+    if (__any(st.top == -INFINITY)) refer<T, D, KEYS>(st, s, factor, false);
+    float sum = exponentials<T, D, KEYS>(st, s, factor);
+    bool again, lower = false;
+    if constexpr (Held<T>::kLowers) {
+        // in one comparison what is nearly never so, NaN and 0 (nothing seen) among it
+        constexpr uint32_t kFrom = __builtin_bit_cast(uint32_t, Held<T>::kLeast), kTo = __builtin_bit_cast(uint32_t, Held<T>::kMost);
+        again = __any(__float_as_uint(sum) - kFrom > kTo - kFrom);
+        if (again) {
+            const bool lowers = sum > 0.0f && st.sum < Held<T>::kLowered;
+            lower = lowers && sum < Held<T>::kLow;
+            again = __any(sum > Held<T>::kMost || (lowers && sum < Held<T>::kLeast));
+        }
+    } else {
+        again = __any(sum > Held<T>::kMost);
+    }
+    if (again) {
         scores<T, D, KEYS>(s, q, k, f);
         if (partly) mask<KEYS>(s, first_key, row);
-        raise<D, KEYS>(st, s, factor);
-        sum = exponentials<D, KEYS>(st, s, factor);
+        refer<T, D, KEYS>(st, s, factor, lower);
+        sum = exponentials<T, D, KEYS>(st, s, factor);
     }
     st.sum += sum;
 #pragma unroll
@@ -179,9 +224,9 @@ __device__ __forceinline__ void finish(const ForwardArgs& a, const Piece& p, uin
 {
     const uint32_t half = threadIdx.x % kWave / 32;
     const uint32_t token = row / a.seq.group, head = kv_head * a.seq.group + row % a.seq.group;
-    const float sum = both_sum(st.sum);
+    const float sum = sum_of<T>(st);
     // a row that sees nothing: zeros, and -inf
-    const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float scale = sum == 0.0f ? 0.0f : Held<T>::kDown / sum;
     const bool there = token < p.stored;
     const uint64_t flat = (static_cast<uint64_t>(p.batch) * a.seq.rows + p.first + token) * a.heads + head;
     if (a.parts > 1) {
@@ -239,7 +284,7 @@ __device__ __forceinline__ void load_row(s16x8 (&q)[D / 16], const char* row, bo
 // for each exponential the vector instructions bind, 15 to a product, and the launch is as long as its longest piece.  Two variants took fewer cycles and no less time, as the clock sank with them (1.95 GHz
 // in a first launch, 1.6 to 1.7 under load): scores of the next tile between the exponentials of this
 // one (541), and eight waves that take turns at multiplying and at exponentials (530).
-template <typename T, int D> __global__ __launch_bounds__(256, 2) void attention_kernel(ForwardArgs a)
+template <typename T, int D> __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_kernel(ForwardArgs a)
 {
     constexpr uint32_t kBytes = Tile<D>::kBytes;
     __shared__ __attribute__((aligned(1024))) char shared[4 * kBytes];
@@ -401,7 +446,7 @@ template <typename T, int D> __global__ __launch_bounds__(kFewWaves * 64, 1) voi
         arrived<0>();
     }
     // the waves' states, each shrunk to the largest of their maxima, added in the order of the waves
-    st.sum = both_sum(st.sum);
+    st.sum = sum_of<T>(st);
     __syncthreads();                                     // no tile is read any more
     constexpr uint32_t kRow = D + 4;                     // keeps 32 rows' accesses in different banks
     static_assert(kFewWaves * 32 * (kRow + 2) * 4 <= kFewWaves * kOwn, "the states fit the tiles' place");
@@ -436,7 +481,7 @@ template <typename T, int D> __global__ __launch_bounds__(kFewWaves * 64, 1) voi
     // from lanes of rows that may not be there: before any lane leaves
     const float row_sum = __shfl(sum, static_cast<int>(out_row % 32)), row_top = __shfl(top, static_cast<int>(out_row % 32));
     if (out_token >= p.stored) return;
-    const float scale = row_sum == 0.0f ? 0.0f : 1.0f / row_sum;
+    const float scale = row_sum == 0.0f ? 0.0f : Held<T>::kDown / row_sum;
     const uint64_t flat = (static_cast<uint64_t>(p.batch) * a.seq.rows + p.first + out_token) * a.heads + head;
     char* to = const_cast<char*>(a.out.at(p.batch, p.first + out_token, head));
     float* part_to = a.partial + (static_cast<uint64_t>(part) * a.rows_all + flat) * D;
