@@ -18,9 +18,9 @@
 // same order: a row that sees one key has O = V and exactly no dS.
 //
 // P and dS are rounded to the operands' 16 bits before the last three products, as the matrix cores take them, and
-// delta, but for short sequences and windows, is that of the O that was given, itself rounded: bf16 gradients of q and k are 2.7e-3 off where rounding the exact
-// ones is 1.7e-3 off, fp16 3.5e-4 and 2.1e-4.  A delta from the sums of P dP would not have O's rounding, but would be
-// wrong with an lse over more keys than the call has.  Everything else is fp32.
+// delta, but for short sequences and windows, is that of the O that was given, itself rounded: bf16 gradients of q and k
+// are 2.7e-3 off where rounding the exact ones is 1.7e-3 off, fp16 3.5e-4 and 2.1e-4.  A delta from the sums of P dP
+// would not have O's rounding, but would be wrong with an lse over more keys than the call has.  Everything else is fp32.
 #include "attention_tile.h"
 
 #include <algorithm>
@@ -203,11 +203,11 @@ __device__ __forceinline__ void store_row(char* to, const f32x16 (&x)[D / 32], f
         }
 }
 
-// Workgroups that see no more tiles than these make delta from P and dP instead, in 32 bits, which takes as long again as
+// Workgroups whose rows see no more keys than these make delta from P and dP instead, in 32 bits, which takes as long again as
 // two of the three products: out is rounded, and where a row sees few keys dP - delta may be much smaller than
-// either.  Two tokens, two heads: grads were 0.22 off; windows of two or three keys 0.03.  With three tiles, those of 128
-// rows in windows of up to 64 keys, what is beyond is at most 2.9e-3 off.
-constexpr int32_t kOwnTiles = 3;
+// either.  Two tokens, two heads: grads were 0.22 off; windows of two or three keys 0.03.  128 rows in windows of 64
+// keys see 191, in three tiles or, where the first begins inside one, four.  What is beyond is at most 2.8e-3 off.
+constexpr int32_t kOwnKeys = 192;
 
 // 128 rows to a workgroup, 32 to a wave, tiles of 64 keys as in the forward pass, and two workgroups on a compute unit.
 // 8192 tokens in five packed documents of 717 to 3588, 32/8 heads of 128 in bf16: 261 us, 0.89 PFLOP/s of its three
@@ -281,7 +281,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_q_ke
     Fragments<D> f;
     f.init();
     const float factor = a.scale * kLog2E;
-    if (tile < end && end - tile <= kOwnTiles) {
+    if (tile < end && all.hi - all.lo <= kOwnKeys) {
         // delta from P and dP themselves, in a pass of its own
         float products = 0.0f, sum = 0.0f;
         uint32_t buffer = 0;

@@ -513,3 +513,16 @@ def test_many_sequences(hip_device):
     """More than the 64 that are looked through at a time."""
     lengths = [(7 * b) % 23 for b in range(200)]
     Case(hip_device, BF16, lengths, lengths, 2, 1, 64).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 128), (3, 3, 64), (4, 2, 80)])
+@pytest.mark.parametrize("window", [2, 3, 8, 32, 64])
+@pytest.mark.parametrize("more", [1, 5, 30, 62])
+@pytest.mark.parametrize("packed", [True, False])
+def test_gradients_of_rows_that_see_few_keys_wherever_these_begin(hip_device, dtype, heads, kv_heads, dim, window, more, packed):
+    """With more keys than queries 128 rows' windows begin anywhere in a tile of keys, and reach into four of them."""
+    queries = [300, 140]
+    case = Case(hip_device, dtype, queries, [n + more for n in queries], heads, kv_heads, dim, packed=packed, window=window)
+    out, lse = case.run()
+    case.check_grads(case.grad(out, lse), out, lse, exact=True)
