@@ -194,8 +194,9 @@ int la_attention_grad(const la_attention_t* call, void* workspace, uint64_t work
  * pairs (a, b) -> (a cos - b sin, b cos + a sin), pair j by cos and sin [position][j] of fp32 tables with
  * `positions` rows of rotated / 2; in fp32, rounded once.  Pairs are elements (j, j + rotated / 2), or with
  * interleaved != 0 (2 j, 2 j + 1).  Row i has position at[i] (int32 or int64), or i where `at` is null; one outside
- * the tables makes the rotated elements of its row NaN.  Results may be written over their inputs, not over
- * one another.
+ * the tables makes the rotated elements of its row NaN.  q_out may be q and k_out may be k, element for element; otherwise
+ * results share no memory with what the call reads or with one another (LA_EINVAL), though they may lie between one
+ * another as parts of one projection do.
  */
 typedef struct {
     int dtype;
@@ -222,9 +223,10 @@ int la_qk_norm_rotary(const la_rotary_t* call, la_stream_t stream);
 
 /*
  * The gradients of la_qk_norm_rotary from those of its results, grad_q and grad_k: towards x, into q_out and
- * k_out (which may be grad_q and grad_k), and towards the weights that there are, into grad_q_weight and
- * grad_k_weight (dtype or LA_F32), added to with accumulate != 0.  q and k are its inputs; without weights they are
- * not read and may be null.  Sums are fp32 in a fixed order.
+ * k_out (which may be grad_q and grad_k, or q and k, element for element), and towards the weights that there are, into
+ * grad_q_weight and grad_k_weight (dtype or LA_F32), added to with accumulate != 0.  q and k are its inputs; without
+ * weights they are not read and may be null.  The other results share no memory with one another, nor q_out and k_out
+ * with what else the call reads (LA_EINVAL).  Sums are fp32 in a fixed order.
  * workspace: la_qk_norm_rotary_grad_workspace(call) bytes, 16-byte aligned.
  */
 uint64_t la_qk_norm_rotary_grad_workspace(const la_rotary_t* call);

@@ -10,6 +10,7 @@
 // two 16-byte accesses each in 16-bit types, whose elements are pairs of one another, so a
 // head's sum needs three exchanges and the rotation none.  A wave stays on one token,
 // whose row of the tables it reads once for all heads it takes.
+#include "memory_overlap.h"
 #include "ops_common.h"
 
 #include <algorithm>
@@ -434,7 +435,41 @@ int check_reach(const la_rotary_t& c)
     return LA_OK;
 }
 
-bool same_results(const la_rotary_t& c) { return c.n && c.heads && c.kv_heads && c.q_out.data == c.k_out.data; }
+la_memory::Place place_of(const la_rotary_t& c, const la_heads_t& h, uint64_t heads)
+{
+    const uint64_t size = static_cast<uint64_t>(dtype_bytes(c.dtype));
+    return {reinterpret_cast<uintptr_t>(h.data), c.dim * size, {c.n, heads, 1}, {h.row_stride * size, h.head_stride * size, 0}};
+}
+
+// Heads are read and written by waves of their own, in no order: a result lies exactly where heads of its own kind are read,
+// each read whole before it is written, or where nothing is read; and no two results share memory.  The scales'
+// gradients are written after everything is read.
+bool results_apart(const la_rotary_t& c, bool grad)
+{
+    using la_memory::flat;
+    using la_memory::Place;
+    using la_memory::shared;
+    const uint64_t size = static_cast<uint64_t>(dtype_bytes(c.dtype)), table = c.positions * (c.rotated / 2) * sizeof(float);
+    const Place outs[] = {place_of(c, c.q_out, c.heads), place_of(c, c.k_out, c.kv_heads)};
+    const bool x_read[] = {!grad || c.q_weight, !grad || c.k_weight};
+    const Place none{}, heads[] = {x_read[0] ? place_of(c, c.q, c.heads) : none, x_read[1] ? place_of(c, c.k, c.kv_heads) : none,
+                                   grad ? place_of(c, c.grad_q, c.heads) : none, grad ? place_of(c, c.grad_k, c.kv_heads) : none};
+    const Place others[] = {flat(c.q_weight, c.dim * size), flat(c.k_weight, c.dim * size), flat(c.cos, table), flat(c.sin, table),
+                            flat(c.at, c.at ? c.n * static_cast<uint64_t>(dtype_bytes(c.at_dtype)) : 0)};
+    for (int out = 0; out < 2; ++out) {
+        for (int k = 0; k < 4; ++k)
+            if (shared(outs[out], heads[k]) && !(k % 2 == out && same(outs[out], heads[k]))) return false;
+        for (const Place& other : others)
+            if (shared(outs[out], other)) return false;
+    }
+    if (shared(outs[0], outs[1])) return false;
+    if (!grad) return true;
+    const uint64_t bytes = c.dim * static_cast<uint64_t>(dtype_bytes(c.weight_grad_dtype));
+    const Place scales[] = {c.q_weight ? flat(c.grad_q_weight, bytes) : none, c.k_weight ? flat(c.grad_k_weight, bytes) : none};
+    for (const Place& of : scales)
+        if (shared(of, outs[0]) || shared(of, outs[1])) return false;
+    return !shared(scales[0], scales[1]);
+}
 
 RotaryArgs args_of(const la_rotary_t& c)
 {
@@ -537,7 +572,7 @@ int la_qk_norm_rotary(const la_rotary_t* call, la_stream_t stream)
     if (c.n == 0 || c.heads + c.kv_heads == 0) return LA_OK;
     if ((c.heads && bad(c.q, c.dtype)) || (c.kv_heads && bad(c.k, c.dtype))) return LA_EINVAL;
     rc = check_reach(c);
-    if (rc == LA_OK && same_results(c)) rc = LA_EINVAL;
+    if (rc == LA_OK && !results_apart(c, false)) rc = LA_EINVAL;
     if (rc != LA_OK) return rc;
     RotaryArgs a = args_of(c);
     const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -571,8 +606,7 @@ int la_qk_norm_rotary_grad(const la_rotary_t* call, void* workspace, uint64_t wo
     if (rc == LA_OK && (!reachable(c.grad_q_weight) || !reachable(c.grad_k_weight) || (normed && !reachable(workspace)) ||
                         (any && (!reachable(c.grad_q.data) || !reachable(c.grad_k.data)))))
         rc = LA_EFAULT;
-    // each result is written by workgroups of its own, in no order
-    if (rc == LA_OK && (same_results(c) || (c.q_weight && c.k_weight && c.grad_q_weight == c.grad_k_weight))) rc = LA_EINVAL;
+    if (rc == LA_OK && !results_apart(c, true)) rc = LA_EINVAL;
     if (rc != LA_OK) return rc;
     RotaryArgs a = args_of(c);
     a.grad_q = rows_of(c.grad_q, c.dtype);

@@ -422,8 +422,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: tor
     [positions, pairs]; the first ``2 * pairs`` elements of a head turn, (a, b) -> (a cos - b sin, b cos + a sin), pair
     j of elements (j, j + pairs), or (2 j, 2 j + 1) if ``interleaved``.  ``positions``: int32 or int64
     [n], row i of the tables for row i by default; one outside the tables makes the rotated elements NaN.
-    ``out``: the two tensors to write instead of new ones: q and k themselves, or memory that the call does not
-    read, rows of a cache for instance.  All in fp32, rounded once."""
+    ``out``: the two tensors to write instead of new ones: q and k themselves, each in its own place, or memory that the call
+    does not read, rows of a cache for instance; not one in the other's.  All in fp32, rounded once."""
     if out is None and stream is None and q.is_cuda:
         done = _ops_lib.calls().qk_norm_rotary(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved, *_here())
         if done is not None:
@@ -445,8 +445,8 @@ def qk_norm_rotary_grad(grad_q: torch.Tensor, grad_k: torch.Tensor, q: Optional[
     """The gradients of ``qk_norm_rotary`` towards its q, k and weights, from those of its results.
 
     q and k are its inputs (None will do for heads that are not normed).  ``out``: where the
-    gradients of q and k go, new tensors by default; ``grad_q`` and ``grad_k`` themselves may be written
-    over.  ``grad_q_weight``, ``grad_k_weight``: the tensors [dim] to write (of the weights' type or
+    gradients of q and k go, new tensors by default; ``grad_q`` and ``grad_k`` (or q and k) themselves, each in its own
+    place, may be written over, nothing else that the call reads.  ``grad_q_weight``, ``grad_k_weight``: the tensors [dim] to write (of the weights' type or
     float32, both of one type, two tensors; new by default), added to with ``accumulate``.  Returns ``(grad_q, grad_k,
     grad_q_weight, grad_k_weight)``, None for a weight that there is not.  Sums are fp32 in a fixed order."""
     if grad_q_weight is None and grad_k_weight is None and not accumulate and out is None and stream is None \

@@ -308,3 +308,73 @@ def test_out_of_memory_is_torchs_error(hip_device, t, stream):
             torch.cuda.set_per_process_memory_fraction(1.0, hip_device)
         call()
         torch.cuda.synchronize()
+
+
+def _normal(t, *shape, dtype=BF16):
+    return t(*shape, dtype=dtype).normal_(generator=torch.Generator(device="cuda").manual_seed(sum(shape)))
+
+
+def _moved(x, by):
+    """The same view `by` elements on in its memory."""
+    return x.as_strided(x.shape, x.stride(), x.storage_offset() + by)
+
+
+def test_rotated_heads_go_to_their_own_place_or_where_nothing_is_read(hip_device, t):
+    """Heads are read and written in no order, so a result that lies over others that are read, or over the other result, is
+    refused; parts of one projection's rows are fine."""
+    n = 130
+    wide = _normal(t, n + 2, 16, 64)
+    q, k, free, more = (wide[1:-1, 4 * i:4 * i + 4] for i in range(4))
+    table, at, scales = _normal(t, n, 32, dtype=torch.float32), t(n * 16, dtype=torch.int64), _normal(t, n * 64)
+    at[:n] = torch.arange(n, device=hip_device).flip(0)
+    how = dict(q_weight=scales[64:128], k_weight=scales[128:192], positions=at[:n])
+    want = ops.qk_norm_rotary(q, k, table, table, **how)
+    kept = wide.clone()
+    for out in ((k, q), (k, more), (free, q), (_moved(q, 16 * 64), more), (_moved(q, -64), more), (_moved(q, 1), more),
+                (free, _moved(k, 64)), (free, _moved(k, -63)), (q, _moved(k, -64)), (free, free), (free, _moved(free, 64)),
+                (_moved(free, 16 * 64), free), (free, _moved(free, 3 * 64 + 63))):
+        with pytest.raises(RuntimeError, match="la_qk_norm_rotary"):
+            ops.qk_norm_rotary(q, k, table, table, out=out, **how)
+        assert torch.equal(wide, kept)
+    for over in (table, at, scales):                         # heads over the other inputs
+        with pytest.raises(RuntimeError, match="la_qk_norm_rotary"):
+            ops.qk_norm_rotary(q, k[:, :1], table, table, out=(free, over.view(BF16).view(n, 1, 64)), **how)
+    for out in ((free, more), (q, more), (more, k), (q, k)):
+        wide.copy_(kept)
+        ops.qk_norm_rotary(q, k, table, table, out=out, **how)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        others = torch.ones_like(wide, dtype=torch.bool)
+        for x in out:
+            others.as_strided(x.shape, x.stride(), x.storage_offset()).zero_()
+        assert torch.equal(wide[others], kept[others])
+
+
+def test_gradients_of_rotated_heads_go_to_their_own_place_or_where_nothing_is_read(hip_device, t):
+    n = 130
+    wide = _normal(t, n + 2, 24, 64)
+    q, k, gq, gk, free, more = (wide[1:-1, 4 * i:4 * i + 4] for i in range(6))
+    table, scales = _normal(t, n, 32, dtype=torch.float32), _normal(t, 4, 64)
+    normed = dict(q_weight=scales[0], k_weight=scales[1])
+    kept = wide.clone()
+
+    def refused(out, how=normed, **more):
+        with pytest.raises(RuntimeError, match="la_qk_norm_rotary_grad"):
+            ops.qk_norm_rotary_grad(gq, gk, q, k, table, table, out=out, **how, **more)
+        assert torch.equal(wide, kept)
+
+    for out in ((gk, gq), (k, q), (gk, more), (free, gq), (free, q), (k, more), (_moved(gq, 64), more), (_moved(q, -64), more),
+                (free, _moved(gk, 24 * 64)), (free, _moved(k, 1)), (free, _moved(free, 64)), (free, free)):
+        refused(out)
+    refused((free, more), grad_q_weight=free[0, 0], grad_k_weight=scales[2])
+    refused((free, more), grad_q_weight=scales[2], grad_k_weight=more[n - 1, 3])
+    refused((free, more), grad_q_weight=scales.view(-1)[128:192], grad_k_weight=scales.view(-1)[160:224])
+    refused((gk, more), how={})
+    refused((free, _moved(free, 64)), how={})
+    for how, outs in ((normed, ((free, more), (gq, gk), (q, k), (gq, k), (free, gk))),
+                      ({}, ((free, more), (gq, gk), (_moved(q, -64), _moved(k, -64)), (k, q)))):      # q and k are not read
+        want = ops.qk_norm_rotary_grad(gq, gk, q, k, table, table, **how)
+        for out in outs:
+            got = ops.qk_norm_rotary_grad(gq, gk, q, k, table, table, out=out, **how)
+            for a, b in zip(got, want):
+                assert a is b is None or torch.equal(a, b)
+            wide.copy_(kept)
