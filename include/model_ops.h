@@ -151,6 +151,7 @@ typedef struct {
  * key; window (with causal; 0: none): only the last `window` of these.
  * A row that sees no key has out 0 and lse -inf; so has a row of no sequence.  What lies
  * beyond a sequence's keys is never looked at, whatever it holds.
+ * out and lse share no memory with one another or with what the call reads (LA_EINVAL), but may lie between it.
  * dtype (of all heads): LA_BF16 or LA_F16; dim at most 128; scale above 0.
  * workspace: la_attention_workspace(call) bytes, 256-byte aligned: partial results where
  * the keys of few rows are shared out among workgroups, and copies of what does not lie
@@ -181,8 +182,8 @@ int la_attention(const la_attention_t* call, void* workspace, uint64_t workspace
  * and lse: P = exp(scale q k - lse), dP = grad_out v, dS = P (dP - sum(grad_out out)),
  *   grad_q = scale dS k,  grad_k = scale dS^T q,  grad_v = P^T grad_out,
  * those of key heads summed over the query heads that share them.  Rows beyond a sequence's length or in no
- * sequence have gradient 0, or with keep_rest != 0 stay as they were.  Nothing is added atomically.  The gradients
- * may lie between one another, as parts of one projection's do, but not where the call reads.
+ * sequence have gradient 0, or with keep_rest != 0 stay as they were.  Nothing is added atomically.  The gradients share
+ * no memory with one another or with what the call reads (LA_EINVAL), but may lie between, as parts of one projection do.
  * workspace: la_attention_grad_workspace(call) bytes, 256-byte aligned.
  */
 uint64_t la_attention_grad_workspace(const la_attention_t* call);

@@ -647,9 +647,8 @@ int la_attention(const la_attention_t* call, void* workspace, uint64_t workspace
     if (!reachable(c.q.data) || !reachable(c.k.data) || !reachable(c.v.data) || !reachable(c.out.data) ||
         !reachable(c.lse.data) || !indices_reachable(c) || (la_attention_workspace(call) && !reachable(workspace)))
         return LA_EFAULT;
-    const Extent written = extent(c, c.out, true);
-    if (!apart(written, extent(c, c.q, true)) || !apart(written, extent(c, c.k, false)) ||
-        !apart(written, extent(c, c.v, false)))
+    if (!results_apart(c, {place_of(c, c.out, true), place_of_lse(c)},
+                       {place_of(c, c.q, true), place_of(c, c.k, false), place_of(c, c.v, false)}))
         return LA_EINVAL;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);

@@ -846,12 +846,9 @@ int la_attention_grad(const la_attention_t* call, void* workspace, uint64_t work
                           c.grad_v.data, c.lse.data})
         if (!reachable(p)) return LA_EFAULT;
     if (!indices_reachable(c) || !reachable(workspace)) return LA_EFAULT;
-    // one kernel writes what the next would read; gradients may lie between one another, as a projection's do
-    for (const Extent& written : {extent(c, c.grad_q, true), extent(c, c.grad_k, false), extent(c, c.grad_v, false)})
-        for (const Extent& read : {extent(c, c.q, true), extent(c, c.k, false), extent(c, c.v, false),
-                                   extent(c, c.out, true), extent(c, c.grad_out, true)})
-            if (!apart(written, read)) return LA_EINVAL;
-    if (keys && (c.grad_k.data == c.grad_v.data || (rows && (c.grad_q.data == c.grad_k.data || c.grad_q.data == c.grad_v.data))))
+    if (!results_apart(c, {place_of(c, c.grad_q, true), place_of(c, c.grad_k, false), place_of(c, c.grad_v, false)},
+                       {place_of(c, c.q, true), place_of(c, c.k, false), place_of(c, c.v, false), place_of(c, c.out, true),
+                        place_of(c, c.grad_out, true), place_of_lse(c)}))
         return LA_EINVAL;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);

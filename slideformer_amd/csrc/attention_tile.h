@@ -18,6 +18,7 @@
 #ifndef SLIDEFORMER_AMD_ATTENTION_TILE_H
 #define SLIDEFORMER_AMD_ATTENTION_TILE_H
 
+#include "memory_overlap.h"
 #include "ops_common.h"
 
 namespace att {
@@ -443,18 +444,38 @@ inline uint64_t packed_bytes(const la_attention_t& c, const la_heads_t& h, bool 
     return ceil_div(rows * (queries ? c.heads : c.kv_heads) * ceil_div(c.dim, 8ull) * 16, 256ull) * 256;
 }
 
-// The memory from the first to the last element of `h`.
-struct Extent {
-    uintptr_t from, to;
-};
-inline Extent extent(const la_attention_t& c, const la_heads_t& h, bool queries)
+inline la_memory::Place place_of(const la_attention_t& c, const la_heads_t& h, bool queries)
 {
-    const uint64_t rows = queries ? c.rows : c.key_rows, heads = queries ? c.heads : c.kv_heads;
-    const uintptr_t from = reinterpret_cast<uintptr_t>(h.data);
-    if (sets(c) * rows == 0) return {from, from};
-    return {from, from + 2 * ((sets(c) - 1) * h.batch_stride + (rows - 1) * h.row_stride + (heads - 1) * h.head_stride + c.dim)};
+    return {reinterpret_cast<uintptr_t>(h.data), 2 * c.dim,
+            {sets(c), queries ? c.rows : c.key_rows, queries ? c.heads : c.kv_heads},
+            {2 * h.batch_stride, 2 * h.row_stride, 2 * h.head_stride}};
 }
-inline bool apart(const Extent& a, const Extent& b) { return a.from == a.to || b.from == b.to || a.to <= b.from || b.to <= a.from; }
+
+// lse: an fp32 to a head.
+inline la_memory::Place place_of_lse(const la_attention_t& c)
+{
+    return {reinterpret_cast<uintptr_t>(c.lse.data), 4, {sets(c), c.rows, c.heads},
+            {4 * c.lse.batch_stride, 4 * c.lse.row_stride, 4 * c.lse.head_stride}};
+}
+
+// Whether results share no memory with one another, with `read`, or with the indices: kernels read and write in no order,
+// and one what the next reads.  They may lie between one another, as parts of a projection's gradient do.
+template <int WRITTEN, int READ>
+inline bool results_apart(const la_attention_t& c, const la_memory::Place (&written)[WRITTEN], const la_memory::Place (&read)[READ])
+{
+    const uint64_t size = c.index_dtype == LA_I64 ? 8 : 4;
+    const la_memory::Place indices[] = {la_memory::flat(c.starts, (c.batch + 1) * size), la_memory::flat(c.key_starts, (c.batch + 1) * size),
+                                        la_memory::flat(c.lengths, c.batch * size), la_memory::flat(c.key_lengths, c.batch * size)};
+    for (int k = 0; k < WRITTEN; ++k) {
+        for (const la_memory::Place& p : read)
+            if (shared(written[k], p)) return false;
+        for (const la_memory::Place& p : indices)
+            if (shared(written[k], p)) return false;
+        for (int m = 0; m < k; ++m)
+            if (shared(written[k], written[m])) return false;
+    }
+    return true;
+}
 
 inline Heads plain(const la_heads_t& h, uint64_t size = 2)
 {

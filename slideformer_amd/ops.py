@@ -597,9 +597,9 @@ def attention_grad(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     """The gradients of ``attention`` towards q, k and v, from that of its out.
 
     ``out`` and ``lse`` are its results (lse in any order of memory), the other arguments those that it had.
-    Probabilities are computed again.  ``grads``: the three tensors to write, like q, k and v (parts of one projection's gradient,
-    for instance), not in memory that the call reads; rows of no sequence stay as they were in them.  Without it they
-    are new, and zero there.
+    Probabilities are computed again.  ``grads``: the three tensors to write, like q, k and v (parts of one projection's
+    gradient, for instance), not in memory that the call reads, nor one in another's; rows of no sequence stay as they
+    were in them.  Without it they are new, and zero there.
     The gradients of a key head are sums over the query heads that share it.  Sums are fp32 in a fixed
     order: equal calls give equal bits."""
     if grads is None and stream is None and q.is_cuda and (window is None or window > 0):

@@ -2,10 +2,12 @@
 refusals on the device."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
-from slideformer_amd import ops
+from slideformer_amd import _lib, _ops_lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -378,3 +380,67 @@ def test_gradients_of_rotated_heads_go_to_their_own_place_or_where_nothing_is_re
             for a, b in zip(got, want):
                 assert a is b is None or torch.equal(a, b)
             wide.copy_(kept)
+
+
+def _fp32_within(wide, first):
+    """Four fp32 to each row of `wide`, from its element `first` on."""
+    return wide.view(torch.float32)[..., 0, :4].as_strided((*wide.shape[:-2], 4), (*(n // 2 for n in wide.stride()[:-2]), 1), first // 2)
+
+
+@pytest.mark.parametrize("packed", [True, False])
+def test_gradients_of_attention_do_not_go_into_one_another(hip_device, t, packed):
+    """Nor into lse.  Between all that is read and written is fine, row by row."""
+    rows = (130,) if packed else (2, 65)
+    wide = _normal(t, *rows, 25, 64)
+    q, g, out, gq = (wide[..., 4 * i:4 * i + 4, :] for i in range(4))
+    k, v, gk, gv = (wide[..., 16 + 2 * i:18 + 2 * i, :] for i in range(4))
+    how = dict(starts=torch.tensor([0, 60, 130], device=hip_device)) if packed else {}
+    o, lse = ops.attention(q, k, v, **how)
+    out.copy_(o)
+    want = ops.attention_grad(g, q, k, v, out, lse, **how)
+    kept = wide.clone()
+
+    def refused(grads, lse=lse):
+        with pytest.raises(RuntimeError, match="la_attention_grad"):
+            ops.attention_grad(g, q, k, v, out, lse, grads=grads, **how)
+        assert torch.equal(wide, kept)
+
+    for grads in ((gq, gk, _moved(gk, 64)), (gq, _moved(gv, 64), gv), (gq, _moved(gk, 65), gv), (_moved(gq, 64 * 8 - 63), gk, gv),
+                  (_moved(gq, -1), gk, gv), (gq, _moved(gk, -64), gv), (gq, gk, _moved(gk, 1)), (gq, gk, gk), (gq, gv, gv)):
+        refused(grads)
+    for first in (12 * 64 + 100, 21 * 64 + 56, 22 * 64 - 2):     # the last from grad_k's last element on
+        refused((gq, gk, gv), lse=_fp32_within(wide, first))
+    within = _fp32_within(wide, 24 * 64 + 8)
+    within.copy_(lse)
+    kept.copy_(wide)
+    for a, b in zip(ops.attention_grad(g, q, k, v, out, within, grads=(gq, gk, gv), **how), want):
+        assert torch.equal(a, b)
+    for x in (wide, kept):
+        for of in (slice(12, 16), slice(20, 24)):
+            x[..., of, :] = 0
+    assert torch.equal(wide.view(torch.int16), kept.view(torch.int16))       # bits: lse's halves may be NaN
+
+
+def test_results_of_attention_in_memory_of_the_callers(hip_device, t):
+    """Through the C-ABI, which takes out and lse: not where the call reads, indices among it, nor in one another."""
+    wide, buf = _normal(t, 4, 14, 64), torch.tensor([0, 3, 4] + [4] * 253, device=hip_device)
+    q, k, v, free = wide[:, :4], wide[:, 4:6], wide[:, 6:8], wide[:, 8:12]
+    starts, lse = buf[:3], _fp32_within(wide, 13 * 64)
+    want = ops.attention(q, k, v, starts=starts)
+    lib, kept = _ops_lib.load(), wide.clone()
+
+    def run(out, lse):
+        device, call = ops._attention_call(q, k, v, True, None, None, starts, None, None, None)
+        call.out, call.lse = ops._heads(out, "out", device, 3), ops._row_values(lse, "lse", device, q)
+        work = torch.empty(1 << 16, dtype=torch.uint8, device=device)
+        assert lib.la_attention_workspace(ctypes.byref(call)) <= work.numel()
+        return lib.la_attention(ctypes.byref(call), work.data_ptr(), work.numel(), torch.cuda.current_stream().cuda_stream)
+
+    for out, where in ((q, lse), (_moved(q, 64), lse), (wide[:, 5:9], lse), (_moved(free, -65), lse), (buf.view(BF16).view(4, 4, 64), lse),
+                       (free, _fp32_within(wide, 9 * 64)), (free, _fp32_within(wide, 12 * 64 - 2)), (free, _fp32_within(wide, 6)),
+                       (free, _fp32_within(wide, 8 * 64 - 2)), (free, buf.view(torch.float32)[2:18].view(4, 4))):
+        assert run(out, where) == _lib.LA_EINVAL
+        assert torch.equal(wide, kept) and buf[:4].tolist() == [0, 3, 4, 4]
+    assert run(free, lse) == _lib.LA_OK
+    assert torch.equal(free, want[0]) and torch.equal(lse, want[1])
+    assert torch.equal(wide[:, :8], kept[:, :8])
