@@ -38,23 +38,23 @@ struct ForwardArgs {
     int aligned;                    // rows of the result may be written 16 bytes at a time
 };
 
-// How P is held, relative to a row's reference st.top: times 2^kUp.  Exponentials need the maximum of no tile but a row's
-// first: those of later ones add up to less than kMost nearly always, and where they do not, the scores are made again and
-// the references raised.  Looking for the maximum of every tile instead is 21 more vector instructions of about 165, which
-// bind heads of 64.
+// How P is held, relative to a row's reference st.top: times 2^kUp.  Exponentials need the maximum of no tile but a
+// row's first: those of later ones add up to less than kMost nearly always, and where they do not, the scores are made
+// again and the references raised.  Looking for the maximum of every tile instead is 21 more vector instructions of about
+// 165, which bind heads of 64.
 template <typename T> struct Held {
     static constexpr bool kLowers = false;
     static constexpr float kUp = 0.0f, kDown = 1.0f, kMost = 4096.0f;
 };
 // fp16 holds 2^-24 to 65504, and where one key is far above the others, as a text's first token often is, the others are
-// below that beside it: 65536 of them, 17.5 lower, were 3 % off together, where the first one's value is small.  So P is held
-// times 2^9, and where a tile's sum is less than kLeast, the reference is lowered to the tile's maximum, and `sum` and `out`,
-// in fp32, raised by as much; so are the wave's other rows whose sum is less than kLow, which would soon be next.  A
-// probability is then off by half a step, or by 2^-20 of its tile's sum.  Lowering ends with sums of kLowered and
-// more, beside which what is lower still is nothing in fp16 results; it is by 2^kStep at the most, so that sums of products
-// stay below 2^(kStep + 50) * 65504.
-// 8192 tokens, causal, 32 and 8 heads of 128: 562 us, and 553 with P held times 1 as bf16's; 8 x 1024, 12 heads of 64: 28.9
-// and 27.4; with a first key 17.5 above the others 563 and 29.5.
+// below that beside it: 40000 of them, 17.5 lower, gave results up to 49 % off where the first one's value is small.  So
+// P is held times 2^9, and where a tile's sum is less than kLeast, the reference is lowered to the tile's maximum, and
+// `sum` and `out`, in fp32, raised by as much; so are the wave's other rows whose sum is less than kLow, which would soon
+// be next.  A probability is then off by half a step, or by 2^-20 of its tile's sum.  Lowering ends with sums of kLowered
+// and more, beside which what is lower still is nothing in fp16 results; it is by 2^kStep at the most, so that sums of
+// products stay below 2^(kStep + 50) * 65504.
+// 8192 tokens, causal, 32 and 8 heads of 128: 562 us, and 553 with P held times 1 as bf16's; 8 x 1024, 12 heads of 64:
+// 28.9 and 27.4; with a first key 17.5 above the others 563 and 29.5.
 template <> struct Held<_Float16> {
     static constexpr bool kLowers = true;
     static constexpr float kUp = 9.0f, kDown = 0x1p-9f, kMost = 65024.0f;    // 127 * 2^9; each term is below 65504
@@ -163,7 +163,8 @@ __device__ __forceinline__ void take(State<D>& st, const s16x8 (&q)[D / 16], con
     bool again, lower = false;
     if constexpr (Held<T>::kLowers) {
         // in one comparison what is nearly never so, NaN and 0 (nothing seen) among it
-        constexpr uint32_t kFrom = __builtin_bit_cast(uint32_t, Held<T>::kLeast), kTo = __builtin_bit_cast(uint32_t, Held<T>::kMost);
+        constexpr uint32_t kFrom = __builtin_bit_cast(uint32_t, Held<T>::kLeast);
+        constexpr uint32_t kTo = __builtin_bit_cast(uint32_t, Held<T>::kMost);
         again = __any(__float_as_uint(sum) - kFrom > kTo - kFrom);
         if (again) {
             const bool lowers = sum > 0.0f && st.sum < Held<T>::kLowered;
@@ -279,11 +280,13 @@ __device__ __forceinline__ void load_row(s16x8 (&q)[D / 16], const char* row, bo
 
 // 128 rows to a workgroup, 32 to a wave; all waves go over the same tiles of 64 keys, two of which are
 // in LDS: one in work, the next on its way.  Two workgroups on a compute unit (four of D = 64), each in the
-// other's pauses.  8192 tokens, causal, 32 and 8 heads of 128 in bf16: 525 us, 1.05 PFLOP/s, the matrix cores busy 57 % of
-// the cycles.  8 x 1024 tokens, causal, 12 heads of 64: 27 us, 0.49 PFLOP/s, matrix cores busy 31 %: with half the products
-// for each exponential the vector instructions bind, 15 to a product, and the launch is as long as its longest piece.  Two variants took fewer cycles and no less time, as the clock sank with them (1.95 GHz
-// in a first launch, 1.6 to 1.7 under load): scores of the next tile between the exponentials of this
-// one (541), and eight waves that take turns at multiplying and at exponentials (530).
+// other's pauses.  8192 tokens, causal, 32 and 8 heads of 128 in bf16: 511 us, 1.08 PFLOP/s, the matrix cores busy 60 % of
+// the cycles (launches settle at that after some twenty; those first ones, while the clock is found, take 522 to 677).
+// 8 x 1024 tokens, causal, 12 heads of 64: 28 us, 0.46 PFLOP/s, matrix cores busy 31 %: with half the products for each
+// exponential the vector instructions bind, 15 to a product, and the launch is as long as its longest piece.  Two
+// variants took fewer cycles and no less time, as the clock sank with them (1.95 GHz in a first launch, 1.6 to 1.7 under
+// load): scores of the next tile between the exponentials of this one, and eight waves that take turns at multiplying and
+// at exponentials (541 and 530, where this took 525).
 template <typename T, int D> __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_kernel(ForwardArgs a)
 {
     constexpr uint32_t kBytes = Tile<D>::kBytes;
@@ -363,8 +366,9 @@ template <typename T, int D> __global__ __launch_bounds__(256, D == 64 ? 3 : 2) 
 // with tiles of its own in LDS and without waiting for the others, and join at the end.  Two waves, so that
 // two workgroups or more are on a compute unit and one's start and end are under the other's loads.
 // Bound by memory: a wave takes 0.8 us for 32 keys where loads do not bind.  16 rows of 32/8 heads of 128 over caches
-// of 8192 filled to 5600 on average, 367 MB: 75 us, 4.9 TB/s; one row over 65536, 268 MB: 44.6 us, 6.0 TB/s.  With five tiles in a ring, four of them
-// on their way, one row over 65536 keys of eight heads took 47.9 us instead of 44.4, with four waves 46.5.
+// of 8192 filled to 5600 on average, 367 MB: 76 us, 4.8 TB/s; one row over 65536, 268 MB: 43.7 us, 6.1 TB/s.  With five
+// tiles in a ring, four of them on their way, one row over 65536 keys of eight heads took 47.9 us instead of 44.4, with
+// four waves 46.5.
 constexpr uint32_t kFewWaves = 2;
 
 template <typename T, int D> __global__ __launch_bounds__(kFewWaves * 64, 1) void few_rows_kernel(ForwardArgs a)

@@ -210,9 +210,10 @@ __device__ __forceinline__ void store_row(char* to, const f32x16 (&x)[D / 32], f
 constexpr int32_t kOwnKeys = 192;
 
 // 128 rows to a workgroup, 32 to a wave, tiles of 64 keys as in the forward pass, and two workgroups on a compute unit.
-// 8192 tokens in five packed documents of 717 to 3588, 32/8 heads of 128 in bf16: 261 us, 0.89 PFLOP/s of its three
-// products; 8 x 1024 tokens, 12 heads of 64, 34 us.  The matrix cores are busy 51 and 35 % of the cycles: between a tile's
-// scores and its sums a wave has exponentials, and one other wave whose products could go on meanwhile.
+// 8192 tokens in five packed documents of 717 to 3588, 32/8 heads of 128 in bf16: 244 us, 0.95 PFLOP/s of its three
+// products (261 in the first twenty launches, while the clock is found); 8 x 1024 tokens, 12 heads of 64, 33 us.  The
+// matrix cores are busy 51 and 35 % of the cycles: between a tile's scores and its sums a wave has exponentials, and one
+// other wave whose products could go on meanwhile.
 template <typename T, int D> __global__ __launch_bounds__(256, 2) void grad_q_kernel(GradArgs a)
 {
     constexpr uint32_t kBytes = Tile<D>::kBytes;
@@ -545,10 +546,10 @@ template <typename T, int D> struct Keys {
 // 128 keys to a workgroup, 32 to a wave; all waves go over the same tiles of 64 rows of one query
 // head after the other.  Four tiles are in LDS: one whose sums are made, one whose scores are, two on their way.  One wave
 // on a SIMD (two of D = 64): both sums and both own operands of 128 keys take 360 registers.
-// 8192 tokens in five packed documents of 717 to 3588, 32/8 heads of 128 in bf16: 445 us, 0.69 PFLOP/s of its four
-// products; 8 x 1024 tokens, 12 heads of 64, 46 us.  The matrix cores are busy 51 and 35 % of the cycles, bound by issue
-// (a wave alone issues an instruction in 5.5 cycles, a product takes 32); and compute units have work 71 % of the first
-// case's time, for the longest document's first keys are the longest chain.  Two parts for each such piece took 10 % longer
+// 8192 tokens in five packed documents of 717 to 3588, 32/8 heads of 128 in bf16: 389 us, 0.79 PFLOP/s of its four
+// products (440 in the first twenty launches); 8 x 1024 tokens, 12 heads of 64, 45 us.  The matrix cores are busy 51 and
+// 35 % of the cycles, bound by issue (a wave alone issues an instruction in 5.5 cycles, a product takes 32); and compute
+// units have work 71 % of the first case's time, for the longest document's first keys are the longest chain.  Two parts for each such piece took 10 % longer
 // with the card full, probably since their rows do not come from L2 together.
 template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_kernel(GradArgs a)
 {

@@ -461,15 +461,18 @@ inline la_memory::Place place_of_lse(const la_attention_t& c)
 // Whether results share no memory with one another, with `read`, or with the indices: kernels read and write in no order,
 // and one what the next reads.  They may lie between one another, as parts of a projection's gradient do.
 template <int WRITTEN, int READ>
-inline bool results_apart(const la_attention_t& c, const la_memory::Place (&written)[WRITTEN], const la_memory::Place (&read)[READ])
+inline bool results_apart(const la_attention_t& c, const la_memory::Place (&written)[WRITTEN],
+                          const la_memory::Place (&read)[READ])
 {
+    using la_memory::flat;
+    using la_memory::Place;
     const uint64_t size = c.index_dtype == LA_I64 ? 8 : 4;
-    const la_memory::Place indices[] = {la_memory::flat(c.starts, (c.batch + 1) * size), la_memory::flat(c.key_starts, (c.batch + 1) * size),
-                                        la_memory::flat(c.lengths, c.batch * size), la_memory::flat(c.key_lengths, c.batch * size)};
+    const Place indices[] = {flat(c.starts, (c.batch + 1) * size), flat(c.key_starts, (c.batch + 1) * size),
+                             flat(c.lengths, c.batch * size), flat(c.key_lengths, c.batch * size)};
     for (int k = 0; k < WRITTEN; ++k) {
-        for (const la_memory::Place& p : read)
+        for (const Place& p : read)
             if (shared(written[k], p)) return false;
-        for (const la_memory::Place& p : indices)
+        for (const Place& p : indices)
             if (shared(written[k], p)) return false;
         for (int m = 0; m < k; ++m)
             if (shared(written[k], written[m])) return false;

@@ -182,8 +182,10 @@ template <typename T> __device__ __forceinline__ T* head_at(const HeadRows& r, u
 }
 
 // One wave takes U query heads, or key heads, of a token for each of its groups of lanes, all loads first.
-// Bound by memory: 8192 tokens of 32 and 8 heads of 128 in bf16, 172 MB, take 35.0 us, 4.9 TB/s, what a copy of
-// 2 GiB reaches; 40.7 with stores that stay in the caches, 36.5 with U = 2.
+// Bound by memory: 8192 tokens of 32 and 8 heads of 128 in bf16, 172 MB, take 32.6 us, 5.3 TB/s, where a copy of
+// 2 GiB reaches 4.9; 37.0 with stores that stay in the caches, 1.5 more with U = 2.  With the attention that reads them next
+// the stores past the caches gain for shorter batches and lose a little for longer ones: 1100 tokens in windows of 128
+// 24.2 us and 27.0, 2048 28.4 and 29.7, 8192 94 and 95; causal, 2048 tokens 62 and 63, two times 2048 103.5 and 100.1.
 template <typename T, bool INTERLEAVED, bool WHOLE, int U> __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a)
 {
     constexpr int V = Elem<T>::kCount;
