@@ -223,7 +223,7 @@ template <typename T, int D>
 __device__ __forceinline__ void finish(const ForwardArgs& a, const Piece& p, uint32_t kv_head, uint32_t part, uint32_t row,
                                        State<D>& st)
 {
-    const uint32_t half = threadIdx.x % kWave / 32;
+    const uint32_t half = lane_now() / 32;
     const uint32_t token = row / a.seq.group, head = kv_head * a.seq.group + row % a.seq.group;
     const float sum = sum_of<T>(st);
     // a row that sees nothing: zeros, and -inf
@@ -359,7 +359,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, D == 64 ? 3 : 2) 
             }
         }
     }
-    finish<T, D>(a, p, kv_head, part, row, st);
+    finish<T, D>(a, p, kv_head, part, wave_row + lane_now() % 32, st);
 }
 
 // At most 32 rows to a workgroup (a single new token's heads): its waves take the same rows and different keys, each

@@ -19,7 +19,7 @@
 //
 // P and dS are rounded to the operands' 16 bits before the last three products, as the matrix cores take them, and
 // delta, but for short sequences and windows, is that of the O that was given, itself rounded: bf16 gradients of q and k
-// are 2.7e-3 off where rounding the exact ones is 1.7e-3 off, fp16 3.5e-4 and 2.1e-4.  A delta from the sums of P dP
+// are up to 2.8e-3 off where rounding the exact ones is 1.7e-3 off, fp16 3.5e-4 and 2.1e-4.  A delta from the sums of P dP
 // would not have O's rounding, but would be wrong with an lse over more keys than the call has.  Everything else is fp32.
 #include "attention_tile.h"
 

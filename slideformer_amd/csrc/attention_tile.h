@@ -92,6 +92,9 @@ __device__ __forceinline__ float both_sum(float x)
 // probabilities up to 1 notices.
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// threadIdx.x % kWave, made anew: kept from a kernel's start it takes a register through its loop.
+__device__ __forceinline__ uint32_t lane_now() { return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
+
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ uint64_t uniform(uint64_t x)
 {

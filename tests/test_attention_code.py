@@ -118,3 +118,21 @@ def test_the_checks_find_what_they_look_for():
     assert not _hazards(["v_readfirstlane_b32 s4, v1", "s_nop 4", "buffer_load_dwordx4 v1, s[4:7], 0 offen lds", *quiet])
     loop = [".L0:", "a", "s_cbranch_vccz .L1", "b", ".L1:", "c", "s_branch .L0"]
     assert _paths(loop) == [["a", "s_cbranch_vccz .L1", "b", "c", "s_branch .L0"], ["a", "s_cbranch_vccz .L1", "c", "s_branch .L0"]]
+
+
+@pytest.mark.slow
+def test_attention_keeps_its_rows_in_registers(tmp_path):
+    """No kernel of the forward pass has scratch memory, and those of heads of 64 let three waves on a SIMD."""
+    out = tmp_path / "attention.s"
+    flags = [f for f in build.BASE_FLAGS if f not in ("-shared", "-fPIC", "-Wall")]
+    subprocess.run([build.hipcc(), *flags, "--cuda-device-only", "-S", "-I",
+                    os.path.join(build.REPO_DIR, "include"), "-o", str(out),
+                    os.path.join(build.CSRC, "attention.hip")], check=True, capture_output=True)
+    text = out.read_text()
+    kernels = re.findall(r"\.amdhsa_kernel (\S+)(.*?)\.end_amdhsa_kernel", text, re.S)
+    assert len(kernels) == 13, [name for name, _ in kernels]     # two types, two sizes, three kernels; the copy into chunks
+    for name, fields in kernels:
+        got = {k: int(v) for k, v in re.findall(r"\.amdhsa_(private_segment_fixed_size|next_free_vgpr) (\d+)", fields)}
+        assert got["private_segment_fixed_size"] == 0, name
+        if "16attention_kernel" in name and "Li64" in name:
+            assert got["next_free_vgpr"] <= 168, name            # 512 for three, in eights
