@@ -549,8 +549,8 @@ template <typename T, int D> struct Keys {
 // 8192 tokens in five packed documents of 717 to 3588, 32/8 heads of 128 in bf16: 389 us, 0.79 PFLOP/s of its four
 // products (440 in the first twenty launches); 8 x 1024 tokens, 12 heads of 64, 45 us.  The matrix cores are busy 51 and
 // 35 % of the cycles, bound by issue (a wave alone issues an instruction in 5.5 cycles, a product takes 32); and compute
-// units have work 71 % of the first case's time, for the longest document's first keys are the longest chain.  Two parts for each such piece took 10 % longer
-// with the card full, probably since their rows do not come from L2 together.
+// units have work 71 % of the first case's time, for the longest document's first keys are the longest chain.  Two parts
+// for each such piece took 10 % longer with the card full, probably since their rows do not come from L2 together.
 template <typename T, int D> __global__ __launch_bounds__(256, 1) void grad_kv_kernel(GradArgs a)
 {
     using Mine = Keys<T, D>;
